@@ -9,6 +9,7 @@ in libsmla.so (C ABI: include/smla.h):
 * ``smla.indexer``      — indexer scoring and exact top-k selection
 * ``smla.norm_rope``    — ``ref_torch/norm_rope.py`` (tables for the kernels)
 * ``smla.mla``          — ``v4mlx/mla.py`` projections
+* ``smla.paged``        — the paged latent cache: attention, append, slots forked and grown, compaction
 * ``smla.workloads``    — seeded synthetic inputs of the benchmark configurations
 """
 from . import _lib  # noqa: F401

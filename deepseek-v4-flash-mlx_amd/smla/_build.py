@@ -8,7 +8,7 @@ from concurrent.futures import ThreadPoolExecutor
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(_HERE), "csrc")
 SOURCES = ["attn.hip", "attn_decode.hip", "indexer.hip", "topk.hip", "pool.hip", "qat.hip", "linear.hip",
-           "gemm.hip", "capi.hip"]
+           "gemm.hip", "paged.hip", "paged_attn.hip", "capi.hip"]
 OUT = os.path.join(_HERE, "libsmla.so")
 # linker version script: only the smla_* C entry points are exported
 EXPORTS = os.path.join(CSRC, "libsmla.map")
@@ -18,9 +18,10 @@ FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC",
          # not know the feature; that is harmless)
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
-# per-source additions.  attn_decode.hip: MFMA accumulators in VGPRs (its online-softmax rescale
+# per-source additions.  attn_decode.hip, paged_attn.hip: MFMA accumulators in VGPRs (its online-softmax rescale
 # touches them with VALU ops; with AGPR accumulators every P.V step would copy them both ways)
-EXTRA = {"attn_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"]}
+_VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=true"]
+EXTRA = {"attn_decode.hip": _VGPR_FORM, "paged_attn.hip": _VGPR_FORM}
 
 
 def _compile(hipcc, src, obj):

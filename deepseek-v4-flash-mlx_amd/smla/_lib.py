@@ -77,6 +77,17 @@ _SIGNATURES = {
                               _i64, _vp, _vp, _int, _vp, _sz, _vp]),
     "smla_o_proj": (_int, [_vp, _int, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _int,
                            _i64, _vp, _vp, _int, _vp]),
+    "smla_paged_attn_workspace": (_sz, [_i64] * 3),
+    "smla_paged_attn": (_int, [_vp, _int, _vp, _int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
+                               _i64, _f32, _vp, _i64, _i64, _int, _vp, _int, _vp, _sz, _vp]),
+    "smla_paged_append": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _f32,
+                                 _int, _int, _vp, _vp, _int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "smla_update_pages_workspace": (_sz, [_i64] * 2),
+    "smla_update_pages": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
+                                 _i64, _i64, _vp, _i64, _i64, _vp, _sz, _vp]),
+    "smla_compact_pages_workspace": (_sz, [_i64]),
+    "smla_compact_pages": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp,
+                                  _i64, _i64, _vp, _sz, _vp]),
 }
 
 # sim modes of smla_gated_pool / smla_ring_step, flags of smla_rotate_fp4
@@ -85,6 +96,8 @@ QAT_ROTATE, QAT_FP4 = 1, 2
 
 # phases of smla_sparse_attn_ex, flags of smla_index_decode
 ATTN_SPLIT, ATTN_MERGE = 1, 2
+# flags of smla_paged_append and smla_paged_attn (FILL)
+PAGED_NORM_Q, PAGED_NORM_KV, PAGED_FILL = 1, 2, 4
 INDEX_EXACT = 1
 
 

@@ -40,6 +40,10 @@
  *   smla_linear_ws            v4mlx/mla.py:16-18               (the same, with a workspace)
  *   smla_linear_pair_ws       ref_torch/compressor.py:28-29    kv and score projections in one launch
  *   smla_q_up                 oracle/decode_engine.py:78-80    q_up, per-head norm and RoPE of a prompt
+ *   smla_paged_attn           oracle/decode_engine.py:107-117  the attention of a ragged batch over pages of rows
+ *   smla_paged_append         oracle/decode_engine.py:78-84    q / kv norms, RoPE, quantisation, write to pages
+ *   smla_update_pages         oracle/v4_fast.py:150-159        copies of sequences' caches (clone_states), as pages
+ *   smla_compact_pages        (none: the reference's caches are contiguous)
  *   smla_o_proj, _ws          oracle/decode_engine.py:118-119  inverse RoPE of o's rope dims + o_grouped
  *                             v4mlx/mla.py:42-56               o_grouped(o, wo_a, wo_b)
  */
@@ -516,6 +520,84 @@ int smla_o_proj_ws(const void* o, int o_dtype, const int32_t* pos, const float* 
                    int64_t rd, int64_t G, int64_t R, const void* wo_a, const void* wo_b, int w_dtype,
                    int64_t dim, void* mid, void* y, int y_dtype, void* workspace, size_t workspace_bytes,
                    void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Paged latent cache.  A pool is n_pages pages of P rows of D channels (pages [n_pages, P, D]: BF16, or
+ * FP8_E4M3 codes with page_scales [n_pages, P, D/64] fp32, row value = decode(code) * scale).  Row j of
+ * sequence b is row j % P of page table[b, j / P] (table: B rows of cols entries, ld_table elements apart).
+ * All integers are int32 on the device and none is read by the host, so a captured call follows
+ * them.  A page id outside [0, n_pages) is no page: such rows are not read, written or counted.
+ * Several sequences may share a page; rows are then appended only past the rows they share
+ * (smla_update_pages keeps it so).  n_pages * P < 2^31.
+ *
+ * A batch is ragged: B sequences with lens[b] rows in the cache, the last cu[b+1] - cu[b] of them those
+ * of the tokens cu[b] .. cu[b+1]-1 (cu [B+1], cu[0] = 0, not decreasing, cu[B] <= T); token t sits at position
+ * lens[b] - (cu[b+1] - cu[b]) + t - cu[b].  What belongs to tokens at and behind cu[B] is left as it was,
+ * or, with SMLA_PAGED_FILL, set to 0. */
+enum { SMLA_PAGED_NORM_Q = 1, SMLA_PAGED_NORM_KV = 2, SMLA_PAGED_FILL = 4 };
+
+/* smla_paged_attn: attention of those tokens over their sequences' rows, after the rows are in the cache.
+ *   q [T, H, D] BF16, D 576 or 512; out [T, H, DV] BF16, DV 512; any H; attn_sink [H] fp32 or NULL
+ * Token at position p attends rows j <= p; with window > 0 those with j > p - window or j < first (a
+ * sliding window and the first rows).  scale multiplies q.row; the sink adds exp(sink) to the
+ * denominator.  A token that sees no row gives 0.  Rows a token does not see may hold anything,
+ * infinities and NaN too; a row it sees that scores NaN or +inf gives NaN.
+ * flags: 0 or SMLA_PAGED_FILL.  q, pages, out and workspace 16-byte aligned.  Sums and softmax statistics
+ * are fp32; probabilities, and the partial sums of tokens whose rows are split over workgroups, are
+ * rounded to bf16 before their products and joins.  The result does not depend on the order in which
+ * workgroups run.  workspace: smla_paged_attn_workspace(T, H, B) bytes, not shared by calls that overlap. */
+size_t smla_paged_attn_workspace(int64_t T, int64_t H, int64_t B);
+int smla_paged_attn(const void* q, int q_dtype, const void* pages, int page_dtype, const float* page_scales,
+                    int64_t n_pages, int64_t P, const int32_t* table, int64_t ld_table, int64_t cols,
+                    const int32_t* lens, const int32_t* cu, int64_t B, int64_t T, int64_t H, int64_t D, int64_t DV,
+                    float scale, const float* attn_sink, int64_t window, int64_t first, int flags, void* out,
+                    int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* smla_paged_append: the tokens' queries and latent rows from their projections, in one launch.
+ *   q [T, H, D] (tokens ldq elements apart; H = 0: none) and kv [T, D] (ldkv apart), both F32 or BF16
+ * With SMLA_PAGED_NORM_Q / SMLA_PAGED_NORM_KV the first norm_dims channels of every query head / row are
+ * RMS-normed (eps; weights q_w / kv_w [norm_dims] fp32, NULL: none); then the last rd channels are rotated to
+ * the token's position as in smla_rope (cos_t, sin_t [n_pos, rd/2] fp32).  Queries go to q_out [T, H, D] BF16,
+ * the row to its page: BF16 (sim SMLA_SIM_FP8: its first D - rd channels fp8 round-tripped) or e4m3 codes and
+ * scales, quantised as smla_quant_fp8_pow2 does.  A token at a position outside [0, n_pos) (rd > 0) writes
+ * nothing (SMLA_PAGED_FILL: zero queries); a row past the table's columns or whose entry is no
+ * page is not stored.  D a multiple of 64 up to 1024, rd and norm_dims multiples of 4, ldq and ldkv too; rd a
+ * multiple of 64 with SMLA_SIM_FP8; q and kv aligned to four of their elements, q_out and pages to 8 bytes. */
+int smla_paged_append(const void* q, int64_t ldq, const void* kv, int64_t ldkv, int x_dtype, int64_t T, int64_t H,
+                      int64_t D, int64_t norm_dims, const float* q_w, const float* kv_w, const float* cos_t,
+                      const float* sin_t, int64_t n_pos, int64_t rd, float eps, int sim, int flags, void* q_out,
+                      void* pages, int page_dtype, float* scales, int64_t n_pages, int64_t P, const int32_t* table,
+                      int64_t ld_table, int64_t cols, const int32_t* lens, const int32_t* cu, int64_t B, void* stream);
+
+/* smla_update_pages: what happens to S slots between two steps, all at once.  Slot s becomes a copy of slot
+ * parent[s] as it was before the call (s: itself, -1: an empty slot) with grow[s] >= 0 more rows:
+ *   - its parent's whole pages are shared; of a partly filled last page the rows in use are copied to a
+ *     fresh page, unless the slot keeps its own (parent[s] == s);
+ *   - fresh pages are the free ones (refs 0) in ascending order, taken by the slots in order;
+ *   - granted[s] = 1 if parent[s] and grow[s] are valid, the rows fit M pages and the pages that slots 0 .. s ask
+ *     for are at most the free ones; else 0, and the slot stays as it was.
+ * In: table [S, M] (ld_table), lens [S], refs [n_pages] (how many entries name each page).  Out, all other
+ * buffers than the inputs: table_out [S, M] dense (-1 past a slot's pages), lens_out, refs_out, granted [S].
+ * Pages given up by the call are free from refs_out on.  Rows are copied within `layers` pools that share the table
+ * (layer l at pages + l layer_bytes; row_bytes a row), and likewise within scales (NULL: none).
+ * workspace: smla_update_pages_workspace(S, n_pages) bytes, 4-byte aligned. */
+size_t smla_update_pages_workspace(int64_t S, int64_t n_pages);
+int smla_update_pages(const int32_t* table, int64_t ld_table, int64_t S, int64_t M, const int32_t* lens,
+                      const int32_t* refs, int64_t n_pages, int64_t P, const int32_t* parent, const int32_t* grow,
+                      int32_t* table_out, int32_t* lens_out, int32_t* refs_out, int32_t* granted, void* pages,
+                      int64_t layers, int64_t layer_bytes, int64_t row_bytes, void* scales, int64_t scale_layer_bytes,
+                      int64_t scale_row_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
+/* smla_compact_pages: the live pages (refs > 0) moved to the ids below their number: the i-th live page at or
+ * past it goes to the i-th free id below it, in every layer; the others stay.  table_out [S, M] names the new ids
+ * (-1 for an entry that names no live page), refs_out their counts, live [1] their number; all other buffers
+ * than the inputs.  The moved pages' old places keep their rows.  Other arguments as above.
+ * workspace: smla_compact_pages_workspace(n_pages) bytes, 4-byte aligned. */
+size_t smla_compact_pages_workspace(int64_t n_pages);
+int smla_compact_pages(const int32_t* table, int64_t ld_table, int64_t S, int64_t M, const int32_t* refs,
+                       int64_t n_pages, int64_t P, int32_t* table_out, int32_t* refs_out, int32_t* live, void* pages,
+                       int64_t layers, int64_t layer_bytes, int64_t row_bytes, void* scales, int64_t scale_layer_bytes,
+                       int64_t scale_row_bytes, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
