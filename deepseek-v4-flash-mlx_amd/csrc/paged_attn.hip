@@ -6,19 +6,28 @@
 // j > p - window or j < first.  out = sum_j e^(s_j - m) row_j[:512] / (sum_j e^(s_j - m) + e^(sink - m)) with
 // s_j = scale q.row_j; a token that sees no row gives 0.
 //
-// A sequence's (token, head) pairs are rows of q, n_b * H of them in a run; a tile is 64 of them (one token
-// of 64 heads, four of 16).  The rows a tile visits are numbered through: entry e < nf is row e (the first
-// rows, where the window starts behind them), entry e >= nf row lo + e - nf.  A work item is a run of `rps`
-// entries of one tile; every workgroup finds its item from the lengths itself (no plan launch, no host
-// read): with few tiles rps is the smallest that gives every compute unit at most one item, with many
-// it only cuts entries that one workgroup would be long busy with.  Tiles of several items leave (m, l, O)
-// states that paged_merge_kernel joins.
+// A sequence's (token, head) pairs are rows of q, n_b * H of them in a run; a tile is 32 NB of them.  The rows
+// a tile visits are numbered through: entry e < nf is row e (the first rows, where the window starts
+// behind them), entry e >= nf row lo + e - nf.  A work item is a run of `rps` entries of one tile; every
+// workgroup finds its item from the lengths itself (no plan launch, no host read): with few tiles rps is the
+// smallest that gives every compute unit at most one item, with many it only cuts entries that one workgroup
+// would be long busy with.  Tiles of several items leave (m, l, O) states that paged_merge_kernel joins.
 //
-// The workgroup is the sparse decode kernel's: 12 waves, 4 that score 16 rows of q each (S^T = K Q^T,
-// online softmax, P to LDS) and 8 that accumulate O^T += V^T P^T, one tile of 32 rows apart, rows copied
-// HBM -> LDS into a ring by the value waves (fp8 rows: loaded, converted, written).  Row numbers come
-// through an LDS ring of 8 tiles that score wave 0 fills seven tiles ahead, so a row list of any length
-// costs one table read per row.
+// A workgroup is 8 waves of up to 256 registers, two per SIMD, and walks its entries in tiles of 32 rows, two
+// roles one tile apart with one barrier between:
+//   * score waves 0 .. NB-1: S^T = K Q^T of 32 q rows (v_mfma_f32_16x16x32_bf16, rows as M; the 32 rows' Q^T
+//     stays in 144 registers, so a K fragment read from LDS serves two products), online softmax with a lazy
+//     maximum, P in bf16 and the rescale factor to LDS;
+//   * value waves 3 .. 7: O^T += V^T P^T (v_mfma_f32_32x32x16_bf16) of 3 or 4 blocks of 32 value columns and all
+//     the tile's q rows, so each V^T fragment (ds_read_b64_tr_b16) is read by one wave and serves NB products.
+//     Wave 3 shares its SIMD with value wave 7 instead of a score wave and takes four blocks, the others three.
+// At NB = 3 the matrix pipes of SIMDs 0 .. 2 have 1152 + 576 cycles a tile, SIMD 3 has 1344, against about
+// 6.8 KB of LDS traffic a row (53 cycles of 128 bytes): both near balance, where 64 q rows on 12
+// waves of 168 registers (16 rows' Q^T a score wave) read 8.4 KB for two thirds of the products.
+//
+// Rows come HBM -> LDS by DMA into a ring of NBUF tiles, copies issued by the value waves (fp8 rows: loaded,
+// converted, written).  Row numbers go through an LDS ring of 8 tiles that score wave 0 fills seven tiles
+// ahead, so a row list of any length costs one table read per row.
 //
 // Rows masked for some of a tile's q rows may hold anything (rows not yet written, pages of id -1 read as
 // row 0): their probability is 0, and where a masked score is not finite the value waves take the tile's
@@ -31,12 +40,14 @@ namespace {
 typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i32x4_t lds_i32x4_t;
 typedef __attribute__((address_space(3))) u32x2_t lds_u32x2_t;
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
-constexpr int kTileQ = 64;       // q rows of a tile
-constexpr int kIdTiles = 8;      // tiles of the row-number ring
-constexpr int kMinRows = 64;     // fewest entries of an item
+constexpr int kIdTiles = 8;        // tiles of the row-number ring
+constexpr int kMinRows = 64;       // fewest entries of an item
 constexpr int kMinRowsMany = 256;  // the same with more tiles than compute units
-constexpr int kHeader = 256;     // workspace bytes before the states
+constexpr int kHeader = 256;       // workspace bytes before the states
+constexpr int kWaves = 8, kFirstValue = 3, kValueWaves = 5;
+constexpr int kUnits = 16;         // blocks of 32 value columns
 
 struct PagedArgs {
   const uint16_t* q;
@@ -51,8 +62,10 @@ struct PagedArgs {
   float scale;
 };
 
-template <int D, int NBUF_>
+template <int D, int NB_, int NBUF_>
 struct GeoP {
+  static constexpr int NB = NB_;
+  static constexpr int TILEQ = 32 * NB;  // q rows of a tile
   static constexpr int ROWB = D * 2;
   static constexpr bool TAIL = D > 512;
   static constexpr int MSTRIDE = 1056;  // LDS bytes per row, columns 0..511
@@ -60,20 +73,18 @@ struct GeoP {
   static constexpr int TAIL_BYTES = TAIL ? kTileRows * 128 : 0;
   static constexpr int TILE_BYTES = MAIN_BYTES + TAIL_BYTES;
   static constexpr int NBUF = NBUF_;
-  static constexpr int PSTRIDE = 80;  // bytes per q row in a P buffer: 32 probabilities, then padding (a flag in row 16 hg)
-  static constexpr int PBUF = kTileQ * PSTRIDE;
+  static constexpr int PSTRIDE = 80;  // bytes per q row in a P buffer: 32 probabilities, then padding (a flag in rows 32 s)
+  static constexpr int PBUF = TILEQ * PSTRIDE;
   static constexpr int P_OFF = NBUF * TILE_BYTES;
-  static constexpr int AL_OFF = P_OFF + 2 * PBUF;
-  static constexpr int IDS_OFF = AL_OFF + 2 * kTileQ * 4;
-  static constexpr int LOOP_END = IDS_OFF + kIdTiles * kTileRows * 4;
-  static constexpr int STAGE = kTileQ * (1024 + 16);
-  static constexpr int ML_OFF = LOOP_END > STAGE ? LOOP_END : STAGE;
-  static constexpr int LDS_BYTES = ML_OFF + kTileQ * 2 * 4;
-  static constexpr int NW = 12;
+  static constexpr int AL_OFF = P_OFF + 2 * PBUF;  // rescale factors; after the loop (m, l)
+  static constexpr int IDS_OFF = AL_OFF + 2 * TILEQ * 4;
+  static constexpr int LDS_BYTES = IDS_OFF + kIdTiles * kTileRows * 4;
   static constexpr int KSTEPS = D / 32;
   static constexpr int NDMA = kTileRows + (TAIL ? kTileRows / 8 : 0);
+  static constexpr int STATE_O = kUnits * NB * 2048;                     // bytes of a state's O^T
+  static constexpr int STATE_F = TILEQ * 2 + kValueWaves * NB * 64;       // floats: (m, l), then scales
   static_assert(LDS_BYTES <= 160 * 1024, "LDS budget");
-  static_assert(NBUF >= 3, "Q takes the last two slots; tile 0 needs one more");
+  static_assert(NB <= kFirstValue && NBUF >= 3, "roles; a tile scored, one consumed, one on its way");
   static_assert(kIdTiles >= NBUF + 2, "row numbers are written before their copies are issued");
 };
 
@@ -98,9 +109,10 @@ __device__ inline uint32_t finite2(uint32_t w) {
 // The plan.  One lane per sequence, 64 at a time; every workgroup computes the same.
 struct Seq {
   int beg, n, len;  // first token, tokens, cache rows
-  int tiles, span;  // tiles of 64 q rows; entries that a tile may visit
+  int tiles, span;  // tiles of q rows; entries that a tile may visit
 };
 
+template <int TILEQ>
 __device__ inline Seq load_seq(const PagedArgs& a, int b) {
   Seq s{0, 0, 0, 0, 0};
   if (b < a.B) {
@@ -108,11 +120,11 @@ __device__ inline Seq load_seq(const PagedArgs& a, int b) {
     s.beg = min(max(c0, 0), a.T);
     s.n = max(min(c1, a.T) - s.beg, 0);
     s.len = max(len, 0);
-    s.tiles = (int)(((uint32_t)s.n * (uint32_t)a.H + kTileQ - 1) / kTileQ);
+    s.tiles = (int)(((uint32_t)s.n * (uint32_t)a.H + TILEQ - 1) / TILEQ);
     const int64_t cap = (int64_t)a.cols * a.P;
     int64_t span = s.len < cap ? s.len : cap;
     if (a.window > 0) {
-      const int64_t w = (int64_t)a.window + a.first + (kTileQ + a.H - 1) / a.H;  // + 1 token - 1
+      const int64_t w = (int64_t)a.window + a.first + (TILEQ + a.H - 1) / a.H;  // + 1 token - 1
       span = span < w ? span : w;
     }
     s.span = (int)span;
@@ -125,11 +137,12 @@ __device__ inline int splits_of(const Seq& s, int rps) { return max(1, ceil_div(
 __device__ inline int wave_sum_i(int v) { return __builtin_amdgcn_readlane(wave_incl_scan(v), 63); }
 
 // Entries per item (a multiple of 32).  s0: sequences 0..63, kept in registers by the caller.
+template <int TILEQ>
 __device__ inline int plan_rps(const PagedArgs& a, const Seq& s0, int lane) {
   float work = 0.f;
   int tiles = 0, most = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const Seq s = b0 == 0 ? s0 : load_seq(a, b0 + lane);
+    const Seq s = b0 == 0 ? s0 : load_seq<TILEQ>(a, b0 + lane);
     work += wave_sum_dpp((float)s.tiles * (float)s.span);
     tiles += wave_sum_i(s.tiles);
     most = max(most, (int)wave_max_dpp((float)(s.tiles > 0 ? s.span / kTileRows + 1 : 0)));
@@ -146,7 +159,7 @@ __device__ inline int plan_rps(const PagedArgs& a, const Seq& s0, int lane) {
     const int mid = lo + (hi - lo) / 2;
     int items = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-      const Seq s = b0 == 0 ? s0 : load_seq(a, b0 + lane);
+      const Seq s = b0 == 0 ? s0 : load_seq<TILEQ>(a, b0 + lane);
       items += wave_sum_i(s.tiles * splits_of(s, mid * kTileRows));
     }
     if (items <= a.cus) hi = mid;
@@ -161,10 +174,11 @@ struct Item {
   Seq s;
   int b, tile, split, nsplit, slot;
 };
+template <int TILEQ>
 __device__ inline bool find_item(const PagedArgs& a, const Seq& s0, int lane, int rps, int w, bool by_tile, Item& it) {
   int before = 0, slots = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const Seq s = b0 == 0 ? s0 : load_seq(a, b0 + lane);
+    const Seq s = b0 == 0 ? s0 : load_seq<TILEQ>(a, b0 + lane);
     const int ns = splits_of(s, rps);
     const int states = ns > 1 ? s.tiles * ns : 0;
     const int mine = by_tile ? (ns > 1 ? s.tiles : 0) : s.tiles * ns;
@@ -193,468 +207,521 @@ __device__ inline bool find_item(const PagedArgs& a, const Seq& s0, int lane, in
   return false;
 }
 
-// states in the workspace: (m, l) of 64 rows per slot, then per slot a 64 KB block of O^T in bf16, in the
-// order of the value waves' accumulators
-__device__ inline float* state_ml(const PagedArgs& a, int slot) {
-  return (float*)(a.ws + kHeader) + (int64_t)slot * (2 * kTileQ);
-}
-__device__ inline uint8_t* state_o(const PagedArgs& a, int slot) {
-  return a.ws + kHeader + (int64_t)a.slots * (2 * kTileQ * 4) + (int64_t)slot * 65536;
+// row number of row j of a sequence's table (-1: not asked for, or a page id out of range)
+__device__ inline int row_number(const PagedArgs& a, const int32_t* trow, int j, bool asked) {
+  int id = -1;
+  if (asked) {
+    const uint32_t col = (uint32_t)j / (uint32_t)a.P;
+    const int page = trow[col];
+    if (page >= 0 && page < a.n_pages) id = page * a.P + (j - (int)col * a.P);
+  }
+  return id;
 }
 
-constexpr int kDmaWaves = 8;
+// States in the workspace, one slot per item of a split tile: (m, l) of its q rows and the scales of its values, then
+// (all slots' apart) O^T in fp16, a power of two per lane and wave taken out, in the order of the accumulators.
 template <class G>
-__device__ inline int dma_count(int w) {
-  return w < 4 ? 0 : (G::NDMA - (w - 4) + kDmaWaves - 1) / kDmaWaves;
+__device__ inline float* state_f(const PagedArgs& a, int slot) {
+  return (float*)(a.ws + kHeader) + (int64_t)slot * G::STATE_F;
+}
+template <class G>
+__device__ inline uint8_t* state_o(const PagedArgs& a, int slot) {
+  return a.ws + kHeader + (int64_t)a.slots * (G::STATE_F * 4) + (int64_t)slot * G::STATE_O;
 }
 
-template <int D, int NBUF, bool FP8>
-__global__ __launch_bounds__(768) void paged_attn_kernel(const PagedArgs a) {
-  using G = GeoP<D, NBUF>;
-  extern __shared__ __align__(16) uint8_t lds_generic[];
-  lds_u8_t* lds = (lds_u8_t*)lds_generic;
+// value wave vi (0 .. 4; wave kFirstValue + vi): first block and blocks
+__device__ inline constexpr int units_of(int vi) { return vi == 0 ? 4 : 3; }
+__device__ inline constexpr int first_unit(int vi) { return vi == 0 ? 0 : 1 + 3 * vi; }
+
+// What a workgroup works on, the same in all its waves.
+struct Work {
+  int slot;    // state slot, -1: the tile's only item
+  int nh;      // q rows here
+  int64_t row0;  // first of them in q and out
+  int m0, p0, p_lo, p_hi;  // the first one's number in its sequence; positions of the sequence's first token, the tile's first and last
+  int lo, nf;  // entry e < nf: row e; e >= nf: row lo + e - nf
+  int e_begin, e_end, ntiles;
+};
+
+// ---- row copies of one tile, dealt to the value waves (one instruction a row for columns 0..511, one per 8 rows for
+// the rope tails, XOR-swizzled by row)
+template <class G>
+__device__ inline void issue_tile(const PagedArgs& a, uint32_t lds_base, const lds_i32_t* ids_s, int vi, int lane, int tl) {
+  const lds_i32_t* id = ids_s + (tl % kIdTiles) * kTileRows;
+  const uint32_t tbase = lds_base + (uint32_t)((tl % G::NBUF) * G::TILE_BYTES);
+  auto rowp = [&](int r) { return (const uint8_t*)a.pages + (int64_t)max(id[r], 0) * G::ROWB; };
+#pragma unroll
+  for (int k = 0; k < (G::NDMA + kValueWaves - 1) / kValueWaves; k++) {
+    const int x = vi + kValueWaves * k;
+    if (x < kTileRows) {
+      dma16(rowp(x) + 16 * lane, __builtin_amdgcn_readfirstlane(tbase + x * G::MSTRIDE));
+    } else if (x < G::NDMA) {
+      const int r0 = (x - kTileRows) * 8, r = r0 + (lane >> 3);
+      dma16(rowp(r) + 1024 + 16 * ((lane & 7) ^ (r & 7)), __builtin_amdgcn_readfirstlane(tbase + G::MAIN_BYTES + r0 * 128));
+    }
+  }
+}
+
+// ---- fp8 rows (e4m3 codes, one fp32 scale per 64 columns): a tile's codes in pieces of 16, 64 pieces at a time dealt
+// to the value waves; main columns first, then the rope tails, so no wave instruction mixes the two
+template <int D>
+struct F8 {
+  static constexpr int N = kTileRows * (D / 16) / 64;               // pieces of 64
+  static constexpr int K = (N + kValueWaves - 1) / kValueWaves;
+  u32x4_t v[K];
+  float s[K];
+};
+template <int D>
+__device__ inline void f8_place(int x, int lane, int& r, int& cc) {
+  if (x < 16) {
+    r = 2 * x + (lane >> 5);
+    cc = lane & 31;
+  } else {
+    r = (x - 16) * 16 + (lane >> 2);
+    cc = 32 + (lane & 3);
+  }
+}
+template <int D>
+__device__ inline void f8_load(const PagedArgs& a, const lds_i32_t* ids_s, int vi, int lane, int tl, F8<D>& f) {
+  const lds_i32_t* id = ids_s + (tl % kIdTiles) * kTileRows;
+#pragma unroll
+  for (int k = 0; k < F8<D>::K; k++) {
+    const int x = vi + kValueWaves * k;
+    if (x < F8<D>::N) {
+      int r, cc;
+      f8_place<D>(x, lane, r, cc);
+      const int64_t row = max(id[r], 0);
+      f.v[k] = *(const u32x4_t*)((const uint8_t*)a.pages + row * D + 16 * cc);
+      f.s[k] = a.page_scales[row * (D / 64) + (cc >> 2)];
+    }
+  }
+}
+template <class G, int D>
+__device__ inline void f8_store(lds_u8_t* lds, int vi, int lane, int tl, const F8<D>& f) {
+  lds_u8_t* slot = lds + (tl % G::NBUF) * G::TILE_BYTES;
+#pragma unroll
+  for (int k = 0; k < F8<D>::K; k++) {
+    const int x = vi + kValueWaves * k;
+    if (x < F8<D>::N) {
+      int r, cc;
+      f8_place<D>(x, lane, r, cc);
+      uint32_t w[8];
+      // a normal power-of-two scale: code x scale is a bf16 value, given exactly by the scaled
+      // converter; any other scale: the fp32 product rounded to bf16
+      const uint32_t su = __float_as_uint(f.s[k]);
+      if ((su & 0x7fffffu) == 0 && su - 0x00800000u < 0x7f000000u) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          w[2 * j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f.v[k][j], f.s[k], false));
+          w[2 * j + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f.v[k][j], f.s[k], true));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const f32x2_t x0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)f.v[k][j], false);
+          const f32x2_t x1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)f.v[k][j], true);
+          w[2 * j] = pack_bf16x2(x0.x * f.s[k], x0.y * f.s[k]);
+          w[2 * j + 1] = pack_bf16x2(x1.x * f.s[k], x1.y * f.s[k]);
+        }
+      }
+      const u32x4_t w0 = {w[0], w[1], w[2], w[3]}, w1 = {w[4], w[5], w[6], w[7]};
+      if (x < 16) {
+        *(lds_u32x4_t*)(slot + r * G::MSTRIDE + 32 * cc) = w0;
+        *(lds_u32x4_t*)(slot + r * G::MSTRIDE + 32 * cc + 16) = w1;
+      } else {
+        const int l0 = 2 * (cc - 32);
+        *(lds_u32x4_t*)(slot + G::MAIN_BYTES + r * 128 + 16 * (l0 ^ (r & 7))) = w0;
+        *(lds_u32x4_t*)(slot + G::MAIN_BYTES + r * 128 + 16 * ((l0 + 1) ^ (r & 7))) = w1;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Score wave `wave` < NB: q rows 32 wave .. + 31.
+template <class G, int D>
+__device__ inline void score_role(const PagedArgs& a, const Work& w, const int32_t* trow, lds_u8_t* lds, int wave, int lane) {
   lds_i32_t* ids_s = (lds_i32_t*)(lds + G::IDS_OFF);
   lds_f32_t* al_s = (lds_f32_t*)(lds + G::AL_OFF);
-  lds_f32_t* ml_s = (lds_f32_t*)(lds + G::ML_OFF);
-  const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const bool scorer = wave < 4;
   const int g = lane >> 4, c = lane & 15;
-
-  Item it;
-  int rps;
-  {
-    const Seq s0 = load_seq(a, lane);
-    rps = plan_rps(a, s0, lane);
-    if (blockIdx.x == 0 && tid == 0) *(int*)a.ws = rps;
-    if (!find_item(a, s0, lane, rps, blockIdx.x, false, it)) return;
+  const bool idle = 32 * wave >= w.nh;  // no q rows: barriers (and row numbers) only
+  // Q^T: q row 32 wave + 16 n + c, K step j: elements 32 j + 8 g .. + 7 (rows past nh read the tile's first)
+  bf16x8_t qf[2][G::KSTEPS];
+  int eh[2], el[2];
+#pragma unroll
+  for (int n = 0; n < 2; n++) {
+    const int r = 32 * wave + 16 * n + c;
+    const int rr = r < w.nh ? r : 0;
+    const uint8_t* qr = (const uint8_t*)(a.q + (w.row0 + rr) * D) + 16 * g;
+#pragma unroll
+    for (int j = 0; j < G::KSTEPS; j++) qf[n][j] = as_bf16x8(__builtin_nontemporal_load((const u32x4_t*)(qr + 64 * j)));
+    // entries that the q row sees: e < eh, and e < first or e >= el
+    const int pc = w.p0 + (int)((uint32_t)(w.m0 + rr) / (uint32_t)a.H);
+    eh[n] = pc + 1 - w.lo + w.nf;
+    el[n] = a.window > 0 ? pc - a.window + 1 - w.lo + w.nf : 0;
   }
-  if (it.nsplit > 1 && it.slot + it.nsplit > a.slots) return;  // lengths that no batch of T tokens has
-  const int rows_b = it.s.n * a.H, m0 = it.tile * kTileQ;
-  const int nh = min(kTileQ, rows_b - m0);  // q rows here
-  const int64_t row0 = (int64_t)it.s.beg * a.H + m0;
-  const int p0 = it.s.len - it.s.n;                                   // position of the first token
-  const int p_lo = p0 + (int)((uint32_t)m0 / (uint32_t)a.H);           // of the tile's first and last
-  const int p_hi = p0 + (int)((uint32_t)(m0 + nh - 1) / (uint32_t)a.H);
-  const int w_lo = p_lo - a.window + 1;
-  const int lo = a.window > 0 && w_lo > 0 ? w_lo : 0;
-  const int nf = min(a.first, lo);
-  const int64_t cap = (int64_t)a.cols * a.P;
-  const int top = (int)min((int64_t)p_hi + 1, cap);  // rows below it
-  const int entries = max(0, top - lo + nf);
-  const int e_begin = it.split * rps, e_end = min(entries, e_begin + rps);
-  const int ntiles = e_end > e_begin ? (e_end - e_begin + kTileRows - 1) / kTileRows : 0;
-  const int32_t* trow = a.table + it.b * a.ld_table;
-  // row number of entry e (-1: none, or a page id out of range)
-  auto row_number = [&](int e) -> int {
-    const int j = e < nf ? e : lo + (e - nf);
-    int id = -1;
-    if (e < e_end) {
-      const uint32_t col = (uint32_t)j / (uint32_t)a.P;
-      const int page = trow[col];
-      if (page >= 0 && page < a.n_pages) id = page * a.P + (j - (int)col * a.P);
-    }
-    return id;
-  };
-
-  // ---- Q rows: two tiles of 32 in the last two ring slots (rows past nh read the tile's first)
-  constexpr int QS = G::NBUF - 2;
-  auto issue_rows = [&](int slot, auto&& rowp, bool nt) {
-    const uint32_t tbase = lds_base + (uint32_t)(slot * G::TILE_BYTES);
-    if (wave < 4) return;
-#pragma unroll
-    for (int k = 0; k < (G::NDMA + kDmaWaves - 1) / kDmaWaves; k++) {
-      const int x = wave - 4 + kDmaWaves * k;
-      if (x < kTileRows) {
-        const uint32_t ld = __builtin_amdgcn_readfirstlane(tbase + x * G::MSTRIDE);
-        if (nt)
-          dma16_nt(rowp(x) + 16 * lane, ld);
-        else
-          dma16(rowp(x) + 16 * lane, ld);
-      } else if (x < G::NDMA) {
-        const int r0 = (x - kTileRows) * 8;
-        const int r = r0 + (lane >> 3);
-        const int ch = (lane & 7) ^ (r & 7);  // rope tails XOR-swizzled by row
-        const uint32_t ld = __builtin_amdgcn_readfirstlane(tbase + G::MAIN_BYTES + r0 * 128);
-        if (nt)
-          dma16_nt(rowp(r) + 1024 + 16 * ch, ld);
-        else
-          dma16(rowp(r) + 1024 + 16 * ch, ld);
-      }
-    }
-  };
-  {
-    const uint8_t* qrow0 = (const uint8_t*)(a.q + row0 * D);
-    for (int qt = 0; qt < 2; qt++)
-      issue_rows(
-          QS + qt,
-          [&](int r) {
-            const int hl = 32 * qt + r;
-            return qrow0 + (hl < nh ? hl : 0) * (int64_t)G::ROWB;
-          },
-          it.nsplit == 1);
+  // entries below eh_all and outside [first, el_all) are seen by every q row of the tile
+  const int eh_all = w.p_lo + 1 - w.lo + w.nf, el_all = a.window > 0 ? w.p_hi - a.window + 1 - w.lo + w.nf : 0;
+  if (idle) {  // nothing to rescale, and no flags
+    al_s[(lane >> 5) * G::TILEQ + 32 * wave + (lane & 31)] = 1.f;
+    if (lane < 2) *(lds_i32_t*)(lds + G::P_OFF + lane * G::PBUF + 32 * wave * G::PSTRIDE + 64) = 0;
   }
-  // ---- the first eight tiles' row numbers, a score thread each
-  if (scorer) ids_s[tid] = row_number(e_begin + tid);
-  lds_barrier();
-
-  auto issue_tile = [&](int tl) {
-    if constexpr (!FP8) {
-      const lds_i32_t* tid_s = ids_s + (tl % kIdTiles) * kTileRows;
-      issue_rows(tl % G::NBUF,
-                 [&](int r) { return (const uint8_t*)a.pages + (int64_t)max(tid_s[r], 0) * G::ROWB; }, false);
-    }
-  };
-  const int my_dma = FP8 ? 0 : dma_count<G>(wave);
-
-  // ---- fp8 rows: see attn_decode_kernel (16 codes per lane and chunk; main and rope columns apart)
-  constexpr int F8_CH = D / 16;
-  constexpr int F8_K = (kTileRows * F8_CH + 511) / 512;
-  struct F8Regs {
-    u32x4_t v[F8_K];
-    float s[F8_K];
-  };
-  auto f8_chunk = [&](int vl, int k, int& r, int& cc) -> bool {
-    if (k < 2) {
-      const int ci = vl + 512 * k;
-      r = ci >> 5;
-      cc = ci & 31;
-      return true;
-    }
-    r = vl >> 2;
-    cc = 32 + (vl & 3);
-    return vl < 128;
-  };
-  auto f8_load = [&](int tl, F8Regs& fr) {
-    const lds_i32_t* tid_s = ids_s + (tl % kIdTiles) * kTileRows;
-    const int vl = (wave - 4) * 64 + lane;
-#pragma unroll
-    for (int k = 0; k < F8_K; k++) {
-      int r, cc;
-      if (f8_chunk(vl, k, r, cc)) {
-        const int64_t row = max(tid_s[r], 0);
-        fr.v[k] = *(const u32x4_t*)((const uint8_t*)a.pages + row * D + 16 * cc);
-        fr.s[k] = a.page_scales[row * (D / 64) + (cc >> 2)];
-      }
-    }
-  };
-  auto f8_store = [&](int tl, const F8Regs& fr) {
-    lds_u8_t* slot = lds + (tl % G::NBUF) * G::TILE_BYTES;
-    const int vl = (wave - 4) * 64 + lane;
-#pragma unroll
-    for (int k = 0; k < F8_K; k++) {
-      int r, cc;
-      if (f8_chunk(vl, k, r, cc)) {
-        uint32_t w[8];
-        // a normal power-of-two scale: code x scale is a bf16 value, given exactly by the scaled
-        // converter; any other scale: the fp32 product rounded to bf16
-        const uint32_t su = __float_as_uint(fr.s[k]);
-        if ((su & 0x7fffffu) == 0 && su - 0x00800000u < 0x7f000000u) {
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            w[2 * j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(fr.v[k][j], fr.s[k], false));
-            w[2 * j + 1] =
-                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(fr.v[k][j], fr.s[k], true));
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const f32x2_t lo2 = __builtin_amdgcn_cvt_pk_f32_fp8((int)fr.v[k][j], false);
-            const f32x2_t hi2 = __builtin_amdgcn_cvt_pk_f32_fp8((int)fr.v[k][j], true);
-            w[2 * j] = pack_bf16x2(lo2.x * fr.s[k], lo2.y * fr.s[k]);
-            w[2 * j + 1] = pack_bf16x2(hi2.x * fr.s[k], hi2.y * fr.s[k]);
-          }
-        }
-        const u32x4_t w0 = {w[0], w[1], w[2], w[3]}, w1 = {w[4], w[5], w[6], w[7]};
-        if (k < 2) {
-          *(lds_u32x4_t*)(slot + r * G::MSTRIDE + 32 * cc) = w0;
-          *(lds_u32x4_t*)(slot + r * G::MSTRIDE + 32 * cc + 16) = w1;
-        } else {
-          const int l0 = 2 * (cc - 32);
-          *(lds_u32x4_t*)(slot + G::MAIN_BYTES + r * 128 + 16 * (l0 ^ (r & 7))) = w0;
-          *(lds_u32x4_t*)(slot + G::MAIN_BYTES + r * 128 + 16 * ((l0 + 1) ^ (r & 7))) = w1;
+  float m_ref[2] = {-SMLA_INF, -SMLA_INF}, l_lane[2] = {0.f, 0.f};
+  int next_id = 0;  // row numbers on their way: tile i + 7, read in iteration i - 1 and written in iteration i
+  for (int i = 0; i <= w.ntiles; i++) {
+    if (i < w.ntiles) {
+      if (wave == 0 && lane < kTileRows) {
+        if (i > 0 && i + kIdTiles - 1 < w.ntiles) ids_s[((i + kIdTiles - 1) % kIdTiles) * kTileRows + lane] = next_id;
+        if (i + kIdTiles < w.ntiles) {
+          const int e = w.e_begin + (i + kIdTiles) * kTileRows + lane;
+          next_id = row_number(a, trow, e < w.nf ? e : w.lo + (e - w.nf), e < w.e_end);
         }
       }
-    }
-  };
-
-  // ---- prologue copies: tiles 0 .. NBUF-3
-  for (int tl = 0; tl < min(ntiles, QS); tl++) issue_tile(tl);
-  F8Regs f8r;
-  if constexpr (FP8) {
-    if (!scorer) {
-      for (int tl = 0; tl < min(ntiles, QS); tl++) {
-        f8_load(tl, f8r);
-        f8_store(tl, f8r);
-      }
-      if (QS < ntiles) f8_load(QS, f8r);
-    }
-  }
-  wait_vm(FP8 ? 0 : max(0, min(QS, ntiles) - 1) * my_dma);
-  lds_barrier();
-
-  auto end_iteration = [&](int i) {
-    if constexpr (!FP8) {
-      if (i + 1 < ntiles) wait_vm(max(0, min(i + G::NBUF - 2, ntiles - 1) - (i + 1)) * my_dma);
-    }
-    lds_barrier();
-    if (i + G::NBUF - 1 < ntiles) issue_tile(i + G::NBUF - 1);
-  };
-
-  if (scorer) {
-    const int hg = wave;
-    bf16x8_t qf[G::KSTEPS];
-    {
-      const lds_u8_t* qb = lds + (QS + (hg >> 1)) * G::TILE_BYTES;
-      const int qr = (hg & 1) * 16 + c;
-#pragma unroll
-      for (int j = 0; j < G::KSTEPS; j++) {
-        if (!G::TAIL || j < 16) {
-          qf[j] = as_bf16x8(*(const lds_u32x4_t*)(qb + qr * G::MSTRIDE + 16 * g + 64 * j));
-        } else {
-          const int lch = 4 * (j - 16) + g;
-          qf[j] = as_bf16x8(*(const lds_u32x4_t*)(qb + G::MAIN_BYTES + qr * 128 + 16 * (lch ^ (qr & 7))));
-        }
-      }
-    }
-    lds_barrier();  // Q slots free
-    if (ntiles > QS) issue_tile(QS);
-    // entries that q row 16 hg + c sees: e < eh, and e < first or e >= el
-    const int m = min(m0 + hg * 16 + c, rows_b - 1);
-    const int pc = p0 + (int)((uint32_t)m / (uint32_t)a.H);
-    const int eh = pc + 1 - lo + nf;
-    const int el = a.window > 0 ? pc - a.window + 1 - lo + nf : 0;
-    // entries below eh_all and outside [first, el_all) are seen by every q row of the tile
-    const int eh_all = p_lo + 1 - lo + nf, el_all = a.window > 0 ? p_hi - a.window + 1 - lo + nf : 0;
-    float m_ref = -SMLA_INF, l_lane = 0.f;
-    const int kq_off = c * G::MSTRIDE + 16 * g;
-    // row numbers on their way: tile i + 7, read in iteration i - 1 and written in iteration i
-    int next_id = 0;
-    for (int i = 0; i <= ntiles; i++) {
-      if (i < ntiles) {
+      if (!idle) {
         const lds_u8_t* buf = lds + (i % G::NBUF) * G::TILE_BYTES;
-        auto ldk = [&](int j, int blk) -> u32x4_t {
-          if (!G::TAIL || j < 16) return *(const lds_u32x4_t*)(buf + kq_off + blk * 16 * G::MSTRIDE + 64 * j);
-          const int r = 16 * blk + c, lch = 4 * (j - 16) + g;
+        auto ldk = [&](int j, int h) -> u32x4_t {
+          if (!G::TAIL || j < 16) return *(const lds_u32x4_t*)(buf + (16 * h + c) * G::MSTRIDE + 16 * g + 64 * j);
+          const int r = 16 * h + c, lch = 4 * (j - 16) + g;
           return *(const lds_u32x4_t*)(buf + G::MAIN_BYTES + r * 128 + 16 * (lch ^ (r & 7)));
         };
-        constexpr int PF = 6;
-        u32x4_t ka[PF], kb[PF];
+        constexpr int PF = 4;
+        u32x4_t kf[2][PF];
 #pragma unroll
         for (int j = 0; j < PF; j++) {
-          ka[j] = ldk(j, 0);
-          kb[j] = ldk(j, 1);
+          kf[0][j] = ldk(j, 0);
+          kf[1][j] = ldk(j, 1);
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (wave == 0 && lane < kTileRows) {
-          if (i > 0 && i + kIdTiles - 1 < ntiles) ids_s[((i + kIdTiles - 1) % kIdTiles) * kTileRows + lane] = next_id;
-          if (i + kIdTiles < ntiles) next_id = row_number(e_begin + (i + kIdTiles) * kTileRows + lane);
-        }
-        f32x4_t s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+        f32x4_t s[2][2];  // half of the rows, q rows
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int n = 0; n < 2; n++) s[h][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < G::KSTEPS; j++) {
-          const u32x4_t a0 = ka[j % PF], a1 = kb[j % PF];
+          const u32x4_t k0 = kf[0][j % PF], k1 = kf[1][j % PF];
           if (j + PF < G::KSTEPS) {
-            ka[j % PF] = ldk(j + PF, 0);
-            kb[j % PF] = ldk(j + PF, 1);
+            kf[0][j % PF] = ldk(j + PF, 0);
+            kf[1][j % PF] = ldk(j + PF, 1);
           }
-          s0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a0), qf[j], s0, 0, 0, 0);
-          s1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a1), qf[j], s1, 0, 0, 0);
-          __builtin_amdgcn_sched_barrier(0);
+          s[0][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k0), qf[0][j], s[0][0], 0, 0, 0);
+          s[0][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k0), qf[1][j], s[0][1], 0, 0, 0);
+          s[1][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k1), qf[0][j], s[1][0], 0, 0, 0);
+          s[1][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k1), qf[1][j], s[1][1], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);  // keep the reads PF steps ahead of their products
         }
-        float x[8];
-        const lds_i32_t* tid_s = ids_s + (i % kIdTiles) * kTileRows;
-        const i32x4_t v0 = *(const lds_i32x4_t*)(tid_s + 4 * g);
-        const i32x4_t v1 = *(const lds_i32x4_t*)(tid_s + 16 + 4 * g);
-        const int e0 = e_begin + i * kTileRows;
-        const bool open = e0 + kTileRows <= eh_all && (e0 >= el_all || e0 + kTileRows <= a.first);
+        const lds_i32_t* id = ids_s + (i % kIdTiles) * kTileRows;
+        const i32x4_t v0 = *(const lds_i32x4_t*)(id + 4 * g), v1 = *(const lds_i32x4_t*)(id + 16 + 4 * g);
+        const int e0 = w.e_begin + i * kTileRows;
+        const int least = min(min(min(v0[0], v0[1]), min(v0[2], v0[3])), min(min(v1[0], v1[1]), min(v1[2], v1[3])));
+        const bool open = e0 + kTileRows <= eh_all && (e0 >= el_all || e0 + kTileRows <= a.first) &&
+                          __builtin_amdgcn_ballot_w64(least < 0) == 0;
         bool odd = false;  // a masked score that is not finite
-        if (open) {
+        if (!open) {
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            x[k] = v0[k] >= 0 ? s0[k] * a.scale : -SMLA_INF;
-            x[4 + k] = v1[k] >= 0 ? s1[k] * a.scale : -SMLA_INF;
-            odd |= (v0[k] < 0 && !(fabsf(s0[k]) < SMLA_INF)) | (v1[k] < 0 && !(fabsf(s1[k]) < SMLA_INF));
+          for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+              const int e = e0 + 4 * g + (k & 3) + 16 * (k >> 2);
+              const float x = s[k >> 2][n][k & 3];
+              const bool ok = (k < 4 ? v0[k & 3] : v1[k & 3]) >= 0 && e < eh[n] && (e < a.first || e >= el[n]);
+              odd |= !ok && !(fabsf(x) < SMLA_INF);
+              s[k >> 2][n][k & 3] = ok ? x * a.scale : -SMLA_INF;
+            }
+        }
+        const float sc = open ? a.scale : 1.f;  // masked tiles are scaled above
+        const uint64_t any_odd = __builtin_amdgcn_ballot_w64(odd);
+        lds_u8_t* pb = lds + G::P_OFF + (i & 1) * G::PBUF + (32 * wave + c) * G::PSTRIDE;
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+          float x[8];
+#pragma unroll
+          for (int k = 0; k < 8; k++) x[k] = s[k >> 2][n][k & 3] * sc;
+          float mt = x[0];
+#pragma unroll
+          for (int k = 1; k < 8; k++) mt = fmaxf(mt, x[k]);
+          mt = rows4_reduce(mt, [](float x, float y) { return fmaxf(x, y); });
+          float alpha = 1.f;
+          if ((mt > m_ref[n] + kRescaleSlack) || (m_ref[n] == -SMLA_INF && mt > -SMLA_INF)) {
+            alpha = (m_ref[n] > -SMLA_INF) ? __expf(m_ref[n] - mt) : 0.f;
+            l_lane[n] *= alpha;
+            m_ref[n] = mt;
           }
-        } else {
+          float p[8];
 #pragma unroll
           for (int k = 0; k < 8; k++) {
-            const int e = e0 + 4 * g + (k & 3) + 16 * (k >> 2);
-            const int id = k < 4 ? v0[k & 3] : v1[k & 3];
-            const float s = k < 4 ? s0[k & 3] : s1[k & 3];
-            const bool ok = id >= 0 && e < eh && (e < a.first || e >= el);
-            x[k] = ok ? s * a.scale : -SMLA_INF;
-            odd |= !ok && !(fabsf(s) < SMLA_INF);
+            // a NaN score stays NaN also where no maximum is set yet
+            p[k] = (m_ref[n] > -SMLA_INF) ? __expf(x[k] - m_ref[n]) : (x[k] == -SMLA_INF ? 0.f : x[k]);
+            l_lane[n] += p[k];
           }
+          *(lds_u32x2_t*)(pb + 16 * n * G::PSTRIDE + 8 * g) = u32x2_t{pack2(p[0], p[1]), pack2(p[2], p[3])};
+          *(lds_u32x2_t*)(pb + 16 * n * G::PSTRIDE + 32 + 8 * g) = u32x2_t{pack2(p[4], p[5]), pack2(p[6], p[7])};
+          if (g == 0) al_s[(i & 1) * G::TILEQ + 32 * wave + 16 * n + c] = alpha;
         }
-        const uint64_t any_odd = __builtin_amdgcn_ballot_w64(odd);
-        float mt = x[0];
-#pragma unroll
-        for (int k = 1; k < 8; k++) mt = fmaxf(mt, x[k]);
-        mt = rows4_reduce(mt, [](float x, float y) { return fmaxf(x, y); });
-        float alpha = 1.f;
-        if ((mt > m_ref + kRescaleSlack) || (m_ref == -SMLA_INF && mt > -SMLA_INF)) {
-          alpha = (m_ref > -SMLA_INF) ? __expf(m_ref - mt) : 0.f;
-          l_lane *= alpha;
-          m_ref = mt;
-        }
-        float p[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-          // a NaN score stays NaN also where no maximum is set yet
-          const float e = (m_ref > -SMLA_INF) ? __expf(x[k] - m_ref) : (x[k] == -SMLA_INF ? 0.f : x[k]);
-          p[k] = bf16_round(e);
-          l_lane += p[k];
-        }
-        lds_u8_t* pb = lds + G::P_OFF + (i & 1) * G::PBUF + (hg * 16 + c) * G::PSTRIDE;
-        *(lds_u32x2_t*)(pb + 8 * g) = u32x2_t{pack2(p[0], p[1]), pack2(p[2], p[3])};
-        *(lds_u32x2_t*)(pb + 32 + 8 * g) = u32x2_t{pack2(p[4], p[5]), pack2(p[6], p[7])};
-        if (g == 0) al_s[(i & 1) * kTileQ + hg * 16 + c] = alpha;
         if (lane == 0) *(lds_i32_t*)(pb + 64) = any_odd != 0;
       }
-      end_iteration(i);
     }
-    const float l_tot = rows4_reduce(l_lane, [](float x, float y) { return x + y; });
-    const int hl = hg * 16 + c;
+    lds_barrier();
+  }
+  // (m, l): for the value waves' final scaling, or the state's
+#pragma unroll
+  for (int n = 0; n < 2; n++) {
+    const float l = rows4_reduce(l_lane[n], [](float x, float y) { return x + y; });
+    const int r = 32 * wave + 16 * n + c;
     if (g == 0) {
-      ml_s[hl * 2] = m_ref;
-      ml_s[hl * 2 + 1] = l_tot;
-      if (it.nsplit > 1) *(f32x2_t*)(state_ml(a, it.slot + it.split) + 2 * hl) = f32x2_t{m_ref, l_tot};
+      if (w.slot >= 0) *(f32x2_t*)(state_f<G>(a, w.slot) + 2 * r) = f32x2_t{m_ref[n], l};
+      al_s[2 * r] = m_ref[n];
+      al_s[2 * r + 1] = l;
     }
-    if (it.nsplit > 1) return;
-    lds_barrier();  // (m, l) in LDS
-    lds_barrier();  // the output block is staged
+  }
+  lds_barrier();
+}
+
+// ---------------------------------------------------------------------------------------------
+// Value wave vi with NU blocks of 32 columns from block u0 on.
+template <class G, int D, bool FP8, int NU>
+__device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* lds, int vi, int u0, int lane) {
+  constexpr int NB = G::NB;
+  const lds_i32_t* ids_s = (const lds_i32_t*)(lds + G::IDS_OFF);
+  const lds_f32_t* al_s = (const lds_f32_t*)(lds + G::AL_OFF);
+  const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
+  const int nb = (w.nh + 31) / 32;  // blocks of q rows in use (the others' products are not stored)
+  const int my_dma = (G::NDMA - vi + kValueWaves - 1) / kValueWaves;
+  f32x16_t o[NU][NB];
+#pragma unroll
+  for (int u = 0; u < NU; u++)
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) o[u][n][r] = 0.f;
+  // V^T provider address inside a 16-row step: group j = lane >> 4 covers value columns 16 (j & 1) .. of a block and
+  // rows 8 (j >> 1) ..; lane J = lane & 15 supplies row J >> 2, columns 4 (J & 3) .. + 3
+  const int vj = lane >> 4, vJ = lane & 15;
+  const int tr_off = (8 * (vj >> 1) + (vJ >> 2)) * G::MSTRIDE + 2 * (32 * u0 + 16 * (vj & 1) + 4 * (vJ & 3));
+  const int pr_off = (lane & 31) * G::PSTRIDE + 16 * (lane >> 5);
+  F8<D> f8;
+  // ---- the first copies: every slot (row copies), or tiles 0 .. NBUF-3 (fp8, and the next one's codes)
+  if constexpr (FP8) {
+    for (int tl = 0; tl < min(w.ntiles, G::NBUF - 2); tl++) {
+      f8_load<D>(a, ids_s, vi, lane, tl, f8);
+      f8_store<G, D>(lds, vi, lane, tl, f8);
+    }
+    if (G::NBUF - 2 < w.ntiles) f8_load<D>(a, ids_s, vi, lane, G::NBUF - 2, f8);
   } else {
-    const int vw = wave - 4;
-    const int hp = vw & 1, dq = vw >> 1;
-    lds_barrier();  // pairs with the score waves' barrier after their Q^T reads
-    if (ntiles > QS) issue_tile(QS);
-    f32x16_t o[4];
-#pragma unroll
-    for (int mb = 0; mb < 4; mb++)
-#pragma unroll
-      for (int r = 0; r < 16; r++) o[mb][r] = 0.f;
-    const int vj = lane >> 4, vJ = lane & 15;
-    const int tr_off = (8 * (vj >> 1) + (vJ >> 2)) * G::MSTRIDE + 2 * (128 * dq + 16 * (vj & 1) + 4 * (vJ & 3));
-    const int pr_off = (32 * hp + (lane & 31)) * G::PSTRIDE + 16 * (lane >> 5);
-    for (int i = 0; i <= ntiles; i++) {
-      if constexpr (FP8) {
-        if (i + G::NBUF - 2 < ntiles) {
-          f8_store(i + G::NBUF - 2, f8r);
-          if (i + G::NBUF - 1 < ntiles) f8_load(i + G::NBUF - 1, f8r);
-        }
+    for (int tl = 0; tl < min(w.ntiles, G::NBUF); tl++) issue_tile<G>(a, lds_base, ids_s, vi, lane, tl);
+    wait_vm(max(0, min(G::NBUF, w.ntiles) - 1) * my_dma);  // tile 0 has landed
+  }
+  lds_barrier();
+  for (int i = 0; i <= w.ntiles; i++) {
+    if constexpr (FP8) {
+      // tile i + NBUF - 2 goes to the slot of tile i - 2, consumed before the last barrier
+      if (i + G::NBUF - 2 < w.ntiles) {
+        f8_store<G, D>(lds, vi, lane, i + G::NBUF - 2, f8);
+        if (i + G::NBUF - 1 < w.ntiles) f8_load<D>(a, ids_s, vi, lane, i + G::NBUF - 1, f8);
       }
-      if (i >= 1) {
-        const int tp = i - 1;
-        const lds_u8_t* buf = lds + (tp % G::NBUF) * G::TILE_BYTES;
-        const lds_u8_t* pbuf = lds + G::P_OFF + (tp & 1) * G::PBUF;
-        const float al = al_s[(tp & 1) * kTileQ + 32 * hp + (lane & 31)];
-        const int odd = *(const lds_i32_t*)(pbuf + 32 * hp * G::PSTRIDE + 64) |
-                        *(const lds_i32_t*)(pbuf + (32 * hp + 16) * G::PSTRIDE + 64);
+    }
+    if (i >= 1) {
+      const int tp = i - 1;  // tile scored in the last iteration
+      const lds_u8_t* buf = lds + (tp % G::NBUF) * G::TILE_BYTES;
+      const lds_u8_t* pbuf = lds + G::P_OFF + (tp & 1) * G::PBUF;
+      int odd = 0;
+#pragma unroll
+      for (int n = 0; n < NB; n++) {
+        odd |= *(const lds_i32_t*)(pbuf + 32 * n * G::PSTRIDE + 64);
+        const float al = al_s[(tp & 1) * G::TILEQ + 32 * n + (lane & 31)];
         if (__builtin_amdgcn_ballot_w64(al != 1.f)) {
 #pragma unroll
-          for (int mb = 0; mb < 4; mb++) o[mb] *= al;
+          for (int u = 0; u < NU; u++) o[u][n] *= al;
         }
-        auto step = [&](bool clean) {
-#pragma unroll
-          for (int ks = 0; ks < 2; ks++) {
-            const bf16x8_t pf = as_bf16x8(*(const lds_u32x4_t*)(pbuf + pr_off + 32 * ks));
-            const lds_u8_t* vb = buf + tr_off + 16 * ks * G::MSTRIDE;
-#pragma unroll
-            for (int mb = 0; mb < 4; mb++) {
-              const v4i16_t vlo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vb + 64 * mb));
-              const v4i16_t vhi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vb + 64 * mb + 4 * G::MSTRIDE));
-              bf16x8_t va = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(vlo, vhi, 0, 1, 2, 3, 4, 5, 6, 7));
-              if (clean) {
-                u32x4_t w = __builtin_bit_cast(u32x4_t, va);
-#pragma unroll
-                for (int k = 0; k < 4; k++) w[k] = finite2(w[k]);
-                va = as_bf16x8(w);
-              }
-              o[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pf, o[mb], 0, 0, 0);
-            }
-          }
-        };
-        if (__builtin_amdgcn_readfirstlane(odd)) step(true);
-        else step(false);
       }
-      end_iteration(i);
-    }
-    if (it.nsplit > 1) {
-      // O^T straight from the accumulators (attn_decode_kernel's order): 1 KB pieces ((vw * 4 + mb) * 2 + h),
-      // in which lane l's 16 bytes are values 128 dq + 32 mb + 16 h + 8 (l >> 5) .. + 7 of q row 32 hp + (l & 31)
-      uint8_t* blk = state_o(a, it.slot + it.split) + vw * 8192 + 16 * lane;
+      if (__builtin_amdgcn_readfirstlane(odd)) {
+        // this wave's columns (nobody else reads them by now): 64 NU bytes of each of 32 rows, 16 bytes a lane
+        lds_u8_t* mine = lds + (tp % G::NBUF) * G::TILE_BYTES + 64 * u0;
+        for (int x = lane; x < kTileRows * 4 * NU; x += 64) {
+          const int row = x / (4 * NU);
+          lds_u32x4_t* at = (lds_u32x4_t*)(mine + row * G::MSTRIDE + 16 * (x - row * (4 * NU)));
+          u32x4_t y = *at;
 #pragma unroll
-      for (int mb = 0; mb < 4; mb++) {
+          for (int k = 0; k < 4; k++) y[k] = finite2(y[k]);
+          *at = y;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ks++) {
+        bf16x8_t pf[NB];
+#pragma unroll
+        for (int n = 0; n < NB; n++) pf[n] = as_bf16x8(*(const lds_u32x4_t*)(pbuf + pr_off + 32 * n * G::PSTRIDE + 32 * ks));
+        const lds_u8_t* vb = buf + tr_off + 16 * ks * G::MSTRIDE;
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+          const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vb + 64 * u));
+          const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vb + 64 * u + 4 * G::MSTRIDE));
+          const bf16x8_t va = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (int n = 0; n < NB; n++) o[u][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pf[n], o[u][n], 0, 0, 0);
+        }
+      }
+    }
+    // tile i + 1 has landed; the slot of the consumed tile i - 1 takes tile i + NBUF - 1
+    if constexpr (!FP8) {
+      // (the newest requested: NBUF - 1 at first, then i + NBUF - 2)
+      if (i + 1 < w.ntiles) wait_vm(max(0, min(max(i + G::NBUF - 2, G::NBUF - 1), w.ntiles - 1) - (i + 1)) * my_dma);
+    }
+    lds_barrier();
+    if constexpr (!FP8) {
+      if (i >= 1 && i + G::NBUF - 1 < w.ntiles) issue_tile<G>(a, lds_base, ids_s, vi, lane, i + G::NBUF - 1);
+    }
+  }
+  lds_barrier();  // (m, l) in LDS
+#pragma unroll
+  for (int n = 0; n < NB; n++) {
+    if (n >= nb) continue;
+    const int r = 32 * n + (lane & 31);
+    // O^T of block u: register k holds column 8 (k >> 2) + 4 (lane >> 5) + (k & 3) of q row r; one lane swap per
+    // pair of packed registers gives each lane 8 columns in a row, 16 h + 8 (lane >> 5) .. + 7
+    if (w.slot >= 0) {
+      // the lane's largest magnitude sets its scale: fp16 keeps 11 bits of every value that matters beside it
+      float top = 0.f;
+#pragma unroll
+      for (int u = 0; u < NU; u++)
+#pragma unroll
+        for (int k = 0; k < 16; k++) top = fmaxf(top, fabsf(o[u][n][k]));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);  // 2^(e-127) <= top < 2^(e-126)
+      const float inv = __uint_as_float((254u - e) << 23);
+      state_f<G>(a, w.slot)[2 * G::TILEQ + (vi * NB + n) * 64 + lane] = __uint_as_float(e << 23);
+      uint8_t* blk = state_o<G>(a, w.slot) + (u0 * NB + n) * 2048 + 16 * lane;
+#pragma unroll
+      for (int u = 0; u < NU; u++) {
         uint32_t d[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) d[k] = pack2(o[mb][2 * k], o[mb][2 * k + 1]);
+        for (int k = 0; k < 8; k++)
+          d[k] = __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)(o[u][n][2 * k] * inv), (_Float16)(o[u][n][2 * k + 1] * inv)});
 #pragma unroll
         for (int k = 0; k < 8; k += 4) {
           const auto x0 = __builtin_amdgcn_permlane32_swap(d[k], d[k + 2], false, false);
           const auto x1 = __builtin_amdgcn_permlane32_swap(d[k + 1], d[k + 3], false, false);
-          const u32x4_t v4 = {x0[0], x1[0], x0[1], x1[1]};
-          __builtin_nontemporal_store(v4, (u32x4_t*)(blk + (mb * 2 + (k >> 2)) * 1024));
+          __builtin_nontemporal_store(u32x4_t{x0[0], x1[0], x0[1], x1[1]}, (u32x4_t*)(blk + u * NB * 2048 + (k >> 2) * 1024));
         }
       }
-      return;
-    }
-    lds_barrier();  // (m, l) in LDS
-    const int hl = 32 * hp + (lane & 31);
-    const float M = ml_s[hl * 2], L = ml_s[hl * 2 + 1];
-    float inv = 0.f;  // no row seen: 0
-    if (!(L == 0.f)) {
-      const float snk = a.sink && hl < nh ? a.sink[(uint32_t)(m0 + hl) % (uint32_t)a.H] : -SMLA_INF;
-      inv = 1.0f / (L + (snk == -SMLA_INF ? 0.f : __expf(snk - M)));
-    }
-    const int dvb = 128 * dq + 4 * (lane >> 5);
-    lds_u8_t* srow = lds + hl * (1024 + 16);
-#pragma unroll
-    for (int mb = 0; mb < 4; mb++)
-#pragma unroll
-      for (int qd = 0; qd < 4; qd++) {
-        const f32x4_t v = f32x4_t{o[mb][4 * qd], o[mb][4 * qd + 1], o[mb][4 * qd + 2], o[mb][4 * qd + 3]} * inv;
-        *(lds_u32x2_t*)(srow + 2 * (dvb + 32 * mb + 8 * qd)) = u32x2_t{pack2(v[0], v[1]), pack2(v[2], v[3])};
+    } else {
+      const float M = al_s[2 * r], L = al_s[2 * r + 1];
+      float inv = 0.f;  // no row seen: 0
+      if (!(L == 0.f)) {
+        const float snk = a.sink && r < w.nh ? a.sink[(uint32_t)(w.m0 + r) % (uint32_t)a.H] : -SMLA_INF;
+        inv = 1.0f / (L + (snk == -SMLA_INF ? 0.f : __expf(snk - M)));
       }
-    lds_barrier();
+      uint8_t* dst = (uint8_t*)(a.out + (w.row0 + r) * 512 + 32 * u0 + 8 * (lane >> 5));
+#pragma unroll
+      for (int u = 0; u < NU; u++) {
+        uint32_t d[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) d[k] = pack2(o[u][n][2 * k] * inv, o[u][n][2 * k + 1] * inv);
+#pragma unroll
+        for (int k = 0; k < 8; k += 4) {
+          const auto x0 = __builtin_amdgcn_permlane32_swap(d[k], d[k + 2], false, false);
+          const auto x1 = __builtin_amdgcn_permlane32_swap(d[k + 1], d[k + 3], false, false);
+          if (r < w.nh) *(u32x4_t*)(dst + 64 * u + 8 * k) = u32x4_t{x0[0], x1[0], x0[1], x1[1]};
+        }
+      }
+    }
   }
-  // the tile's q rows are consecutive rows of out
-  uint8_t* dst = (uint8_t*)(a.out + row0 * 512);
-  for (int i = tid; i < nh * 64; i += G::NW * 64)
-    __builtin_nontemporal_store(*(const lds_u32x4_t*)(lds + (i >> 6) * (1024 + 16) + (i & 63) * 16),
-                                (u32x4_t*)(dst + (int64_t)i * 16));
+}
+
+template <int D, int NB, int NBUF, bool FP8>
+__global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedArgs a) {
+  using G = GeoP<D, NB, NBUF>;
+  extern __shared__ __align__(16) uint8_t lds_generic[];
+  lds_u8_t* lds = (lds_u8_t*)lds_generic;
+  lds_i32_t* ids_s = (lds_i32_t*)(lds + G::IDS_OFF);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Item it;
+  int rps;
+  {
+    const Seq s0 = load_seq<G::TILEQ>(a, lane);
+    rps = plan_rps<G::TILEQ>(a, s0, lane);
+    if (blockIdx.x == 0 && tid == 0) *(int*)a.ws = rps;
+    if (!find_item<G::TILEQ>(a, s0, lane, rps, blockIdx.x, false, it)) return;
+  }
+  if (it.nsplit > 1 && it.slot + it.nsplit > a.slots) return;  // lengths that no batch of T tokens has
+  Work w;
+  const int rows_b = it.s.n * a.H;
+  w.m0 = it.tile * G::TILEQ;
+  w.slot = it.nsplit > 1 ? it.slot + it.split : -1;
+  w.nh = min(G::TILEQ, rows_b - w.m0);
+  w.row0 = (int64_t)it.s.beg * a.H + w.m0;
+  w.p0 = it.s.len - it.s.n;
+  w.p_lo = w.p0 + (int)((uint32_t)w.m0 / (uint32_t)a.H);
+  w.p_hi = w.p0 + (int)((uint32_t)(w.m0 + w.nh - 1) / (uint32_t)a.H);
+  const int w_lo = w.p_lo - a.window + 1;
+  w.lo = a.window > 0 && w_lo > 0 ? w_lo : 0;
+  w.nf = min(a.first, w.lo);
+  const int64_t cap = (int64_t)a.cols * a.P;
+  const int top = (int)min((int64_t)w.p_hi + 1, cap);  // rows below it
+  const int entries = max(0, top - w.lo + w.nf);
+  w.e_begin = it.split * rps;
+  w.e_end = min(entries, w.e_begin + rps);
+  w.ntiles = w.e_end > w.e_begin ? (w.e_end - w.e_begin + kTileRows - 1) / kTileRows : 0;
+  const int32_t* trow = a.table + it.b * a.ld_table;
+  if (tid < kIdTiles * kTileRows) {  // the first eight tiles' row numbers
+    const int e = w.e_begin + tid;
+    ids_s[tid] = row_number(a, trow, e < w.nf ? e : w.lo + (e - w.nf), e < w.e_end);
+  }
+  lds_barrier();
+  if (wave < kFirstValue) {
+    if (wave < NB) {
+      lds_barrier();  // tile 0 has landed
+      score_role<G, D>(a, w, trow, lds, wave, lane);
+    } else {
+      for (int i = 0; i < w.ntiles + 3; i++) lds_barrier();
+    }
+  } else if (wave == kFirstValue) {
+    value_role<G, D, FP8, units_of(0)>(a, w, lds, 0, first_unit(0), lane);
+  } else {
+    value_role<G, D, FP8, units_of(1)>(a, w, lds, wave - kFirstValue, first_unit(wave - kFirstValue), lane);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
-// Joins the states of split tiles: a workgroup of 4 waves takes a 1 KB piece (8 values of 64 q rows' half)
-// of one tile, wave w the splits w, w + 4, .. eight at a time with a running maximum, the waves' sums then
-// through LDS in a fixed order.  Workgroups walk the pieces of all split tiles; with `fill` they also clear
-// the rows behind the last sequence.
+// Joins the states of split tiles: a workgroup of 4 waves takes a 1 KB piece (8 values of 32 q rows, twice) of one tile,
+// wave w the splits w, w + 4, .. eight at a time with a running maximum, the waves' sums then through LDS in a
+// fixed order.  Workgroups walk the pieces of all split tiles; with `fill` they also clear the rows behind the
+// last sequence.
 constexpr int kMergeWaves = 4, kMergeBatch = 8;
 
+template <int D, int NB>
 __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const PagedArgs a) {
+  using G = GeoP<D, NB, 3>;
+  constexpr int kPieces = kUnits * NB * 2;
   __shared__ float red[kMergeWaves][64][10];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Seq s0 = load_seq(a, lane);
+  const Seq s0 = load_seq<G::TILEQ>(a, lane);
   const int rps = __builtin_amdgcn_readfirstlane(*(const int*)a.ws);
-  for (int64_t w = blockIdx.x;; w += gridDim.x) {
+  for (int64_t x = blockIdx.x;; x += gridDim.x) {
     Item it;
-    if (!find_item(a, s0, lane, rps, (int)(w >> 6), true, it)) break;
-    if (it.slot + it.nsplit > a.slots) continue;
-    const int piece = (int)(w & 63);
-    const int row = 32 * ((piece >> 3) & 1) + (lane & 31);  // vw = piece / 8: hp = vw & 1, dq = vw >> 1
+    const int tile = (int)(x / kPieces), piece = (int)(x - (int64_t)tile * kPieces);
+    if (!find_item<G::TILEQ>(a, s0, lane, rps, tile, true, it)) break;
+    const int m0 = it.tile * G::TILEQ, rows_b = it.s.n * a.H;
+    const int u = piece / (2 * NB), n = (piece >> 1) % NB, half = piece & 1;
+    if (it.slot + it.nsplit > a.slots || m0 + 32 * n >= rows_b) continue;
+    const int vi = u < 4 ? 0 : (u - 1) / 3;
+    const int row = 32 * n + (lane & 31);
     float m = -SMLA_INF, l = 0.f, acc[8];
 #pragma unroll
     for (int k = 0; k < 8; k++) acc[k] = 0.f;
     for (int sp0 = wave; sp0 < it.nsplit; sp0 += kMergeWaves * kMergeBatch) {
       f32x2_t ml[kMergeBatch];
+      float sc[kMergeBatch];
       u32x4_t v[kMergeBatch];
 #pragma unroll
       for (int k = 0; k < kMergeBatch; k++) {
         const int sp = sp0 + kMergeWaves * k;
         if (sp < it.nsplit) {
-          ml[k] = *(const f32x2_t*)(state_ml(a, it.slot + sp) + 2 * row);
-          v[k] = *(const u32x4_t*)(state_o(a, it.slot + sp) + piece * 1024 + 16 * lane);
+          const float* f = state_f<G>(a, it.slot + sp);
+          ml[k] = *(const f32x2_t*)(f + 2 * row);
+          sc[k] = f[2 * G::TILEQ + (vi * NB + n) * 64 + lane];
+          v[k] = *(const u32x4_t*)(state_o<G>(a, it.slot + sp) + piece * 1024 + 16 * lane);
         }
       }
       float top = m;
@@ -672,10 +739,13 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
           // a state without a maximum has l = 0 (nothing seen) or NaN
           const float e = ml[k][0] > -SMLA_INF ? __expf(ml[k][0] - m) : 1.f;
           l += ml[k][1] * e;
+          const float es = e * sc[k];
 #pragma unroll
           for (int j = 0; j < 4; j++) {
-            acc[2 * j] += __uint_as_float(v[k][j] << 16) * e;
-            acc[2 * j + 1] += __uint_as_float(v[k][j] & 0xffff0000u) * e;
+            const uint32_t word = v[k][j];  // (a bit cast of a vector's element itself takes element 0)
+            const f16x2_t h2 = __builtin_bit_cast(f16x2_t, word);
+            acc[2 * j] += (float)h2[0] * es;
+            acc[2 * j + 1] += (float)h2[1] * es;
           }
         }
     }
@@ -699,18 +769,16 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
 #pragma unroll
         for (int j = 0; j < 8; j++) y[j] += red[k][lane][2 + j] * e;
       }
-      const int m0 = it.tile * kTileQ, rows_b = it.s.n * a.H;
       if (m0 + row < rows_b) {
         float inv = 0.f;
         if (!(sum == 0.f)) {
           const float snk = a.sink ? a.sink[(uint32_t)(m0 + row) % (uint32_t)a.H] : -SMLA_INF;
           inv = 1.0f / (sum + (snk == -SMLA_INF ? 0.f : __expf(snk - top)));
         }
-        const int vw = piece >> 3, dv = 128 * (vw >> 1) + 32 * ((piece >> 1) & 3) + 16 * (piece & 1) + 8 * (lane >> 5);
         u32x4_t o;
 #pragma unroll
         for (int j = 0; j < 4; j++) o[j] = pack2(y[2 * j] * inv, y[2 * j + 1] * inv);
-        *(u32x4_t*)(a.out + ((int64_t)it.s.beg * a.H + m0 + row) * 512 + dv) = o;
+        *(u32x4_t*)(a.out + ((int64_t)it.s.beg * a.H + m0 + row) * 512 + 32 * u + 16 * half + 8 * (lane >> 5)) = o;
       }
     }
   }
@@ -721,25 +789,31 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
   }
 }
 
-template <int D, int NBUF, bool FP8>
-int launch_paged(const PagedArgs& a, int64_t grid, hipStream_t st) {
-  using G = GeoP<D, NBUF>;
-  auto kern = paged_attn_kernel<D, NBUF, FP8>;
-  static std::atomic<uint64_t> lds_attr{0};
-  if (hipError_t e = smla_set_dynamic_lds((const void*)kern, G::LDS_BYTES, lds_attr); e != hipSuccess) return (int)e;
-  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(G::NW * 64), G::LDS_BYTES, st, a);
-  SMLA_HIP_CHECK_LAUNCH();
-  return SMLA_OK;
-}
-
 // Tiles that T tokens of B sequences can make, and the state slots that their plan can use: with at most one
 // item per compute unit one slot each, else two per half share of work.
-int64_t most_tiles(int64_t T, int64_t H, int64_t B) { return T * H / kTileQ + (B < T ? B : T); }
-int64_t plan_slots(int64_t T, int64_t H, int64_t B, int cus) {
-  return most_tiles(T, H, B) <= cus ? cus : 4 * (int64_t)cus + 64;
-}
+int64_t most_tiles(int64_t T, int64_t H, int64_t B, int nb) { return T * H / (32 * nb) + (B < T ? B : T); }
+int64_t plan_slots(int64_t tiles, int cus) { return tiles <= cus ? cus : 4 * (int64_t)cus + 64; }
+// q rows per tile / 32: where the sequences have no more than 64 on average, tiles of 64 leave LDS for a fourth ring slot
+// (steps of one or few tokens are bound by the rows' arrival); longer runs of q rows share a row among 96
+int tile_blocks(int64_t T, int64_t H, int64_t B) { return T * H <= 64 * B ? 2 : 3; }
 bool plan_sizes(int64_t T, int64_t H, int64_t B) {
-  return T >= 0 && H > 0 && B > 0 && T <= 0x7fffffff && H <= 0x7fffffff && B <= 0xfffff && T * H <= 0x7fffffc0;
+  return T >= 0 && H > 0 && B > 0 && T <= 0x7fffffff && H <= 0x7fffffff && B <= 0xfffff && T * H <= 0x7fffff80;
+}
+
+template <int D, int NB, int NBUF, bool FP8>
+int launch_paged(const PagedArgs& a, int64_t tiles, hipStream_t st) {
+  using G = GeoP<D, NB, NBUF>;
+  auto kern = paged_attn_kernel<D, NB, NBUF, FP8>;
+  static std::atomic<uint64_t> lds_attr{0};
+  if (hipError_t e = smla_set_dynamic_lds((const void*)kern, G::LDS_BYTES, lds_attr); e != hipSuccess) return (int)e;
+  const int64_t grid = tiles <= a.cus ? a.cus : tiles + 2 * (int64_t)a.cus + 64;
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * kWaves), G::LDS_BYTES, st, a);
+  SMLA_HIP_CHECK_LAUNCH();
+  const int64_t pieces = tiles * kUnits * NB * 2, most = 8 * (int64_t)a.cus;
+  hipLaunchKernelGGL((paged_merge_kernel<D, NB>), dim3((unsigned)(pieces < most ? pieces : most)), dim3(64 * kMergeWaves), 0,
+                     st, a);
+  SMLA_HIP_CHECK_LAUNCH();
+  return SMLA_OK;
 }
 
 }  // namespace
@@ -748,7 +822,10 @@ bool plan_sizes(int64_t T, int64_t H, int64_t B) {
 extern "C" size_t smla_paged_attn_workspace(int64_t T, int64_t H, int64_t B) {
   using namespace smla_attn;
   if (!plan_sizes(T, H, B)) return 0;
-  return (size_t)(kHeader + plan_slots(T, H, B, smla_num_cus()) * (2 * kTileQ * 4 + 65536));
+  const int nb = tile_blocks(T, H, B);
+  const int64_t state = nb == 2 ? GeoP<512, 2, 3>::STATE_O + 4 * GeoP<512, 2, 3>::STATE_F
+                                : GeoP<512, 3, 3>::STATE_O + 4 * GeoP<512, 3, 3>::STATE_F;
+  return (size_t)(kHeader + plan_slots(most_tiles(T, H, B, nb), smla_num_cus()) * state);
 }
 
 extern "C" int smla_paged_attn(const void* q, int q_dtype, const void* pages, int page_dtype, const float* page_scales,
@@ -790,20 +867,19 @@ extern "C" int smla_paged_attn(const void* q, int q_dtype, const void* pages, in
   a.window = (int)window;
   a.first = window > 0 ? (int)first : 0;
   a.cus = smla_num_cus();
-  a.slots = (int)plan_slots(T, H, B, a.cus);
   a.fill = (flags & SMLA_PAGED_FILL) != 0;
   a.scale = scale;
-  const int64_t tiles = most_tiles(T, H, B);
-  const int64_t grid = tiles <= a.cus ? a.cus : tiles + 2 * (int64_t)a.cus + 64;
+  const int nb = tile_blocks(T, H, B);
+  const int64_t tiles = most_tiles(T, H, B, nb);
+  a.slots = (int)plan_slots(tiles, a.cus);
   const hipStream_t st = (hipStream_t)stream;
-  int rc;
-  if (page_dtype == SMLA_FP8_E4M3)
-    rc = D == 576 ? launch_paged<576, 3, true>(a, grid, st) : launch_paged<512, 3, true>(a, grid, st);
-  else
-    rc = D == 576 ? launch_paged<576, 3, false>(a, grid, st) : launch_paged<512, 3, false>(a, grid, st);
-  if (rc != 0) return rc;
-  const int64_t pieces = tiles * 64, most = 8 * (int64_t)a.cus;
-  hipLaunchKernelGGL(paged_merge_kernel, dim3((unsigned)(pieces < most ? pieces : most)), dim3(64 * kMergeWaves), 0, st, a);
-  SMLA_HIP_CHECK_LAUNCH();
-  return SMLA_OK;
+  const bool fp8 = page_dtype == SMLA_FP8_E4M3;
+#define SMLA_PAGED(DD, NB, NBUF) return fp8 ? launch_paged<DD, NB, NBUF, true>(a, tiles, st) : launch_paged<DD, NB, NBUF, false>(a, tiles, st)
+  if (nb == 2) {
+    if (D == 576) SMLA_PAGED(576, 2, 4);
+    SMLA_PAGED(512, 2, 4);
+  }
+  if (D == 576) SMLA_PAGED(576, 3, 3);
+  SMLA_PAGED(512, 3, 4);
+#undef SMLA_PAGED
 }
