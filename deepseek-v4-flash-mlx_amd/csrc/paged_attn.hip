@@ -338,14 +338,21 @@ __device__ inline void f8_store(lds_u8_t* lds, int vi, int lane, int tl, const F
 }
 
 // ---------------------------------------------------------------------------------------------
-// Score wave `wave` < NB: q rows 32 wave .. + 31.
+// Score wave `wave` < NB: q rows 32 wave .. + 31.  A tile goes in two halves of 16 rows: the second half's products
+// run while the first half's exponentials are taken between them (an element a K step, placed by hand:
+// the products leave the vector pipe idle three cycles of four), so only the second half's are left at the end.
+// Scores are kept in base 2; a maximum further than 2^11.5 above the reference moves the reference, everything else
+// stays below e^8 of it.
 template <class G, int D>
 __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32_t* trow, lds_u8_t* lds, int wave, int lane) {
   lds_i32_t* ids_s = (lds_i32_t*)(lds + G::IDS_OFF);
   lds_f32_t* al_s = (lds_f32_t*)(lds + G::AL_OFF);
   const int g = lane >> 4, c = lane & 15;
   const bool idle = 32 * wave >= w.nh;  // no q rows: barriers (and row numbers) only
-  // Q^T: q row 32 wave + 16 n + c, K step j: elements 32 j + 8 g .. + 7 (rows past nh read the tile's first)
+  constexpr float kLog2e = 1.44269504088896340736f;
+  const float c2 = fabsf(a.scale) * kLog2e;
+  // Q^T: q row 32 wave + 16 n + c, K step j: elements 32 j + 8 g .. + 7 (rows past nh read the tile's first);
+  // a negative scale's sign goes into q
   bf16x8_t qf[2][G::KSTEPS];
   int eh[2], el[2];
 #pragma unroll
@@ -360,13 +367,20 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
     eh[n] = pc + 1 - w.lo + w.nf;
     el[n] = a.window > 0 ? pc - a.window + 1 - w.lo + w.nf : 0;
   }
+  if (a.scale < 0.f) {
+#pragma unroll
+    for (int n = 0; n < 2; n++)
+#pragma unroll
+      for (int j = 0; j < G::KSTEPS; j++) qf[n][j] = as_bf16x8(__builtin_bit_cast(u32x4_t, qf[n][j]) ^ 0x80008000u);
+  }
   // entries below eh_all and outside [first, el_all) are seen by every q row of the tile
   const int eh_all = w.p_lo + 1 - w.lo + w.nf, el_all = a.window > 0 ? w.p_hi - a.window + 1 - w.lo + w.nf : 0;
   if (idle) {  // nothing to rescale, and no flags
     al_s[(lane >> 5) * G::TILEQ + 32 * wave + (lane & 31)] = 1.f;
     if (lane < 2) *(lds_i32_t*)(lds + G::P_OFF + lane * G::PBUF + 32 * wave * G::PSTRIDE + 64) = 0;
   }
-  float m_ref[2] = {-SMLA_INF, -SMLA_INF}, l_lane[2] = {0.f, 0.f};
+  // m_ref: the reference (-inf: none yet); m_sub: what is taken off a score (0 without a reference)
+  float m_ref[2] = {-SMLA_INF, -SMLA_INF}, m_sub[2] = {0.f, 0.f}, l_lane[2] = {0.f, 0.f};
   int next_id = 0;  // row numbers on their way: tile i + 7, read in iteration i - 1 and written in iteration i
   for (int i = 0; i <= w.ntiles; i++) {
     if (i < w.ntiles) {
@@ -379,85 +393,126 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
       }
       if (!idle) {
         const lds_u8_t* buf = lds + (i % G::NBUF) * G::TILE_BYTES;
-        auto ldk = [&](int j, int h) -> u32x4_t {
+        // fragment f of the tile: half f / KSTEPS, K step f % KSTEPS
+        auto ldk = [&](int f) -> u32x4_t {
+          const int h = f / G::KSTEPS, j = f - h * G::KSTEPS;
           if (!G::TAIL || j < 16) return *(const lds_u32x4_t*)(buf + (16 * h + c) * G::MSTRIDE + 16 * g + 64 * j);
           const int r = 16 * h + c, lch = 4 * (j - 16) + g;
           return *(const lds_u32x4_t*)(buf + G::MAIN_BYTES + r * 128 + 16 * (lch ^ (r & 7)));
         };
-        constexpr int PF = 4;
-        u32x4_t kf[2][PF];
+        constexpr int PF = 6;
+        u32x4_t kf[PF];
 #pragma unroll
-        for (int j = 0; j < PF; j++) {
-          kf[0][j] = ldk(j, 0);
-          kf[1][j] = ldk(j, 1);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        f32x4_t s[2][2];  // half of the rows, q rows
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-          for (int n = 0; n < 2; n++) s[h][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < G::KSTEPS; j++) {
-          const u32x4_t k0 = kf[0][j % PF], k1 = kf[1][j % PF];
-          if (j + PF < G::KSTEPS) {
-            kf[0][j % PF] = ldk(j + PF, 0);
-            kf[1][j % PF] = ldk(j + PF, 1);
-          }
-          s[0][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k0), qf[0][j], s[0][0], 0, 0, 0);
-          s[0][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k0), qf[1][j], s[0][1], 0, 0, 0);
-          s[1][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k1), qf[0][j], s[1][0], 0, 0, 0);
-          s[1][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k1), qf[1][j], s[1][1], 0, 0, 0);
-          __builtin_amdgcn_sched_barrier(0);  // keep the reads PF steps ahead of their products
-        }
+        for (int f = 0; f < PF; f++) kf[f] = ldk(f);
         const lds_i32_t* id = ids_s + (i % kIdTiles) * kTileRows;
         const i32x4_t v0 = *(const lds_i32x4_t*)(id + 4 * g), v1 = *(const lds_i32x4_t*)(id + 16 + 4 * g);
         const int e0 = w.e_begin + i * kTileRows;
-        const int least = min(min(min(v0[0], v0[1]), min(v0[2], v0[3])), min(min(v1[0], v1[1]), min(v1[2], v1[3])));
-        const bool open = e0 + kTileRows <= eh_all && (e0 >= el_all || e0 + kTileRows <= a.first) &&
-                          __builtin_amdgcn_ballot_w64(least < 0) == 0;
         bool odd = false;  // a masked score that is not finite
-        if (!open) {
+        float alpha[2] = {1.f, 1.f};
+        bool open = false;
+        float cm = 1.f;
+        // scores of a half that are masked or tiles not open: scaled, -inf where the q row does not see the row
+        auto mask = [&](f32x4_t (&s)[2], const i32x4_t& v, int e1) {
 #pragma unroll
           for (int n = 0; n < 2; n++)
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-              const int e = e0 + 4 * g + (k & 3) + 16 * (k >> 2);
-              const float x = s[k >> 2][n][k & 3];
-              const bool ok = (k < 4 ? v0[k & 3] : v1[k & 3]) >= 0 && e < eh[n] && (e < a.first || e >= el[n]);
-              odd |= !ok && !(fabsf(x) < SMLA_INF);
-              s[k >> 2][n][k & 3] = ok ? x * a.scale : -SMLA_INF;
+            for (int k = 0; k < 4; k++) {
+              const int e = e1 + 4 * g + k;
+              const bool ok = v[k] >= 0 && e < eh[n] && (e < a.first || e >= el[n]);
+              odd |= !ok && !(fabsf(s[n][k]) < SMLA_INF);
+              s[n][k] = ok ? s[n][k] * c2 : -SMLA_INF;
             }
+        };
+        // moves the references where a score is past them: factor[n] = e^(old - new)
+        auto raise = [&](const f32x4_t (&s)[2], float (&factor)[2]) -> bool {
+          float top[2];
+#pragma unroll
+          for (int n = 0; n < 2; n++) top[n] = fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3])) * cm;
+          constexpr float kSlack = kRescaleSlack * kLog2e;
+          if (__builtin_amdgcn_ballot_w64(top[0] > m_ref[0] + kSlack || top[1] > m_ref[1] + kSlack) == 0) return false;
+#pragma unroll
+          for (int n = 0; n < 2; n++) {
+            const float t = rows4_reduce(top[n], [](float x, float y) { return fmaxf(x, y); });
+            factor[n] = 1.f;
+            if (t > m_ref[n] + kSlack) {
+              factor[n] = m_ref[n] > -SMLA_INF ? __builtin_amdgcn_exp2f(m_ref[n] - t) : 0.f;
+              l_lane[n] *= factor[n];
+              m_ref[n] = m_sub[n] = t;
+            }
+          }
+          return true;
+        };
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4_t s0[2], s1[2], t[2];  // a half's scores: even and odd K steps apart until its end
+        float p[2][8];
+#pragma unroll
+        for (int n = 0; n < 2; n++) s0[n] = t[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < G::KSTEPS; j++) {
+          const bf16x8_t k = as_bf16x8(kf[j % PF]);
+          kf[j % PF] = ldk(j + PF);
+#pragma unroll
+          for (int n = 0; n < 2; n++) {
+            if (j & 1) t[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[n][j], t[n], 0, 0, 0);
+            else s0[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[n][j], s0[n], 0, 0, 0);
+          }
+          if (j == 1) {
+            const int least = min(min(min(v0[0], v0[1]), min(v0[2], v0[3])), min(min(v1[0], v1[1]), min(v1[2], v1[3])));
+            open = e0 + kTileRows <= eh_all && (e0 >= el_all || e0 + kTileRows <= a.first) &&
+                   __builtin_amdgcn_ballot_w64(least < 0) == 0;
+            cm = open ? c2 : 1.f;
+          }
+          __builtin_amdgcn_sched_barrier(0);  // keep the reads PF steps ahead of their products
         }
-        const float sc = open ? a.scale : 1.f;  // masked tiles are scaled above
-        const uint64_t any_odd = __builtin_amdgcn_ballot_w64(odd);
+#pragma unroll
+        for (int n = 0; n < 2; n++) s0[n] += t[n];
+        if (!open) mask(s0, v0, e0);
+        raise(s0, alpha);
+#pragma unroll
+        for (int n = 0; n < 2; n++) s1[n] = t[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < G::KSTEPS; j++) {
+          const int f = G::KSTEPS + j;
+          const bf16x8_t k = as_bf16x8(kf[f % PF]);
+          if (j + PF < G::KSTEPS) kf[f % PF] = ldk(f + PF);
+#pragma unroll
+          for (int n = 0; n < 2; n++) {
+            if (j & 1) t[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[n][j], t[n], 0, 0, 0);
+            else s1[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[n][j], s1[n], 0, 0, 0);
+          }
+          if (j < 8) {
+            const int n = j >> 2, x = j & 3;
+            p[n][x] = __builtin_amdgcn_exp2f(s0[n][x] * cm - m_sub[n]);
+            l_lane[n] += p[n][x];
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int n = 0; n < 2; n++) s1[n] += t[n];
+        if (!open) mask(s1, v1, e0 + 16);
+        float later[2];
+        if (raise(s1, later)) {  // the first half's were taken against the old reference
+#pragma unroll
+          for (int n = 0; n < 2; n++) {
+            alpha[n] *= later[n];
+#pragma unroll
+            for (int x = 0; x < 4; x++) p[n][x] *= later[n];
+          }
+        }
         lds_u8_t* pb = lds + G::P_OFF + (i & 1) * G::PBUF + (32 * wave + c) * G::PSTRIDE;
 #pragma unroll
         for (int n = 0; n < 2; n++) {
-          float x[8];
 #pragma unroll
-          for (int k = 0; k < 8; k++) x[k] = s[k >> 2][n][k & 3] * sc;
-          float mt = x[0];
-#pragma unroll
-          for (int k = 1; k < 8; k++) mt = fmaxf(mt, x[k]);
-          mt = rows4_reduce(mt, [](float x, float y) { return fmaxf(x, y); });
-          float alpha = 1.f;
-          if ((mt > m_ref[n] + kRescaleSlack) || (m_ref[n] == -SMLA_INF && mt > -SMLA_INF)) {
-            alpha = (m_ref[n] > -SMLA_INF) ? __expf(m_ref[n] - mt) : 0.f;
-            l_lane[n] *= alpha;
-            m_ref[n] = mt;
+          for (int x = 0; x < 4; x++) {
+            p[n][4 + x] = __builtin_amdgcn_exp2f(s1[n][x] * cm - m_sub[n]);
+            l_lane[n] += p[n][4 + x];
           }
-          float p[8];
-#pragma unroll
-          for (int k = 0; k < 8; k++) {
-            // a NaN score stays NaN also where no maximum is set yet
-            p[k] = (m_ref[n] > -SMLA_INF) ? __expf(x[k] - m_ref[n]) : (x[k] == -SMLA_INF ? 0.f : x[k]);
-            l_lane[n] += p[k];
-          }
-          *(lds_u32x2_t*)(pb + 16 * n * G::PSTRIDE + 8 * g) = u32x2_t{pack2(p[0], p[1]), pack2(p[2], p[3])};
-          *(lds_u32x2_t*)(pb + 16 * n * G::PSTRIDE + 32 + 8 * g) = u32x2_t{pack2(p[4], p[5]), pack2(p[6], p[7])};
-          if (g == 0) al_s[(i & 1) * G::TILEQ + 32 * wave + 16 * n + c] = alpha;
+          *(lds_u32x2_t*)(pb + 16 * n * G::PSTRIDE + 8 * g) = u32x2_t{pack2(p[n][0], p[n][1]), pack2(p[n][2], p[n][3])};
+          *(lds_u32x2_t*)(pb + 16 * n * G::PSTRIDE + 32 + 8 * g) = u32x2_t{pack2(p[n][4], p[n][5]), pack2(p[n][6], p[n][7])};
+          if (g == 0) al_s[(i & 1) * G::TILEQ + 32 * wave + 16 * n + c] = alpha[n];
         }
+        const uint64_t any_odd = __builtin_amdgcn_ballot_w64(odd);
         if (lane == 0) *(lds_i32_t*)(pb + 64) = any_odd != 0;
       }
     }
@@ -610,7 +665,7 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
       float inv = 0.f;  // no row seen: 0
       if (!(L == 0.f)) {
         const float snk = a.sink && r < w.nh ? a.sink[(uint32_t)(w.m0 + r) % (uint32_t)a.H] : -SMLA_INF;
-        inv = 1.0f / (L + (snk == -SMLA_INF ? 0.f : __expf(snk - M)));
+        inv = 1.0f / (L + (snk == -SMLA_INF ? 0.f : __builtin_amdgcn_exp2f(snk * 1.44269504088896340736f - M)));
       }
       uint8_t* dst = (uint8_t*)(a.out + (w.row0 + r) * 512 + 32 * u0 + 8 * (lane >> 5));
 #pragma unroll
@@ -728,7 +783,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
 #pragma unroll
       for (int k = 0; k < kMergeBatch; k++)
         if (sp0 + kMergeWaves * k < it.nsplit) top = fmaxf(top, ml[k][0]);
-      const float keep = m > -SMLA_INF ? __expf(m - top) : (top == m ? 1.f : 0.f);
+      const float keep = m > -SMLA_INF ? __builtin_amdgcn_exp2f(m - top) : (top == m ? 1.f : 0.f);
       l *= keep;
 #pragma unroll
       for (int j = 0; j < 8; j++) acc[j] *= keep;
@@ -737,7 +792,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
       for (int k = 0; k < kMergeBatch; k++)
         if (sp0 + kMergeWaves * k < it.nsplit) {
           // a state without a maximum has l = 0 (nothing seen) or NaN
-          const float e = ml[k][0] > -SMLA_INF ? __expf(ml[k][0] - m) : 1.f;
+          const float e = ml[k][0] > -SMLA_INF ? __builtin_amdgcn_exp2f(ml[k][0] - m) : 1.f;
           l += ml[k][1] * e;
           const float es = e * sc[k];
 #pragma unroll
@@ -764,7 +819,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
       for (int j = 0; j < 8; j++) y[j] = 0.f;
 #pragma unroll
       for (int k = 0; k < kMergeWaves; k++) {
-        const float mk = red[k][lane][0], e = mk > -SMLA_INF ? __expf(mk - top) : 1.f;
+        const float mk = red[k][lane][0], e = mk > -SMLA_INF ? __builtin_amdgcn_exp2f(mk - top) : 1.f;
         sum += red[k][lane][1] * e;
 #pragma unroll
         for (int j = 0; j < 8; j++) y[j] += red[k][lane][2 + j] * e;
@@ -773,7 +828,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
         float inv = 0.f;
         if (!(sum == 0.f)) {
           const float snk = a.sink ? a.sink[(uint32_t)(m0 + row) % (uint32_t)a.H] : -SMLA_INF;
-          inv = 1.0f / (sum + (snk == -SMLA_INF ? 0.f : __expf(snk - top)));
+          inv = 1.0f / (sum + (snk == -SMLA_INF ? 0.f : __builtin_amdgcn_exp2f(snk * 1.44269504088896340736f - top)));
         }
         u32x4_t o;
 #pragma unroll
