@@ -14,7 +14,7 @@
 // would be long busy with.  Tiles of several items leave (m, l, O) states that paged_merge_kernel joins.
 //
 // A workgroup is 8 waves of up to 256 registers, two per SIMD, and walks its entries in tiles of 32 rows, two
-// roles one tile apart with one barrier between:
+// roles with one barrier a tile between:
 //   * score waves 0 .. NB-1: S^T = K Q^T of 32 q rows (v_mfma_f32_16x16x32_bf16, rows as M; the 32 rows' Q^T
 //     stays in 144 registers, so a K fragment read from LDS serves two products), online softmax with a lazy
 //     maximum, P in bf16 and the rescale factor to LDS;
@@ -25,8 +25,8 @@
 // 6.8 KB of LDS traffic a row (53 cycles of 128 bytes): both near balance, where 64 q rows on 12
 // waves of 168 registers (16 rows' Q^T a score wave) read 8.4 KB for two thirds of the products.
 //
-// Rows come HBM -> LDS by DMA into a ring of NBUF tiles, copies issued by the value waves (fp8 rows: loaded,
-// converted, written).  Row numbers go through an LDS ring of 8 tiles that score wave 0 fills seven tiles
+// Rows come HBM -> LDS by DMA into a ring of four tiles, copies issued by the value waves (fp8 rows: loaded,
+// converted, written).  Row numbers go through an LDS ring of 8 tiles that score wave 0 fills six tiles
 // ahead, so a row list of any length costs one table read per row.
 //
 // Rows masked for some of a tile's q rows may hold anything (rows not yet written, pages of id -1 read as
@@ -62,30 +62,35 @@ struct PagedArgs {
   float scale;
 };
 
-template <int D, int NB_, int NBUF_>
+// LDS layouts without bank conflicts (128 bytes an access cycle).  16-byte chunk ch of row r's columns 0..511 lies at chunk
+// ch ^ row_swizzle(r) of its 1024 bytes: the eight rows of a K read's cycle then fall on eight chunks, and the four rows
+// of a transposed V read's on four pairs of chunks.  Chunk ch of q row r's 64 bytes of P lies at ch ^ ((r >> 1) & 3).
+__device__ inline constexpr int row_swizzle(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+__device__ inline constexpr int p_at(int r, int ch) { return 64 * r + 16 * (ch ^ ((r >> 1) & 3)); }
+
+template <int D, int NB_>
 struct GeoP {
   static constexpr int NB = NB_;
   static constexpr int TILEQ = 32 * NB;  // q rows of a tile
   static constexpr int ROWB = D * 2;
   static constexpr bool TAIL = D > 512;
-  static constexpr int MSTRIDE = 1056;  // LDS bytes per row, columns 0..511
-  static constexpr int MAIN_BYTES = kTileRows * MSTRIDE;
+  static constexpr int MAIN_BYTES = kTileRows * 1024;  // columns 0..511 of 32 rows, in swizzled 16-byte chunks
   static constexpr int TAIL_BYTES = TAIL ? kTileRows * 128 : 0;
   static constexpr int TILE_BYTES = MAIN_BYTES + TAIL_BYTES;
-  static constexpr int NBUF = NBUF_;
-  static constexpr int PSTRIDE = 80;  // bytes per q row in a P buffer: 32 probabilities, then padding (a flag in rows 32 s)
-  static constexpr int PBUF = TILEQ * PSTRIDE;
+  static constexpr int NBUF = 4;
+  static constexpr int PBUF = TILEQ * 64;  // 32 probabilities a q row (p_at)
   static constexpr int P_OFF = NBUF * TILE_BYTES;
   static constexpr int AL_OFF = P_OFF + 2 * PBUF;  // rescale factors; after the loop (m, l)
   static constexpr int IDS_OFF = AL_OFF + 2 * TILEQ * 4;
-  static constexpr int LDS_BYTES = IDS_OFF + kIdTiles * kTileRows * 4;
+  static constexpr int FLAG_OFF = IDS_OFF + kIdTiles * kTileRows * 4;  // a flag per P buffer and score wave
+  static constexpr int LDS_BYTES = FLAG_OFF + 2 * 4 * 4;
   static constexpr int KSTEPS = D / 32;
   static constexpr int NDMA = kTileRows + (TAIL ? kTileRows / 8 : 0);
   static constexpr int STATE_O = kUnits * NB * 2048;                     // bytes of a state's O^T
   static constexpr int STATE_F = TILEQ * 2 + kValueWaves * NB * 64;       // floats: (m, l), then scales
   static_assert(LDS_BYTES <= 160 * 1024, "LDS budget");
   static_assert(NB <= kFirstValue && NBUF >= 3, "roles; a tile scored, one consumed, one on its way");
-  static_assert(kIdTiles >= NBUF + 2, "row numbers are written before their copies are issued");
+  static_assert(kIdTiles >= NBUF + 4, "row numbers are written before their copies are issued");
 };
 
 __device__ inline uint32_t pack2(float a, float b) { return pack_bf16x2(a, b); }
@@ -233,6 +238,9 @@ __device__ inline uint8_t* state_o(const PagedArgs& a, int slot) {
 __device__ inline constexpr int units_of(int vi) { return vi == 0 ? 4 : 3; }
 __device__ inline constexpr int first_unit(int vi) { return vi == 0 ? 0 : 1 + 3 * vi; }
 
+// the k-th of a tile's copies that value wave vi makes (the wave with four blocks is dealt last)
+__device__ inline constexpr int dealt(int vi, int k) { return kValueWaves - 1 - vi + kValueWaves * k; }
+
 // What a workgroup works on, the same in all its waves.
 struct Work {
   int slot;    // state slot, -1: the tile's only item
@@ -252,9 +260,9 @@ __device__ inline void issue_tile(const PagedArgs& a, uint32_t lds_base, const l
   auto rowp = [&](int r) { return (const uint8_t*)a.pages + (int64_t)max(id[r], 0) * G::ROWB; };
 #pragma unroll
   for (int k = 0; k < (G::NDMA + kValueWaves - 1) / kValueWaves; k++) {
-    const int x = vi + kValueWaves * k;
+    const int x = dealt(vi, k);
     if (x < kTileRows) {
-      dma16(rowp(x) + 16 * lane, __builtin_amdgcn_readfirstlane(tbase + x * G::MSTRIDE));
+      dma16(rowp(x) + 16 * (lane ^ row_swizzle(x)), __builtin_amdgcn_readfirstlane(tbase + x * 1024));
     } else if (x < G::NDMA) {
       const int r0 = (x - kTileRows) * 8, r = r0 + (lane >> 3);
       dma16(rowp(r) + 1024 + 16 * ((lane & 7) ^ (r & 7)), __builtin_amdgcn_readfirstlane(tbase + G::MAIN_BYTES + r0 * 128));
@@ -286,7 +294,7 @@ __device__ inline void f8_load(const PagedArgs& a, const lds_i32_t* ids_s, int v
   const lds_i32_t* id = ids_s + (tl % kIdTiles) * kTileRows;
 #pragma unroll
   for (int k = 0; k < F8<D>::K; k++) {
-    const int x = vi + kValueWaves * k;
+    const int x = dealt(vi, k);
     if (x < F8<D>::N) {
       int r, cc;
       f8_place<D>(x, lane, r, cc);
@@ -301,7 +309,7 @@ __device__ inline void f8_store(lds_u8_t* lds, int vi, int lane, int tl, const F
   lds_u8_t* slot = lds + (tl % G::NBUF) * G::TILE_BYTES;
 #pragma unroll
   for (int k = 0; k < F8<D>::K; k++) {
-    const int x = vi + kValueWaves * k;
+    const int x = dealt(vi, k);
     if (x < F8<D>::N) {
       int r, cc;
       f8_place<D>(x, lane, r, cc);
@@ -326,8 +334,9 @@ __device__ inline void f8_store(lds_u8_t* lds, int vi, int lane, int tl, const F
       }
       const u32x4_t w0 = {w[0], w[1], w[2], w[3]}, w1 = {w[4], w[5], w[6], w[7]};
       if (x < 16) {
-        *(lds_u32x4_t*)(slot + r * G::MSTRIDE + 32 * cc) = w0;
-        *(lds_u32x4_t*)(slot + r * G::MSTRIDE + 32 * cc + 16) = w1;
+        const int ch = (2 * cc) ^ row_swizzle(r);
+        *(lds_u32x4_t*)(slot + r * 1024 + 16 * ch) = w0;
+        *(lds_u32x4_t*)(slot + r * 1024 + 16 * (ch ^ 1)) = w1;
       } else {
         const int l0 = 2 * (cc - 32);
         *(lds_u32x4_t*)(slot + G::MAIN_BYTES + r * 128 + 16 * (l0 ^ (r & 7))) = w0;
@@ -338,11 +347,13 @@ __device__ inline void f8_store(lds_u8_t* lds, int vi, int lane, int tl, const F
 }
 
 // ---------------------------------------------------------------------------------------------
-// Score wave `wave` < NB: q rows 32 wave .. + 31.  A tile goes in two halves of 16 rows: the second half's products
-// run while the first half's exponentials are taken between them (an element a K step, placed by hand:
-// the products leave the vector pipe idle three cycles of four), so only the second half's are left at the end.
-// Scores are kept in base 2; a maximum further than 2^11.5 above the reference moves the reference, everything else
-// stays below e^8 of it.
+// Score wave `wave` < NB: q rows 32 wave .. + 31.  A tile goes in two halves of 16 rows, and an iteration is half a tile
+// late: it finishes tile i - 1 (second half's products, between which the first half's exponentials are taken, an
+// element a K step) and begins tile i (first half's products, between which tile i - 1's second exponentials are
+// taken and its P written).  The products leave the vector pipe idle three cycles of four, so the softmax costs
+// little beside them, and what an iteration reads first has been in LDS since the one before.
+// Scores are kept in base 2; a maximum further than e^8 above the reference moves the reference, everything else stays
+// below e^8 of it.
 template <class G, int D>
 __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32_t* trow, lds_u8_t* lds, int wave, int lane) {
   lds_i32_t* ids_s = (lds_i32_t*)(lds + G::IDS_OFF);
@@ -377,147 +388,187 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
   const int eh_all = w.p_lo + 1 - w.lo + w.nf, el_all = a.window > 0 ? w.p_hi - a.window + 1 - w.lo + w.nf : 0;
   if (idle) {  // nothing to rescale, and no flags
     al_s[(lane >> 5) * G::TILEQ + 32 * wave + (lane & 31)] = 1.f;
-    if (lane < 2) *(lds_i32_t*)(lds + G::P_OFF + lane * G::PBUF + 32 * wave * G::PSTRIDE + 64) = 0;
+    if (lane < 2) *(lds_i32_t*)(lds + G::FLAG_OFF + 16 * lane + 4 * wave) = 0;
   }
+  // K^T of row c: chunk 4 j + g of the main columns (even and odd K steps), chunk 4 (j - 16) + g of the tail
+  const int k_even = 1024 * c + 16 * (g ^ row_swizzle(c)), k_odd = 1024 * c + 16 * ((4 + g) ^ row_swizzle(c));
+  const int t_even = G::MAIN_BYTES + 128 * c + 16 * (g ^ (c & 7)), t_odd = G::MAIN_BYTES + 128 * c + 16 * ((4 + g) ^ (c & 7));
   // m_ref: the reference (-inf: none yet); m_sub: what is taken off a score (0 without a reference)
   float m_ref[2] = {-SMLA_INF, -SMLA_INF}, m_sub[2] = {0.f, 0.f}, l_lane[2] = {0.f, 0.f};
-  int next_id = 0;  // row numbers on their way: tile i + 7, read in iteration i - 1 and written in iteration i
-  for (int i = 0; i <= w.ntiles; i++) {
-    if (i < w.ntiles) {
-      if (wave == 0 && lane < kTileRows) {
-        if (i > 0 && i + kIdTiles - 1 < w.ntiles) ids_s[((i + kIdTiles - 1) % kIdTiles) * kTileRows + lane] = next_id;
-        if (i + kIdTiles < w.ntiles) {
-          const int e = w.e_begin + (i + kIdTiles) * kTileRows + lane;
-          next_id = row_number(a, trow, e < w.nf ? e : w.lo + (e - w.nf), e < w.e_end);
-        }
+  // the row number of tile 7's entry lane & 31 as column and place in its page, and 32 rows' step
+  int col = 0, off = 0, page = -1;
+  const int step_col = (int)((uint32_t)kTileRows / (uint32_t)a.P), step_off = kTileRows - step_col * a.P;
+  {
+    const int e = w.e_begin + (kIdTiles - 1) * kTileRows + (lane & 31), j = e < w.nf ? e : w.lo + (e - w.nf);
+    col = (int)((uint32_t)j / (uint32_t)a.P);
+    off = j - col * a.P;
+    if (e < w.e_end) page = trow[col];
+  }
+  // page: of tile i + 6's entry, read in iteration i - 1 and used in iteration i, so that nothing waits for it
+  auto row_numbers = [&](int i) {
+    if (wave != 0) return;
+    // tile i + 6's to the slot of tile i - 2, which nobody masks by any more (both halves of the wave alike)
+    if (i + 6 < w.ntiles)
+      ids_s[((i + 6) % kIdTiles) * kTileRows + (lane & 31)] = (uint32_t)page < (uint32_t)a.n_pages ? page * a.P + off : -1;
+    if (i + 7 < w.ntiles) {
+      const int e = w.e_begin + (i + 7) * kTileRows + (lane & 31);
+      // rows follow each other by 32, but where the first rows end
+      off += step_off;
+      col += step_col;
+      if (off >= a.P) {
+        off -= a.P;
+        col++;
       }
-      if (!idle) {
-        const lds_u8_t* buf = lds + (i % G::NBUF) * G::TILE_BYTES;
-        // fragment f of the tile: half f / KSTEPS, K step f % KSTEPS
-        auto ldk = [&](int f) -> u32x4_t {
-          const int h = f / G::KSTEPS, j = f - h * G::KSTEPS;
-          if (!G::TAIL || j < 16) return *(const lds_u32x4_t*)(buf + (16 * h + c) * G::MSTRIDE + 16 * g + 64 * j);
-          const int r = 16 * h + c, lch = 4 * (j - 16) + g;
-          return *(const lds_u32x4_t*)(buf + G::MAIN_BYTES + r * 128 + 16 * (lch ^ (r & 7)));
-        };
-        constexpr int PF = 6;
-        u32x4_t kf[PF];
+      if (w.nf > 0 && w.e_begin + (i + 6) * kTileRows < w.nf) {
+        const int j = e < w.nf ? e : w.lo + (e - w.nf);
+        col = (int)((uint32_t)j / (uint32_t)a.P);
+        off = j - col * a.P;
+      }
+      page = -1;
+      if (e < w.e_end) page = trow[col];
+    }
+  };
+  bool odd = false;               // a masked score of the tile is not finite
+  float alpha[2] = {1.f, 1.f};    // e^(old - new reference) of the tile's q rows
+  float cm = 1.f;                 // what turns the tile's scores to base 2 (c2; 1: masked, and scaled, already)
+  f32x4_t s0[2], s1[2];           // scores of the halves
+  float p[2][8];
+  constexpr int PF = G::TAIL ? 6 : 4;  // fragments read ahead (a divisor of a half's K steps)
+  static_assert(G::KSTEPS % PF == 0, "a half's fragments start at kf[0]");
+  u32x4_t kf[PF];
+  // K step j of half h of a tile
+  auto ldk = [&](const lds_u8_t* buf, int h, int j) -> u32x4_t {
+    if (!G::TAIL || j < 16) return *(const lds_u32x4_t*)(buf + ((j & 1) ? k_odd : k_even) + 16 * 1024 * h + 128 * (j >> 1));
+    return *(const lds_u32x4_t*)(buf + ((j & 1) ? t_odd : t_even) + 16 * 128 * h);
+  };
+  auto tile_at = [&](int i) { return lds + (i % G::NBUF) * G::TILE_BYTES; };
+  // scores of a half where some q row does not see some row: scaled, -inf there
+  auto mask = [&](f32x4_t (&s)[2], int i, int h) {
+    const i32x4_t v = *(const lds_i32x4_t*)(ids_s + (i % kIdTiles) * kTileRows + 16 * h + 4 * g);
+    const int e1 = w.e_begin + i * kTileRows + 16 * h + 4 * g;
 #pragma unroll
-        for (int f = 0; f < PF; f++) kf[f] = ldk(f);
-        const lds_i32_t* id = ids_s + (i % kIdTiles) * kTileRows;
-        const i32x4_t v0 = *(const lds_i32x4_t*)(id + 4 * g), v1 = *(const lds_i32x4_t*)(id + 16 + 4 * g);
-        const int e0 = w.e_begin + i * kTileRows;
-        bool odd = false;  // a masked score that is not finite
-        float alpha[2] = {1.f, 1.f};
-        bool open = false;
-        float cm = 1.f;
-        // scores of a half that are masked or tiles not open: scaled, -inf where the q row does not see the row
-        auto mask = [&](f32x4_t (&s)[2], const i32x4_t& v, int e1) {
+    for (int n = 0; n < 2; n++)
 #pragma unroll
-          for (int n = 0; n < 2; n++)
+      for (int k = 0; k < 4; k++) {  // (without branches)
+        const bool ok = (v[k] >= 0) & (e1 + k < eh[n]) & ((e1 + k < a.first) | (e1 + k >= el[n]));
+        odd |= !ok & !(fabsf(s[n][k]) < SMLA_INF);
+        const float x = s[n][k] * c2;
+        s[n][k] = ok ? x : -SMLA_INF;
+      }
+  };
+  // moves the references where a score is past them: factor[n] = e^(old - new)
+  auto raise = [&](const f32x4_t (&s)[2], float (&factor)[2]) -> bool {
+    float top[2];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-              const int e = e1 + 4 * g + k;
-              const bool ok = v[k] >= 0 && e < eh[n] && (e < a.first || e >= el[n]);
-              odd |= !ok && !(fabsf(s[n][k]) < SMLA_INF);
-              s[n][k] = ok ? s[n][k] * c2 : -SMLA_INF;
-            }
-        };
-        // moves the references where a score is past them: factor[n] = e^(old - new)
-        auto raise = [&](const f32x4_t (&s)[2], float (&factor)[2]) -> bool {
-          float top[2];
+    for (int n = 0; n < 2; n++) top[n] = fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3])) * cm;
+    constexpr float kSlack = kRescaleSlack * kLog2e;
+    if (__builtin_amdgcn_ballot_w64(top[0] > m_ref[0] + kSlack || top[1] > m_ref[1] + kSlack) == 0) return false;
 #pragma unroll
-          for (int n = 0; n < 2; n++) top[n] = fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3])) * cm;
-          constexpr float kSlack = kRescaleSlack * kLog2e;
-          if (__builtin_amdgcn_ballot_w64(top[0] > m_ref[0] + kSlack || top[1] > m_ref[1] + kSlack) == 0) return false;
+    for (int n = 0; n < 2; n++) {
+      const float x = rows4_reduce(top[n], [](float x, float y) { return fmaxf(x, y); });
+      factor[n] = 1.f;
+      if (x > m_ref[n] + kSlack) {
+        factor[n] = m_ref[n] > -SMLA_INF ? __builtin_amdgcn_exp2f(m_ref[n] - x) : 0.f;
+        l_lane[n] *= factor[n];
+        m_ref[n] = m_sub[n] = x;
+      }
+    }
+    return true;
+  };
+  // the products of one half (h of tile buf's rows) into s; `between` j runs after K step j's, and the fragments that
+  // follow (of half nh of tile next) are read ahead
+  auto products = [&](f32x4_t (&s)[2], const lds_u8_t* buf, int h, const lds_u8_t* next, int nh, auto&& between) {
 #pragma unroll
-          for (int n = 0; n < 2; n++) {
-            const float t = rows4_reduce(top[n], [](float x, float y) { return fmaxf(x, y); });
-            factor[n] = 1.f;
-            if (t > m_ref[n] + kSlack) {
-              factor[n] = m_ref[n] > -SMLA_INF ? __builtin_amdgcn_exp2f(m_ref[n] - t) : 0.f;
-              l_lane[n] *= factor[n];
-              m_ref[n] = m_sub[n] = t;
-            }
-          }
-          return true;
-        };
-        __builtin_amdgcn_sched_barrier(0);
-        f32x4_t s0[2], s1[2], t[2];  // a half's scores: even and odd K steps apart until its end
-        float p[2][8];
+    for (int n = 0; n < 2; n++) s[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int n = 0; n < 2; n++) s0[n] = t[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < G::KSTEPS; j++) {
+      const bf16x8_t k = as_bf16x8(kf[j % PF]);
+      kf[j % PF] = j + PF < G::KSTEPS ? ldk(buf, h, j + PF) : ldk(next, nh, j + PF - G::KSTEPS);
 #pragma unroll
-        for (int j = 0; j < G::KSTEPS; j++) {
-          const bf16x8_t k = as_bf16x8(kf[j % PF]);
-          kf[j % PF] = ldk(j + PF);
+      for (int n = 0; n < 2; n++) s[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[n][j], s[n], 0, 0, 0);
+      between(j);
+      __builtin_amdgcn_sched_barrier(0);  // keep the reads PF steps ahead of their products
+    }
+  };
+  // first half of tile i: its products, then masks and references
+  auto first_half = [&](int i, auto&& between) {
+    products(s0, tile_at(i), 0, tile_at(i), 1, between);
+    const i32x4_t v0 = *(const lds_i32x4_t*)(ids_s + (i % kIdTiles) * kTileRows + 4 * (lane & 7));
+    const int least = min(min(v0[0], v0[1]), min(v0[2], v0[3])), e0 = w.e_begin + i * kTileRows;
+    const bool open = e0 + kTileRows <= eh_all && (e0 >= el_all || e0 + kTileRows <= a.first) &&
+                      __builtin_amdgcn_ballot_w64(least < 0) == 0;
+    cm = open ? c2 : 1.f;
+    odd = false;
+    alpha[0] = alpha[1] = 1.f;
+    if (!open) mask(s0, i, 0);
+    raise(s0, alpha);
+    return open;
+  };
+  auto expo = [&](const f32x4_t (&s)[2], int h, float scale, int x) {
+    const int n = x >> 2, k = x & 3;
+    p[n][4 * h + k] = __builtin_amdgcn_exp2f(s[n][k] * scale - m_sub[n]);
+    l_lane[n] += p[n][4 * h + k];
+  };
+  // P and the rescale factors of tile i - 1, written while the next tile's first products run
+  auto put = [&](int i, int part) {
+    const int n = part >> 1, r = 32 * wave + 16 * n + c;
+    lds_u8_t* pb = lds + G::P_OFF + (i & 1) * G::PBUF + 8 * (g & 1);
+    if ((part & 1) == 0)
+      *(lds_u32x2_t*)(pb + p_at(r, g >> 1)) = u32x2_t{pack2(p[n][0], p[n][1]), pack2(p[n][2], p[n][3])};
+    else
+      *(lds_u32x2_t*)(pb + p_at(r, 2 + (g >> 1))) = u32x2_t{pack2(p[n][4], p[n][5]), pack2(p[n][6], p[n][7])};
+  };
+  auto put_alpha = [&](int i, float al0, float al1, bool flag) {
+    al_s[(i & 1) * G::TILEQ + 32 * wave + (lane & 31)] = (lane & 16) ? al1 : al0;
+    const uint64_t any = __builtin_amdgcn_ballot_w64(flag);
+    if (lane == 0) *(lds_i32_t*)(lds + G::FLAG_OFF + 16 * (i & 1) + 4 * wave) = any != 0;
+  };
+  bool open = false;
+  // the compiler's own count: no load is in flight from here on but row_numbers' one, so the loop waits for none
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  if (!idle && w.ntiles > 0) {
 #pragma unroll
-          for (int n = 0; n < 2; n++) {
-            if (j & 1) t[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[n][j], t[n], 0, 0, 0);
-            else s0[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[n][j], s0[n], 0, 0, 0);
-          }
-          if (j == 1) {
-            const int least = min(min(min(v0[0], v0[1]), min(v0[2], v0[3])), min(min(v1[0], v1[1]), min(v1[2], v1[3])));
-            open = e0 + kTileRows <= eh_all && (e0 >= el_all || e0 + kTileRows <= a.first) &&
-                   __builtin_amdgcn_ballot_w64(least < 0) == 0;
-            cm = open ? c2 : 1.f;
-          }
-          __builtin_amdgcn_sched_barrier(0);  // keep the reads PF steps ahead of their products
-        }
-#pragma unroll
-        for (int n = 0; n < 2; n++) s0[n] += t[n];
-        if (!open) mask(s0, v0, e0);
-        raise(s0, alpha);
-#pragma unroll
-        for (int n = 0; n < 2; n++) s1[n] = t[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int j = 0; j < G::KSTEPS; j++) {
-          const int f = G::KSTEPS + j;
-          const bf16x8_t k = as_bf16x8(kf[f % PF]);
-          if (j + PF < G::KSTEPS) kf[f % PF] = ldk(f + PF);
-#pragma unroll
-          for (int n = 0; n < 2; n++) {
-            if (j & 1) t[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[n][j], t[n], 0, 0, 0);
-            else s1[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[n][j], s1[n], 0, 0, 0);
-          }
-          if (j < 8) {
-            const int n = j >> 2, x = j & 3;
-            p[n][x] = __builtin_amdgcn_exp2f(s0[n][x] * cm - m_sub[n]);
-            l_lane[n] += p[n][x];
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-#pragma unroll
-        for (int n = 0; n < 2; n++) s1[n] += t[n];
-        if (!open) mask(s1, v1, e0 + 16);
-        float later[2];
-        if (raise(s1, later)) {  // the first half's were taken against the old reference
-#pragma unroll
-          for (int n = 0; n < 2; n++) {
-            alpha[n] *= later[n];
-#pragma unroll
-            for (int x = 0; x < 4; x++) p[n][x] *= later[n];
-          }
-        }
-        lds_u8_t* pb = lds + G::P_OFF + (i & 1) * G::PBUF + (32 * wave + c) * G::PSTRIDE;
+    for (int j = 0; j < PF; j++) kf[j] = ldk(tile_at(0), 0, j);
+    open = first_half(0, [](int) {});
+  }
+  lds_barrier();
+  for (int i = 1; i <= w.ntiles; i++) {
+    if (!idle) {
+      const bool more = i < w.ntiles;
+      products(s1, tile_at(i - 1), 1, tile_at(i), 0, [&](int j) {
+        if (j < 8) expo(s0, 0, cm, j);
+        if (j == 9) row_numbers(i);
+      });
+      if (!open) mask(s1, i - 1, 1);
+      float later[2];
+      if (raise(s1, later)) {  // the first half's were taken against the old reference
 #pragma unroll
         for (int n = 0; n < 2; n++) {
+          alpha[n] *= later[n];
 #pragma unroll
-          for (int x = 0; x < 4; x++) {
-            p[n][4 + x] = __builtin_amdgcn_exp2f(s1[n][x] * cm - m_sub[n]);
-            l_lane[n] += p[n][4 + x];
-          }
-          *(lds_u32x2_t*)(pb + 16 * n * G::PSTRIDE + 8 * g) = u32x2_t{pack2(p[n][0], p[n][1]), pack2(p[n][2], p[n][3])};
-          *(lds_u32x2_t*)(pb + 16 * n * G::PSTRIDE + 32 + 8 * g) = u32x2_t{pack2(p[n][4], p[n][5]), pack2(p[n][6], p[n][7])};
-          if (g == 0) al_s[(i & 1) * G::TILEQ + 32 * wave + 16 * n + c] = alpha[n];
+          for (int x = 0; x < 4; x++) p[n][x] *= later[n];
         }
-        const uint64_t any_odd = __builtin_amdgcn_ballot_w64(odd);
-        if (lane == 0) *(lds_i32_t*)(pb + 64) = any_odd != 0;
+      }
+      const float al0 = alpha[0], al1 = alpha[1], cm1 = cm;
+      const bool flag = odd;
+      if (more) {
+        open = first_half(i, [&](int j) {
+          if (j < 8) expo(s1, 1, cm1, j);
+          if (j >= 8 && j < 12) put(i - 1, j - 8);
+          if (j == 12) put_alpha(i - 1, al0, al1, flag);
+        });
+      } else {
+#pragma unroll
+        for (int x = 0; x < 8; x++) expo(s1, 1, cm1, x);
+#pragma unroll
+        for (int x = 0; x < 4; x++) put(i - 1, x);
+        put_alpha(i - 1, al0, al1, flag);
       }
     }
     lds_barrier();
   }
+  lds_barrier();  // (the value waves' last tile)
   // (m, l): for the value waves' final scaling, or the state's
 #pragma unroll
   for (int n = 0; n < 2; n++) {
@@ -541,7 +592,7 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
   const lds_f32_t* al_s = (const lds_f32_t*)(lds + G::AL_OFF);
   const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
   const int nb = (w.nh + 31) / 32;  // blocks of q rows in use (the others' products are not stored)
-  const int my_dma = (G::NDMA - vi + kValueWaves - 1) / kValueWaves;
+  const int my_dma = (G::NDMA - dealt(vi, 0) + kValueWaves - 1) / kValueWaves;
   f32x16_t o[NU][NB];
 #pragma unroll
   for (int u = 0; u < NU; u++)
@@ -550,83 +601,113 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
 #pragma unroll
       for (int r = 0; r < 16; r++) o[u][n][r] = 0.f;
   // V^T provider address inside a 16-row step: group j = lane >> 4 covers value columns 16 (j & 1) .. of a block and
-  // rows 8 (j >> 1) ..; lane J = lane & 15 supplies row J >> 2, columns 4 (J & 3) .. + 3
+  // rows 8 (j >> 1) ..; lane J = lane & 15 supplies row J >> 2, columns 4 (J & 3) .. + 3.  Two blocks on, the swizzle is the
+  // same: blocks u and u + 2 lie 128 bytes apart
   const int vj = lane >> 4, vJ = lane & 15;
-  const int tr_off = (8 * (vj >> 1) + (vJ >> 2)) * G::MSTRIDE + 2 * (32 * u0 + 16 * (vj & 1) + 4 * (vJ & 3));
-  const int pr_off = (lane & 31) * G::PSTRIDE + 16 * (lane >> 5);
+  int tr_lo[2], tr_hi[2];  // rows vJ >> 2 and 4 + (vJ >> 2) of each eight
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    const int row = 8 * (vj >> 1) + (vJ >> 2), ch = 4 * (u0 + u) + 2 * (vj & 1) + ((vJ & 3) >> 1);
+    tr_lo[u] = 1024 * row + 16 * (ch ^ row_swizzle(row)) + 8 * (vJ & 1);
+    tr_hi[u] = 1024 * (row + 4) + 16 * (ch ^ row_swizzle(row + 4)) + 8 * (vJ & 1);
+  }
+  int pr[2];  // chunk 2 ks + (lane >> 5) of q row lane & 31 (+ 32 n)
+#pragma unroll
+  for (int ks = 0; ks < 2; ks++) pr[ks] = p_at(lane & 31, 2 * ks + (lane >> 5));
   F8<D> f8;
-  // ---- the first copies: every slot (row copies), or tiles 0 .. NBUF-3 (fp8, and the next one's codes)
+  // ---- the first copies: every slot (row copies), or tile 0 (fp8, and the next one's codes)
   if constexpr (FP8) {
-    for (int tl = 0; tl < min(w.ntiles, G::NBUF - 2); tl++) {
-      f8_load<D>(a, ids_s, vi, lane, tl, f8);
-      f8_store<G, D>(lds, vi, lane, tl, f8);
+    if (w.ntiles > 0) {
+      f8_load<D>(a, ids_s, vi, lane, 0, f8);
+      f8_store<G, D>(lds, vi, lane, 0, f8);
+      if (w.ntiles > 1) f8_load<D>(a, ids_s, vi, lane, 1, f8);
     }
-    if (G::NBUF - 2 < w.ntiles) f8_load<D>(a, ids_s, vi, lane, G::NBUF - 2, f8);
   } else {
     for (int tl = 0; tl < min(w.ntiles, G::NBUF); tl++) issue_tile<G>(a, lds_base, ids_s, vi, lane, tl);
     wait_vm(max(0, min(G::NBUF, w.ntiles) - 1) * my_dma);  // tile 0 has landed
   }
   lds_barrier();
-  for (int i = 0; i <= w.ntiles; i++) {
+  // Iteration i: the score waves finish tile i - 1 and begin tile i, tile i - 2 is consumed here, and tile i + 1 goes
+  // to the slot of tile i - 3, to be there at the iteration's end.
+  for (int i = 0; i <= w.ntiles + 1; i++) {
     if constexpr (FP8) {
-      // tile i + NBUF - 2 goes to the slot of tile i - 2, consumed before the last barrier
-      if (i + G::NBUF - 2 < w.ntiles) {
-        f8_store<G, D>(lds, vi, lane, i + G::NBUF - 2, f8);
-        if (i + G::NBUF - 1 < w.ntiles) f8_load<D>(a, ids_s, vi, lane, i + G::NBUF - 1, f8);
+      if (i + 1 < w.ntiles) {
+        f8_store<G, D>(lds, vi, lane, i + 1, f8);
+        if (i + 2 < w.ntiles) f8_load<D>(a, ids_s, vi, lane, i + 2, f8);
       }
+    } else {
+      if (i >= 3 && i + 1 < w.ntiles) issue_tile<G>(a, lds_base, ids_s, vi, lane, i + 1);
     }
-    if (i >= 1) {
-      const int tp = i - 1;  // tile scored in the last iteration
-      const lds_u8_t* buf = lds + (tp % G::NBUF) * G::TILE_BYTES;
+    if (i >= 2) {
+      const int tp = i - 2;  // its P was written in the last iteration
+      lds_u8_t* buf = lds + (tp % G::NBUF) * G::TILE_BYTES;
       const lds_u8_t* pbuf = lds + G::P_OFF + (tp & 1) * G::PBUF;
-      int odd = 0;
+      // step st: rows 16 (st / NU) .. + 15, block st % NU; V^T is read AHEAD steps early
+      constexpr int AHEAD = NU * NB < 12 ? 2 : 1;  // (192 accumulators leave room for one)
+      const lds_u8_t *lo0 = buf + tr_lo[0], *lo1 = buf + tr_lo[1], *hi0 = buf + tr_hi[0], *hi1 = buf + tr_hi[1];
+      auto ldv = [&](int st) -> u32x4_t {
+        const int u = st % NU, at = 16 * 1024 * (st / NU) + 128 * (u >> 1);
+        const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(((u & 1) ? lo1 : lo0) + at));
+        const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(((u & 1) ? hi1 : hi0) + at));
+        return __builtin_bit_cast(u32x4_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      };
+      auto ldp = [&](int ks, int n) { return as_bf16x8(*(const lds_u32x4_t*)(pbuf + pr[ks] + 32 * 64 * n)); };
+      float al[NB];
 #pragma unroll
-      for (int n = 0; n < NB; n++) {
-        odd |= *(const lds_i32_t*)(pbuf + 32 * n * G::PSTRIDE + 64);
-        const float al = al_s[(tp & 1) * G::TILEQ + 32 * n + (lane & 31)];
-        if (__builtin_amdgcn_ballot_w64(al != 1.f)) {
+      for (int n = 0; n < NB; n++) al[n] = al_s[(tp & 1) * G::TILEQ + 32 * n + (lane & 31)];
+      const i32x4_t flag = *(const lds_i32x4_t*)(lds + G::FLAG_OFF + 16 * (tp & 1));
+      bf16x8_t pf[NB];
+      u32x4_t va[AHEAD + 1];
 #pragma unroll
-          for (int u = 0; u < NU; u++) o[u][n] *= al;
-        }
+      for (int n = 0; n < NB; n++) pf[n] = ldp(0, n);
+#pragma unroll
+      for (int st = 0; st < AHEAD; st++) va[st] = ldv(st);
+      __builtin_amdgcn_sched_barrier(0);
+      bool turn = false;
+#pragma unroll
+      for (int n = 0; n < NB; n++) turn |= al[n] != 1.f;
+      if (__builtin_amdgcn_ballot_w64(turn)) {
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+          for (int u = 0; u < NU; u++) o[u][n] *= al[n];
       }
+      int odd = flag[0];
+#pragma unroll
+      for (int n = 1; n < NB; n++) odd |= flag[n];
       if (__builtin_amdgcn_readfirstlane(odd)) {
-        // this wave's columns (nobody else reads them by now): 64 NU bytes of each of 32 rows, 16 bytes a lane
-        lds_u8_t* mine = lds + (tp % G::NBUF) * G::TILE_BYTES + 64 * u0;
+        // this wave's columns (nobody else reads them by now): 4 NU chunks of each of 32 rows
         for (int x = lane; x < kTileRows * 4 * NU; x += 64) {
-          const int row = x / (4 * NU);
-          lds_u32x4_t* at = (lds_u32x4_t*)(mine + row * G::MSTRIDE + 16 * (x - row * (4 * NU)));
+          const int row = x / (4 * NU), ch = 4 * u0 + x - row * (4 * NU);
+          lds_u32x4_t* at = (lds_u32x4_t*)(buf + row * 1024 + 16 * (ch ^ row_swizzle(row)));
           u32x4_t y = *at;
 #pragma unroll
           for (int k = 0; k < 4; k++) y[k] = finite2(y[k]);
           *at = y;
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int st = 0; st < AHEAD; st++) va[st] = ldv(st);
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int ks = 0; ks < 2; ks++) {
-        bf16x8_t pf[NB];
+      for (int st = 0; st < 2 * NU; st++) {
+        const bf16x8_t v = as_bf16x8(va[st % (AHEAD + 1)]);
+        if (st + AHEAD < 2 * NU) va[(st + AHEAD) % (AHEAD + 1)] = ldv(st + AHEAD);
 #pragma unroll
-        for (int n = 0; n < NB; n++) pf[n] = as_bf16x8(*(const lds_u32x4_t*)(pbuf + pr_off + 32 * n * G::PSTRIDE + 32 * ks));
-        const lds_u8_t* vb = buf + tr_off + 16 * ks * G::MSTRIDE;
-#pragma unroll
-        for (int u = 0; u < NU; u++) {
-          const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vb + 64 * u));
-          const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vb + 64 * u + 4 * G::MSTRIDE));
-          const bf16x8_t va = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-          for (int n = 0; n < NB; n++) o[u][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pf[n], o[u][n], 0, 0, 0);
+        for (int n = 0; n < NB; n++) {
+          o[st % NU][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, pf[n], o[st % NU][n], 0, 0, 0);
+          if (st == NU - 1) pf[n] = ldp(1, n);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-    // tile i + 1 has landed; the slot of the consumed tile i - 1 takes tile i + NBUF - 1
     if constexpr (!FP8) {
-      // (the newest requested: NBUF - 1 at first, then i + NBUF - 2)
-      if (i + 1 < w.ntiles) wait_vm(max(0, min(max(i + G::NBUF - 2, G::NBUF - 1), w.ntiles - 1) - (i + 1)) * my_dma);
+      // tile i + 1 has landed (the newest requested: 3 at first, then i + 1)
+      if (i >= 2) wait_vm(0);
+      else if (i + 1 < w.ntiles) wait_vm(max(0, min(3, w.ntiles - 1) - (i + 1)) * my_dma);
     }
     lds_barrier();
-    if constexpr (!FP8) {
-      if (i >= 1 && i + G::NBUF - 1 < w.ntiles) issue_tile<G>(a, lds_base, ids_s, vi, lane, i + G::NBUF - 1);
-    }
   }
   lds_barrier();  // (m, l) in LDS
 #pragma unroll
@@ -684,9 +765,9 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
   }
 }
 
-template <int D, int NB, int NBUF, bool FP8>
+template <int D, int NB, bool FP8>
 __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedArgs a) {
-  using G = GeoP<D, NB, NBUF>;
+  using G = GeoP<D, NB>;
   extern __shared__ __align__(16) uint8_t lds_generic[];
   lds_u8_t* lds = (lds_u8_t*)lds_generic;
   lds_i32_t* ids_s = (lds_i32_t*)(lds + G::IDS_OFF);
@@ -729,7 +810,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedArgs
       lds_barrier();  // tile 0 has landed
       score_role<G, D>(a, w, trow, lds, wave, lane);
     } else {
-      for (int i = 0; i < w.ntiles + 3; i++) lds_barrier();
+      for (int i = 0; i < w.ntiles + 4; i++) lds_barrier();
     }
   } else if (wave == kFirstValue) {
     value_role<G, D, FP8, units_of(0)>(a, w, lds, 0, first_unit(0), lane);
@@ -747,7 +828,7 @@ constexpr int kMergeWaves = 4, kMergeBatch = 8;
 
 template <int D, int NB>
 __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const PagedArgs a) {
-  using G = GeoP<D, NB, 3>;
+  using G = GeoP<D, NB>;
   constexpr int kPieces = kUnits * NB * 2;
   __shared__ float red[kMergeWaves][64][10];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -848,17 +929,17 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
 // item per compute unit one slot each, else two per half share of work.
 int64_t most_tiles(int64_t T, int64_t H, int64_t B, int nb) { return T * H / (32 * nb) + (B < T ? B : T); }
 int64_t plan_slots(int64_t tiles, int cus) { return tiles <= cus ? cus : 4 * (int64_t)cus + 64; }
-// q rows per tile / 32: where the sequences have no more than 64 on average, tiles of 64 leave LDS for a fourth ring slot
-// (steps of one or few tokens are bound by the rows' arrival); longer runs of q rows share a row among 96
+// q rows per tile / 32: where the sequences have no more than 64 on average (steps of one or few tokens, bound by the
+// rows' arrival), tiles of 64 have fewer products to wait for; longer runs of q rows share a row among 96
 int tile_blocks(int64_t T, int64_t H, int64_t B) { return T * H <= 64 * B ? 2 : 3; }
 bool plan_sizes(int64_t T, int64_t H, int64_t B) {
   return T >= 0 && H > 0 && B > 0 && T <= 0x7fffffff && H <= 0x7fffffff && B <= 0xfffff && T * H <= 0x7fffff80;
 }
 
-template <int D, int NB, int NBUF, bool FP8>
+template <int D, int NB, bool FP8>
 int launch_paged(const PagedArgs& a, int64_t tiles, hipStream_t st) {
-  using G = GeoP<D, NB, NBUF>;
-  auto kern = paged_attn_kernel<D, NB, NBUF, FP8>;
+  using G = GeoP<D, NB>;
+  auto kern = paged_attn_kernel<D, NB, FP8>;
   static std::atomic<uint64_t> lds_attr{0};
   if (hipError_t e = smla_set_dynamic_lds((const void*)kern, G::LDS_BYTES, lds_attr); e != hipSuccess) return (int)e;
   const int64_t grid = tiles <= a.cus ? a.cus : tiles + 2 * (int64_t)a.cus + 64;
@@ -878,8 +959,8 @@ extern "C" size_t smla_paged_attn_workspace(int64_t T, int64_t H, int64_t B) {
   using namespace smla_attn;
   if (!plan_sizes(T, H, B)) return 0;
   const int nb = tile_blocks(T, H, B);
-  const int64_t state = nb == 2 ? GeoP<512, 2, 3>::STATE_O + 4 * GeoP<512, 2, 3>::STATE_F
-                                : GeoP<512, 3, 3>::STATE_O + 4 * GeoP<512, 3, 3>::STATE_F;
+  const int64_t state = nb == 2 ? GeoP<512, 2>::STATE_O + 4 * GeoP<512, 2>::STATE_F
+                                : GeoP<512, 3>::STATE_O + 4 * GeoP<512, 3>::STATE_F;
   return (size_t)(kHeader + plan_slots(most_tiles(T, H, B, nb), smla_num_cus()) * state);
 }
 
@@ -929,12 +1010,12 @@ extern "C" int smla_paged_attn(const void* q, int q_dtype, const void* pages, in
   a.slots = (int)plan_slots(tiles, a.cus);
   const hipStream_t st = (hipStream_t)stream;
   const bool fp8 = page_dtype == SMLA_FP8_E4M3;
-#define SMLA_PAGED(DD, NB, NBUF) return fp8 ? launch_paged<DD, NB, NBUF, true>(a, tiles, st) : launch_paged<DD, NB, NBUF, false>(a, tiles, st)
+#define SMLA_PAGED(DD, NB) return fp8 ? launch_paged<DD, NB, true>(a, tiles, st) : launch_paged<DD, NB, false>(a, tiles, st)
   if (nb == 2) {
-    if (D == 576) SMLA_PAGED(576, 2, 4);
-    SMLA_PAGED(512, 2, 4);
+    if (D == 576) SMLA_PAGED(576, 2);
+    SMLA_PAGED(512, 2);
   }
-  if (D == 576) SMLA_PAGED(576, 3, 3);
-  SMLA_PAGED(512, 3, 4);
+  if (D == 576) SMLA_PAGED(576, 3);
+  SMLA_PAGED(512, 3);
 #undef SMLA_PAGED
 }
