@@ -15,9 +15,8 @@
 //
 // A workgroup is 8 waves of up to 256 registers, two per SIMD, and walks its entries in tiles of 32 rows, two
 // roles with one barrier a tile between:
-//   * score waves 0 .. NB-1: S^T = K Q^T of 32 q rows (v_mfma_f32_16x16x32_bf16, rows as M; the 32 rows' Q^T
-//     stays in 144 registers, so a K fragment read from LDS serves two products), online softmax with a lazy
-//     maximum, P in bf16 and the rescale factor to LDS;
+//   * score waves 0 .. NB-1: S^T = K Q^T of 32 q rows (v_mfma_f32_32x32x16_bf16, rows as M; the 32 q rows' Q^T
+//     stays in 144 registers), online softmax with a lazy maximum, P in bf16 and the rescale factor to LDS;
 //   * value waves 3 .. 7: O^T += V^T P^T (v_mfma_f32_32x32x16_bf16) of 3 or 4 blocks of 32 value columns and all
 //     the tile's q rows, so each V^T fragment (ds_read_b64_tr_b16) is read by one wave and serves NB products.
 //     Wave 3 shares its SIMD with value wave 7 instead of a score wave and takes four blocks, the others three.
@@ -45,6 +44,7 @@ typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 constexpr int kIdTiles = 8;        // tiles of the row-number ring
 constexpr int kMinRows = 64;       // fewest entries of an item
 constexpr int kMinRowsMany = 256;  // the same with more tiles than compute units
+constexpr int kMinPart = 4096, kMostParts = 4, kMostItems = 16, kPartRows = 256;  // parts of many tiles (plan_rps)
 constexpr int kHeader = 256;       // workspace bytes before the states
 constexpr int kWaves = 8, kFirstValue = 3, kValueWaves = 5;
 constexpr int kUnits = 16;         // blocks of 32 value columns
@@ -62,11 +62,12 @@ struct PagedArgs {
   float scale;
 };
 
-// LDS layouts without bank conflicts (128 bytes an access cycle).  16-byte chunk ch of row r's columns 0..511 lies at chunk
-// ch ^ row_swizzle(r) of its 1024 bytes: the eight rows of a K read's cycle then fall on eight chunks, and the four rows
-// of a transposed V read's on four pairs of chunks.  Chunk ch of q row r's 64 bytes of P lies at ch ^ ((r >> 1) & 3).
-__device__ inline constexpr int row_swizzle(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
-__device__ inline constexpr int p_at(int r, int ch) { return 64 * r + 16 * (ch ^ ((r >> 1) & 3)); }
+// LDS layouts without bank conflicts (64 banks: 256 bytes an access cycle).  16-byte chunk ch of row r's columns 0..511 lies
+// at chunk ch ^ row_swizzle(r) of its 1024 bytes: the 16 rows of a K read's cycle fall on 16 chunks, and the four
+// rows of a transposed V read's (64 bytes each) on four groups of four.  Chunk ch of q row r's 64 bytes of P lies at
+// ch ^ ((r >> 2) & 3).  Measured: 4.7 cycles a 1 KB read against 8.0 with swizzles that repeat every 128 bytes.
+__device__ inline constexpr int row_swizzle(int r) { return ((r & 3) << 2) | ((r >> 2) & 3); }
+__device__ inline constexpr int p_at(int r, int ch) { return 64 * r + 16 * (ch ^ ((r >> 2) & 3)); }
 
 template <int D, int NB_>
 struct GeoP {
@@ -84,7 +85,6 @@ struct GeoP {
   static constexpr int IDS_OFF = AL_OFF + 2 * TILEQ * 4;
   static constexpr int FLAG_OFF = IDS_OFF + kIdTiles * kTileRows * 4;  // a flag per P buffer and score wave
   static constexpr int LDS_BYTES = FLAG_OFF + 2 * 4 * 4;
-  static constexpr int KSTEPS = D / 32;
   static constexpr int NDMA = kTileRows + (TAIL ? kTileRows / 8 : 0);
   static constexpr int STATE_O = kUnits * NB * 2048;                     // bytes of a state's O^T
   static constexpr int STATE_F = TILEQ * 2 + kValueWaves * NB * 64;       // floats: (m, l), then scales
@@ -94,14 +94,6 @@ struct GeoP {
 };
 
 __device__ inline uint32_t pack2(float a, float b) { return pack_bf16x2(a, b); }
-
-template <class Op>
-__device__ inline float rows4_reduce(float v, Op op) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
 
 // the bf16 pair with an infinite or NaN half set to 0
 __device__ inline uint32_t finite2(uint32_t w) {
@@ -141,7 +133,7 @@ __device__ inline int ceil_div(int a, int b) { return (int)(((uint32_t)a + (uint
 __device__ inline int splits_of(const Seq& s, int rps) { return max(1, ceil_div(s.span, rps)); }
 __device__ inline int wave_sum_i(int v) { return __builtin_amdgcn_readlane(wave_incl_scan(v), 63); }
 
-// Entries per item (a multiple of 32).  s0: sequences 0..63, kept in registers by the caller.
+// Most entries per item (a multiple of 32; a sequence's splits are equal parts of its entries).  s0: sequences 0..63, kept in registers by the caller.
 template <int TILEQ>
 __device__ inline int plan_rps(const PagedArgs& a, const Seq& s0, int lane) {
   float work = 0.f;
@@ -155,7 +147,25 @@ __device__ inline int plan_rps(const PagedArgs& a, const Seq& s0, int lane) {
   if (tiles > a.cus) {
     // more tiles than compute units: items of at most half a unit's share
     const float share = work / (float)(2 * a.cus * kTileRows);
-    return max(kMinRowsMany, ((int)fminf(share, 16777216.f) + 1) * kTileRows);
+    const int best = max(kMinRowsMany / kTileRows, (int)fminf(share, 16777216.f) + 1);
+    if (most < kMinPart / kTileRows * 2 || 2 * (int64_t)tiles > kMostItems * a.cus) return best * kTileRows;
+    // few rounds of long tiles: parts of them fill the last round better; a part costs about kPartRows entries more
+    float least = 0.f;
+    int rps = best;
+    for (int k = 1; k <= kMostParts && most / k >= kMinPart / kTileRows && k * tiles <= kMostItems * a.cus; k++) {
+      const int unit = min(best, (most + k - 1) / k);
+      int items = 0;
+      for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const Seq s = b0 == 0 ? s0 : load_seq<TILEQ>(a, b0 + lane);
+        items += wave_sum_i(s.tiles * splits_of(s, unit * kTileRows));
+      }
+      const float cost = (float)ceil_div(items, a.cus) * (work / (float)items + (float)kPartRows);
+      if (k == 1 || cost < least) {
+        least = cost;
+        rps = unit;
+      }
+    }
+    return rps * kTileRows;
   }
   // units of 32 entries: the fewest that give at most one item per compute unit
   int lo = max(kMinRows / kTileRows, (int)fminf(work / (float)(a.cus * kTileRows), 16777216.f));
@@ -238,9 +248,6 @@ __device__ inline uint8_t* state_o(const PagedArgs& a, int slot) {
 __device__ inline constexpr int units_of(int vi) { return vi == 0 ? 4 : 3; }
 __device__ inline constexpr int first_unit(int vi) { return vi == 0 ? 0 : 1 + 3 * vi; }
 
-// the k-th of a tile's copies that value wave vi makes (the wave with four blocks is dealt last)
-__device__ inline constexpr int dealt(int vi, int k) { return kValueWaves - 1 - vi + kValueWaves * k; }
-
 // What a workgroup works on, the same in all its waves.
 struct Work {
   int slot;    // state slot, -1: the tile's only item
@@ -251,21 +258,36 @@ struct Work {
   int e_begin, e_end, ntiles;
 };
 
-// ---- row copies of one tile, dealt to the value waves (one instruction a row for columns 0..511, one per 8 rows for
-// the rope tails, XOR-swizzled by row)
+// ---- row copies of one tile, dealt to the value waves (one instruction a row for columns 0..511, one per 8 rows for the
+// rope tails, XOR-swizzled by row).  The row numbers are in registers by then (RowIds, read from the ring an
+// iteration before), and a row's address is scalar: a copy costs its wave a few issue slots.
+struct RowIds {
+  int mine, tail;  // of row lane & 31; of the lane's row of this wave's tail copy
+};
+// the k-th copy or fp8 piece of a tile that value wave vi takes (the wave with four blocks is dealt last)
+__device__ inline constexpr int dealt(int vi, int k) { return kValueWaves - 1 - vi + kValueWaves * k; }
 template <class G>
-__device__ inline void issue_tile(const PagedArgs& a, uint32_t lds_base, const lds_i32_t* ids_s, int vi, int lane, int tl) {
+__device__ inline RowIds read_ids(const lds_i32_t* ids_s, int vi, int lane, int tl) {
   const lds_i32_t* id = ids_s + (tl % kIdTiles) * kTileRows;
+  // copies 32 .. 35 are the tails': wave vi has number 32 + t, t = (dealt(vi, 0) - 32) mod 5, if that is below 4
+  const int t = (dealt(vi, 0) + 3) % kValueWaves;
+  return RowIds{max(id[lane & 31], 0), G::TAIL && t < 4 ? max(id[8 * t + (lane >> 3)], 0) : 0};
+}
+template <class G>
+__device__ inline void issue_tile(const PagedArgs& a, uint32_t lds_base, const RowIds& id, int vi, int lane, int tl) {
   const uint32_t tbase = lds_base + (uint32_t)((tl % G::NBUF) * G::TILE_BYTES);
-  auto rowp = [&](int r) { return (const uint8_t*)a.pages + (int64_t)max(id[r], 0) * G::ROWB; };
 #pragma unroll
   for (int k = 0; k < (G::NDMA + kValueWaves - 1) / kValueWaves; k++) {
     const int x = dealt(vi, k);
     if (x < kTileRows) {
-      dma16(rowp(x) + 16 * (lane ^ row_swizzle(x)), __builtin_amdgcn_readfirstlane(tbase + x * 1024));
+      const uint64_t row = (uint64_t)(uintptr_t)a.pages + (uint64_t)(uint32_t)__builtin_amdgcn_readlane(id.mine, x) * G::ROWB;
+      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(tbase + x * 1024),
+                   "v"(16 * (lane ^ row_swizzle(x))), "s"(row)
+                   : "memory", "m0");
     } else if (x < G::NDMA) {
       const int r0 = (x - kTileRows) * 8, r = r0 + (lane >> 3);
-      dma16(rowp(r) + 1024 + 16 * ((lane & 7) ^ (r & 7)), __builtin_amdgcn_readfirstlane(tbase + G::MAIN_BYTES + r0 * 128));
+      dma16((const uint8_t*)a.pages + (int64_t)id.tail * G::ROWB + 1024 + 16 * ((lane & 7) ^ (r & 7)),
+            __builtin_amdgcn_readfirstlane(tbase + G::MAIN_BYTES + r0 * 128));
     }
   }
 }
@@ -347,58 +369,55 @@ __device__ inline void f8_store(lds_u8_t* lds, int vi, int lane, int tl, const F
 }
 
 // ---------------------------------------------------------------------------------------------
-// Score wave `wave` < NB: q rows 32 wave .. + 31.  A tile goes in two halves of 16 rows, and an iteration is half a tile
-// late: it finishes tile i - 1 (second half's products, between which the first half's exponentials are taken, an
-// element a K step) and begins tile i (first half's products, between which tile i - 1's second exponentials are
-// taken and its P written).  The products leave the vector pipe idle three cycles of four, so the softmax costs
-// little beside them, and what an iteration reads first has been in LDS since the one before.
+// Score wave `wave` < NB: q rows 32 wave .. + 31, one to a lane pair (lanes r and r + 32 share q row r and the tile's rows in
+// runs of four).  Iteration i multiplies tile i (D / 16 products of 32 rows x 32 q rows x 16, 32 cycles of the matrix
+// pipe each) and, in the issue slots that the products leave, turns tile i - 1's scores to probabilities and writes
+// them: nothing of the softmax but the look at its maximum, which fills the wait for the first K fragments, stands by itself.
 // Scores are kept in base 2; a maximum further than e^8 above the reference moves the reference, everything else stays
 // below e^8 of it.
 template <class G, int D>
 __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32_t* trow, lds_u8_t* lds, int wave, int lane) {
   lds_i32_t* ids_s = (lds_i32_t*)(lds + G::IDS_OFF);
   lds_f32_t* al_s = (lds_f32_t*)(lds + G::AL_OFF);
-  const int g = lane >> 4, c = lane & 15;
+  constexpr int STEPS = D / 16;
+  const int h = lane >> 5, r = 32 * wave + (lane & 31);  // half, q row of the tile
   const bool idle = 32 * wave >= w.nh;  // no q rows: barriers (and row numbers) only
   constexpr float kLog2e = 1.44269504088896340736f;
   const float c2 = fabsf(a.scale) * kLog2e;
-  // Q^T: q row 32 wave + 16 n + c, K step j: elements 32 j + 8 g .. + 7 (rows past nh read the tile's first);
-  // a negative scale's sign goes into q
-  bf16x8_t qf[2][G::KSTEPS];
-  int eh[2], el[2];
+  // Q^T of q row r, step j: elements 16 j + 8 h .. + 7 (rows past nh read the tile's first); a negative scale's sign goes
+  // into q
+  bf16x8_t qf[STEPS];
+  const int rr = r < w.nh ? r : 0;
+  {
+    const uint8_t* qr = (const uint8_t*)(a.q + (w.row0 + rr) * D) + 16 * h;
 #pragma unroll
-  for (int n = 0; n < 2; n++) {
-    const int r = 32 * wave + 16 * n + c;
-    const int rr = r < w.nh ? r : 0;
-    const uint8_t* qr = (const uint8_t*)(a.q + (w.row0 + rr) * D) + 16 * g;
-#pragma unroll
-    for (int j = 0; j < G::KSTEPS; j++) qf[n][j] = as_bf16x8(__builtin_nontemporal_load((const u32x4_t*)(qr + 64 * j)));
-    // entries that the q row sees: e < eh, and e < first or e >= el
-    const int pc = w.p0 + (int)((uint32_t)(w.m0 + rr) / (uint32_t)a.H);
-    eh[n] = pc + 1 - w.lo + w.nf;
-    el[n] = a.window > 0 ? pc - a.window + 1 - w.lo + w.nf : 0;
+    for (int j = 0; j < STEPS; j++) qf[j] = as_bf16x8(__builtin_nontemporal_load((const u32x4_t*)(qr + 32 * j)));
   }
   if (a.scale < 0.f) {
 #pragma unroll
-    for (int n = 0; n < 2; n++)
-#pragma unroll
-      for (int j = 0; j < G::KSTEPS; j++) qf[n][j] = as_bf16x8(__builtin_bit_cast(u32x4_t, qf[n][j]) ^ 0x80008000u);
+    for (int j = 0; j < STEPS; j++) qf[j] = as_bf16x8(__builtin_bit_cast(u32x4_t, qf[j]) ^ 0x80008000u);
   }
+  // entries that the q row sees: e < eh, and e < first or e >= eh - span
+  const int eh = w.p0 + (int)((uint32_t)(w.m0 + rr) / (uint32_t)a.H) + 1 - w.lo + w.nf;
+  const uint32_t span = a.window > 0 ? (uint32_t)a.window : 0x7fffffffu;
   // entries below eh_all and outside [first, el_all) are seen by every q row of the tile
   const int eh_all = w.p_lo + 1 - w.lo + w.nf, el_all = a.window > 0 ? w.p_hi - a.window + 1 - w.lo + w.nf : 0;
   if (idle) {  // nothing to rescale, and no flags
-    al_s[(lane >> 5) * G::TILEQ + 32 * wave + (lane & 31)] = 1.f;
+    al_s[h * G::TILEQ + r] = 1.f;
     if (lane < 2) *(lds_i32_t*)(lds + G::FLAG_OFF + 16 * lane + 4 * wave) = 0;
   }
-  // K^T of row c: chunk 4 j + g of the main columns (even and odd K steps), chunk 4 (j - 16) + g of the tail
-  const int k_even = 1024 * c + 16 * (g ^ row_swizzle(c)), k_odd = 1024 * c + 16 * ((4 + g) ^ row_swizzle(c));
-  const int t_even = G::MAIN_BYTES + 128 * c + 16 * (g ^ (c & 7)), t_odd = G::MAIN_BYTES + 128 * c + 16 * ((4 + g) ^ (c & 7));
-  // m_ref: the reference (-inf: none yet); m_sub: what is taken off a score (0 without a reference)
-  float m_ref[2] = {-SMLA_INF, -SMLA_INF}, m_sub[2] = {0.f, 0.f}, l_lane[2] = {0.f, 0.f};
+  // K of row lane & 31, step j: chunk 2 j + h of the main columns, 2 (j - 32) + h of the tail; the swizzle only turns bits,
+  // so a step's address is step 0's xor 32 (j mod 8) (j mod 4 in the tail), and 256 (j / 8) on
+  const uint32_t k_at = (uint32_t)(uintptr_t)lds + 1024 * (lane & 31) + 16 * (h ^ row_swizzle(lane & 31));
+  const uint32_t t_at = (uint32_t)(uintptr_t)lds + G::MAIN_BYTES + 128 * (lane & 31) + 16 * (h ^ (lane & 7));
+  // the reference; below every score while there is none (exponentials of -inf against it are 0, and the first score seen
+  // is past it)
+  constexpr float kSlack = kRescaleSlack * kLog2e;
+  float m_ref = -3e38f, l_lane = 0.f;
   // the row number of tile 7's entry lane & 31 as column and place in its page, and 32 rows' step
   int col = 0, off = 0, page = -1;
   const int step_col = (int)((uint32_t)kTileRows / (uint32_t)a.P), step_off = kTileRows - step_col * a.P;
-  {
+  if (wave == 0) {
     const int e = w.e_begin + (kIdTiles - 1) * kTileRows + (lane & 31), j = e < w.nf ? e : w.lo + (e - w.nf);
     col = (int)((uint32_t)j / (uint32_t)a.P);
     off = j - col * a.P;
@@ -428,157 +447,134 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
       if (e < w.e_end) page = trow[col];
     }
   };
-  bool odd = false;               // a masked score of the tile is not finite
-  float alpha[2] = {1.f, 1.f};    // e^(old - new reference) of the tile's q rows
-  float cm = 1.f;                 // what turns the tile's scores to base 2 (c2; 1: masked, and scaled, already)
-  f32x4_t s0[2], s1[2];           // scores of the halves
-  float p[2][8];
-  constexpr int PF = G::TAIL ? 6 : 4;  // fragments read ahead (a divisor of a half's K steps)
-  static_assert(G::KSTEPS % PF == 0, "a half's fragments start at kf[0]");
-  u32x4_t kf[PF];
-  // K step j of half h of a tile
-  auto ldk = [&](const lds_u8_t* buf, int h, int j) -> u32x4_t {
-    if (!G::TAIL || j < 16) return *(const lds_u32x4_t*)(buf + ((j & 1) ? k_odd : k_even) + 16 * 1024 * h + 128 * (j >> 1));
-    return *(const lds_u32x4_t*)(buf + ((j & 1) ? t_odd : t_even) + 16 * 128 * h);
-  };
-  auto tile_at = [&](int i) { return lds + (i % G::NBUF) * G::TILE_BYTES; };
-  // scores of a half where some q row does not see some row: scaled, -inf there
-  auto mask = [&](f32x4_t (&s)[2], int i, int h) {
-    const i32x4_t v = *(const lds_i32x4_t*)(ids_s + (i % kIdTiles) * kTileRows + 16 * h + 4 * g);
-    const int e1 = w.e_begin + i * kTileRows + 16 * h + 4 * g;
+  // scores of a tile of which some q row does not see some row: scaled, -inf there
+  auto mask = [&](f32x16_t& s, int i) -> bool {
+    bool odd = false;  // a masked score is not finite
+    const lds_i32_t* id = ids_s + (i % kIdTiles) * kTileRows + 4 * h;
+    const int e0 = w.e_begin + i * kTileRows + 4 * h;
 #pragma unroll
-    for (int n = 0; n < 2; n++)
+    for (int q = 0; q < 4; q++) {
+      const i32x4_t v = *(const lds_i32x4_t*)(id + 8 * q);
 #pragma unroll
       for (int k = 0; k < 4; k++) {  // (without branches)
-        const bool ok = (v[k] >= 0) & (e1 + k < eh[n]) & ((e1 + k < a.first) | (e1 + k >= el[n]));
-        odd |= !ok & !(fabsf(s[n][k]) < SMLA_INF);
-        const float x = s[n][k] * c2;
-        s[n][k] = ok ? x : -SMLA_INF;
-      }
-  };
-  // moves the references where a score is past them: factor[n] = e^(old - new)
-  auto raise = [&](const f32x4_t (&s)[2], float (&factor)[2]) -> bool {
-    float top[2];
-#pragma unroll
-    for (int n = 0; n < 2; n++) top[n] = fmaxf(fmaxf(s[n][0], s[n][1]), fmaxf(s[n][2], s[n][3])) * cm;
-    constexpr float kSlack = kRescaleSlack * kLog2e;
-    if (__builtin_amdgcn_ballot_w64(top[0] > m_ref[0] + kSlack || top[1] > m_ref[1] + kSlack) == 0) return false;
-#pragma unroll
-    for (int n = 0; n < 2; n++) {
-      const float x = rows4_reduce(top[n], [](float x, float y) { return fmaxf(x, y); });
-      factor[n] = 1.f;
-      if (x > m_ref[n] + kSlack) {
-        factor[n] = m_ref[n] > -SMLA_INF ? __builtin_amdgcn_exp2f(m_ref[n] - x) : 0.f;
-        l_lane[n] *= factor[n];
-        m_ref[n] = m_sub[n] = x;
+        const int e = e0 + 8 * q + k;
+        const float x = s[4 * q + k];
+        const bool ok = (v[k] >= 0) & (e < eh) & ((e < a.first) | (e >= (int)((uint32_t)eh - span)));
+        odd |= !ok & !(fabsf(x) < SMLA_INF);
+        s[4 * q + k] = ok ? x * c2 : -SMLA_INF;
       }
     }
-    return true;
+    return odd;
   };
-  // the products of one half (h of tile buf's rows) into s; `between` j runs after K step j's, and the fragments that
-  // follow (of half nh of tile next) are read ahead
-  auto products = [&](f32x4_t (&s)[2], const lds_u8_t* buf, int h, const lds_u8_t* next, int nh, auto&& between) {
+  // whether every q row of the tile sees every row of tile i (its row numbers v are all there)
+  auto is_open = [&](int i, const i32x4_t& v) -> bool {
+    const int e0 = w.e_begin + i * kTileRows;
+    return e0 + kTileRows <= eh_all && (e0 >= el_all || e0 + kTileRows <= a.first) &&
+           __builtin_amdgcn_ballot_w64(min(min(v[0], v[1]), min(v[2], v[3])) < 0) == 0;
+  };
+  auto ids_of = [&](int i) { return *(const lds_i32x4_t*)(ids_s + (i % kIdTiles) * kTileRows + 4 * (lane & 7)); };
+  constexpr int PF = G::TAIL ? 5 : 8;  // fragments read ahead
+  u32x4_t kf[PF];
+  auto ldk = [&](uint32_t buf, int j) -> u32x4_t {
+    const uint32_t at = !G::TAIL || j < 32 ? ((buf + k_at) ^ (32 * (j & 7))) + 256 * (j >> 3) : (buf + t_at) ^ (32 * (j & 3));
+    return *(const lds_u32x4_t*)(uintptr_t)at;
+  };
+  // the products of tile i; `between` j runs after step j's
+  auto products = [&](f32x16_t& s, int i, auto&& before, auto&& between) {
+    const uint32_t buf = (uint32_t)((i % G::NBUF) * G::TILE_BYTES);
 #pragma unroll
-    for (int n = 0; n < 2; n++) s[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < PF; j++) kf[j] = ldk(buf, j);
+#pragma unroll
+    for (int k = 0; k < 16; k++) s[k] = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
+    before();
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int j = 0; j < G::KSTEPS; j++) {
+    for (int j = 0; j < STEPS; j++) {
       const bf16x8_t k = as_bf16x8(kf[j % PF]);
-      kf[j % PF] = j + PF < G::KSTEPS ? ldk(buf, h, j + PF) : ldk(next, nh, j + PF - G::KSTEPS);
-#pragma unroll
-      for (int n = 0; n < 2; n++) s[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[n][j], s[n], 0, 0, 0);
+      if (j + PF < STEPS) kf[j % PF] = ldk(buf, j + PF);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[j], s, 0, 0, 0);
       between(j);
       __builtin_amdgcn_sched_barrier(0);  // keep the reads PF steps ahead of their products
     }
   };
-  // first half of tile i: its products, then masks and references
-  auto first_half = [&](int i, auto&& between) {
-    products(s0, tile_at(i), 0, tile_at(i), 1, between);
-    const i32x4_t v0 = *(const lds_i32x4_t*)(ids_s + (i % kIdTiles) * kTileRows + 4 * (lane & 7));
-    const int least = min(min(v0[0], v0[1]), min(v0[2], v0[3])), e0 = w.e_begin + i * kTileRows;
-    const bool open = e0 + kTileRows <= eh_all && (e0 >= el_all || e0 + kTileRows <= a.first) &&
-                      __builtin_amdgcn_ballot_w64(least < 0) == 0;
-    cm = open ? c2 : 1.f;
-    odd = false;
-    alpha[0] = alpha[1] = 1.f;
-    if (!open) mask(s0, i, 0);
-    raise(s0, alpha);
-    return open;
-  };
-  auto expo = [&](const f32x4_t (&s)[2], int h, float scale, int x) {
-    const int n = x >> 2, k = x & 3;
-    p[n][4 * h + k] = __builtin_amdgcn_exp2f(s[n][k] * scale - m_sub[n]);
-    l_lane[n] += p[n][4 * h + k];
-  };
-  // P and the rescale factors of tile i - 1, written while the next tile's first products run
-  auto put = [&](int i, int part) {
-    const int n = part >> 1, r = 32 * wave + 16 * n + c;
-    lds_u8_t* pb = lds + G::P_OFF + (i & 1) * G::PBUF + 8 * (g & 1);
-    if ((part & 1) == 0)
-      *(lds_u32x2_t*)(pb + p_at(r, g >> 1)) = u32x2_t{pack2(p[n][0], p[n][1]), pack2(p[n][2], p[n][3])};
-    else
-      *(lds_u32x2_t*)(pb + p_at(r, 2 + (g >> 1))) = u32x2_t{pack2(p[n][4], p[n][5]), pack2(p[n][6], p[n][7])};
-  };
-  auto put_alpha = [&](int i, float al0, float al1, bool flag) {
-    al_s[(i & 1) * G::TILEQ + 32 * wave + (lane & 31)] = (lane & 16) ? al1 : al0;
-    const uint64_t any = __builtin_amdgcn_ballot_w64(flag);
-    if (lane == 0) *(lds_i32_t*)(lds + G::FLAG_OFF + 16 * (i & 1) + 4 * wave) = any != 0;
-  };
   bool open = false;
-  // the compiler's own count: no load is in flight from here on but row_numbers' one, so the loop waits for none
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-  if (!idle && w.ntiles > 0) {
+  // Iteration i: tile i's products into `now`, tile i - 1's scores `old` to P.
+  auto iteration = [&](int i, f32x16_t& now, f32x16_t& old) {
+    const bool more = i < w.ntiles;
+    const float cm = open ? c2 : 1.f;  // what turns tile i - 1's scores to base 2 (1: masked, and scaled, already)
+    float alpha = 1.f;                 // e^(old - new reference)
+    bool odd = false;
+    if (!open) odd = mask(old, i - 1);
+    auto look = [&]() {  // the reference moves to the tile's maximum where that is past it
+      float x = fmaxf(old[0], old[1]);
 #pragma unroll
-    for (int j = 0; j < PF; j++) kf[j] = ldk(tile_at(0), 0, j);
-    open = first_half(0, [](int) {});
-  }
-  lds_barrier();
-  for (int i = 1; i <= w.ntiles; i++) {
-    if (!idle) {
-      const bool more = i < w.ntiles;
-      products(s1, tile_at(i - 1), 1, tile_at(i), 0, [&](int j) {
-        if (j < 8) expo(s0, 0, cm, j);
-        if (j == 9) row_numbers(i);
-      });
-      if (!open) mask(s1, i - 1, 1);
-      float later[2];
-      if (raise(s1, later)) {  // the first half's were taken against the old reference
-#pragma unroll
-        for (int n = 0; n < 2; n++) {
-          alpha[n] *= later[n];
-#pragma unroll
-          for (int x = 0; x < 4; x++) p[n][x] *= later[n];
+      for (int k = 2; k < 16; k += 2) x = fmaxf(fmaxf(x, old[k]), old[k + 1]);
+      x *= cm;
+      if (__builtin_amdgcn_ballot_w64(x > m_ref + kSlack)) {
+        const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+        if (x > m_ref + kSlack) {
+          alpha = __builtin_amdgcn_exp2f(m_ref - x);
+          l_lane *= alpha;
+          m_ref = x;
         }
       }
-      const float al0 = alpha[0], al1 = alpha[1], cm1 = cm;
-      const bool flag = odd;
-      if (more) {
-        open = first_half(i, [&](int j) {
-          if (j < 8) expo(s1, 1, cm1, j);
-          if (j >= 8 && j < 12) put(i - 1, j - 8);
-          if (j == 12) put_alpha(i - 1, al0, al1, flag);
-        });
-      } else {
+    };
+    auto expo = [&](int k) { old[k] = __builtin_amdgcn_exp2f(old[k] * cm - m_ref); };
+    auto put = [&](int q) {
+      l_lane += (old[4 * q] + old[4 * q + 1]) + (old[4 * q + 2] + old[4 * q + 3]);
+      *(lds_u32x2_t*)(lds + G::P_OFF + ((i - 1) & 1) * G::PBUF + p_at(r, q) + 8 * h) =
+          u32x2_t{pack2(old[4 * q], old[4 * q + 1]), pack2(old[4 * q + 2], old[4 * q + 3])};
+    };
+    auto put_alpha = [&]() {
+      al_s[((i - 1) & 1) * G::TILEQ + r] = alpha;
+      const uint64_t any = __builtin_amdgcn_ballot_w64(odd);
+      if (lane == 0) *(lds_i32_t*)(lds + G::FLAG_OFF + 16 * ((i - 1) & 1) + 4 * wave) = any != 0;
+    };
+    if (more) {
+      i32x4_t v;
+      bool next = false;
+      products(now, i, look, [&](int j) {
+        if (j < 16) expo(j);
+        if (j >= 16 && j < 24 && (j & 1) == 0) put((j - 16) / 2);
+        if (j == 24) put_alpha();
+        if (j == 25) v = ids_of(i);
+        if (j == 26) row_numbers(i);
+        if (j == 29) next = is_open(i, v);
+      });
+      open = next;
+    } else {
+      look();
 #pragma unroll
-        for (int x = 0; x < 8; x++) expo(s1, 1, cm1, x);
+      for (int k = 0; k < 16; k++) expo(k);
 #pragma unroll
-        for (int x = 0; x < 4; x++) put(i - 1, x);
-        put_alpha(i - 1, al0, al1, flag);
-      }
+      for (int q = 0; q < 4; q++) put(q);
+      put_alpha();
     }
+  };
+  // the compiler's own count: no load is in flight from here on but row_numbers' one, so the loop waits for none
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  f32x16_t s0, s1;
+  if (!idle && w.ntiles > 0) {
+    open = is_open(0, ids_of(0));
+    products(s0, 0, [] {}, [](int) {});
+  }
+  lds_barrier();
+  for (int i = 1; i <= w.ntiles; i += 2) {
+    if (!idle) iteration(i, s1, s0);
+    lds_barrier();
+    if (i + 1 > w.ntiles) break;
+    if (!idle) iteration(i + 1, s0, s1);
     lds_barrier();
   }
   lds_barrier();  // (the value waves' last tile)
   // (m, l): for the value waves' final scaling, or the state's
-#pragma unroll
-  for (int n = 0; n < 2; n++) {
-    const float l = rows4_reduce(l_lane[n], [](float x, float y) { return x + y; });
-    const int r = 32 * wave + 16 * n + c;
-    if (g == 0) {
-      if (w.slot >= 0) *(f32x2_t*)(state_f<G>(a, w.slot) + 2 * r) = f32x2_t{m_ref[n], l};
-      al_s[2 * r] = m_ref[n];
-      al_s[2 * r + 1] = l;
-    }
+  const float l = l_lane + __shfl_xor(l_lane, 32, 64);
+  if (h == 0) {
+    if (w.slot >= 0) *(f32x2_t*)(state_f<G>(a, w.slot) + 2 * r) = f32x2_t{m_ref, l};
+    al_s[2 * r] = m_ref;
+    al_s[2 * r + 1] = l;
   }
   lds_barrier();
 }
@@ -593,6 +589,7 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
   const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
   const int nb = (w.nh + 31) / 32;  // blocks of q rows in use (the others' products are not stored)
   const int my_dma = (G::NDMA - dealt(vi, 0) + kValueWaves - 1) / kValueWaves;
+  RowIds ids{0, 0};  // of the next tile to request
   f32x16_t o[NU][NB];
 #pragma unroll
   for (int u = 0; u < NU; u++)
@@ -601,16 +598,14 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
 #pragma unroll
       for (int r = 0; r < 16; r++) o[u][n][r] = 0.f;
   // V^T provider address inside a 16-row step: group j = lane >> 4 covers value columns 16 (j & 1) .. of a block and
-  // rows 8 (j >> 1) ..; lane J = lane & 15 supplies row J >> 2, columns 4 (J & 3) .. + 3.  Two blocks on, the swizzle is the
-  // same: blocks u and u + 2 lie 128 bytes apart
+  // rows 8 (j >> 1) ..; lane J = lane & 15 supplies row J >> 2, columns 4 (J & 3) .. + 3.  Of a block's chunk the swizzle
+  // turns the number in its group of four (alike in all blocks) and, by the row's two low bits, the block's place
+  // among four
   const int vj = lane >> 4, vJ = lane & 15;
-  int tr_lo[2], tr_hi[2];  // rows vJ >> 2 and 4 + (vJ >> 2) of each eight
-#pragma unroll
-  for (int u = 0; u < 2; u++) {
-    const int row = 8 * (vj >> 1) + (vJ >> 2), ch = 4 * (u0 + u) + 2 * (vj & 1) + ((vJ & 3) >> 1);
-    tr_lo[u] = 1024 * row + 16 * (ch ^ row_swizzle(row)) + 8 * (vJ & 1);
-    tr_hi[u] = 1024 * (row + 4) + 16 * (ch ^ row_swizzle(row + 4)) + 8 * (vJ & 1);
-  }
+  const int tr_row = 8 * (vj >> 1) + (vJ >> 2), tr_ch = 2 * (vj & 1) + ((vJ & 3) >> 1);
+  const int tr_lo = 1024 * tr_row + 16 * (tr_ch ^ (row_swizzle(tr_row) & 3)) + 8 * (vJ & 1);  // rows vJ >> 2 of each eight
+  const int tr_hi = 1024 * (tr_row + 4) + 16 * (tr_ch ^ (row_swizzle(tr_row + 4) & 3)) + 8 * (vJ & 1);  // 4 + (vJ >> 2)
+  const int tr_turn = 64 * (vJ >> 2);
   int pr[2];  // chunk 2 ks + (lane >> 5) of q row lane & 31 (+ 32 n)
 #pragma unroll
   for (int ks = 0; ks < 2; ks++) pr[ks] = p_at(lane & 31, 2 * ks + (lane >> 5));
@@ -623,7 +618,9 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
       if (w.ntiles > 1) f8_load<D>(a, ids_s, vi, lane, 1, f8);
     }
   } else {
-    for (int tl = 0; tl < min(w.ntiles, G::NBUF); tl++) issue_tile<G>(a, lds_base, ids_s, vi, lane, tl);
+    for (int tl = 0; tl < min(w.ntiles, G::NBUF); tl++)
+      issue_tile<G>(a, lds_base, read_ids<G>(ids_s, vi, lane, tl), vi, lane, tl);
+    if (G::NBUF < w.ntiles) ids = read_ids<G>(ids_s, vi, lane, G::NBUF);
     wait_vm(max(0, min(G::NBUF, w.ntiles) - 1) * my_dma);  // tile 0 has landed
   }
   lds_barrier();
@@ -636,7 +633,10 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
         if (i + 2 < w.ntiles) f8_load<D>(a, ids_s, vi, lane, i + 2, f8);
       }
     } else {
-      if (i >= 3 && i + 1 < w.ntiles) issue_tile<G>(a, lds_base, ids_s, vi, lane, i + 1);
+      if (i >= 3 && i + 1 < w.ntiles) {
+        issue_tile<G>(a, lds_base, ids, vi, lane, i + 1);
+        if (i + 2 < w.ntiles) ids = read_ids<G>(ids_s, vi, lane, i + 2);
+      }
     }
     if (i >= 2) {
       const int tp = i - 2;  // its P was written in the last iteration
@@ -644,11 +644,11 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
       const lds_u8_t* pbuf = lds + G::P_OFF + (tp & 1) * G::PBUF;
       // step st: rows 16 (st / NU) .. + 15, block st % NU; V^T is read AHEAD steps early
       constexpr int AHEAD = NU * NB < 12 ? 2 : 1;  // (192 accumulators leave room for one)
-      const lds_u8_t *lo0 = buf + tr_lo[0], *lo1 = buf + tr_lo[1], *hi0 = buf + tr_hi[0], *hi1 = buf + tr_hi[1];
+      const lds_u8_t *vlo = buf + tr_lo, *vhi = buf + tr_hi;
       auto ldv = [&](int st) -> u32x4_t {
-        const int u = st % NU, at = 16 * 1024 * (st / NU) + 128 * (u >> 1);
-        const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(((u & 1) ? lo1 : lo0) + at));
-        const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(((u & 1) ? hi1 : hi0) + at));
+        const int u = u0 + st % NU, at = 16 * 1024 * (st / NU), block = ((64 * (u & 3)) ^ tr_turn) + 256 * (u >> 2);
+        const v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vlo + block + at));
+        const v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(vhi + block + at));
         return __builtin_bit_cast(u32x4_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
       };
       auto ldp = [&](int ks, int n) { return as_bf16x8(*(const lds_u32x4_t*)(pbuf + pr[ks] + 32 * 64 * n)); };
@@ -768,7 +768,7 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
 template <int D, int NB, bool FP8>
 __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedArgs a) {
   using G = GeoP<D, NB>;
-  extern __shared__ __align__(16) uint8_t lds_generic[];
+  extern __shared__ __align__(256) uint8_t lds_generic[];
   lds_u8_t* lds = (lds_u8_t*)lds_generic;
   lds_i32_t* ids_s = (lds_i32_t*)(lds + G::IDS_OFF);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -796,8 +796,9 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedArgs
   const int64_t cap = (int64_t)a.cols * a.P;
   const int top = (int)min((int64_t)w.p_hi + 1, cap);  // rows below it
   const int entries = max(0, top - w.lo + w.nf);
-  w.e_begin = it.split * rps;
-  w.e_end = min(entries, w.e_begin + rps);
+  const int part = ceil_div(ceil_div(it.s.span, it.nsplit), kTileRows) * kTileRows;
+  w.e_begin = (int)min((int64_t)it.split * part, (int64_t)entries);
+  w.e_end = min(entries, w.e_begin + part);
   w.ntiles = w.e_end > w.e_begin ? (w.e_end - w.e_begin + kTileRows - 1) / kTileRows : 0;
   const int32_t* trow = a.table + it.b * a.ld_table;
   if (tid < kIdTiles * kTileRows) {  // the first eight tiles' row numbers
@@ -926,9 +927,18 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
 }
 
 // Tiles that T tokens of B sequences can make, and the state slots that their plan can use: with at most one
-// item per compute unit one slot each, else two per half share of work.
+// item per compute unit one slot each, else two per half share of work, or the parts that long tiles may be cut into.
 int64_t most_tiles(int64_t T, int64_t H, int64_t B, int nb) { return T * H / (32 * nb) + (B < T ? B : T); }
-int64_t plan_slots(int64_t tiles, int cus) { return tiles <= cus ? cus : 4 * (int64_t)cus + 64; }
+int64_t plan_slots(int64_t tiles, int cus, int64_t span) {
+  if (tiles <= cus) return cus;
+  const int64_t whole = 4 * (int64_t)cus + 64, most = kMostItems * (int64_t)cus, parts = kMostParts * tiles < most ? kMostParts * tiles : most;
+  return span < 2 * kMinPart || parts < whole ? whole : parts;
+}
+// entries that a tile of these calls may visit
+int64_t most_entries(int64_t rows, int64_t window, int64_t first, int64_t H) {
+  const int64_t w = window + first + 128 + H;
+  return window > 0 && w < rows ? w : rows;
+}
 // q rows per tile / 32: where the sequences have no more than 64 on average (steps of one or few tokens, bound by the
 // rows' arrival), tiles of 64 have fewer products to wait for; longer runs of q rows share a row among 96
 int tile_blocks(int64_t T, int64_t H, int64_t B) { return T * H <= 64 * B ? 2 : 3; }
@@ -942,7 +952,8 @@ int launch_paged(const PagedArgs& a, int64_t tiles, hipStream_t st) {
   auto kern = paged_attn_kernel<D, NB, FP8>;
   static std::atomic<uint64_t> lds_attr{0};
   if (hipError_t e = smla_set_dynamic_lds((const void*)kern, G::LDS_BYTES, lds_attr); e != hipSuccess) return (int)e;
-  const int64_t grid = tiles <= a.cus ? a.cus : tiles + 2 * (int64_t)a.cus + 64;
+  const int64_t grid = tiles <= a.cus ? a.cus : tiles + a.slots;
+
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * kWaves), G::LDS_BYTES, st, a);
   SMLA_HIP_CHECK_LAUNCH();
   const int64_t pieces = tiles * kUnits * NB * 2, most = 8 * (int64_t)a.cus;
@@ -955,13 +966,14 @@ int launch_paged(const PagedArgs& a, int64_t tiles, hipStream_t st) {
 }  // namespace
 }  // namespace smla_attn
 
-extern "C" size_t smla_paged_attn_workspace(int64_t T, int64_t H, int64_t B) {
+extern "C" size_t smla_paged_attn_workspace(int64_t T, int64_t H, int64_t B, int64_t rows, int64_t window,
+                                            int64_t first) {
   using namespace smla_attn;
-  if (!plan_sizes(T, H, B)) return 0;
+  if (!plan_sizes(T, H, B) || rows < 0 || window < 0 || first < 0) return 0;
   const int nb = tile_blocks(T, H, B);
   const int64_t state = nb == 2 ? GeoP<512, 2>::STATE_O + 4 * GeoP<512, 2>::STATE_F
                                 : GeoP<512, 3>::STATE_O + 4 * GeoP<512, 3>::STATE_F;
-  return (size_t)(kHeader + plan_slots(most_tiles(T, H, B, nb), smla_num_cus()) * state);
+  return (size_t)(kHeader + plan_slots(most_tiles(T, H, B, nb), smla_num_cus(), most_entries(rows, window, first, H)) * state);
 }
 
 extern "C" int smla_paged_attn(const void* q, int q_dtype, const void* pages, int page_dtype, const float* page_scales,
@@ -981,7 +993,7 @@ extern "C" int smla_paged_attn(const void* q, int q_dtype, const void* pages, in
   if (window < 0 || first < 0 || window > 0x3fffffff || first > 0x3fffffff || (flags & ~SMLA_PAGED_FILL)) return SMLA_E_RANGE;
   if (!plan_sizes(T, H, B) || n_pages > 0x7fffffff || P > 0x7fffffff || n_pages * P > 0x7fffffff || cols > 0x7fffffff)
     return SMLA_E_RANGE;
-  if (!usable_workspace(workspace, workspace_bytes, smla_paged_attn_workspace(T, H, B))) return SMLA_E_WORKSPACE;
+  if (!usable_workspace(workspace, workspace_bytes, smla_paged_attn_workspace(T, H, B, cols * P, window, first))) return SMLA_E_WORKSPACE;
   if (T == 0) return SMLA_OK;
   PagedArgs a{};
   a.q = (const uint16_t*)q;
@@ -1007,7 +1019,7 @@ extern "C" int smla_paged_attn(const void* q, int q_dtype, const void* pages, in
   a.scale = scale;
   const int nb = tile_blocks(T, H, B);
   const int64_t tiles = most_tiles(T, H, B, nb);
-  a.slots = (int)plan_slots(tiles, a.cus);
+  a.slots = (int)plan_slots(tiles, a.cus, most_entries(cols * P, window, first, H));
   const hipStream_t st = (hipStream_t)stream;
   const bool fp8 = page_dtype == SMLA_FP8_E4M3;
 #define SMLA_PAGED(DD, NB) return fp8 ? launch_paged<DD, NB, true>(a, tiles, st) : launch_paged<DD, NB, false>(a, tiles, st)

@@ -77,7 +77,7 @@ _SIGNATURES = {
                               _i64, _vp, _vp, _int, _vp, _sz, _vp]),
     "smla_o_proj": (_int, [_vp, _int, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _int,
                            _i64, _vp, _vp, _int, _vp]),
-    "smla_paged_attn_workspace": (_sz, [_i64] * 3),
+    "smla_paged_attn_workspace": (_sz, [_i64] * 6),
     "smla_paged_attn": (_int, [_vp, _int, _vp, _int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
                                _i64, _f32, _vp, _i64, _i64, _int, _vp, _int, _vp, _sz, _vp]),
     "smla_paged_append": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _f32,

@@ -1035,7 +1035,7 @@ def _paged_attn_(q: torch.Tensor, pages: torch.Tensor, page_scales: Optional[tor
         return
     if not q.is_contiguous():
         q = q.contiguous()
-    wsb = _lib.lib().smla_paged_attn_workspace(T, H, B)
+    wsb = _lib.lib().smla_paged_attn_workspace(T, H, B, table.shape[1] * pages.shape[1], window, first)
     ws = torch.empty(wsb, dtype=torch.uint8, device=q.device)
     _launch(q, "smla_paged_attn", q.data_ptr(), _lib.BF16, pages.data_ptr(), code, _p(page_scales), pages.shape[0],
             pages.shape[1], table.data_ptr(), table.stride(0), table.shape[1], lens.data_ptr(), cu.data_ptr(), B, T, H, D,

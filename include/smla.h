@@ -545,8 +545,9 @@ enum { SMLA_PAGED_NORM_Q = 1, SMLA_PAGED_NORM_KV = 2, SMLA_PAGED_FILL = 4 };
  * flags: 0 or SMLA_PAGED_FILL.  q, pages, out and workspace 16-byte aligned.  Sums and softmax statistics
  * are fp32; probabilities, and the partial sums of tokens whose rows are split over workgroups, are
  * rounded to bf16 before their products and joins.  The result does not depend on the order in which
- * workgroups run.  workspace: smla_paged_attn_workspace(T, H, B) bytes, not shared by calls that overlap. */
-size_t smla_paged_attn_workspace(int64_t T, int64_t H, int64_t B);
+ * workgroups run.  workspace: smla_paged_attn_workspace(T, H, B, rows, window, first) bytes, rows = cols * P, not shared
+ * by calls that overlap. */
+size_t smla_paged_attn_workspace(int64_t T, int64_t H, int64_t B, int64_t rows, int64_t window, int64_t first);
 int smla_paged_attn(const void* q, int q_dtype, const void* pages, int page_dtype, const float* page_scales,
                     int64_t n_pages, int64_t P, const int32_t* table, int64_t ld_table, int64_t cols,
                     const int32_t* lens, const int32_t* cu, int64_t B, int64_t T, int64_t H, int64_t D, int64_t DV,

@@ -121,6 +121,26 @@ def test_attn_more_tiles_than_compute_units(dev):
     _run_attn(dev, [300, 1], [300, 1500], 64, 512, 64, seed=5)
 
 
+def test_attn_long_tiles_in_parts(dev):
+    """Few rounds of long tiles: parts of them go through states, equal to the same tokens asked one by one."""
+    from smla import paged
+    announce("paged_attn 600 tokens of 64 heads over 9000 rows")
+    g = torch.Generator().manual_seed(8)
+    T, L, P = 600, 9000, 64
+    pages = torch.randn(L // P + 4, P, 512, generator=g).to(torch.bfloat16).to(dev)
+    table = torch.randperm(L // P + 4, generator=g)[:-(-L // P)].to(torch.int32)[None].to(dev)
+    q = torch.randn(T, 64, 512, generator=g).to(torch.bfloat16).to(dev)
+    out = paged.paged_attn(q, pages, table, _i32([L], dev), _i32([0, T], dev), 512 ** -0.5)
+    kv = pages[table[0].long()].reshape(-1, 512)[:L].float()
+    for t in (0, 1, 299, 598, 599):
+        n = L - T + t + 1
+        one = paged.paged_attn(q[t:t + 1], pages, table, _i32([n], dev), _i32([0, 1], dev), 512 ** -0.5)[0]
+        p = torch.softmax(q[t].float() @ kv[:n].T * 512 ** -0.5, dim=-1)
+        want = p @ kv[:n]
+        for x in (out[t], one):
+            assert ((x.float() - want).norm(dim=-1) <= 3 * BF16 * want.norm(dim=-1)).all(), t
+
+
 @pytest.mark.parametrize("window,first", [(1, 0), (1, 1), (8, 0), (8, 4), (40, 37), (128, 4), (64, 500), (1000, 2), (1 << 29, 1 << 29)])
 @pytest.mark.parametrize("H", [16, 64])
 def test_attn_window_and_first_rows(dev, window, first, H):

@@ -97,9 +97,11 @@ def test_compact_pages_arguments(change, status):
 def test_workspace_sizes():
     from smla import _lib
     lib = _lib.lib()
-    assert lib.smla_paged_attn_workspace(-1, 16, 1) == 0 and lib.smla_paged_attn_workspace(1, 0, 1) == 0
-    few, many = lib.smla_paged_attn_workspace(1, 64, 1), lib.smla_paged_attn_workspace(4096, 64, 1)
-    assert 0 < few < many < 1 << 28
+    size = lib.smla_paged_attn_workspace
+    assert size(-1, 16, 1, 64, 0, 0) == size(1, 0, 1, 64, 0, 0) == size(1, 16, 1, -1, 0, 0) == size(1, 16, 1, 64, -1, 0) == 0
+    few, many, long = size(1, 64, 1, 4096, 0, 0), size(4096, 64, 1, 4096, 0, 0), size(4096, 64, 1, 1 << 20, 0, 0)
+    assert 0 < few < many < long < 1 << 29
+    assert size(4096, 64, 1, 1 << 20, 128, 4) == many       # a window keeps the tiles short
     assert lib.smla_update_pages_workspace(0, 1) == 0 and lib.smla_compact_pages_workspace(0) == 0
 
 
