@@ -248,6 +248,9 @@ __device__ inline uint8_t* state_o(const PagedArgs& a, int slot) {
 __device__ inline constexpr int units_of(int vi) { return vi == 0 ? 4 : 3; }
 __device__ inline constexpr int first_unit(int vi) { return vi == 0 ? 0 : 1 + 3 * vi; }
 
+// chunk ch (16 bytes) of output row r where the finished rows are staged (over the ring)
+__device__ inline constexpr int out_at(int r, int ch) { return 1024 * r + 16 * (ch ^ (r & 15)); }
+
 // What a workgroup works on, the same in all its waves.
 struct Work {
   int slot;    // state slot, -1: the tile's only item
@@ -273,6 +276,14 @@ __device__ inline RowIds read_ids(const lds_i32_t* ids_s, int vi, int lane, int 
   const int t = (dealt(vi, 0) + 3) % kValueWaves;
   return RowIds{max(id[lane & 31], 0), G::TAIL && t < 4 ? max(id[8 * t + (lane >> 3)], 0) : 0};
 }
+// 1 KB from a row at a scalar address, chunks swizzled; nt: not kept in the L2
+__device__ inline void copy_row(uint32_t lds_dst, uint64_t row, int x, int lane, bool nt) {
+  const int at = 16 * (lane ^ row_swizzle(x));
+  if (nt)
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds_dst), "v"(at), "s"(row) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_dst), "v"(at), "s"(row) : "memory", "m0");
+}
 template <class G>
 __device__ inline void issue_tile(const PagedArgs& a, uint32_t lds_base, const RowIds& id, int vi, int lane, int tl) {
   const uint32_t tbase = lds_base + (uint32_t)((tl % G::NBUF) * G::TILE_BYTES);
@@ -281,13 +292,26 @@ __device__ inline void issue_tile(const PagedArgs& a, uint32_t lds_base, const R
     const int x = dealt(vi, k);
     if (x < kTileRows) {
       const uint64_t row = (uint64_t)(uintptr_t)a.pages + (uint64_t)(uint32_t)__builtin_amdgcn_readlane(id.mine, x) * G::ROWB;
-      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(tbase + x * 1024),
-                   "v"(16 * (lane ^ row_swizzle(x))), "s"(row)
-                   : "memory", "m0");
+      copy_row(tbase + x * 1024, row, x, lane, false);
     } else if (x < G::NDMA) {
       const int r0 = (x - kTileRows) * 8, r = r0 + (lane >> 3);
       dma16((const uint8_t*)a.pages + (int64_t)id.tail * G::ROWB + 1024 + 16 * ((lane & 7) ^ (r & 7)),
             __builtin_amdgcn_readfirstlane(tbase + G::MAIN_BYTES + r0 * 128));
+    }
+  }
+}
+// the same for 32 rows whose addresses `rowp` gives
+template <class G, class F>
+__device__ inline void copy_rows(uint32_t tbase, int vi, int lane, bool nt, F&& rowp) {
+#pragma unroll
+  for (int k = 0; k < (G::NDMA + kValueWaves - 1) / kValueWaves; k++) {
+    const int x = dealt(vi, k);
+    if (x < kTileRows) {
+      copy_row(tbase + x * 1024, rowp(x), x, lane, nt);
+    } else if (x < G::NDMA) {
+      const int r0 = (x - kTileRows) * 8, r = r0 + (lane >> 3);
+      dma16_nt((const uint8_t*)rowp(r) + 1024 + 16 * ((lane & 7) ^ (r & 7)),
+               __builtin_amdgcn_readfirstlane(tbase + G::MAIN_BYTES + r0 * 128));
     }
   }
 }
@@ -384,19 +408,7 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
   const bool idle = 32 * wave >= w.nh;  // no q rows: barriers (and row numbers) only
   constexpr float kLog2e = 1.44269504088896340736f;
   const float c2 = fabsf(a.scale) * kLog2e;
-  // Q^T of q row r, step j: elements 16 j + 8 h .. + 7 (rows past nh read the tile's first); a negative scale's sign goes
-  // into q
-  bf16x8_t qf[STEPS];
-  const int rr = r < w.nh ? r : 0;
-  {
-    const uint8_t* qr = (const uint8_t*)(a.q + (w.row0 + rr) * D) + 16 * h;
-#pragma unroll
-    for (int j = 0; j < STEPS; j++) qf[j] = as_bf16x8(__builtin_nontemporal_load((const u32x4_t*)(qr + 32 * j)));
-  }
-  if (a.scale < 0.f) {
-#pragma unroll
-    for (int j = 0; j < STEPS; j++) qf[j] = as_bf16x8(__builtin_bit_cast(u32x4_t, qf[j]) ^ 0x80008000u);
-  }
+  const int rr = r < w.nh ? r : 0;  // (rows past nh are the tile's first)
   // entries that the q row sees: e < eh, and e < first or e >= eh - span
   const int eh = w.p0 + (int)((uint32_t)(w.m0 + rr) / (uint32_t)a.H) + 1 - w.lo + w.nf;
   const uint32_t span = a.window > 0 ? (uint32_t)a.window : 0x7fffffffu;
@@ -410,6 +422,20 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
   // so a step's address is step 0's xor 32 (j mod 8) (j mod 4 in the tail), and 256 (j / 8) on
   const uint32_t k_at = (uint32_t)(uintptr_t)lds + 1024 * (lane & 31) + 16 * (h ^ row_swizzle(lane & 31));
   const uint32_t t_at = (uint32_t)(uintptr_t)lds + G::MAIN_BYTES + 128 * (lane & 31) + 16 * (h ^ (lane & 7));
+  auto ldk = [&](uint32_t buf, int j) -> u32x4_t {
+    const uint32_t at = !G::TAIL || j < 32 ? ((buf + k_at) ^ (32 * (j & 7))) + 256 * (j >> 3) : (buf + t_at) ^ (32 * (j & 3));
+    return *(const lds_u32x4_t*)(uintptr_t)at;
+  };
+  // Q^T of q row r, step j: elements 16 j + 8 h .. + 7, from the ring slot that its 32 q rows came to in a tile's layout; a
+  // negative scale's sign goes into q
+  bf16x8_t qf[STEPS];
+#pragma unroll
+  for (int j = 0; j < STEPS; j++) qf[j] = as_bf16x8(ldk((1 + wave) * G::TILE_BYTES, j));
+  if (a.scale < 0.f) {
+#pragma unroll
+    for (int j = 0; j < STEPS; j++) qf[j] = as_bf16x8(__builtin_bit_cast(u32x4_t, qf[j]) ^ 0x80008000u);
+  }
+  lds_barrier();  // Q's slots are free
   // the reference; below every score while there is none (exponentials of -inf against it are 0, and the first score seen
   // is past it)
   constexpr float kSlack = kRescaleSlack * kLog2e;
@@ -475,10 +501,6 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
   auto ids_of = [&](int i) { return *(const lds_i32x4_t*)(ids_s + (i % kIdTiles) * kTileRows + 4 * (lane & 7)); };
   constexpr int PF = G::TAIL ? 5 : 8;  // fragments read ahead
   u32x4_t kf[PF];
-  auto ldk = [&](uint32_t buf, int j) -> u32x4_t {
-    const uint32_t at = !G::TAIL || j < 32 ? ((buf + k_at) ^ (32 * (j & 7))) + 256 * (j >> 3) : (buf + t_at) ^ (32 * (j & 3));
-    return *(const lds_u32x4_t*)(uintptr_t)at;
-  };
   // the products of tile i; `between` j runs after step j's
   auto products = [&](f32x16_t& s, int i, auto&& before, auto&& between) {
     const uint32_t buf = (uint32_t)((i % G::NBUF) * G::TILE_BYTES);
@@ -610,7 +632,12 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
 #pragma unroll
   for (int ks = 0; ks < 2; ks++) pr[ks] = p_at(lane & 31, 2 * ks + (lane >> 5));
   F8<D> f8;
-  // ---- the first copies: every slot (row copies), or tile 0 (fp8, and the next one's codes)
+  // ---- Q rows to ring slots 1 .. NB in a tile's layout, then tile 0 (fp8: and the next one's codes)
+#pragma unroll
+  for (int n = 0; n < NB; n++)
+    if (32 * n < w.nh)
+      copy_rows<G>(lds_base + (1 + n) * G::TILE_BYTES, vi, lane, true,
+                   [&](int x) { return (uint64_t)(uintptr_t)a.q + (uint64_t)(w.row0 + (32 * n + x < w.nh ? 32 * n + x : 0)) * G::ROWB; });
   if constexpr (FP8) {
     if (w.ntiles > 0) {
       f8_load<D>(a, ids_s, vi, lane, 0, f8);
@@ -618,12 +645,16 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
       if (w.ntiles > 1) f8_load<D>(a, ids_s, vi, lane, 1, f8);
     }
   } else {
-    for (int tl = 0; tl < min(w.ntiles, G::NBUF); tl++)
+    if (w.ntiles > 0) issue_tile<G>(a, lds_base, read_ids<G>(ids_s, vi, lane, 0), vi, lane, 0);
+  }
+  wait_vm(0);
+  lds_barrier();
+  lds_barrier();  // the score waves have read Q
+  if constexpr (!FP8) {
+    for (int tl = 1; tl < min(w.ntiles, G::NBUF); tl++)
       issue_tile<G>(a, lds_base, read_ids<G>(ids_s, vi, lane, tl), vi, lane, tl);
     if (G::NBUF < w.ntiles) ids = read_ids<G>(ids_s, vi, lane, G::NBUF);
-    wait_vm(max(0, min(G::NBUF, w.ntiles) - 1) * my_dma);  // tile 0 has landed
   }
-  lds_barrier();
   // Iteration i: the score waves finish tile i - 1 and begin tile i, tile i - 2 is consumed here, and tile i + 1 goes
   // to the slot of tile i - 3, to be there at the iteration's end.
   for (int i = 0; i <= w.ntiles + 1; i++) {
@@ -748,7 +779,6 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
         const float snk = a.sink && r < w.nh ? a.sink[(uint32_t)(w.m0 + r) % (uint32_t)a.H] : -SMLA_INF;
         inv = 1.0f / (L + (snk == -SMLA_INF ? 0.f : __builtin_amdgcn_exp2f(snk * 1.44269504088896340736f - M)));
       }
-      uint8_t* dst = (uint8_t*)(a.out + (w.row0 + r) * 512 + 32 * u0 + 8 * (lane >> 5));
 #pragma unroll
       for (int u = 0; u < NU; u++) {
         uint32_t d[8];
@@ -758,7 +788,7 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
         for (int k = 0; k < 8; k += 4) {
           const auto x0 = __builtin_amdgcn_permlane32_swap(d[k], d[k + 2], false, false);
           const auto x1 = __builtin_amdgcn_permlane32_swap(d[k + 1], d[k + 3], false, false);
-          if (r < w.nh) *(u32x4_t*)(dst + 64 * u + 8 * k) = u32x4_t{x0[0], x1[0], x0[1], x1[1]};
+          *(lds_u32x4_t*)(lds + out_at(r, 4 * (u0 + u) + (k >> 1) + (lane >> 5))) = u32x4_t{x0[0], x1[0], x0[1], x1[1]};
         }
       }
     }
@@ -808,16 +838,22 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedArgs
   lds_barrier();
   if (wave < kFirstValue) {
     if (wave < NB) {
-      lds_barrier();  // tile 0 has landed
+      lds_barrier();  // Q and tile 0 have landed
       score_role<G, D>(a, w, trow, lds, wave, lane);
     } else {
-      for (int i = 0; i < w.ntiles + 4; i++) lds_barrier();
+      for (int i = 0; i < w.ntiles + 5; i++) lds_barrier();
     }
   } else if (wave == kFirstValue) {
     value_role<G, D, FP8, units_of(0)>(a, w, lds, 0, first_unit(0), lane);
   } else {
     value_role<G, D, FP8, units_of(1)>(a, w, lds, wave - kFirstValue, first_unit(wave - kFirstValue), lane);
   }
+  if (w.slot >= 0) return;
+  lds_barrier();  // the rows are staged
+  // the tile's q rows are consecutive rows of out, a kilobyte each; nothing here reads them again
+  uint8_t* dst = (uint8_t*)(a.out + w.row0 * 512) + 16 * lane;
+  for (int r = wave; r < w.nh; r += kWaves)
+    __builtin_nontemporal_store(*(const lds_u32x4_t*)(lds + out_at(r, lane)), (u32x4_t*)(dst + (int64_t)r * 1024));
 }
 
 // ---------------------------------------------------------------------------------------------
