@@ -8,8 +8,8 @@
 //  * paged_append_kernel : per new token, the per-head RMS norm and RoPE of its query heads and the norm,
 //                          RoPE and quantisation of its latent row, written to the row's page.  One wave
 //                          per (token, head) row; nothing is read twice.
-//  * update_plan / update_apply : slot s becomes a copy of slot parent[s] plus grow[s] rows.
-//  * compact_plan / compact_apply : live pages moved to the pool's first ids.
+//  * update_one / update_plan + update_apply : slot s becomes a copy of slot parent[s] plus grow[s] rows.
+//  * compact_one / compact_plan + compact_apply : live pages moved to the pool's first ids.
 #include "smla_internal.h"
 
 namespace {
@@ -199,9 +199,15 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
 // ---------------------------------------------------------------------------------------------
 // pages: shared pieces
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanPages = 8;           // pages per thread of a plan's scan step
+constexpr int kWavePages = 1024;        // most pages of a wave in one step of a scan over refs
+constexpr int kStepPages = kPlanThreads / 64 * kWavePages;
 constexpr int64_t kCopyChunk = 16384;   // bytes of one copy item
-constexpr int kCopyThreads = 256;
+constexpr int kCopyThreads = 256;       // threads that copy an item together
+// One launch does all where every workgroup can plan for itself: inputs are read only, so that all plans agree, and the plan
+// fits the LDS: pools of one scan step, up to 1024 slots, and few enough table entries for one workgroup.  Measured
+// against two launches: 32 slots of 128 entries and 1500 pages 7.2 us (4.6 + 3.3), 300 pages moved together 7.3 us (7.1 + 4.0),
+// 8192 pages 69.7 us (16.5 + 60.3), and a launch less for the host, 3 us.  Larger ones are planned once.
+constexpr int64_t kOneEntries = 32768;
 
 // Exclusive prefix sum of v over the workgroup (16 waves); total: the sum.
 __device__ inline int block_excl(int v, int* red, int& total) {
@@ -221,15 +227,60 @@ __device__ inline int block_excl(int v, int* red, int& total) {
   return before + incl - v;
 }
 
+__device__ inline int wave_id() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
+
+// A wave's share of a scan over refs: `per` pages (a multiple of 64) from base on, a coalesced load and a ballot per 64; bit l of
+// m[k] for page base + 64 k + l: a free page (refs 0) or a live one (refs > 0).  v: the counts, 0 past the pages n.
+constexpr int kBallots = kWavePages / 64;
+template <bool FREE>
+__device__ inline int wave_pages(const int32_t* refs, int64_t n, int64_t base, int per, int (&v)[kBallots],
+                                 uint64_t (&m)[kBallots]) {
+  const int lane = threadIdx.x & 63, left = (int)min(max(n - base, (int64_t)0), (int64_t)per);
+  const int32_t* at = refs + min(base, n - 1);
+  int sum = 0;
+#pragma unroll
+  for (int k = 0; k < kBallots; k++) v[k] = 64 * k + lane < left ? at[64 * k + lane] : 0;
+#pragma unroll
+  for (int k = 0; k < kBallots; k++) {
+    m[k] = __builtin_amdgcn_ballot_w64(FREE ? (v[k] == 0) & (64 * k + lane < left) : v[k] > 0);
+    sum += (int)__builtin_popcountll(m[k]);
+  }
+  return sum;
+}
+// pages of a wave where 16 share n of them (one step)
+__device__ inline int per_wave(int n) { return (n + kPlanThreads - 1) / kPlanThreads * 64; }
+// Sums of a wave-uniform x over the waves before this one (returned) and over all (total).
+__device__ inline int waves_excl(int x, int* red, int& total) {
+  const int wave = wave_id();
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[wave] = x;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; w++) {
+    before += w < wave ? red[w] : 0;
+    total += red[w];
+  }
+  return before;
+}
+// set bits of m below bit k (0 and less: none, 64 and more: all)
+__device__ inline int bits_below(uint64_t m, int64_t k) {
+  return k <= 0 ? 0 : (int)__builtin_popcountll(k >= 64 ? m : m & ((1ull << k) - 1));
+}
+__device__ inline int lane_below(uint64_t m) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
+
 struct Pool {
   uint8_t* base;
   int64_t layer_bytes;
   int64_t page_bytes, row_bytes;
 };
 
-// n bytes by the workgroup, 16 at a time where both sides are aligned (four loads in flight per thread)
+// n bytes by kCopyThreads threads, 16 at a time where both sides are aligned (four loads in flight per thread)
 __device__ inline void copy_span(uint8_t* dst, const uint8_t* src, int64_t n) {
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x % kCopyThreads;
   const uintptr_t mix = (uintptr_t)dst | (uintptr_t)src;
   if ((mix & 15) == 0) {
     const int64_t nv = n / 16;
@@ -278,7 +329,7 @@ struct PageArgs {
 // What slot s asks for: rows of its parent, rows after growing, its whole pages taken from the parent,
 // pages after growing; false: an argument out of range.
 struct SlotNeed {
-  int have, next, full, pages;
+  int have, next, full, pages, parent;
   bool keep;
 };
 __device__ inline bool slot_need(const PageArgs& a, int s, SlotNeed& n) {
@@ -286,6 +337,7 @@ __device__ inline bool slot_need(const PageArgs& a, int s, SlotNeed& n) {
   if (p < -1 || p >= a.S || g < 0) return false;
   n.have = p >= 0 ? a.lens[p] : 0;
   n.keep = p == s;
+  n.parent = p;
   if (n.have < 0 || (int64_t)n.have + g > 0x7fffffff) return false;
   n.next = n.have + g;
   const uint32_t P = (uint32_t)a.P;
@@ -295,16 +347,116 @@ __device__ inline bool slot_need(const PageArgs& a, int s, SlotNeed& n) {
   return pages <= a.M;
 }
 
+// What becomes of slot s: its first fresh rank (-1: refused), the slot it copies, entries it shares with that, entries
+// afterwards and before, rows of a tail page to copy (0: none).
+struct SlotPlan {
+  int at, parent, full, pages, held, tail;
+};
+__device__ inline SlotPlan slot_plan(const PageArgs& a, int s, int at, const SlotNeed& n) {
+  const int len = a.lens[s];
+  return SlotPlan{at, n.parent, n.full, n.pages, len > 0 ? (int)(((uint32_t)len + (uint32_t)a.P - 1) / (uint32_t)a.P) : 0,
+                  n.keep ? 0 : n.have - n.full * a.P};
+}
+// Entry c of slot s after the update, fresh(k) the fresh page of rank k; count(page, by) for every change of a page's holders.
+template <class Fresh, class Count>
+__device__ inline int slot_entry(const PageArgs& a, int s, int c, const SlotPlan& n, Fresh&& fresh, Count&& count) {
+  const int old = a.table[s * a.ld_table + c];
+  if (n.at < 0) return old;
+  const int now = c < n.full ? a.table[n.parent * a.ld_table + c] : c < n.pages ? fresh(n.at + c - n.full) : -1;
+  if (n.parent == s) {
+    if (c >= n.full && c < n.pages) count(now, 1);
+  } else {
+    if (c < n.held) count(old, -1);
+    if (c < n.pages) count(now, 1);
+  }
+  return now;
+}
+// the tail page of a slot: item `part` of layer `layer` of its copy to page dst
+__device__ inline void copy_tail(const PageArgs& a, const SlotPlan& n, int64_t dst, int layer, int64_t part) {
+  const int64_t src = a.table[n.parent * a.ld_table + n.full];
+  if (src < 0 || src >= a.n_pages || src == dst) return;
+  copy_item(a.p0, a.p1, layer, src, dst, n.tail, part, a.parts);
+}
+
 // ---------------------------------------------------------------------------------------------
-// update.  Workspace: [0] copies, [1 .. S] first fresh rank of a granted slot (-1: refused), [1 + S .. 1 + 2S]
-// slots whose tail page is copied, then the fresh pages in rank order.
+// update in one launch.  Every workgroup plans (prefix sums of the pages that slots ask for, and the free pages in
+// ascending order); workgroup 0 writes the tables and counts refs in the LDS (integer sums: any order gives the same), the
+// others copy tail pages, each 256 threads an item at a time.
+struct UpdateLds {
+  int count[kStepPages];
+  uint16_t fresh[kStepPages];
+  SlotPlan slot[kPlanThreads];
+  uint16_t copies[kPlanThreads];
+  int red[kPlanThreads / 64];
+};
+__global__ __launch_bounds__(kPlanThreads) void update_one_kernel(const PageArgs a) {
+  extern __shared__ __align__(16) uint8_t lds_update[];
+  UpdateLds& l = *(UpdateLds*)lds_update;
+  const int tid = threadIdx.x, lane = tid & 63, per = per_wave(a.n_pages), base = wave_id() * per;
+  int v[kBallots];
+  uint64_t m[kBallots];
+  const int mine = wave_pages<true>(a.refs, a.n_pages, base, per, v, m);
+  SlotNeed n;
+  bool ok = tid < a.S && slot_need(a, tid, n);
+  int total, found, ncopy;
+  const int ask = ok ? n.pages - n.full : 0;
+  const int at = block_excl(ask, l.red, total);
+  int free = waves_excl(mine, l.red, found);  // free pages below the wave's next 64
+#pragma unroll
+  for (int k = 0; k < kBallots; k++) {
+    if (64 * k >= per) break;
+    const int rank = free + lane_below(m[k]);
+    if ((m[k] >> lane) & 1) l.fresh[rank] = (uint16_t)(base + 64 * k + lane);
+    free += (int)__builtin_popcountll(m[k]);
+  }
+  ok = ok && at + ask <= found;
+  const bool copy = ok && !n.keep && n.have > n.full * a.P;
+  const int slot = block_excl(copy, l.red, ncopy);
+  if (tid < a.S) l.slot[tid] = ok ? slot_plan(a, tid, at, n) : SlotPlan{-1};
+  if (copy) l.copies[slot] = (uint16_t)tid;
+  if (blockIdx.x > 0) {
+    __syncthreads();
+    const int64_t items = (int64_t)ncopy * a.items_per_copy * a.layers;
+    constexpr int kGroups = kPlanThreads / kCopyThreads;
+    for (int64_t i = (int64_t)(blockIdx.x - 1) * kGroups + tid / kCopyThreads; i < items; i += (int64_t)(gridDim.x - 1) * kGroups) {
+      const int64_t cl = i / a.items_per_copy;
+      const SlotPlan& p = l.slot[l.copies[cl / a.layers]];
+      copy_tail(a, p, l.fresh[p.at], (int)(cl % a.layers), i - cl * a.items_per_copy);
+    }
+    return;
+  }
+  if (tid < a.S) {
+    a.granted[tid] = ok;
+    a.lens_out[tid] = ok ? n.next : a.lens[tid];
+  }
+#pragma unroll
+  for (int k = 0; k < kBallots; k++)
+    if (64 * k < per) l.count[base + 64 * k + lane] = v[k];
+  __syncthreads();
+  const int entries = a.S * a.M;
+#pragma unroll 4
+  for (int i = tid; i < entries; i += kPlanThreads) {
+    const int s = (int)((uint32_t)i / (uint32_t)a.M), c = i - s * a.M;
+    a.table_out[i] = slot_entry(a, s, c, l.slot[s], [&](int k) { return (int)l.fresh[k]; }, [&](int page, int by) {
+      if (page >= 0 && page < a.n_pages) atomicAdd(&l.count[page], by);
+    });
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kBallots; k++) {
+    const int p = base + 64 * k + lane;
+    if (64 * k < per && p < a.n_pages) a.refs_out[p] = l.count[p];
+  }
+}
+
+// In two.  Workspace: [0] copies, [1 .. S] first fresh rank of a granted slot (-1: refused), [1 + S .. 1 + 2S] slots whose
+// tail page is copied, then the fresh pages in rank order.
 //
-// Workgroup 0 plans (prefix sums of the pages that slots ask for, and the free pages in ascending order until there
-// are enough); the others copy refs, which update_apply then counts up and down.
+// Workgroup 0 plans; the others copy refs, which update_apply then counts up and down.
 __global__ __launch_bounds__(kPlanThreads) void update_plan_kernel(const PageArgs a) {
   __shared__ int red[kPlanThreads / 64];
   __shared__ int ncopy;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
   if (blockIdx.x > 0) {
     const int64_t i = (int64_t)(blockIdx.x - 1) * kPlanThreads + tid;
     if (i < a.n_pages) a.refs_out[i] = a.refs[i];
@@ -321,32 +473,31 @@ __global__ __launch_bounds__(kPlanThreads) void update_plan_kernel(const PageArg
     const bool ok = s < a.S && slot_need(a, s, n);
     int sum;
     const int at = block_excl(ok ? n.pages - n.full : 0, red, sum);
-    if (s < a.S) rank[s] = ok ? total + at : -1;
-    total += sum;
+    // (past 31 bits more pages are asked for than there are: refused)
+    const int64_t first = (int64_t)total + at;
+    if (s < a.S) rank[s] = ok && first <= a.n_pages ? (int)first : -1;
+    total = (int)min((int64_t)total + sum, (int64_t)0x3fffffff);
   }
   int found = 0;
-  for (int64_t base = 0; base < a.n_pages && found < total; base += kPlanThreads * kPlanPages) {
-    const int64_t first = base + (int64_t)tid * kPlanPages;
-    int r[kPlanPages], k = 0;
+  for (int64_t step = 0; step < a.n_pages && found < total; step += kStepPages) {
+    const int64_t base = step + wave_id() * kWavePages;
+    int v[kBallots], sum;
+    uint64_t m[kBallots];
+    const int mine = wave_pages<true>(a.refs, a.n_pages, base, kWavePages, v, m);
+    int free = found + waves_excl(mine, red, sum);
 #pragma unroll
-    for (int j = 0; j < kPlanPages; j++) r[j] = first + j < a.n_pages ? a.refs[first + j] : 1;
-#pragma unroll
-    for (int j = 0; j < kPlanPages; j++) k += r[j] == 0;
-    int sum;
-    int at = found + block_excl(k, red, sum);
-#pragma unroll
-    for (int j = 0; j < kPlanPages; j++)
-      if (r[j] == 0) {
-        if (at < total) fresh[at] = (int)(first + j);
-        at++;
-      }
+    for (int k = 0; k < kBallots; k++) {
+      const int at = free + lane_below(m[k]);
+      if (((m[k] >> lane) & 1) && at < total) fresh[at] = (int)(base + 64 * k + lane);
+      free += (int)__builtin_popcountll(m[k]);
+    }
     found += sum;
   }
   __syncthreads();
   for (int s = tid; s < a.S; s += kPlanThreads) {
     SlotNeed n;
     const int at = rank[s];
-    const bool ok = at >= 0 && slot_need(a, s, n) && at + n.pages - n.full <= found;
+    const bool ok = at >= 0 && slot_need(a, s, n) && (int64_t)at + n.pages - n.full <= found;
     if (!ok) rank[s] = -1;
     a.granted[s] = ok;
     a.lens_out[s] = ok ? n.next : a.lens[s];
@@ -356,104 +507,149 @@ __global__ __launch_bounds__(kPlanThreads) void update_plan_kernel(const PageArg
   if (tid == 0) a.ws[0] = ncopy;
 }
 
-// The first `row_blocks` workgroups write the table entries and count refs (integer sums: any order
-// gives the same), the others copy tail pages, an item of kCopyChunk bytes at a time.
+// The first `row_blocks` workgroups write the table entries and count refs, the others copy tail pages, an item of
+// kCopyChunk bytes at a time.
 __global__ __launch_bounds__(kCopyThreads) void update_apply_kernel(const PageArgs a, int row_blocks) {
   const int32_t* rank = a.ws + 1;
   const int32_t* copies = rank + a.S;
   const int32_t* fresh = copies + a.S;
   if ((int)blockIdx.x < row_blocks) {
-    const int64_t n = (int64_t)a.S * a.M;
-    for (int64_t i = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x; i < n; i += (int64_t)row_blocks * kCopyThreads) {
+    const int64_t all = (int64_t)a.S * a.M;
+    for (int64_t i = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x; i < all; i += (int64_t)row_blocks * kCopyThreads) {
       const int s = (int)((uint32_t)i / (uint32_t)a.M), c = (int)((uint32_t)i - (uint32_t)s * (uint32_t)a.M);
+      SlotNeed n;
       const int at = rank[s];
-      const int old = a.table[s * a.ld_table + c];
-      int now = old;
-      if (at >= 0) {
-        SlotNeed sn;
-        slot_need(a, s, sn);
-        now = c < sn.full ? a.table[a.parent[s] * a.ld_table + c] : c < sn.pages ? fresh[at + c - sn.full] : -1;
-        auto count = [&](int page, int by) {
-          if (page >= 0 && page < a.n_pages) atomicAdd(a.refs_out + page, by);
-        };
-        if (sn.keep) {
-          if (c >= sn.full && c < sn.pages) count(now, 1);
-        } else {
-          if ((int64_t)c * a.P < a.lens[s]) count(old, -1);
-          if (c < sn.pages) count(now, 1);
-        }
-      }
-      a.table_out[i] = now;
+      if (at >= 0) slot_need(a, s, n);
+      a.table_out[i] = slot_entry(a, s, c, at >= 0 ? slot_plan(a, s, at, n) : SlotPlan{-1}, [&](int k) { return fresh[k]; }, [&](int page, int by) {
+        if (page >= 0 && page < a.n_pages) atomicAdd(a.refs_out + page, by);
+      });
     }
     return;
   }
   const int64_t items = (int64_t)a.ws[0] * a.items_per_copy * a.layers;
   for (int64_t i = (int64_t)blockIdx.x - row_blocks; i < items; i += (int64_t)gridDim.x - row_blocks) {
-    const int64_t cl = i / a.items_per_copy, part = i - cl * a.items_per_copy;
-    const int s = copies[cl / a.layers], layer = (int)(cl % a.layers);
+    const int64_t cl = i / a.items_per_copy;
+    const int s = copies[cl / a.layers];
     SlotNeed n;
     slot_need(a, s, n);
-    const int64_t src = a.table[a.parent[s] * a.ld_table + n.full], dst = fresh[rank[s]];
-    if (src < 0 || src >= a.n_pages || src == dst) continue;
-    copy_item(a.p0, a.p1, layer, src, dst, n.have - (int64_t)n.full * a.P, part, a.parts);
+    copy_tail(a, slot_plan(a, s, rank[s], n), fresh[rank[s]], (int)(cl % a.layers), i - cl * a.items_per_copy);
   }
 }
 
 // ---------------------------------------------------------------------------------------------
-// compact.  Workspace: [0] live pages, [1] moved pages, then rank [n_pages] (a moving page's or a hole's),
+// compact.  With L live pages, L0 of them below id L: a hole is a free page below L, its rank the free pages below it; a mover
+// a live page from L on, its rank the live pages below it less L0; the mover of a rank goes to the hole of that rank.
+//
+// In one launch: every workgroup plans and copies its share of the pages, each 256 threads an item at a time;
+// workgroup 0 writes refs, and the table's entries are spread over all.
+struct CompactLds {
+  uint16_t to[kStepPages];  // where a page's rows are afterwards (0xffff: not a live page)
+  uint16_t holes[kStepPages / 2], movers[kStepPages / 2];
+  int red[kPlanThreads / 64];
+};
+__global__ __launch_bounds__(kPlanThreads) void compact_one_kernel(const PageArgs a) {
+  extern __shared__ __align__(16) uint8_t lds_compact[];
+  CompactLds& l = *(CompactLds*)lds_compact;
+  const int tid = threadIdx.x, lane = tid & 63, per = per_wave(a.n_pages), base = wave_id() * per;
+  uint64_t m[kBallots];
+  int live, low = 0, mine;
+  {
+    int v[kBallots];
+    mine = wave_pages<false>(a.refs, a.n_pages, base, per, v, m);
+  }
+  const int before = waves_excl(mine, l.red, live);
+#pragma unroll
+  for (int k = 0; k < kBallots; k++)
+    if (64 * k < per) low += bits_below(m[k], live - (base + 64 * k));
+  int l0;
+  waves_excl(low, l.red, l0);
+  int below = before;  // live pages below the wave's next 64
+#pragma unroll
+  for (int k = 0; k < kBallots; k++) {
+    if (64 * k >= per) break;
+    const int p = base + 64 * k + lane, rank = below + lane_below(m[k]);
+    const bool is = (m[k] >> lane) & 1;
+    l.to[p] = (uint16_t)(is ? p : 0xffff);
+    if (is && p >= live) l.movers[rank - l0] = (uint16_t)p;
+    if (!is && p < live) l.holes[p - rank] = (uint16_t)p;
+    below += (int)__builtin_popcountll(m[k]);
+  }
+  const int moved = live - l0;
+  __syncthreads();
+  for (int i = tid; i < moved; i += kPlanThreads) l.to[l.movers[i]] = l.holes[i];
+  const int64_t items = (int64_t)moved * a.items_per_copy * a.layers;
+  constexpr int kGroups = kPlanThreads / kCopyThreads;
+  for (int64_t i = (int64_t)blockIdx.x * kGroups + tid / kCopyThreads; i < items; i += (int64_t)gridDim.x * kGroups) {
+    const int64_t cl = i / a.items_per_copy, at = cl / a.layers;
+    copy_item(a.p0, a.p1, (int)(cl % a.layers), l.movers[at], l.holes[at], a.P, i - cl * a.items_per_copy, a.parts);
+  }
+  __syncthreads();
+  const int64_t n = (int64_t)a.S * a.M;
+  for (int64_t i = (int64_t)blockIdx.x * kPlanThreads + tid; i < n; i += (int64_t)gridDim.x * kPlanThreads) {
+    const uint32_t s = (uint32_t)i / (uint32_t)a.M, c = (uint32_t)i - s * (uint32_t)a.M;
+    const int page = a.table[s * a.ld_table + c];
+    const int to = page >= 0 && page < a.n_pages ? l.to[page] : 0xffff;
+    a.table_out[i] = to == 0xffff ? -1 : to;
+  }
+  if (blockIdx.x > 0) return;
+  if (tid == 0) a.live[0] = live;
+  below = before;
+#pragma unroll
+  for (int k = 0; k < kBallots; k++) {
+    if (64 * k >= per) break;
+    const int p = base + 64 * k + lane, rank = below + lane_below(m[k]);
+    below += (int)__builtin_popcountll(m[k]);
+    if (p >= a.n_pages) continue;
+    const bool is = (m[k] >> lane) & 1;
+    const int r = a.refs[!is && p < live ? l.movers[p - rank] : p];
+    a.refs_out[p] = is && p >= live ? 0 : r;
+  }
+}
+
+// In two.  Workspace: [0] live pages, [1] moved pages, then rank [n_pages] (a moving page's or a hole's),
 // holes [n_pages], movers [n_pages].
 __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(const PageArgs a) {
   __shared__ int red[kPlanThreads / 64];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
   int32_t* rank = a.ws + 2;
   int32_t* holes = rank + a.n_pages;
   int32_t* movers = holes + a.n_pages;
-  int mine = 0;
-  for (int64_t base = 0; base < a.n_pages; base += kPlanThreads * kPlanPages) {
+  int v[kBallots], mine = 0, live;
+  uint64_t m[kBallots];
+  for (int64_t step = 0; step < a.n_pages; step += kStepPages)
+    mine += wave_pages<false>(a.refs, a.n_pages, step + wave_id() * kWavePages, kWavePages, v, m);
+  waves_excl(mine, red, live);
+  int before = 0, l0 = 0;  // live pages of the steps so far; of those, below `live`
+  for (int64_t step = 0; step < a.n_pages; step += kStepPages) {
+    const int64_t base = step + wave_id() * kWavePages;
+    const int here = wave_pages<false>(a.refs, a.n_pages, base, kWavePages, v, m);
+    int sum, lsum, low = 0;
+    int below = before + waves_excl(here, red, sum);
 #pragma unroll
-    for (int j = 0; j < kPlanPages; j++) {
-      const int64_t i = base + (int64_t)j * kPlanThreads + tid;
-      mine += i < a.n_pages && a.refs[i] > 0;
-    }
-  }
-  int live;
-  block_excl(mine, red, live);
-  int before = 0, moved = 0;  // live pages before the step; of those, at live or beyond
-  for (int64_t base = 0; base < a.n_pages; base += kPlanThreads * kPlanPages) {
-    const int64_t first = base + (int64_t)tid * kPlanPages;
-    int r[kPlanPages], k = 0;
+    for (int k = 0; k < kBallots; k++) low += bits_below(m[k], live - (base + 64 * k));
+    waves_excl(low, red, lsum);
+    before += sum;
+    l0 += lsum;  // (all of L0 where the step has a page past `live`)
 #pragma unroll
-    for (int j = 0; j < kPlanPages; j++) r[j] = first + j < a.n_pages ? a.refs[first + j] : 0;
-#pragma unroll
-    for (int j = 0; j < kPlanPages; j++) k += r[j] > 0;
-    int sum;
-    int at = before + block_excl(k, red, sum);  // live pages below the next id
-    int past = 0;                               // moving pages of this thread
-#pragma unroll
-    for (int j = 0; j < kPlanPages; j++) past += r[j] > 0 && first + j >= live;
-    int msum;
-    int mat = moved + block_excl(past, red, msum);
-#pragma unroll
-    for (int j = 0; j < kPlanPages; j++) {
-      const int64_t i = first + j;
-      if (i >= a.n_pages) continue;
-      if (r[j] > 0) {
-        if (i >= live) {
-          rank[i] = mat;
-          movers[mat++] = (int)i;
+    for (int k = 0; k < kBallots; k++) {
+      const int64_t p = base + 64 * k + lane;
+      const int at = below + lane_below(m[k]);
+      below += (int)__builtin_popcountll(m[k]);
+      if (p >= a.n_pages) continue;
+      if ((m[k] >> lane) & 1) {
+        if (p >= live) {
+          rank[p] = at - l0;
+          movers[at - l0] = (int)p;
         }
-        at++;
-      } else if (i < live) {
-        rank[i] = (int)i - at;
-        holes[(int)i - at] = (int)i;
+      } else if (p < live) {
+        rank[p] = (int)p - at;
+        holes[(int)p - at] = (int)p;
       }
     }
-    before += sum;
-    moved += msum;
   }
   if (tid == 0) {
     a.ws[0] = live;
-    a.ws[1] = moved;
+    a.ws[1] = live - l0;
     a.live[0] = live;
   }
 }
@@ -520,7 +716,7 @@ PageArgs page_args(const int32_t* table, int64_t ld_table, int64_t S, int64_t M,
 }
 
 // workgroups of the table part and of the copies: a few per compute unit, each walking its share
-int row_blocks(const PageArgs& a, int64_t n) {
+int row_blocks(int64_t n) {
   const int64_t want = (n + kCopyThreads - 1) / kCopyThreads, most = 2 * smla_num_cus();
   return (int)(want < most ? want : most);
 }
@@ -528,11 +724,23 @@ int copy_blocks(const PageArgs& a, int64_t entries) {
   const int64_t want = entries * a.items_per_copy * a.layers, most = 8 * smla_num_cus();
   return (int)(want < most ? want : most);
 }
+// workgroups of kPlanThreads for the copies of a call in one launch
+int one_blocks(const PageArgs& a, int64_t entries, int64_t most) {
+  const int64_t groups = kPlanThreads / kCopyThreads, want = (entries * a.items_per_copy * a.layers + groups - 1) / groups;
+  return (int)(want < most ? want : most);
+}
+bool update_in_one(int64_t S, int64_t M, int64_t n_pages) {
+  return S <= kPlanThreads && n_pages <= kStepPages && S * M <= kOneEntries;
+}
+bool compact_in_one(int64_t n_pages) { return n_pages <= kStepPages; }
+bool has_workspace(const void* ws, size_t bytes, size_t need) {
+  return need == 0 || (ws && ((uintptr_t)ws & 3) == 0 && bytes >= need);
+}
 
 }  // namespace
 
-extern "C" size_t smla_update_pages_workspace(int64_t S, int64_t n_pages) {
-  return S > 0 && n_pages > 0 ? (size_t)(1 + 2 * S + n_pages) * 4 : 0;
+extern "C" size_t smla_update_pages_workspace(int64_t S, int64_t M, int64_t n_pages) {
+  return S > 0 && M > 0 && n_pages > 0 && !update_in_one(S, M, n_pages) ? (size_t)(1 + 2 * S + n_pages) * 4 : 0;
 }
 
 extern "C" int smla_update_pages(const int32_t* table, int64_t ld_table, int64_t S, int64_t M, const int32_t* lens,
@@ -546,25 +754,33 @@ extern "C" int smla_update_pages(const int32_t* table, int64_t ld_table, int64_t
                          row_bytes, scales, scale_layer_bytes, scale_row_bytes, workspace);
   if (int rc = check_pages(a, S, M, n_pages, P, layers); rc != 0) return rc;
   if (lens_out == lens) return SMLA_E_UNSUPPORTED;
-  if (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < smla_update_pages_workspace(S, n_pages))
-    return SMLA_E_WORKSPACE;
+  if (!has_workspace(workspace, workspace_bytes, smla_update_pages_workspace(S, M, n_pages))) return SMLA_E_WORKSPACE;
   a.lens = lens;
   a.parent = parent;
   a.grow = grow;
   a.lens_out = lens_out;
   a.granted = granted;
   const hipStream_t st = (hipStream_t)stream;
+  if (update_in_one(S, M, n_pages)) {
+    static std::atomic<uint64_t> lds_attr{0};
+    if (hipError_t e = smla_set_dynamic_lds((const void*)update_one_kernel, sizeof(UpdateLds), lds_attr); e != hipSuccess)
+      return (int)e;
+    hipLaunchKernelGGL(update_one_kernel, dim3((unsigned)(1 + one_blocks(a, S, smla_num_cus()))), dim3(kPlanThreads),
+                       sizeof(UpdateLds), st, a);
+    SMLA_HIP_CHECK_LAUNCH();
+    return SMLA_OK;
+  }
   hipLaunchKernelGGL(update_plan_kernel, dim3((unsigned)(1 + (n_pages + kPlanThreads - 1) / kPlanThreads)),
                      dim3(kPlanThreads), 0, st, a);
   SMLA_HIP_CHECK_LAUNCH();
-  const int rb = row_blocks(a, S * M);
+  const int rb = row_blocks(S * M);
   hipLaunchKernelGGL(update_apply_kernel, dim3((unsigned)(rb + copy_blocks(a, S))), dim3(kCopyThreads), 0, st, a, rb);
   SMLA_HIP_CHECK_LAUNCH();
   return SMLA_OK;
 }
 
 extern "C" size_t smla_compact_pages_workspace(int64_t n_pages) {
-  return n_pages > 0 ? (size_t)(2 + 3 * n_pages) * 4 : 0;
+  return n_pages > 0 && !compact_in_one(n_pages) ? (size_t)(2 + 3 * n_pages) * 4 : 0;
 }
 
 extern "C" int smla_compact_pages(const int32_t* table, int64_t ld_table, int64_t S, int64_t M, const int32_t* refs,
@@ -576,13 +792,21 @@ extern "C" int smla_compact_pages(const int32_t* table, int64_t ld_table, int64_
   PageArgs a = page_args(table, ld_table, S, M, refs, n_pages, P, table_out, refs_out, pages, layers, layer_bytes,
                          row_bytes, scales, scale_layer_bytes, scale_row_bytes, workspace);
   if (int rc = check_pages(a, S, M, n_pages, P, layers); rc != 0) return rc;
-  if (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < smla_compact_pages_workspace(n_pages))
-    return SMLA_E_WORKSPACE;
+  if (!has_workspace(workspace, workspace_bytes, smla_compact_pages_workspace(n_pages))) return SMLA_E_WORKSPACE;
   a.live = live;
   const hipStream_t st = (hipStream_t)stream;
+  if (compact_in_one(n_pages)) {
+    static std::atomic<uint64_t> lds_attr{0};
+    if (hipError_t e = smla_set_dynamic_lds((const void*)compact_one_kernel, sizeof(CompactLds), lds_attr); e != hipSuccess)
+      return (int)e;
+    hipLaunchKernelGGL(compact_one_kernel, dim3((unsigned)(1 + one_blocks(a, n_pages / 2, smla_num_cus() - 1))),
+                       dim3(kPlanThreads), sizeof(CompactLds), st, a);
+    SMLA_HIP_CHECK_LAUNCH();
+    return SMLA_OK;
+  }
   hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
   SMLA_HIP_CHECK_LAUNCH();
-  const int rb = row_blocks(a, S * M > n_pages ? S * M : n_pages);
+  const int rb = row_blocks(S * M > n_pages ? S * M : n_pages);
   hipLaunchKernelGGL(compact_apply_kernel, dim3((unsigned)(rb + copy_blocks(a, (n_pages + 1) / 2))),
                      dim3(kCopyThreads), 0, st, a, rb);
   SMLA_HIP_CHECK_LAUNCH();

@@ -170,6 +170,8 @@ __device__ inline int plan_rps(const PagedArgs& a, const Seq& s0, int lane) {
   // units of 32 entries: the fewest that give at most one item per compute unit
   int lo = max(kMinRows / kTileRows, (int)fminf(work / (float)(a.cus * kTileRows), 16777216.f));
   int hi = max(lo, most + (most >> 20) + 1);  // (most went through fp32)
+  // (sum of tiles x ceil(span / rps) <= work / rps + tiles: enough where that fits, two units more for fp32's rounding)
+  if (tiles < a.cus) hi = max(lo, min(hi, (int)fminf(work / (float)((a.cus - tiles) * kTileRows), 16777216.f) + 2));
   while (lo < hi) {
     const int mid = lo + (hi - lo) / 2;
     int items = 0;

@@ -82,7 +82,7 @@ _SIGNATURES = {
                                _i64, _f32, _vp, _i64, _i64, _int, _vp, _int, _vp, _sz, _vp]),
     "smla_paged_append": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _f32,
                                  _int, _int, _vp, _vp, _int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp]),
-    "smla_update_pages_workspace": (_sz, [_i64] * 2),
+    "smla_update_pages_workspace": (_sz, [_i64] * 3),
     "smla_update_pages": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
                                  _i64, _i64, _vp, _i64, _i64, _vp, _sz, _vp]),
     "smla_compact_pages_workspace": (_sz, [_i64]),

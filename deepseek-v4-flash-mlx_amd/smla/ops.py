@@ -951,26 +951,31 @@ def topk_into(scores, k, out, id_offset=0, nvis=None):
 
 # ----------------------------------------------------------------------------------------------
 # The paged latent cache (smla.paged).
-_current_device = torch.cuda.current_device
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # (a tensor is on it: initialised)
 
 
 def _one_device(t, *rest):
     """All tensors on t's GPU (one launch reads them all)."""
-    dev = t.device
-    if dev.type != "cuda":
+    dev = t.get_device()
+    if dev < 0:
         _on_gpu(t)
     for r in rest:
-        if r is not None and r.device != dev:
-            raise RuntimeError(f"smla paged ops run on one GPU: got tensors on {dev} and {r.device}")
+        if r is not None and r.get_device() != dev:
+            raise RuntimeError(f"smla paged ops run on one GPU: got tensors on {t.device} and {r.device}")
 
 
 def _launch(t, name, *args):
     """``_lib.call`` with t's device current (a launch goes to a stream of the current device)."""
-    if _current_device() == t.device.index:
-        _lib.call(name, *args, _stream(t))
+    dev = t.get_device()
+    if _current_device() == dev:
+        _lib.call(name, *args, _raw_stream(dev))
     else:
         with torch.cuda.device(t.device):
             _lib.call(name, *args, _stream(t))
+
+
+def _f32(t):
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
 def _i32(t, shape, name):
@@ -982,17 +987,17 @@ def _i32(t, shape, name):
 
 def _i32_rows(t, name):
     """An int32 table with unit column stride (rows may lie apart)."""
-    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] == 0 or t.shape[1] == 0:
+    if t.dtype != torch.int32 or t.dim() != 2 or t.numel() == 0:
         raise ValueError(f"{name} must be a non-empty int32 table of two dimensions, got {t.dtype} {list(t.shape)}")
-    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+    return t if t.is_contiguous() or t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
 
 
 def _check_pool(pages, page_scales, dims):
     """The pool's page dtype code; pages and scales are written in place, so they have to be dense."""
     if pages.dim() not in dims or not pages.is_contiguous() or pages.numel() == 0:
         raise ValueError(f"pages must be a dense, non-empty {' or '.join(map(str, dims))}-dimensional pool")
-    fp8 = _is_fp8_rows(pages)
-    if not fp8 and pages.dtype != torch.bfloat16:
+    fp8 = pages.dtype != torch.bfloat16
+    if fp8 and not _is_fp8_rows(pages):
         raise TypeError(f"pages are bf16 or fp8 (e4m3) rows, got {pages.dtype}")
     if fp8 != (page_scales is not None):
         raise ValueError("page_scales go with fp8 pages, and only with them")
@@ -1005,9 +1010,10 @@ def _check_pool(pages, page_scales, dims):
 
 
 def _check_batch(table, lens, cu):
+    """table, lens, cu, sequences, the table's columns and row stride."""
     table = _i32_rows(table, "table")
-    B = table.shape[0]
-    return table, _i32(lens, (B,), "lens"), _i32(cu, (B + 1,), "cu")
+    B, cols = table.shape
+    return table, _i32(lens, (B,), "lens"), _i32(cu, (B + 1,), "cu"), B, cols, table.stride(0) if B > 1 else cols
 
 
 def _paged_attn_(q: torch.Tensor, pages: torch.Tensor, page_scales: Optional[torch.Tensor], table: torch.Tensor,
@@ -1019,7 +1025,8 @@ def _paged_attn_(q: torch.Tensor, pages: torch.Tensor, page_scales: Optional[tor
         raise ValueError(f"expected q [T,H,D] and out [T,H,dv], got {list(q.shape)} and {list(out.shape)}")
     T, H, D = q.shape
     code = _check_pool(pages, page_scales, (3,))
-    if pages.shape[2] != D:
+    n_pages, P, dp = pages.shape
+    if dp != D:
         raise ValueError(f"pages {list(pages.shape)} do not match q {list(q.shape)}")
     if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
         raise TypeError("paged_attn takes bf16 queries and gives bf16")
@@ -1028,18 +1035,16 @@ def _paged_attn_(q: torch.Tensor, pages: torch.Tensor, page_scales: Optional[tor
     if attn_sink is not None:
         if tuple(attn_sink.shape) != (H,):
             raise ValueError(f"attn_sink {list(attn_sink.shape)} must be [{H}]")
-        attn_sink = attn_sink.float().contiguous()
-    table, lens, cu = _check_batch(table, lens, cu)
-    B = table.shape[0]
+        attn_sink = _f32(attn_sink)
+    table, lens, cu, B, cols, ld = _check_batch(table, lens, cu)
     if T == 0:
         return
     if not q.is_contiguous():
         q = q.contiguous()
-    wsb = _lib.lib().smla_paged_attn_workspace(T, H, B, table.shape[1] * pages.shape[1], window, first)
+    wsb = _lib.lib().smla_paged_attn_workspace(T, H, B, cols * P, window, first)
     ws = torch.empty(wsb, dtype=torch.uint8, device=q.device)
-    _launch(q, "smla_paged_attn", q.data_ptr(), _lib.BF16, pages.data_ptr(), code, _p(page_scales), pages.shape[0],
-            pages.shape[1], table.data_ptr(), table.stride(0), table.shape[1], lens.data_ptr(), cu.data_ptr(), B, T, H, D,
-            out.shape[2], scale, _p(attn_sink), window, first, _lib.PAGED_FILL if fill else 0, out.data_ptr(), _lib.BF16,
+    _launch(q, "smla_paged_attn", q.data_ptr(), _lib.BF16, pages.data_ptr(), code, _p(page_scales), n_pages, P,
+            table.data_ptr(), ld, cols, lens.data_ptr(), cu.data_ptr(), B, T, H, D, out.shape[2], scale, _p(attn_sink), window, first, _lib.PAGED_FILL if fill else 0, out.data_ptr(), _lib.BF16,
             ws.data_ptr(), wsb)
 
 
@@ -1054,6 +1059,12 @@ def _(q, pages, page_scales, table, lens, cu, attn_sink, scale, window, first, f
 paged_attn_op_ = _with_eager_route(paged_attn_op_, _paged_attn_)
 
 
+def _norm_weights(w, n, name):
+    if w.shape != (n,):
+        raise ValueError(f"{name} must hold {n} weights, got {list(w.shape)}")
+    return _f32(w)
+
+
 def _paged_append_(q: Optional[torch.Tensor], kv: torch.Tensor, pages: torch.Tensor, page_scales: Optional[torch.Tensor],
                    table: torch.Tensor, lens: torch.Tensor, cu: torch.Tensor, cos_t: torch.Tensor, sin_t: torch.Tensor,
                    q_norm: Optional[torch.Tensor], kv_norm: Optional[torch.Tensor], norm_dims: int, fp8_sim: bool,
@@ -1064,40 +1075,46 @@ def _paged_append_(q: Optional[torch.Tensor], kv: torch.Tensor, pages: torch.Ten
         raise ValueError("expected kv [T,D]")
     T, D = kv.shape
     code = _check_pool(pages, page_scales, (3,))
-    if pages.shape[2] != D:
+    n_pages, P, dp = pages.shape
+    if dp != D:
         raise ValueError(f"pages {list(pages.shape)} do not match kv {list(kv.shape)}")
-    if kv.dtype not in _YDT:
+    xdt = _YDT.get(kv.dtype)
+    if xdt is None:
         raise TypeError("paged_append takes fp32 or bf16 projections")
     # four channels are read at a time
     unit = 4 * kv.element_size() - 1
-    if kv.stride(1) != 1 or kv.stride(0) < D or kv.stride(0) % 4 or kv.data_ptr() & unit:
+    ldkv, s1 = kv.stride()
+    if s1 != 1 or ldkv < D or ldkv % 4 or kv.data_ptr() & unit:
         kv = kv.clone(memory_format=torch.contiguous_format)
+        ldkv = D
     H = ldq = 0
     if q is not None:
-        H = q.shape[1]
         if q.dim() != 3 or q.shape[0] != T or q.shape[2] != D or q.dtype != kv.dtype:
             raise ValueError(f"expected q [{T}, H, {D}] {kv.dtype}, got {list(q.shape)} {q.dtype}")
         if q_out.shape != q.shape or q_out.dtype != torch.bfloat16 or not q_out.is_contiguous() or q_out.data_ptr() & 7:
             raise ValueError("q_out must be contiguous, 8-byte aligned bf16 of q's shape")
-        if H and (q.stride(2) != 1 or q.stride(1) != D or q.stride(0) < H * D or q.stride(0) % 4 or q.data_ptr() & unit):
+        H = q.shape[1]
+        ldq, s1, s2 = q.stride()
+        if H and (s2 != 1 or s1 != D or ldq < H * D or ldq % 4 or q.data_ptr() & unit):
             q = q.clone(memory_format=torch.contiguous_format)
-        ldq = q.stride(0) if T > 1 else H * D
-    for w, name in ((q_norm, "q_norm"), (kv_norm, "kv_norm")):
-        if w is not None and tuple(w.shape) != (norm_dims,):
-            raise ValueError(f"{name} must hold {norm_dims} weights, got {list(w.shape)}")
-    q_norm = None if q_norm is None else q_norm.float().contiguous()
-    kv_norm = None if kv_norm is None else kv_norm.float().contiguous()
+            ldq = H * D
+    if q_norm is not None:
+        q_norm = _norm_weights(q_norm, norm_dims, "q_norm")
+    if kv_norm is not None:
+        kv_norm = _norm_weights(kv_norm, norm_dims, "kv_norm")
     if cos_t.dim() != 2 or cos_t.shape != sin_t.shape:
         raise ValueError("rotation tables must be [n_pos, rd/2]")
-    cos_t, sin_t = cos_t.float().contiguous(), sin_t.float().contiguous()
-    table, lens, cu = _check_batch(table, lens, cu)
+    cos_t, sin_t = _f32(cos_t), _f32(sin_t)
+    n_pos, rd2 = cos_t.shape
+    table, lens, cu, B, cols, ld = _check_batch(table, lens, cu)
     if T == 0:
         return
-    _launch(kv, "smla_paged_append", _p(q), ldq, kv.data_ptr(), kv.stride(0) if T > 1 else D, _YDT[kv.dtype], T, H, D,
-            norm_dims, _p(q_norm), _p(kv_norm), cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0], 2 * cos_t.shape[1], eps,
-            _lib.SIM_FP8 if fp8_sim else _lib.SIM_NONE, flags, _p(q_out), pages.data_ptr(), code, _p(page_scales),
-            pages.shape[0], pages.shape[1], table.data_ptr(), table.stride(0), table.shape[1], lens.data_ptr(),
-            cu.data_ptr(), table.shape[0])
+    if T == 1:
+        ldq, ldkv = H * D, D
+    _launch(kv, "smla_paged_append", _p(q), ldq, kv.data_ptr(), ldkv, xdt, T, H, D, norm_dims, _p(q_norm), _p(kv_norm),
+            cos_t.data_ptr(), sin_t.data_ptr(), n_pos, 2 * rd2, eps, _lib.SIM_FP8 if fp8_sim else _lib.SIM_NONE, flags,
+            _p(q_out), pages.data_ptr(), code, _p(page_scales), n_pages, P, table.data_ptr(), ld, cols, lens.data_ptr(),
+            cu.data_ptr(), B)
 
 
 paged_append_op_ = torch.library.custom_op("smla::paged_append_", mutates_args=("pages", "page_scales", "q_out"),
@@ -1115,8 +1132,7 @@ paged_append_op_ = _with_eager_route(paged_append_op_, _paged_append_)
 def _pool_args(pages, page_scales):
     """(pointer, layers, layer bytes, row bytes) of the rows and (pointer, layer bytes, row bytes) of the scales."""
     code = _check_pool(pages, page_scales, (3, 4))
-    layers = pages.shape[0] if pages.dim() == 4 else 1
-    n_pages, P, D = pages.shape[-3:]
+    layers, n_pages, P, D = pages.shape if pages.dim() == 4 else (1, *pages.shape)
     row = D * (1 if code == _lib.FP8_E4M3 else 2)
     srow = D // 64 * 4
     scales = (None, 0, 0) if page_scales is None else (page_scales.data_ptr(), n_pages * P * srow, srow)
@@ -1133,14 +1149,14 @@ def _update_pages(pages: torch.Tensor, page_scales: Optional[torch.Tensor], tabl
     S, M = table.shape
     lens, parent, grow = _i32(lens, (S,), "lens"), _i32(parent, (S,), "parent"), _i32(grow, (S,), "grow")
     refs = _i32(refs, (n_pages,), "refs")
-    table2, lens2, granted = torch.empty_like(table, memory_format=torch.contiguous_format), torch.empty_like(lens), \
-        torch.empty_like(lens)
-    refs2 = torch.empty_like(refs)
-    wsb = _lib.lib().smla_update_pages_workspace(S, n_pages)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=pages.device)
-    _launch(pages, "smla_update_pages", table.data_ptr(), table.stride(0), S, M, lens.data_ptr(), refs.data_ptr(), n_pages,
-            P, parent.data_ptr(), grow.data_ptr(), table2.data_ptr(), lens2.data_ptr(), refs2.data_ptr(),
-            granted.data_ptr(), *pool, *scales, ws.data_ptr(), wsb)
+    # (a table with its rows apart gives a dense one)
+    table2 = torch.empty_like(table) if table.is_contiguous() else table.new_empty((S, M))
+    lens2, granted, refs2 = torch.empty_like(lens), torch.empty_like(lens), torch.empty_like(refs)
+    wsb = _lib.lib().smla_update_pages_workspace(S, M, n_pages)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=pages.device) if wsb else None
+    _launch(pages, "smla_update_pages", table.data_ptr(), table.stride(0) if S > 1 else M, S, M, lens.data_ptr(),
+            refs.data_ptr(), n_pages, P, parent.data_ptr(), grow.data_ptr(), table2.data_ptr(), lens2.data_ptr(),
+            refs2.data_ptr(), granted.data_ptr(), *pool, *scales, _p(ws), wsb)
     return table2, lens2, refs2, granted
 
 
@@ -1162,13 +1178,14 @@ def _compact_pages(pages: torch.Tensor, page_scales: Optional[torch.Tensor], tab
     _one_device(pages, page_scales, table, refs)
     n_pages, P, pool, scales = _pool_args(pages, page_scales)
     table = _i32_rows(table, "table")
+    S, M = table.shape
     refs = _i32(refs, (n_pages,), "refs")
-    table2, refs2 = torch.empty_like(table, memory_format=torch.contiguous_format), torch.empty_like(refs)
-    live = refs.new_empty(1)
+    table2 = torch.empty_like(table) if table.is_contiguous() else table.new_empty((S, M))
+    refs2, live = torch.empty_like(refs), refs.new_empty(1)
     wsb = _lib.lib().smla_compact_pages_workspace(n_pages)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=pages.device)
-    _launch(pages, "smla_compact_pages", table.data_ptr(), table.stride(0), *table.shape, refs.data_ptr(), n_pages, P,
-            table2.data_ptr(), refs2.data_ptr(), live.data_ptr(), *pool, *scales, ws.data_ptr(), wsb)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=pages.device) if wsb else None
+    _launch(pages, "smla_compact_pages", table.data_ptr(), table.stride(0) if S > 1 else M, S, M, refs.data_ptr(), n_pages,
+            P, table2.data_ptr(), refs2.data_ptr(), live.data_ptr(), *pool, *scales, _p(ws), wsb)
     return table2, refs2, live
 
 

@@ -581,8 +581,9 @@ int smla_paged_append(const void* q, int64_t ldq, const void* kv, int64_t ldkv, 
  * buffers than the inputs: table_out [S, M] dense (-1 past a slot's pages), lens_out, refs_out, granted [S].
  * Pages given up by the call are free from refs_out on.  Rows are copied within `layers` pools that share the table
  * (layer l at pages + l layer_bytes; row_bytes a row), and likewise within scales (NULL: none).
- * workspace: smla_update_pages_workspace(S, n_pages) bytes, 4-byte aligned. */
-size_t smla_update_pages_workspace(int64_t S, int64_t n_pages);
+ * workspace: smla_update_pages_workspace(S, M, n_pages) bytes, 4-byte aligned; none (0, NULL is taken) where one
+ * launch does all. */
+size_t smla_update_pages_workspace(int64_t S, int64_t M, int64_t n_pages);
 int smla_update_pages(const int32_t* table, int64_t ld_table, int64_t S, int64_t M, const int32_t* lens,
                       const int32_t* refs, int64_t n_pages, int64_t P, const int32_t* parent, const int32_t* grow,
                       int32_t* table_out, int32_t* lens_out, int32_t* refs_out, int32_t* granted, void* pages,
@@ -593,7 +594,7 @@ int smla_update_pages(const int32_t* table, int64_t ld_table, int64_t S, int64_t
  * past it goes to the i-th free id below it, in every layer; the others stay.  table_out [S, M] names the new ids
  * (-1 for an entry that names no live page), refs_out their counts, live [1] their number; all other buffers
  * than the inputs.  The moved pages' old places keep their rows.  Other arguments as above.
- * workspace: smla_compact_pages_workspace(n_pages) bytes, 4-byte aligned. */
+ * workspace: smla_compact_pages_workspace(n_pages) bytes, 4-byte aligned; none where one launch does all. */
 size_t smla_compact_pages_workspace(int64_t n_pages);
 int smla_compact_pages(const int32_t* table, int64_t ld_table, int64_t S, int64_t M, const int32_t* refs,
                        int64_t n_pages, int64_t P, int32_t* table_out, int32_t* refs_out, int32_t* live, void* pages,

@@ -409,7 +409,8 @@ def _apply(pool, moves, P):
 
 @pytest.mark.parametrize("S,M,P,n_pages,layers,D,kv", [
     (1, 1, 1, 1, 0, 512, "bf16"), (1, 4, 16, 6, 0, 576, "fp8"), (5, 7, 3, 20, 2, 64, "bf16"), (16, 9, 8, 70, 3, 128, "fp8"),
-    (64, 12, 16, 400, 0, 512, "bf16"), (1500, 5, 4, 5000, 0, 64, "bf16"), (40, 300, 2, 9000, 1, 64, "fp8")])
+    (64, 12, 16, 400, 0, 512, "bf16"), (1500, 5, 4, 5000, 0, 64, "bf16"), (40, 300, 2, 9000, 1, 64, "fp8"),
+    (1024, 32, 2, 16384, 0, 64, "bf16"), (9, 2500, 4, 20000, 0, 64, "bf16"), (7, 5000, 1, 33000, 2, 64, "fp8")])
 def test_update_pages(dev, S, M, P, n_pages, layers, D, kv):
     from smla import paged
     r = random.Random(S + M)
@@ -453,7 +454,8 @@ def test_update_pages_bad_entries(dev):
 
 @pytest.mark.parametrize("S,M,P,n_pages,layers,D,kv", [
     (1, 1, 1, 1, 0, 512, "bf16"), (3, 5, 16, 9, 2, 576, "fp8"), (8, 9, 8, 60, 0, 64, "bf16"), (30, 300, 2, 9000, 0, 64, "fp8"),
-    (64, 64, 4, 20000, 1, 64, "bf16")])
+    (64, 64, 4, 20000, 1, 64, "bf16"), (9, 100, 2, 1025, 3, 64, "bf16"), (9, 2000, 1, 16384, 0, 64, "bf16"),
+    (9, 2000, 1, 16385, 0, 64, "bf16"), (9, 6000, 1, 50000, 0, 64, "fp8")])
 def test_compact_pages(dev, S, M, P, n_pages, layers, D, kv):
     from smla import paged
     r = random.Random(S)

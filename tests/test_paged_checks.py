@@ -67,9 +67,9 @@ def test_paged_append_arguments(change, status):
 UPDATE = ("table ld_table S M lens refs n_pages P parent grow table_out lens_out refs_out granted pages layers layer_bytes "
           "row_bytes scales scale_layer_bytes scale_row_bytes ws ws_bytes stream").split()
 OTHER = ctypes.c_void_p(8192)
-UPDATE_OK = dict(table=FAKE, ld_table=8, S=4, M=8, lens=FAKE, refs=FAKE, n_pages=10, P=16, parent=FAKE, grow=FAKE, table_out=OTHER,
+UPDATE_OK = dict(table=FAKE, ld_table=8, S=4, M=8, lens=FAKE, refs=FAKE, n_pages=20000, P=16, parent=FAKE, grow=FAKE, table_out=OTHER,
                  lens_out=OTHER, refs_out=OTHER, granted=OTHER, pages=FAKE, layers=1, layer_bytes=0, row_bytes=1024, scales=None,
-                 scale_layer_bytes=0, scale_row_bytes=0, ws=FAKE, ws_bytes=(1 + 2 * 4 + 10) * 4, stream=None)
+                 scale_layer_bytes=0, scale_row_bytes=0, ws=FAKE, ws_bytes=(1 + 2 * 4 + 20000) * 4, stream=None)
 BAD_POOL = [(dict(table=None), NULL), (dict(refs=None), NULL), (dict(pages=None), NULL), (dict(table_out=None), NULL),
             (dict(refs_out=None), NULL), (dict(S=0), SHAPE), (dict(M=0), SHAPE), (dict(n_pages=0), SHAPE), (dict(P=0), SHAPE),
             (dict(layers=0), SHAPE), (dict(row_bytes=0), SHAPE), (dict(ld_table=7), SHAPE), (dict(scales=FAKE), SHAPE),
@@ -79,17 +79,17 @@ BAD_POOL = [(dict(table=None), NULL), (dict(refs=None), NULL), (dict(pages=None)
 
 @pytest.mark.parametrize("change,status", BAD_POOL + [
     (dict(lens=None), NULL), (dict(parent=None), NULL), (dict(grow=None), NULL), (dict(lens_out=None), NULL),
-    (dict(granted=None), NULL), (dict(lens_out=FAKE), UNSUP), (dict(ws_bytes=(1 + 2 * 4 + 10) * 4 - 1), WS)])
+    (dict(granted=None), NULL), (dict(lens_out=FAKE), UNSUP), (dict(ws_bytes=(1 + 2 * 4 + 20000) * 4 - 1), WS)])
 def test_update_pages_arguments(change, status):
     assert _call("smla_update_pages", UPDATE, UPDATE_OK, **change) == status
 
 
 COMPACT = ("table ld_table S M refs n_pages P table_out refs_out live pages layers layer_bytes row_bytes scales "
            "scale_layer_bytes scale_row_bytes ws ws_bytes stream").split()
-COMPACT_OK = {k: UPDATE_OK[k] for k in COMPACT if k in UPDATE_OK} | dict(live=OTHER, ws_bytes=32 * 4)
+COMPACT_OK = {k: UPDATE_OK[k] for k in COMPACT if k in UPDATE_OK} | dict(live=OTHER, ws_bytes=60002 * 4)
 
 
-@pytest.mark.parametrize("change,status", BAD_POOL + [(dict(live=None), NULL), (dict(ws_bytes=32 * 4 - 1), WS)])
+@pytest.mark.parametrize("change,status", BAD_POOL + [(dict(live=None), NULL), (dict(ws_bytes=60002 * 4 - 1), WS)])
 def test_compact_pages_arguments(change, status):
     assert _call("smla_compact_pages", COMPACT, COMPACT_OK, **change) == status
 
@@ -102,7 +102,12 @@ def test_workspace_sizes():
     few, many, long = size(1, 64, 1, 4096, 0, 0), size(4096, 64, 1, 4096, 0, 0), size(4096, 64, 1, 1 << 20, 0, 0)
     assert 0 < few < many < long < 1 << 29
     assert size(4096, 64, 1, 1 << 20, 128, 4) == many       # a window keeps the tiles short
-    assert lib.smla_update_pages_workspace(0, 1) == 0 and lib.smla_compact_pages_workspace(0) == 0
+    update, compact = lib.smla_update_pages_workspace, lib.smla_compact_pages_workspace
+    assert update(0, 1, 1) == update(1, 0, 1) == update(1, 1, 0) == compact(0) == 0
+    # one launch, which needs none, up to one step of a scan, 1024 slots and 32768 entries
+    assert update(1024, 32, 16384) == compact(16384) == 0
+    assert update(4, 8, 16385) == 4 * (1 + 8 + 16385) and update(1025, 1, 8) == 4 * (1 + 2050 + 8)
+    assert update(1024, 33, 8) == 4 * (1 + 2048 + 8) and compact(16385) == 4 * (2 + 3 * 16385)
 
 
 def test_python_checks():
