@@ -269,7 +269,7 @@ struct Work {
 struct RowIds {
   int mine, tail;  // of row lane & 31; of the lane's row of this wave's tail copy
 };
-// the k-th copy or fp8 piece of a tile that value wave vi takes (the wave with four blocks is dealt last)
+// the k-th copy of a tile (NB = 3: fp8 piece) that value wave vi takes (the wave with four blocks is dealt last)
 __device__ inline constexpr int dealt(int vi, int k) { return kValueWaves - 1 - vi + kValueWaves * k; }
 template <class G>
 __device__ inline RowIds read_ids(const lds_i32_t* ids_s, int vi, int lane, int tl) {
@@ -318,12 +318,17 @@ __device__ inline void copy_rows(uint32_t tbase, int vi, int lane, bool nt, F&& 
   }
 }
 
-// ---- fp8 rows (e4m3 codes, one fp32 scale per 64 columns): a tile's codes in pieces of 16, 64 pieces at a time dealt
-// to the value waves; main columns first, then the rope tails, so no wave instruction mixes the two
+// ---- fp8 rows (e4m3 codes, one fp32 scale per 64 columns): a tile's codes in pieces of 16, 64 pieces at a time: main columns
+// first, then the rope tails, so no wave instruction mixes the two.  At NB = 2 wave 2 has no q rows and takes most of
+// them, the value waves kShare each; both keep two tiles' codes on their way (2 to 4 draft tokens of 64 sequences, 16 heads:
+// 110 us; all pieces by the value waves 115, one tile ahead 121).  At NB = 3 the value waves share them.
+constexpr int kShare = 2;
 template <int D>
+constexpr int kPieces8 = kTileRows * (D / 16) / 64;
+template <int NB, int D>
+constexpr int kMine8 = NB == 2 ? kShare : (kPieces8<D> + kValueWaves - 1) / kValueWaves;  // a value wave's
+template <int K>
 struct F8 {
-  static constexpr int N = kTileRows * (D / 16) / 64;               // pieces of 64
-  static constexpr int K = (N + kValueWaves - 1) / kValueWaves;
   u32x4_t v[K];
   float s[K];
 };
@@ -337,13 +342,14 @@ __device__ inline void f8_place(int x, int lane, int& r, int& cc) {
     cc = 32 + (lane & 3);
   }
 }
-template <int D>
-__device__ inline void f8_load(const PagedArgs& a, const lds_i32_t* ids_s, int vi, int lane, int tl, F8<D>& f) {
+// pieces x0 + k step, k < K (of the last, those that exist)
+template <int D, int K>
+__device__ inline void f8_load(const PagedArgs& a, const lds_i32_t* ids_s, int x0, int step, int lane, int tl, F8<K>& f) {
   const lds_i32_t* id = ids_s + (tl % kIdTiles) * kTileRows;
 #pragma unroll
-  for (int k = 0; k < F8<D>::K; k++) {
-    const int x = dealt(vi, k);
-    if (x < F8<D>::N) {
+  for (int k = K - 1; k >= 0; k--) {
+    const int x = x0 + k * step;
+    if (x < kPieces8<D>) {
       int r, cc;
       f8_place<D>(x, lane, r, cc);
       const int64_t row = max(id[r], 0);
@@ -352,13 +358,13 @@ __device__ inline void f8_load(const PagedArgs& a, const lds_i32_t* ids_s, int v
     }
   }
 }
-template <class G, int D>
-__device__ inline void f8_store(lds_u8_t* lds, int vi, int lane, int tl, const F8<D>& f) {
+template <class G, int D, int K>
+__device__ inline void f8_store(lds_u8_t* lds, int x0, int step, int lane, int tl, const F8<K>& f) {
   lds_u8_t* slot = lds + (tl % G::NBUF) * G::TILE_BYTES;
 #pragma unroll
-  for (int k = 0; k < F8<D>::K; k++) {
-    const int x = dealt(vi, k);
-    if (x < F8<D>::N) {
+  for (int k = 0; k < K; k++) {
+    const int x = x0 + k * step;
+    if (x < kPieces8<D>) {
       int r, cc;
       f8_place<D>(x, lane, r, cc);
       uint32_t w[8];
@@ -501,7 +507,7 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
            __builtin_amdgcn_ballot_w64(min(min(v[0], v[1]), min(v[2], v[3])) < 0) == 0;
   };
   auto ids_of = [&](int i) { return *(const lds_i32x4_t*)(ids_s + (i % kIdTiles) * kTileRows + 4 * (lane & 7)); };
-  constexpr int PF = G::TAIL ? 5 : 8;  // fragments read ahead
+  constexpr int PF = G::TAIL ? 5 : 4;  // fragments read ahead (more only crowd the LDS at a tile's start)
   u32x4_t kf[PF];
   // the products of tile i; `between` j runs after step j's
   auto products = [&](f32x16_t& s, int i, auto&& before, auto&& between) {
@@ -633,7 +639,12 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
   int pr[2];  // chunk 2 ks + (lane >> 5) of q row lane & 31 (+ 32 n)
 #pragma unroll
   for (int ks = 0; ks < 2; ks++) pr[ks] = p_at(lane & 31, 2 * ks + (lane >> 5));
-  F8<D> f8;
+  // fp8 codes on their way: of one tile, of two where registers are left
+  constexpr bool DEEP = FP8 && NB == 2;
+  F8<kMine8<NB, D>> f8, f8_next;
+  const int x0 = DEEP ? vi : dealt(vi, 0);
+  __builtin_assume(x0 >= 0 && x0 < kValueWaves);
+  const int last = max(w.ntiles - 1, 0);
   // ---- Q rows to ring slots 1 .. NB in a tile's layout, then tile 0 (fp8: and the next one's codes)
 #pragma unroll
   for (int n = 0; n < NB; n++)
@@ -641,15 +652,16 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
       copy_rows<G>(lds_base + (1 + n) * G::TILE_BYTES, vi, lane, true,
                    [&](int x) { return (uint64_t)(uintptr_t)a.q + (uint64_t)(w.row0 + (32 * n + x < w.nh ? 32 * n + x : 0)) * G::ROWB; });
   if constexpr (FP8) {
-    if (w.ntiles > 0) {
-      f8_load<D>(a, ids_s, vi, lane, 0, f8);
-      f8_store<G, D>(lds, vi, lane, 0, f8);
-      if (w.ntiles > 1) f8_load<D>(a, ids_s, vi, lane, 1, f8);
-    }
+    // (past the last tile: the last once more, so that the loads in flight are counted alike on all paths)
+    f8_load<D>(a, ids_s, x0, kValueWaves, lane, 0, f8);
+    f8_store<G, D>(lds, x0, kValueWaves, lane, 0, f8);
+    f8_load<D>(a, ids_s, x0, kValueWaves, lane, min(1, last), f8);
+    if constexpr (DEEP) f8_load<D>(a, ids_s, x0, kValueWaves, lane, min(2, last), f8_next);
   } else {
     if (w.ntiles > 0) issue_tile<G>(a, lds_base, read_ids<G>(ids_s, vi, lane, 0), vi, lane, 0);
   }
-  wait_vm(0);
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), in the compiler's own count too
+  asm volatile("" ::: "memory");
   lds_barrier();
   lds_barrier();  // the score waves have read Q
   if constexpr (!FP8) {
@@ -659,12 +671,10 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
   }
   // Iteration i: the score waves finish tile i - 1 and begin tile i, tile i - 2 is consumed here, and tile i + 1 goes
   // to the slot of tile i - 3, to be there at the iteration's end.
-  for (int i = 0; i <= w.ntiles + 1; i++) {
+  auto iteration = [&](int i, F8<kMine8<NB, D>>& f) {
     if constexpr (FP8) {
-      if (i + 1 < w.ntiles) {
-        f8_store<G, D>(lds, vi, lane, i + 1, f8);
-        if (i + 2 < w.ntiles) f8_load<D>(a, ids_s, vi, lane, i + 2, f8);
-      }
+      if (i + 1 < w.ntiles) f8_store<G, D>(lds, x0, kValueWaves, lane, i + 1, f);
+      f8_load<D>(a, ids_s, x0, kValueWaves, lane, min(i + 2 + DEEP, last), f);
     } else {
       if (i >= 3 && i + 1 < w.ntiles) {
         issue_tile<G>(a, lds_base, ids, vi, lane, i + 1);
@@ -741,6 +751,23 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
       else if (i + 1 < w.ntiles) wait_vm(max(0, min(3, w.ntiles - 1) - (i + 1)) * my_dma);
     }
     lds_barrier();
+  };
+  if constexpr (DEEP) {
+    // in pairs, each register set with its own half (a way out between the halves would make the compiler wait for all
+    // loads); of an odd number the first, which has no products, by itself
+    int i = w.ntiles & 1;
+    if (i) {
+      if (w.ntiles > 1) f8_store<G, D>(lds, x0, kValueWaves, lane, 1, f8);
+      f8 = f8_next;
+      f8_load<D>(a, ids_s, x0, kValueWaves, lane, min(3, last), f8_next);
+      lds_barrier();
+    }
+    for (; i <= w.ntiles; i += 2) {
+      iteration(i, f8);
+      iteration(i + 1, f8_next);
+    }
+  } else {
+    for (int i = 0; i <= w.ntiles + 1; i++) iteration(i, f8);
   }
   lds_barrier();  // (m, l) in LDS
 #pragma unroll
@@ -797,6 +824,40 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
   }
 }
 
+// Wave 2 at NB = 2 over fp8 pages: the pieces that the value waves leave, requested two tiles ahead; it keeps their barriers.
+template <class G, int D>
+__device__ inline void feed_role(const PagedArgs& a, const Work& w, lds_u8_t* lds, int lane) {
+  constexpr int X0 = kShare * kValueWaves, K = kPieces8<D> - X0;
+  const lds_i32_t* ids_s = (const lds_i32_t*)(lds + G::IDS_OFF);
+  const int last = max(w.ntiles - 1, 0);
+  F8<K> f8, f8_next;
+  f8_load<D>(a, ids_s, X0, 1, lane, 0, f8);
+  f8_store<G, D>(lds, X0, 1, lane, 0, f8);
+  f8_load<D>(a, ids_s, X0, 1, lane, min(1, last), f8);
+  f8_load<D>(a, ids_s, X0, 1, lane, min(2, last), f8_next);
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  lds_barrier();
+  lds_barrier();
+  auto iteration = [&](int i, F8<K>& f) {
+    if (i + 1 < w.ntiles) f8_store<G, D>(lds, X0, 1, lane, i + 1, f);
+    f8_load<D>(a, ids_s, X0, 1, lane, min(i + 3, last), f);
+    __builtin_amdgcn_sched_barrier(0);
+    lds_barrier();
+  };
+  int i = w.ntiles & 1;  // (pairs: as in value_role)
+  if (i) {
+    if (w.ntiles > 1) f8_store<G, D>(lds, X0, 1, lane, 1, f8);
+    f8 = f8_next;
+    f8_load<D>(a, ids_s, X0, 1, lane, min(3, last), f8_next);
+    lds_barrier();
+  }
+  for (; i <= w.ntiles; i += 2) {
+    iteration(i, f8);
+    iteration(i + 1, f8_next);
+  }
+  lds_barrier();
+}
+
 template <int D, int NB, bool FP8>
 __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedArgs a) {
   using G = GeoP<D, NB>;
@@ -842,6 +903,8 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedArgs
     if (wave < NB) {
       lds_barrier();  // Q and tile 0 have landed
       score_role<G, D>(a, w, trow, lds, wave, lane);
+    } else if constexpr (FP8 && NB == 2) {
+      feed_role<G, D>(a, w, lds, lane);
     } else {
       for (int i = 0; i < w.ntiles + 5; i++) lds_barrier();
     }
