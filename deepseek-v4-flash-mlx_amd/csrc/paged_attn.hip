@@ -417,9 +417,9 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
   constexpr float kLog2e = 1.44269504088896340736f;
   const float c2 = fabsf(a.scale) * kLog2e;
   const int rr = r < w.nh ? r : 0;  // (rows past nh are the tile's first)
-  // entries that the q row sees: e < eh, and e < first or e >= eh - span
-  const int eh = w.p0 + (int)((uint32_t)(w.m0 + rr) / (uint32_t)a.H) + 1 - w.lo + w.nf;
-  const uint32_t span = a.window > 0 ? (uint32_t)a.window : 0x7fffffffu;
+  // entries that the q row sees: e < eh, and e < first or e >= past
+  const int eh = max(w.p0 + (int)((uint32_t)(w.m0 + rr) / (uint32_t)a.H) + 1 - w.lo + w.nf, 0);
+  const int past = a.window > 0 ? max(eh - a.window, 0) : 0;
   // entries below eh_all and outside [first, el_all) are seen by every q row of the tile
   const int eh_all = w.p_lo + 1 - w.lo + w.nf, el_all = a.window > 0 ? w.p_hi - a.window + 1 - w.lo + w.nf : 0;
   if (idle) {  // nothing to rescale, and no flags
@@ -481,24 +481,22 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
       if (e < w.e_end) page = trow[col];
     }
   };
-  // scores of a tile of which some q row does not see some row: scaled, -inf there
+  // scores of a tile of which some q row does not see some row: scaled, -inf there; whether a masked one is not finite
+  // (0 x it is not 0).  The rows that the q row sees as bits: those whose row number is there (a ballot), below eh, and
+  // from `past` on or below first; then per score a bit spread to a word, and bitwise selects.
   auto mask = [&](f32x16_t& s, int i) -> bool {
-    bool odd = false;  // a masked score is not finite
-    const lds_i32_t* id = ids_s + (i % kIdTiles) * kTileRows + 4 * h;
-    const int e0 = w.e_begin + i * kTileRows + 4 * h;
+    const int e0 = w.e_begin + i * kTileRows;
+    const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(ids_s[(i % kIdTiles) * kTileRows + (lane & 31)] >= 0);
+    auto below = [](int n) -> uint32_t { return n >= 32 ? 0xffffffffu : (1u << max(n, 0)) - 1; };  // the bits below n
+    const uint32_t mine = (there & below(eh - e0) & (~below(past - e0) | below(a.first - e0))) >> (4 * h);
+    float z = 0.f;
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
-      const i32x4_t v = *(const lds_i32x4_t*)(id + 8 * q);
-#pragma unroll
-      for (int k = 0; k < 4; k++) {  // (without branches)
-        const int e = e0 + 8 * q + k;
-        const float x = s[4 * q + k];
-        const bool ok = (v[k] >= 0) & (e < eh) & ((e < a.first) | (e >= (int)((uint32_t)eh - span)));
-        odd |= !ok & !(fabsf(x) < SMLA_INF);
-        s[4 * q + k] = ok ? x * c2 : -SMLA_INF;
-      }
+    for (int k = 0; k < 16; k++) {
+      const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)mine, 8 * (k >> 2) + (k & 3), 1);
+      z = __builtin_fmaf(__uint_as_float(__float_as_uint(s[k]) & ~m), 0.f, z);
+      s[k] = __uint_as_float((__float_as_uint(s[k] * c2) & m) | (__float_as_uint(-SMLA_INF) & ~m));
     }
-    return odd;
+    return !(z == 0.f);
   };
   // whether every q row of the tile sees every row of tile i (its row numbers v are all there)
   auto is_open = [&](int i, const i32x4_t& v) -> bool {
