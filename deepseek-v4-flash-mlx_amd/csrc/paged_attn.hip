@@ -438,7 +438,7 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
   // negative scale's sign goes into q
   bf16x8_t qf[STEPS];
 #pragma unroll
-  for (int j = 0; j < STEPS; j++) qf[j] = as_bf16x8(ldk((1 + wave) * G::TILE_BYTES, j));
+  for (int j = 0; j < STEPS; j++) qf[j] = as_bf16x8(ldk((G::NBUF - G::NB + wave) * G::TILE_BYTES, j));
   if (a.scale < 0.f) {
 #pragma unroll
     for (int j = 0; j < STEPS; j++) qf[j] = as_bf16x8(__builtin_bit_cast(u32x4_t, qf[j]) ^ 0x80008000u);
@@ -643,12 +643,20 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
   const int x0 = DEEP ? vi : dealt(vi, 0);
   __builtin_assume(x0 >= 0 && x0 < kValueWaves);
   const int last = max(w.ntiles - 1, 0);
-  // ---- Q rows to ring slots 1 .. NB in a tile's layout, then tile 0 (fp8: and the next one's codes)
+  // ---- Q rows to the last NB ring slots in a tile's layout (read once: not kept in the L2, unless the tile is split), then
+  // the tiles that the other slots hold (fp8: tile 0, and the next ones' codes)
+  constexpr int EARLY = G::NBUF - NB;
+  auto request_q = [&](bool nt) {
 #pragma unroll
-  for (int n = 0; n < NB; n++)
-    if (32 * n < w.nh)
-      copy_rows<G>(lds_base + (1 + n) * G::TILE_BYTES, vi, lane, true,
-                   [&](int x) { return (uint64_t)(uintptr_t)a.q + (uint64_t)(w.row0 + (32 * n + x < w.nh ? 32 * n + x : 0)) * G::ROWB; });
+    for (int n = 0; n < NB; n++)
+      if (32 * n < w.nh)
+        copy_rows<G>(lds_base + (EARLY + n) * G::TILE_BYTES, vi, lane, nt, [&](int x) {
+          return (uint64_t)(uintptr_t)a.q + (uint64_t)(w.row0 + (32 * n + x < w.nh ? 32 * n + x : 0)) * G::ROWB;
+        });
+  };
+  if (w.slot < 0) request_q(true);
+  else request_q(false);
+  lds_barrier();  // the first row numbers are there
   if constexpr (FP8) {
     // (past the last tile: the last once more, so that the loads in flight are counted alike on all paths)
     f8_load<D>(a, ids_s, x0, kValueWaves, lane, 0, f8);
@@ -656,14 +664,20 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
     f8_load<D>(a, ids_s, x0, kValueWaves, lane, min(1, last), f8);
     if constexpr (DEEP) f8_load<D>(a, ids_s, x0, kValueWaves, lane, min(2, last), f8_next);
   } else {
-    if (w.ntiles > 0) issue_tile<G>(a, lds_base, read_ids<G>(ids_s, vi, lane, 0), vi, lane, 0);
+    for (int tl = 0; tl < min(w.ntiles, EARLY); tl++)
+      issue_tile<G>(a, lds_base, read_ids<G>(ids_s, vi, lane, tl), vi, lane, tl);
   }
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), in the compiler's own count too
-  asm volatile("" ::: "memory");
+  // Q and tile 0 are there
+  if (FP8 || w.ntiles <= 1) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), in the compiler's own count too
+    asm volatile("" ::: "memory");
+  } else {
+    wait_vm((EARLY - 1) * my_dma);
+  }
   lds_barrier();
   lds_barrier();  // the score waves have read Q
   if constexpr (!FP8) {
-    for (int tl = 1; tl < min(w.ntiles, G::NBUF); tl++)
+    for (int tl = EARLY; tl < min(w.ntiles, G::NBUF); tl++)
       issue_tile<G>(a, lds_base, read_ids<G>(ids_s, vi, lane, tl), vi, lane, tl);
     if (G::NBUF < w.ntiles) ids = read_ids<G>(ids_s, vi, lane, G::NBUF);
   }
@@ -892,12 +906,15 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedArgs
   w.e_end = min(entries, w.e_begin + part);
   w.ntiles = w.e_end > w.e_begin ? (w.e_end - w.e_begin + kTileRows - 1) / kTileRows : 0;
   const int32_t* trow = a.table + it.b * a.ld_table;
-  if (tid < kIdTiles * kTileRows) {  // the first eight tiles' row numbers
-    const int e = w.e_begin + tid;
-    ids_s[tid] = row_number(a, trow, e < w.nf ? e : w.lo + (e - w.nf), e < w.e_end);
-  }
-  lds_barrier();
   if (wave < kFirstValue) {
+    // the first eight tiles' row numbers: six, then (wave 0) two, there at the next barrier
+    auto first_numbers = [&](int x) {
+      const int e = w.e_begin + x;
+      ids_s[x] = row_number(a, trow, e < w.nf ? e : w.lo + (e - w.nf), e < w.e_end);
+    };
+    first_numbers(tid);
+    lds_barrier();
+    if (tid < kIdTiles * kTileRows - 64 * kFirstValue) first_numbers(tid + 64 * kFirstValue);
     if (wave < NB) {
       lds_barrier();  // Q and tile 0 have landed
       score_role<G, D>(a, w, trow, lds, wave, lane);
