@@ -148,7 +148,8 @@ __device__ inline int plan_rps(const PagedArgs& a, const Seq& s0, int lane) {
     // more tiles than compute units: items of at most half a unit's share
     const float share = work / (float)(2 * a.cus * kTileRows);
     const int best = max(kMinRowsMany / kTileRows, (int)fminf(share, 16777216.f) + 1);
-    if (most < kMinPart / kTileRows * 2 || 2 * (int64_t)tiles > kMostItems * a.cus) return best * kTileRows;
+    // (past 2 kMinPart entries, where plan_slots has slots for the parts; `most` is one more than whole tiles)
+    if (most <= kMinPart / kTileRows * 2 || 2 * (int64_t)tiles > kMostItems * a.cus) return best * kTileRows;
     // few rounds of long tiles: parts of them fill the last round better; a part costs about kPartRows entries more
     float least = 0.f;
     int rps = best;
@@ -170,8 +171,12 @@ __device__ inline int plan_rps(const PagedArgs& a, const Seq& s0, int lane) {
   // units of 32 entries: the fewest that give at most one item per compute unit
   int lo = max(kMinRows / kTileRows, (int)fminf(work / (float)(a.cus * kTileRows), 16777216.f));
   int hi = max(lo, most + (most >> 20) + 1);  // (most went through fp32)
-  // (sum of tiles x ceil(span / rps) <= work / rps + tiles: enough where that fits, two units more for fp32's rounding)
-  if (tiles < a.cus) hi = max(lo, min(hi, (int)fminf(work / (float)((a.cus - tiles) * kTileRows), 16777216.f) + 2));
+  // (sum of tiles x ceil(span / rps) <= work / rps + tiles: enough where that fits; fp32 sums of at most 256 terms and their
+  // quotient are off by under 1e-4 of it)
+  if (tiles < a.cus) {
+    const float fits = work / (float)((a.cus - tiles) * kTileRows) * 1.0001f;
+    if (fits < (float)hi) hi = max(lo, (int)fits + 2);
+  }
   while (lo < hi) {
     const int mid = lo + (hi - lo) / 2;
     int items = 0;

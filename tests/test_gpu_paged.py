@@ -141,6 +141,26 @@ def test_attn_long_tiles_in_parts(dev):
             assert ((x.float() - want).norm(dim=-1) <= 3 * BF16 * want.norm(dim=-1)).all(), t
 
 
+@pytest.mark.parametrize("L,P", [(8170, 15), (8160, 16), (8192, 64), (8224, 32)])
+def test_attn_tiles_at_the_shortest_length_of_parts(dev, L, P):
+    """Around the length from which tiles are cut into parts: every row is written, whichever way is taken."""
+    from smla import paged
+    announce(f"paged_attn 900 tokens of 64 heads over {L} rows in pages of {P}")
+    g = torch.Generator().manual_seed(L)
+    T, cols = 900, -(-L // P)
+    pages = torch.randn(cols, P, 512, generator=g).to(torch.bfloat16).to(dev)
+    table = torch.randperm(cols, generator=g).to(torch.int32)[None].to(dev)
+    q = torch.randn(T, 64, 512, generator=g).to(torch.bfloat16).to(dev)
+    out = torch.full_like(q, float("nan"))
+    paged.paged_attn(q, pages, table, _i32([L], dev), _i32([0, T], dev), 512 ** -0.5, out=out)
+    assert not out.isnan().any()
+    kv = pages[table[0].long()].reshape(-1, 512)[:L].float()
+    for t in (0, 1, 333, 698, 899):
+        n = L - T + t + 1
+        want = torch.softmax(q[t].float() @ kv[:n].T * 512 ** -0.5, dim=-1) @ kv[:n]
+        assert ((out[t].float() - want).norm(dim=-1) <= 3 * BF16 * want.norm(dim=-1)).all(), t
+
+
 @pytest.mark.parametrize("window,first", [(1, 0), (1, 1), (8, 0), (8, 4), (40, 37), (128, 4), (64, 500), (1000, 2), (1 << 29, 1 << 29)])
 @pytest.mark.parametrize("H", [16, 64])
 def test_attn_window_and_first_rows(dev, window, first, H):
