@@ -1041,9 +1041,11 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
     }
   }
   if (a.fill) {
-    const int64_t from = (int64_t)min(max(a.cu[a.B], 0), a.T) * a.H * 64, to = (int64_t)a.T * a.H * 64;
-    for (int64_t i = from + (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < to; i += (int64_t)gridDim.x * blockDim.x)
-      *(u32x4_t*)(a.out + i * 8) = u32x4_t{0u, 0u, 0u, 0u};
+    // 16-byte pieces of the tokens before the first sequence and behind the last
+    const int64_t tok = (int64_t)a.H * 64, to = a.T * tok, first = min(max(a.cu[0], 0), a.T) * tok;
+    const int64_t gap = max(min(max(a.cu[a.B], 0), a.T) * tok - first, (int64_t)0);
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < to - gap; i += (int64_t)gridDim.x * blockDim.x)
+      *(u32x4_t*)(a.out + (i < first ? i : i + gap) * 8) = u32x4_t{0u, 0u, 0u, 0u};
   }
 }
 
@@ -1114,6 +1116,9 @@ extern "C" int smla_paged_attn(const void* q, int q_dtype, const void* pages, in
   if (window < 0 || first < 0 || window > 0x3fffffff || first > 0x3fffffff || (flags & ~SMLA_PAGED_FILL)) return SMLA_E_RANGE;
   if (!plan_sizes(T, H, B) || n_pages > 0x7fffffff || P > 0x7fffffff || n_pages * P > 0x7fffffff || cols > 0x7fffffff)
     return SMLA_E_RANGE;
+  // rows of q are read while others of out are written
+  const uintptr_t o0 = (uintptr_t)out, q0 = (uintptr_t)q;
+  if (o0 < q0 + (uintptr_t)T * H * D * 2 && q0 < o0 + (uintptr_t)T * H * DV * 2) return SMLA_E_UNSUPPORTED;
   if (!usable_workspace(workspace, workspace_bytes, smla_paged_attn_workspace(T, H, B, cols * P, window, first))) return SMLA_E_WORKSPACE;
   if (T == 0) return SMLA_OK;
   PagedArgs a{};

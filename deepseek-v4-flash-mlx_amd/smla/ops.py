@@ -1039,8 +1039,8 @@ def _paged_attn_(q: torch.Tensor, pages: torch.Tensor, page_scales: Optional[tor
     table, lens, cu, B, cols, ld = _check_batch(table, lens, cu)
     if T == 0:
         return
-    if not q.is_contiguous():
-        q = q.contiguous()
+    if not q.is_contiguous() or q.data_ptr() & 15:     # rows are copied 16 bytes at a time
+        q = q.clone(memory_format=torch.contiguous_format)
     wsb = _lib.lib().smla_paged_attn_workspace(T, H, B, cols * P, window, first)
     ws = torch.empty(wsb, dtype=torch.uint8, device=q.device)
     _launch(q, "smla_paged_attn", q.data_ptr(), _lib.BF16, pages.data_ptr(), code, _p(page_scales), n_pages, P,

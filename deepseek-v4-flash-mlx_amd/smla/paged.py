@@ -23,8 +23,8 @@ def paged_attn(q, pages, table, lens, cu, scale, attn_sink=None, window=0, first
     tokens cu[b] .. cu[b+1]-1, the last rows of its lens[b]; table [B, cols], lens [B], cu [B+1] int32.
     A token at position p attends rows j <= p, with window > 0 those with j > p - window or
     j < first; ``attn_sink`` [H] adds to the denominator as in ``sparse_attn``; a token that sees no
-    row gives 0.  Returns [T, H, dv] bf16: ``out`` when given (rows behind the last sequence are left
-    as they were), else a new tensor (0 there).  One token a sequence, a prompt's chunk and any mix of them
+    row gives 0.  Returns [T, H, dv] bf16: ``out`` when given (apart from q; tokens of no sequence are
+    left as they were), else a new tensor (0 there).  One token a sequence, a prompt's chunk and any mix of them
     are the same call."""
     fill = out is None
     if fill:
@@ -43,8 +43,8 @@ def paged_append(q, kv, pages, table, lens, cu, cos_t, sin_t, kv_norm=None, q_no
     RMS-normed, then the last 2 * cos_t.shape[1] channels rotated to the token's position (``norm_rope.rope_tables``).
     The rows go to their pages: bf16 (``fp8_sim``: the channels before the rotated ones fp8
     round-tripped first) or, with fp8 pages, e4m3 codes and ``page_scales``.  Returns the queries [T, H, D] bf16
-    (``q_out`` when given: rows behind the last sequence or at positions past the tables are left as they
-    were; else 0 there), None without q."""
+    (``q_out`` when given: tokens of no sequence or at positions past the rotation tables are left as
+    they were; else 0 there), None without q."""
     fill = q is not None and q_out is None
     if fill:
         if q.dim() != 3:

@@ -279,6 +279,142 @@ def test_attn_equals_the_dense_path(dev):
     assert rel <= 6 * BF16
 
 
+def test_attn_tokens_of_no_sequence(dev):
+    """Before the first sequence and behind the last: 0 in a new tensor, as they were in one that is given."""
+    from smla import paged
+    announce("paged_attn cu from 3 to 8 of 13 tokens")
+    pages, _, table = _cache(81, [200, 90], 16, 512)
+    q = torch.randn(13, 16, 512, generator=torch.Generator().manual_seed(5)).to(torch.bfloat16)
+    dq, dp, dt = _to(dev, q, pages, table)
+    lens, cu = _i32([200, 90], dev), _i32([3, 5, 8], dev)
+    out = paged.paged_attn(dq, dp, dt, lens, cu, 512 ** -0.5)
+    assert (out[:3] == 0).all() and (out[8:] == 0).all()
+    _check_attn(out[3:8], q[3:8], pages, None, table, [200, 90], [0, 2, 5], None, 0, 0)
+    mine = torch.full_like(out, 7.0)
+    paged.paged_attn(dq, dp, dt, lens, cu, 512 ** -0.5, out=mine)
+    assert (mine[:3] == 7).all() and (mine[8:] == 7).all() and torch.equal(mine[3:8], out[3:8])
+    none = paged.paged_attn(dq, dp, dt, lens, _i32([0, 0, 0], dev), 512 ** -0.5)
+    assert (none == 0).all() and paged.paged_attn(dq[:0], dp, dt, lens, _i32([0, 0, 0], dev), 512 ** -0.5).shape == (0, 16, 512)
+
+
+def test_attn_signs_shared_tables_and_odd_addresses(dev):
+    """A negative scale is the negated query's; sequences may share a table, a page may come twice in one; a query
+    that is not on a 16-byte address is the same query."""
+    from smla import paged
+    announce("paged_attn scale < 0, an expanded table, a repeated page, q at an odd address")
+    pages, _, _ = _cache(82, [160], 16, 576)
+    g = torch.Generator().manual_seed(6)
+    q = torch.randn(6, 3, 576, generator=g).to(torch.bfloat16)
+    table = torch.tensor([[4, 1, 1, 7, 4, 0]], dtype=torch.int32)
+    dq, dp, dt = _to(dev, q, pages, table)
+    lens, cu = [90, 33, 96], [0, 1, 4, 6]
+    args = (dp, dt.expand(3, 6), _i32(lens, dev), _i32(cu, dev))
+    out = paged.paged_attn(dq, *args, 576 ** -0.5)
+    _check_attn(out, q, pages, None, table.expand(3, 6), lens, cu, None, 0, 0)
+    assert torch.equal(paged.paged_attn(-dq, *args, -(576 ** -0.5)), out)
+    odd = torch.empty(dq.numel() + 1, dtype=torch.bfloat16, device=dev)[1:].view_as(dq)
+    odd.copy_(dq)
+    assert torch.equal(paged.paged_attn(odd, *args, 576 ** -0.5), out)
+
+
+@pytest.mark.parametrize("kv,D,P,n_pages", [("bf16", 576, 64, 70000), ("fp8", 512, 64, 150000)])
+def test_rows_past_32_bit_offsets(dev, kv, D, P, n_pages):
+    """Append, attention, a fork and a compaction on pages that lie past 4 GiB from the pool's start."""
+    from smla import paged
+    announce(f"a pool of {n_pages * P * D * (1 if kv == 'fp8' else 2) / 2 ** 30:.1f} GiB, {kv}")
+    g = torch.Generator().manual_seed(7)
+    lens, H = [200, 130], 16
+    small, sscale, stable = _cache(83, lens, P, D, kv, extra=0)
+    n_small = small.shape[0]
+    base = n_pages - n_small - 1        # the last page stays free for the fork
+    assert base * P * D * (1 if kv == "fp8" else 2) > 1 << 32
+    pages = torch.empty(n_pages, P, D, dtype=torch.uint8 if kv == "fp8" else torch.bfloat16, device=dev)
+    scales = None if kv != "fp8" else torch.empty(n_pages, P, D // 64, device=dev)
+    pages[base:base + n_small] = small.view(torch.uint8).to(dev) if kv == "fp8" else small.to(dev)
+    if scales is not None:
+        scales[base:base + n_small] = sscale.to(dev)
+    table = torch.where(stable >= 0, stable + base, stable)
+    q = torch.randn(3, H, D, generator=g).to(torch.bfloat16)
+    cu = [0, 1, 3]
+    dq, dt = _to(dev, q, table)
+    out = paged.paged_attn(dq, pages, dt, _i32(lens, dev), _i32(cu, dev), D ** -0.5, page_scales=scales)
+    _check_attn(out, q, small, sscale, stable, lens, cu, None, 0, 0)
+    # the newest three rows again, by an append of the same token: rows of unit size, elsewhere as they were
+    x = torch.randn(3, D, generator=g)
+    cos, sin = _tables(dev, 256, 64)
+    before = pages[base:base + n_small].clone()
+    paged.paged_append(None, x.to(dev), pages, dt, _i32(lens, dev), _i32(cu, dev), *_to(dev, cos, sin), page_scales=scales)
+    changed = (pages[base:base + n_small] != before).any(-1).cpu()
+    want = torch.zeros_like(changed)
+    for b, p in ((0, 199), (1, 128), (1, 129)):
+        want[stable[b, p // P], p % P] = True
+    assert torch.equal(changed, want)
+    # slot 1 becomes a copy of slot 0, whose tail page goes to the pool's last page
+    refs = torch.ones(n_pages, dtype=torch.int32, device=dev)
+    refs[-1] = 0
+    t2, l2, r2, ok = paged.update_pages(pages, dt, _i32(lens, dev), refs, _i32([0, 0], dev), _i32([0, 0], dev), page_scales=scales)
+    assert ok.tolist() == [1, 1] and l2.tolist() == [200, 200] and int(t2[1, 3]) == n_pages - 1
+    assert torch.equal(pages[-1, :8].view(torch.uint8), pages[int(dt[0, 3]), :8].view(torch.uint8))
+    if scales is not None:
+        assert torch.equal(scales[-1, :8], scales[int(dt[0, 3]), :8])
+    # only the two slots' pages are live: they move to the pool's start
+    refs = torch.zeros_like(refs)
+    for page in t2[t2 >= 0].tolist():
+        refs[page] += 1
+    rows = [pages[t2[s].long()].reshape(-1, D)[:200].clone().view(torch.uint8) for s in range(2)]
+    t3, r3, live = paged.compact_pages(pages, t2, refs, page_scales=scales)
+    assert int(live) == int((refs > 0).sum()) == int(t3.max()) + 1 and int(r3.sum()) == int(refs.sum())
+    for s in range(2):
+        assert torch.equal(pages[t3[s].long()].reshape(-1, D)[:200].view(torch.uint8), rows[s])
+
+
+def test_layers_past_32_bit_offsets(dev):
+    """One launch over layers of more than 4 GiB together: a fork copies its tail page, and a compaction moves pages, in each."""
+    from smla import paged
+    announce("update and compact over 5 layers of 0.9 GiB")
+    layers, n_pages, P, D = 5, 13000, 64, 576
+    pages = torch.empty(layers, n_pages, P, D, dtype=torch.bfloat16, device=dev)
+    fill = torch.randn(layers, 2, P, D, generator=torch.Generator().manual_seed(9)).to(torch.bfloat16).to(dev)
+    pages[:, -2:] = fill
+    table = _i32([[n_pages - 2, n_pages - 1], [-1, -1]], dev)
+    refs = torch.zeros(n_pages, dtype=torch.int32, device=dev)
+    refs[-2:] = 1
+    args = table, _i32([100, 0], dev), refs, _i32([0, 0], dev), _i32([0, 3], dev)
+    t2, l2, r2, ok = paged.update_pages(pages, *args)
+    assert t2.tolist() == [[n_pages - 2, n_pages - 1], [n_pages - 2, 0]] and l2.tolist() == [100, 103] and ok.tolist() == [1, 1]
+    assert torch.equal(pages[:, 0, :36], fill[:, 1, :36])
+    t3, r3, live = paged.compact_pages(pages, t2, r2)
+    assert t3.tolist() == [[1, 2], [1, 0]] and int(live) == 3 and r3[:3].tolist() == [1, 2, 1]
+    assert torch.equal(pages[:, 1:3], fill) and torch.equal(pages[:, 0, :36], fill[:, 1, :36])
+
+
+def test_two_graphs_and_several_calls_in_one(dev):
+    """Two calls captured into one graph and one into another: every replay gives what the eager calls give, whichever ran
+    before, with the lengths of the moment."""
+    from smla import paged
+    announce("paged_attn in two graphs")
+    pages, _, table = _cache(84, [700, 300], 16, 576)
+    q = torch.randn(2, 64, 576, generator=torch.Generator().manual_seed(8)).to(torch.bfloat16)
+    dq, dp, dt = _to(dev, q, pages, table)
+    lens, cu = _i32([700, 300], dev), _i32([0, 1, 2], dev)
+    one = lambda: paged.paged_attn(dq, dp, dt, lens, cu, 576 ** -0.5)  # noqa: E731
+    two = lambda: paged.paged_attn(dq, dp, dt, lens, cu, 576 ** -0.5, window=100, first=2)  # noqa: E731
+    one(), two()
+    torch.cuda.synchronize()
+    a, b = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(a):
+        a_one, a_two = one(), two()
+    with torch.cuda.graph(b):
+        b_one = one()
+    for k, n in enumerate(([700, 300], [1, 300], [512, 33], [699, 0], [700, 300])):
+        lens.copy_(_i32(n, dev))
+        (a if k % 2 else b).replay()
+        (b if k % 2 else a).replay()
+        torch.cuda.synchronize()
+        want = one(), two()
+        assert torch.equal(a_one, want[0]) and torch.equal(a_two, want[1]) and torch.equal(b_one, want[0]), n
+
+
 # ---------------------------------------------------------------------------------------------
 def _tables(dev, n, rd):
     a = torch.arange(n, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(0, rd, 2, dtype=torch.float64) / max(rd, 1))

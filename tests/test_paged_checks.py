@@ -35,6 +35,8 @@ ATTN_OK = dict(q=FAKE, q_dtype=BF16, pages=FAKE, page_dtype=BF16, page_scales=No
     (dict(window=-1), RANGE), (dict(first=-1), RANGE), (dict(window=1 << 30), RANGE), (dict(flags=1), RANGE),
     (dict(n_pages=1 << 20, P=1 << 12), RANGE), (dict(B=1 << 20), RANGE), (dict(T=1 << 30), RANGE), (dict(cols=1 << 31, ld_table=1 << 31), RANGE),
     (dict(ws=None), WS), (dict(ws_bytes=100), WS), (dict(ws=ctypes.c_void_p(4104)), WS),
+    (dict(T=1), UNSUP), (dict(T=1, out=ctypes.c_void_p(4096 + 16 * 576 * 2 - 16)), UNSUP),    # out over q
+    (dict(T=1, q=ctypes.c_void_p(4096 + 16 * 512 * 2 - 16)), UNSUP),
 ])
 def test_paged_attn_arguments(change, status):
     assert _call("smla_paged_attn", ATTN, ATTN_OK, **change) == status
@@ -135,3 +137,35 @@ def test_python_checks():
                             (i32(2, 4), i32(3), i32(3)), (i32(2, 4), i32(2), i32(2)), (i32(2, 4), i32(2).long(), i32(3))):
         with pytest.raises(ValueError):
             ops._check_batch(table, lens, cu)
+
+
+def _paged_calls():
+    from smla import paged
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    bf = lambda *s: torch.empty(*s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    f32 = lambda *s: torch.empty(*s, device="cuda")  # noqa: E731
+    yield ("attn", lambda q, p, t, n, c, s: paged.paged_attn(q, p, t, n, c, 0.04, s, 128, 4),
+           lambda: (bf(9, 16, 576), bf(20, 16, 576), i32(3, 8), i32(3), i32(4), f32(16)), (9, 16, 512), "paged_attn_")
+    yield ("append", lambda q, x, p, t, n, c, cs, sn: paged.paged_append(q, x, p, t, n, c, cs, sn, kv_norm=True),
+           lambda: (f32(9, 16, 512), f32(9, 512), bf(20, 16, 512), i32(3, 8), i32(3), i32(4), f32(128, 32), f32(128, 32)),
+           (9, 16, 512), "paged_append_")
+    yield ("update", lambda p, t, n, r, a, g: paged.update_pages(p, t, n, r, a, g)[0],
+           lambda: (bf(20, 16, 512), i32(3, 8), i32(3), i32(20), i32(3), i32(3)), (3, 8), "update_pages")
+    yield ("compact", lambda p, t, r: paged.compact_pages(p, t, r)[0], lambda: (bf(20, 16, 512), i32(3, 8), i32(20)), (3, 8),
+           "compact_pages")
+
+
+@pytest.mark.parametrize("name,fn,args,shape,op", list(_paged_calls()), ids=lambda v: v if isinstance(v, str) else "")
+def test_paged_calls_trace_as_their_ops(name, fn, args, shape, op):
+    """Without memory behind the tensors nothing but the op itself may ask for a pointer."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    class Call(torch.nn.Module):
+        def forward(self, *a):
+            return fn(*a)
+
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        a = args()
+        assert tuple(fn(*a).shape) == shape
+    program = torch.export.export(Call(), a, strict=False)
+    assert f"smla.{op}.default" in [str(n.target) for n in program.graph.nodes if n.op == "call_function"]
