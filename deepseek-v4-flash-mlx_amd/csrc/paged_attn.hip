@@ -942,101 +942,122 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedArgs
 }
 
 // ---------------------------------------------------------------------------------------------
-// Joins the states of split tiles: a workgroup of 4 waves takes a 1 KB piece (8 values of 32 q rows, twice) of one tile,
-// wave w the splits w, w + 4, .. eight at a time with a running maximum, the waves' sums then through LDS in a
-// fixed order.  Workgroups walk the pieces of all split tiles; with `fill` they also clear the rows behind the
-// last sequence.
+// Joins the states of split tiles, in pieces of 1 KB (8 values of 32 q rows, twice).  A workgroup of 4 waves takes GROUP
+// pieces of a tile at a time: one piece by all four, wave w the splits w, w + 4, .. with a running maximum, the waves'
+// sums then through LDS in a fixed order; where there are many tiles (GROUP 4) and a tile has no more than four splits, a
+// piece a wave, which needs no LDS and no barriers (1366 tiles of 2 or 3 splits: 107 us against 250).
+// Workgroups walk the pieces of all split tiles; with `fill` they also clear the tokens of no sequence.
 constexpr int kMergeWaves = 4, kMergeBatch = 8;
 
-template <int D, int NB>
+template <int D, int NB, int GROUP>
 __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const PagedArgs a) {
   using G = GeoP<D, NB>;
   constexpr int kPieces = kUnits * NB * 2;
   __shared__ float red[kMergeWaves][64][10];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const Seq s0 = load_seq<G::TILEQ>(a, lane);
   const int rps = __builtin_amdgcn_readfirstlane(*(const int*)a.ws);
-  for (int64_t x = blockIdx.x;; x += gridDim.x) {
+  constexpr uint32_t kGroups = kPieces / GROUP;
+  for (uint32_t x = blockIdx.x;; x += gridDim.x) {
     Item it;
-    const int tile = (int)(x / kPieces), piece = (int)(x - (int64_t)tile * kPieces);
-    if (!find_item<G::TILEQ>(a, s0, lane, rps, tile, true, it)) break;
+    const uint32_t tile = x / kGroups, piece0 = (x - tile * kGroups) * GROUP;
+    if (!find_item<G::TILEQ>(a, s0, lane, rps, (int)tile, true, it)) break;
+    if (it.slot + it.nsplit > a.slots) continue;
     const int m0 = it.tile * G::TILEQ, rows_b = it.s.n * a.H;
-    const int u = piece / (2 * NB), n = (piece >> 1) % NB, half = piece & 1;
-    if (it.slot + it.nsplit > a.slots || m0 + 32 * n >= rows_b) continue;
-    const int vi = u < 4 ? 0 : (u - 1) / 3;
-    const int row = 32 * n + (lane & 31);
-    float m = -SMLA_INF, l = 0.f, acc[8];
+    // the splits from, from + step, .. of a piece: maximum, sum, values
+    struct Sum {
+      float m, l, acc[8];
+    };
+    auto gather = [&](int piece, int from, int step) -> Sum {
+      const int u = piece / (2 * NB), n = (piece >> 1) % NB, vi = u < 4 ? 0 : (u - 1) / 3, row = 32 * n + (lane & 31);
+      Sum t;
+      t.m = -SMLA_INF;
+      t.l = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; k++) acc[k] = 0.f;
-    for (int sp0 = wave; sp0 < it.nsplit; sp0 += kMergeWaves * kMergeBatch) {
-      f32x2_t ml[kMergeBatch];
-      float sc[kMergeBatch];
-      u32x4_t v[kMergeBatch];
+      for (int k = 0; k < 8; k++) t.acc[k] = 0.f;
+      for (int sp0 = from; sp0 < it.nsplit; sp0 += step * kMergeBatch) {
+        f32x2_t ml[kMergeBatch];
+        float sc[kMergeBatch];
+        u32x4_t v[kMergeBatch];
 #pragma unroll
-      for (int k = 0; k < kMergeBatch; k++) {
-        const int sp = sp0 + kMergeWaves * k;
-        if (sp < it.nsplit) {
-          const float* f = state_f<G>(a, it.slot + sp);
-          ml[k] = *(const f32x2_t*)(f + 2 * row);
-          sc[k] = f[2 * G::TILEQ + (vi * NB + n) * 64 + lane];
-          v[k] = *(const u32x4_t*)(state_o<G>(a, it.slot + sp) + piece * 1024 + 16 * lane);
-        }
-      }
-      float top = m;
-#pragma unroll
-      for (int k = 0; k < kMergeBatch; k++)
-        if (sp0 + kMergeWaves * k < it.nsplit) top = fmaxf(top, ml[k][0]);
-      const float keep = m > -SMLA_INF ? __builtin_amdgcn_exp2f(m - top) : (top == m ? 1.f : 0.f);
-      l *= keep;
-#pragma unroll
-      for (int j = 0; j < 8; j++) acc[j] *= keep;
-      m = top;
-#pragma unroll
-      for (int k = 0; k < kMergeBatch; k++)
-        if (sp0 + kMergeWaves * k < it.nsplit) {
-          // a state without a maximum has l = 0 (nothing seen) or NaN
-          const float e = ml[k][0] > -SMLA_INF ? __builtin_amdgcn_exp2f(ml[k][0] - m) : 1.f;
-          l += ml[k][1] * e;
-          const float es = e * sc[k];
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const uint32_t word = v[k][j];  // (a bit cast of a vector's element itself takes element 0)
-            const f16x2_t h2 = __builtin_bit_cast(f16x2_t, word);
-            acc[2 * j] += (float)h2[0] * es;
-            acc[2 * j + 1] += (float)h2[1] * es;
+        for (int k = 0; k < kMergeBatch; k++) {
+          const int sp = sp0 + step * k;
+          if (sp < it.nsplit) {
+            const float* f = state_f<G>(a, it.slot + sp);
+            ml[k] = *(const f32x2_t*)(f + 2 * row);
+            sc[k] = f[2 * G::TILEQ + (vi * NB + n) * 64 + lane];
+            v[k] = *(const u32x4_t*)(state_o<G>(a, it.slot + sp) + piece * 1024 + 16 * lane);
           }
         }
-    }
-    __syncthreads();  // the last piece's sums are read
-    red[wave][lane][0] = m;
-    red[wave][lane][1] = l;
+        float top = t.m;
 #pragma unroll
-    for (int j = 0; j < 8; j++) red[wave][lane][2 + j] = acc[j];
-    __syncthreads();
-    if (wave == 0) {
-      float top = m;
+        for (int k = 0; k < kMergeBatch; k++)
+          if (sp0 + step * k < it.nsplit) top = fmaxf(top, ml[k][0]);
+        const float keep = t.m > -SMLA_INF ? __builtin_amdgcn_exp2f(t.m - top) : (top == t.m ? 1.f : 0.f);
+        t.l *= keep;
 #pragma unroll
-      for (int k = 1; k < kMergeWaves; k++) top = fmaxf(top, red[k][lane][0]);
-      float sum = 0.f, y[8];
+        for (int j = 0; j < 8; j++) t.acc[j] *= keep;
+        t.m = top;
 #pragma unroll
-      for (int j = 0; j < 8; j++) y[j] = 0.f;
+        for (int k = 0; k < kMergeBatch; k++)
+          if (sp0 + step * k < it.nsplit) {
+            // a state without a maximum has l = 0 (nothing seen) or NaN
+            const float e = ml[k][0] > -SMLA_INF ? __builtin_amdgcn_exp2f(ml[k][0] - t.m) : 1.f;
+            t.l += ml[k][1] * e;
+            const float es = e * sc[k];
 #pragma unroll
-      for (int k = 0; k < kMergeWaves; k++) {
-        const float mk = red[k][lane][0], e = mk > -SMLA_INF ? __builtin_amdgcn_exp2f(mk - top) : 1.f;
-        sum += red[k][lane][1] * e;
-#pragma unroll
-        for (int j = 0; j < 8; j++) y[j] += red[k][lane][2 + j] * e;
+            for (int j = 0; j < 4; j++) {
+              const uint32_t word = v[k][j];  // (a bit cast of a vector's element itself takes element 0)
+              const f16x2_t h2 = __builtin_bit_cast(f16x2_t, word);
+              t.acc[2 * j] += (float)h2[0] * es;
+              t.acc[2 * j + 1] += (float)h2[1] * es;
+            }
+          }
       }
-      if (m0 + row < rows_b) {
-        float inv = 0.f;
-        if (!(sum == 0.f)) {
-          const float snk = a.sink ? a.sink[(uint32_t)(m0 + row) % (uint32_t)a.H] : -SMLA_INF;
-          inv = 1.0f / (sum + (snk == -SMLA_INF ? 0.f : __builtin_amdgcn_exp2f(snk * 1.44269504088896340736f - top)));
-        }
-        u32x4_t o;
+      return t;
+    };
+    auto finish = [&](int piece, const Sum& t) {
+      const int u = piece / (2 * NB), n = (piece >> 1) % NB, half = piece & 1, row = 32 * n + (lane & 31);
+      if (m0 + row >= rows_b) return;
+      float inv = 0.f;
+      if (!(t.l == 0.f)) {
+        const float snk = a.sink ? a.sink[(uint32_t)(m0 + row) % (uint32_t)a.H] : -SMLA_INF;
+        inv = 1.0f / (t.l + (snk == -SMLA_INF ? 0.f : __builtin_amdgcn_exp2f(snk * 1.44269504088896340736f - t.m)));
+      }
+      u32x4_t o;
 #pragma unroll
-        for (int j = 0; j < 4; j++) o[j] = pack2(y[2 * j] * inv, y[2 * j + 1] * inv);
-        *(u32x4_t*)(a.out + ((int64_t)it.s.beg * a.H + m0 + row) * 512 + 32 * u + 16 * half + 8 * (lane >> 5)) = o;
+      for (int j = 0; j < 4; j++) o[j] = pack2(t.acc[2 * j] * inv, t.acc[2 * j + 1] * inv);
+      *(u32x4_t*)(a.out + ((int64_t)it.s.beg * a.H + m0 + row) * 512 + 32 * u + 16 * half + 8 * (lane >> 5)) = o;
+    };
+    if constexpr (GROUP == kMergeWaves)
+      if (it.nsplit <= kMergeWaves) {
+        finish((int)piece0 + wave, gather((int)piece0 + wave, 0, 1));
+        continue;
+      }
+    for (int piece = (int)piece0; piece < (int)piece0 + GROUP; piece++) {
+      const Sum t = gather(piece, wave, kMergeWaves);
+      __syncthreads();  // the last piece's sums are read
+      red[wave][lane][0] = t.m;
+      red[wave][lane][1] = t.l;
+#pragma unroll
+      for (int j = 0; j < 8; j++) red[wave][lane][2 + j] = t.acc[j];
+      __syncthreads();
+      if (wave == 0) {
+        Sum y;
+        y.m = t.m;
+#pragma unroll
+        for (int k = 1; k < kMergeWaves; k++) y.m = fmaxf(y.m, red[k][lane][0]);
+        y.l = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) y.acc[j] = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMergeWaves; k++) {
+          const float mk = red[k][lane][0], e = mk > -SMLA_INF ? __builtin_amdgcn_exp2f(mk - y.m) : 1.f;
+          y.l += red[k][lane][1] * e;
+#pragma unroll
+          for (int j = 0; j < 8; j++) y.acc[j] += red[k][lane][2 + j] * e;
+        }
+        finish(piece, y);
       }
     }
   }
@@ -1080,8 +1101,9 @@ int launch_paged(const PagedArgs& a, int64_t tiles, hipStream_t st) {
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * kWaves), G::LDS_BYTES, st, a);
   SMLA_HIP_CHECK_LAUNCH();
   const int64_t pieces = tiles * kUnits * NB * 2, most = 8 * (int64_t)a.cus;
-  hipLaunchKernelGGL((paged_merge_kernel<D, NB>), dim3((unsigned)(pieces < most ? pieces : most)), dim3(64 * kMergeWaves), 0,
-                     st, a);
+  const dim3 grid2((unsigned)(pieces < most ? pieces : most)), block2(64 * kMergeWaves);
+  if (pieces >= kMergeWaves * most) hipLaunchKernelGGL((paged_merge_kernel<D, NB, kMergeWaves>), grid2, block2, 0, st, a);
+  else hipLaunchKernelGGL((paged_merge_kernel<D, NB, 1>), grid2, block2, 0, st, a);
   SMLA_HIP_CHECK_LAUNCH();
   return SMLA_OK;
 }
