@@ -943,11 +943,12 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedArgs
 
 // ---------------------------------------------------------------------------------------------
 // Joins the states of split tiles, in pieces of 1 KB (8 values of 32 q rows, twice).  A workgroup of 4 waves takes GROUP
-// pieces of a tile at a time: one piece by all four, wave w the splits w, w + 4, .. with a running maximum, the waves'
-// sums then through LDS in a fixed order; where there are many tiles (GROUP 4) and a tile has no more than four splits, a
-// piece a wave, which needs no LDS and no barriers (1366 tiles of 2 or 3 splits: 107 us against 250).
+// pieces of a tile at a time.  One piece by all four: wave w the splits w, w + 4, .. with a running maximum, the waves'
+// sums then through LDS in a fixed order.  Where there are pieces enough (GROUP 4) and a tile has at most kAlone splits,
+// a piece a wave, which needs no LDS and no barriers: 1366 tiles of 2 or 3 splits 106 us against 254 (4.2 TB/s), 64 tiles of
+// 3 to 6 8.5 against 13.9, 32 tiles of 8 9.6 against 12.9.
 // Workgroups walk the pieces of all split tiles; with `fill` they also clear the tokens of no sequence.
-constexpr int kMergeWaves = 4, kMergeBatch = 8;
+constexpr int kMergeWaves = 4, kMergeBatch = 8, kAlone = 16;
 
 template <int D, int NB, int GROUP>
 __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const PagedArgs a) {
@@ -1030,7 +1031,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
       *(u32x4_t*)(a.out + ((int64_t)it.s.beg * a.H + m0 + row) * 512 + 32 * u + 16 * half + 8 * (lane >> 5)) = o;
     };
     if constexpr (GROUP == kMergeWaves)
-      if (it.nsplit <= kMergeWaves) {
+      if (it.nsplit <= kAlone) {
         finish((int)piece0 + wave, gather((int)piece0 + wave, 0, 1));
         continue;
       }
@@ -1102,7 +1103,7 @@ int launch_paged(const PagedArgs& a, int64_t tiles, hipStream_t st) {
   SMLA_HIP_CHECK_LAUNCH();
   const int64_t pieces = tiles * kUnits * NB * 2, most = 8 * (int64_t)a.cus;
   const dim3 grid2((unsigned)(pieces < most ? pieces : most)), block2(64 * kMergeWaves);
-  if (pieces >= kMergeWaves * most) hipLaunchKernelGGL((paged_merge_kernel<D, NB, kMergeWaves>), grid2, block2, 0, st, a);
+  if (pieces >= kMergeWaves * (int64_t)a.cus) hipLaunchKernelGGL((paged_merge_kernel<D, NB, kMergeWaves>), grid2, block2, 0, st, a);
   else hipLaunchKernelGGL((paged_merge_kernel<D, NB, 1>), grid2, block2, 0, st, a);
   SMLA_HIP_CHECK_LAUNCH();
   return SMLA_OK;
