@@ -20,9 +20,17 @@
 //   * value waves 3 .. 7: O^T += V^T P^T (v_mfma_f32_32x32x16_bf16) of 3 or 4 blocks of 32 value columns and all
 //     the tile's q rows, so each V^T fragment (ds_read_b64_tr_b16) is read by one wave and serves NB products.
 //     Wave 3 shares its SIMD with value wave 7 instead of a score wave and takes four blocks, the others three.
-// At NB = 3 the matrix pipes of SIMDs 0 .. 2 have 1152 + 576 cycles a tile, SIMD 3 has 1344, against about
-// 6.8 KB of LDS traffic a row (53 cycles of 128 bytes): both near balance, where 64 q rows on 12
-// waves of 168 registers (16 rows' Q^T a score wave) read 8.4 KB for two thirds of the products.
+// At NB = 3 the matrix pipes of SIMDs 0 .. 2 have 1152 + 576 cycles a tile (D = 576), SIMD 3 has 1344, and the LDS about
+// 850 (6.8 KB a row at 256 bytes a cycle).  A form with 64 q rows on 12 waves of 168 registers (16 rows' Q^T a score
+// wave) read 8.4 KB a row for two thirds of the products and was 11.6 ms where this one is 7.9.
+// NB = 2 (64 q rows) where a step has few: those steps are bound by the rows' arrival, and a tile has fewer products
+// to wait for.
+//
+// What bounds it, measured: a 2048-token chunk at 32 K (64 heads, D 576) 7.6 to 8.0 ms = 1130 to 1190 TFLOP/s, the matrix
+// pipes (a large library product reaches 1261 on the card); a decode step of 32 sequences of 2 K to 32 K rows 156 us =
+// 5.0 TB/s, HBM; drafts of 64 sequences over fp8 rows 110 us, the conversion to bf16 beside the products; a 4096-token
+// prompt in a 128-row window 200 us, five row tiles an item behind Q's arrival and before the output's leaving (Q and
+// out alone are 113 us of HBM); one token over 4 K rows 11 us and 6 us for the join, latencies.
 //
 // Rows come HBM -> LDS by DMA into a ring of four tiles, copies issued by the value waves (fp8 rows: loaded,
 // converted, written).  Row numbers go through an LDS ring of 8 tiles that score wave 0 fills six tiles
@@ -42,7 +50,7 @@ typedef __attribute__((address_space(3))) u32x2_t lds_u32x2_t;
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kIdTiles = 8;        // tiles of the row-number ring
-constexpr int kMinRows = 64;       // fewest entries of an item
+constexpr int kMinRows = 64;       // fewest entries of an item (one token over 4 K rows, with the join: 64 17.7 us, 128 18.3, 256 20.7)
 constexpr int kMinRowsMany = 256;  // the same with more tiles than compute units
 constexpr int kMinPart = 4096, kMostParts = 4, kMostItems = 16, kPartRows = 256;  // parts of many tiles (plan_rps)
 constexpr int kHeader = 256;       // workspace bytes before the states
