@@ -23,8 +23,7 @@
 // At NB = 3 the matrix pipes of SIMDs 0 .. 2 have 1152 + 576 cycles a tile (D = 576), SIMD 3 has 1344, and the LDS about
 // 850 (6.8 KB a row at 256 bytes a cycle).  A form with 64 q rows on 12 waves of 168 registers (16 rows' Q^T a score
 // wave) read 8.4 KB a row for two thirds of the products and was 11.6 ms where this one is 7.9.
-// NB = 2 (64 q rows) where a step has few: those steps are bound by the rows' arrival, and a tile has fewer products
-// to wait for.
+// NB = 2 (64 q rows) where that makes no more tiles (tile_blocks).
 //
 // What bounds it, measured: a 2048-token chunk at 32 K (64 heads, D 576) 7.6 to 8.0 ms = 1130 to 1190 TFLOP/s, the matrix
 // pipes (a large library product reaches 1261 on the card); a decode step of 32 sequences of 2 K to 32 K rows 156 us =
@@ -1092,9 +1091,14 @@ int64_t most_entries(int64_t rows, int64_t window, int64_t first, int64_t H) {
   const int64_t w = window + first + 128 + H;
   return window > 0 && w < rows ? w : rows;
 }
-// q rows per tile / 32: where the sequences have no more than 64 on average (steps of one or few tokens, bound by the
-// rows' arrival), tiles of 64 have fewer products to wait for; longer runs of q rows share a row among 96
-int tile_blocks(int64_t T, int64_t H, int64_t B) { return T * H <= 64 * B ? 2 : 3; }
+// q rows per tile / 32: 64 where the sequences' q rows, on average, make no more tiles than 96 would, since such a tile has
+// fewer products (and a wave free to convert fp8 rows); else 96, which read the rows less often.  Measured, 64 / 96: 64 q rows
+// a sequence 157 / 161 us (32 sequences of 2 K to 32 K rows), up to 64 over fp8 110 / 157, 128 122 / 131 (fp8 104 / 133),
+// 192 175 / 138, a 2048-token chunk 8.99 / 7.92 ms
+int tile_blocks(int64_t T, int64_t H, int64_t B) {
+  const int64_t r = (T * H + B - 1) / B;
+  return (r + 63) / 64 <= (r + 95) / 96 ? 2 : 3;
+}
 bool plan_sizes(int64_t T, int64_t H, int64_t B) {
   return T >= 0 && H > 0 && B > 0 && T <= 0x7fffffff && H <= 0x7fffffff && B <= 0xfffff && T * H <= 0x7fffff80;
 }

@@ -100,6 +100,15 @@ def test_attn_head_layouts_and_pages(dev, H, D, P, kv):
     _run_attn(dev, [1, 5, 2, 7], [1, 5, 67, 130], H, D, P, kv, seed=H + P)
 
 
+@pytest.mark.parametrize("n", [2, 3, 4, 5, 6, 7])
+@pytest.mark.parametrize("kv,D", [("bf16", 576), ("fp8", 512)])
+def test_attn_tiles_of_both_sizes(dev, n, kv, D):
+    """64 to 224 q rows a sequence: tiles of 64 and of 96, full and partly filled."""
+    announce(f"paged_attn {n} tokens of 32 heads {kv}")
+    _run_attn(dev, [n, n, n], [n, 150, 333], 32, D, 16, kv, seed=n)
+    _run_attn(dev, [1, n, 2 * n - 1], [70, 150, 333], 32, D, 16, kv, window=50, first=3, seed=n + 10)
+
+
 @pytest.mark.parametrize("lens", [[1], [2], [31], [32], [33], [63, 64, 65], [95, 96, 97, 127, 128, 129, 255, 256, 257]])
 def test_attn_one_token_lengths(dev, lens):
     announce(f"paged_attn one token, lens={lens}")
