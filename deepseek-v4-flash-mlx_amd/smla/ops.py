@@ -955,23 +955,25 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 
 
 def _one_device(t, *rest):
-    """All tensors on t's GPU (one launch reads them all)."""
+    """The number of t's GPU, where all tensors have to be (one launch reads them all)."""
     dev = t.get_device()
     if dev < 0:
         _on_gpu(t)
     for r in rest:
         if r is not None and r.get_device() != dev:
             raise RuntimeError(f"smla paged ops run on one GPU: got tensors on {t.device} and {r.device}")
+    return dev
 
 
-def _launch(t, name, *args):
-    """``_lib.call`` with t's device current (a launch goes to a stream of the current device)."""
-    dev = t.get_device()
+def _launch(dev, name, *args):
+    """``_lib.call`` with GPU dev current (a launch goes to a stream of the current device)."""
     if _current_device() == dev:
-        _lib.call(name, *args, _raw_stream(dev))
+        status = getattr(_lib._LIB or _lib.lib(), name)(*args, _raw_stream(dev))
     else:
-        with torch.cuda.device(t.device):
-            _lib.call(name, *args, _stream(t))
+        with torch.cuda.device(dev):
+            status = getattr(_lib.lib(), name)(*args, _raw_stream(dev))
+    if status != 0:
+        _lib.check(name, status)
 
 
 def _f32(t):
@@ -1020,7 +1022,7 @@ def _paged_attn_(q: torch.Tensor, pages: torch.Tensor, page_scales: Optional[tor
                  lens: torch.Tensor, cu: torch.Tensor, attn_sink: Optional[torch.Tensor], scale: float, window: int,
                  first: int, fill: bool, out: torch.Tensor) -> None:
     """``smla_paged_attn`` into out [T, H, DV] (see ``paged.paged_attn``)."""
-    _one_device(q, pages, page_scales, table, lens, cu, attn_sink, out)
+    dev = _one_device(q, pages, page_scales, table, lens, cu, attn_sink, out)
     if q.dim() != 3 or out.dim() != 3 or out.shape[:2] != q.shape[:2]:
         raise ValueError(f"expected q [T,H,D] and out [T,H,dv], got {list(q.shape)} and {list(out.shape)}")
     T, H, D = q.shape
@@ -1043,7 +1045,7 @@ def _paged_attn_(q: torch.Tensor, pages: torch.Tensor, page_scales: Optional[tor
         q = q.clone(memory_format=torch.contiguous_format)
     wsb = _lib.lib().smla_paged_attn_workspace(T, H, B, cols * P, window, first)
     ws = torch.empty(wsb, dtype=torch.uint8, device=q.device)
-    _launch(q, "smla_paged_attn", q.data_ptr(), _lib.BF16, pages.data_ptr(), code, _p(page_scales), n_pages, P,
+    _launch(dev, "smla_paged_attn", q.data_ptr(), _lib.BF16, pages.data_ptr(), code, _p(page_scales), n_pages, P,
             table.data_ptr(), ld, cols, lens.data_ptr(), cu.data_ptr(), B, T, H, D, out.shape[2], scale, _p(attn_sink), window, first, _lib.PAGED_FILL if fill else 0, out.data_ptr(), _lib.BF16,
             ws.data_ptr(), wsb)
 
@@ -1070,7 +1072,7 @@ def _paged_append_(q: Optional[torch.Tensor], kv: torch.Tensor, pages: torch.Ten
                    q_norm: Optional[torch.Tensor], kv_norm: Optional[torch.Tensor], norm_dims: int, fp8_sim: bool,
                    eps: float, flags: int, q_out: Optional[torch.Tensor]) -> None:
     """``smla_paged_append`` (see ``paged.paged_append``)."""
-    _one_device(kv, q, pages, page_scales, table, lens, cu, cos_t, sin_t, q_norm, kv_norm, q_out)
+    dev = _one_device(kv, q, pages, page_scales, table, lens, cu, cos_t, sin_t, q_norm, kv_norm, q_out)
     if kv.dim() != 2:
         raise ValueError("expected kv [T,D]")
     T, D = kv.shape
@@ -1111,7 +1113,7 @@ def _paged_append_(q: Optional[torch.Tensor], kv: torch.Tensor, pages: torch.Ten
         return
     if T == 1:
         ldq, ldkv = H * D, D
-    _launch(kv, "smla_paged_append", _p(q), ldq, kv.data_ptr(), ldkv, xdt, T, H, D, norm_dims, _p(q_norm), _p(kv_norm),
+    _launch(dev, "smla_paged_append", _p(q), ldq, kv.data_ptr(), ldkv, xdt, T, H, D, norm_dims, _p(q_norm), _p(kv_norm),
             cos_t.data_ptr(), sin_t.data_ptr(), n_pos, 2 * rd2, eps, _lib.SIM_FP8 if fp8_sim else _lib.SIM_NONE, flags,
             _p(q_out), pages.data_ptr(), code, _p(page_scales), n_pages, P, table.data_ptr(), ld, cols, lens.data_ptr(),
             cu.data_ptr(), B)
@@ -1143,7 +1145,7 @@ def _update_pages(pages: torch.Tensor, page_scales: Optional[torch.Tensor], tabl
                   refs: torch.Tensor, parent: torch.Tensor, grow: torch.Tensor
                   ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """``smla_update_pages`` (see ``paged.update_pages``): new (table, lens, refs, granted)."""
-    _one_device(pages, page_scales, table, lens, refs, parent, grow)
+    dev = _one_device(pages, page_scales, table, lens, refs, parent, grow)
     n_pages, P, pool, scales = _pool_args(pages, page_scales)
     table = _i32_rows(table, "table")
     S, M = table.shape
@@ -1154,7 +1156,7 @@ def _update_pages(pages: torch.Tensor, page_scales: Optional[torch.Tensor], tabl
     lens2, granted, refs2 = torch.empty_like(lens), torch.empty_like(lens), torch.empty_like(refs)
     wsb = _lib.lib().smla_update_pages_workspace(S, M, n_pages)
     ws = torch.empty(wsb, dtype=torch.uint8, device=pages.device) if wsb else None
-    _launch(pages, "smla_update_pages", table.data_ptr(), table.stride(0) if S > 1 else M, S, M, lens.data_ptr(),
+    _launch(dev, "smla_update_pages", table.data_ptr(), table.stride(0) if S > 1 else M, S, M, lens.data_ptr(),
             refs.data_ptr(), n_pages, P, parent.data_ptr(), grow.data_ptr(), table2.data_ptr(), lens2.data_ptr(),
             refs2.data_ptr(), granted.data_ptr(), *pool, *scales, _p(ws), wsb)
     return table2, lens2, refs2, granted
@@ -1175,7 +1177,7 @@ update_pages_op = _with_eager_route(update_pages_op, _update_pages)
 def _compact_pages(pages: torch.Tensor, page_scales: Optional[torch.Tensor], table: torch.Tensor, refs: torch.Tensor
                    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``smla_compact_pages`` (see ``paged.compact_pages``): new (table, refs, live)."""
-    _one_device(pages, page_scales, table, refs)
+    dev = _one_device(pages, page_scales, table, refs)
     n_pages, P, pool, scales = _pool_args(pages, page_scales)
     table = _i32_rows(table, "table")
     S, M = table.shape
@@ -1184,7 +1186,7 @@ def _compact_pages(pages: torch.Tensor, page_scales: Optional[torch.Tensor], tab
     refs2, live = torch.empty_like(refs), refs.new_empty(1)
     wsb = _lib.lib().smla_compact_pages_workspace(n_pages)
     ws = torch.empty(wsb, dtype=torch.uint8, device=pages.device) if wsb else None
-    _launch(pages, "smla_compact_pages", table.data_ptr(), table.stride(0) if S > 1 else M, S, M, refs.data_ptr(), n_pages,
+    _launch(dev, "smla_compact_pages", table.data_ptr(), table.stride(0) if S > 1 else M, S, M, refs.data_ptr(), n_pages,
             P, table2.data_ptr(), refs2.data_ptr(), live.data_ptr(), *pool, *scales, _p(ws), wsb)
     return table2, refs2, live
 

@@ -52,15 +52,20 @@ def paged_append(q, kv, pages, table, lens, cu, cos_t, sin_t, kv_norm=None, q_no
         q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
     if q is None and q_out is not None:
         raise ValueError("q_out without q")
-    flags, w = _lib.PAGED_FILL if fill else 0, []
-    for norm, bit in ((q_norm, _lib.PAGED_NORM_Q), (kv_norm, _lib.PAGED_NORM_KV)):
-        weights = isinstance(norm, torch.Tensor)
-        if weights or norm:
-            flags |= bit
-        w.append(norm if weights else None)
-    D = kv.shape[-1]
-    ops.paged_append_op_(q, kv, pages, page_scales, table, lens, cu, cos_t, sin_t, w[0], w[1],
-                         min(D, 512) if norm_dims is None else int(norm_dims), bool(fp8_sim), float(eps), flags, q_out)
+    flags = _lib.PAGED_FILL if fill else 0
+    q_weights = kv_weights = None
+    if isinstance(q_norm, torch.Tensor):
+        q_weights, flags = q_norm, flags | _lib.PAGED_NORM_Q
+    elif q_norm:
+        flags |= _lib.PAGED_NORM_Q
+    if isinstance(kv_norm, torch.Tensor):
+        kv_weights, flags = kv_norm, flags | _lib.PAGED_NORM_KV
+    elif kv_norm:
+        flags |= _lib.PAGED_NORM_KV
+    if norm_dims is None:
+        norm_dims = min(kv.shape[-1], 512)
+    ops.paged_append_op_(q, kv, pages, page_scales, table, lens, cu, cos_t, sin_t, q_weights, kv_weights, int(norm_dims),
+                         bool(fp8_sim), float(eps), flags, q_out)
     return q_out
 
 
