@@ -202,12 +202,13 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
 constexpr int kPlanThreads = 1024;
 constexpr int kWavePages = 1024;        // most pages of a wave in one step of a scan over refs
 constexpr int kStepPages = kPlanThreads / 64 * kWavePages;
-constexpr int64_t kCopyChunk = 16384;   // bytes of one copy item
+constexpr int64_t kCopyChunk = 8192;    // bytes of one copy item (16384 leave larger remainders of pages: 61.8 us below for 55.4)
 constexpr int kCopyThreads = 256;       // threads that copy an item together
 // One launch does all where every workgroup can plan for itself: inputs are read only, so that all plans agree, and the plan
 // fits the LDS: pools of one scan step, up to 1024 slots, and few enough table entries for one workgroup.  Measured
 // against two launches: 32 slots of 128 entries and 1500 pages 7.2 us (4.6 + 3.3), 300 pages moved together 7.3 us (7.1 + 4.0),
-// 8192 pages 69.7 us (16.5 + 60.3), and a launch less for the host, 3 us.  Larger ones are planned once.
+// 8192 pages 69.7 us (16.5 + 60.3), and a launch less for the host, 3 us; since then the copies' chunks and nontemporal accesses
+// took the last to 55 us.  Larger ones are planned once.
 constexpr int64_t kOneEntries = 32768;
 
 // Exclusive prefix sum of v over the workgroup (16 waves); total: the sum.
@@ -279,20 +280,31 @@ struct Pool {
   int64_t page_bytes, row_bytes;
 };
 
-// n bytes by kCopyThreads threads, 16 at a time where both sides are aligned (four loads in flight per thread)
+// n bytes by kCopyThreads threads, 16 at a time where both sides are aligned.  NT: not kept in the caches (whole pages of a
+// pool that is larger than those: 8192 pages of 64 x 576 61.8 us against 69.0; a fork's tail page is read soon and stays).
+template <bool NT>
 __device__ inline void copy_span(uint8_t* dst, const uint8_t* src, int64_t n) {
   const int tid = threadIdx.x % kCopyThreads;
   const uintptr_t mix = (uintptr_t)dst | (uintptr_t)src;
   if ((mix & 15) == 0) {
+    constexpr int kLoads = (int)(kCopyChunk / (16 * kCopyThreads));
     const int64_t nv = n / 16;
-    for (int64_t i = tid; i < nv; i += 4 * kCopyThreads) {
-      u32x4_t v[4];
+    const u32x4_t* from = (const u32x4_t*)src;
+    u32x4_t* to = (u32x4_t*)dst;
+    for (int64_t i = tid; i < nv; i += kLoads * kCopyThreads) {
+      u32x4_t v[kLoads];
 #pragma unroll
-      for (int k = 0; k < 4; k++)
-        if (i + k * kCopyThreads < nv) v[k] = *(const u32x4_t*)(src + 16 * (i + k * kCopyThreads));
+      for (int k = 0; k < kLoads; k++)
+        if (i + k * kCopyThreads < nv) {
+          if constexpr (NT) v[k] = __builtin_nontemporal_load(from + i + k * kCopyThreads);
+          else v[k] = from[i + k * kCopyThreads];
+        }
 #pragma unroll
-      for (int k = 0; k < 4; k++)
-        if (i + k * kCopyThreads < nv) *(u32x4_t*)(dst + 16 * (i + k * kCopyThreads)) = v[k];
+      for (int k = 0; k < kLoads; k++)
+        if (i + k * kCopyThreads < nv) {
+          if constexpr (NT) __builtin_nontemporal_store(v[k], to + i + k * kCopyThreads);
+          else to[i + k * kCopyThreads] = v[k];
+        }
     }
     for (int64_t i = nv * 16 + tid; i < n; i += kCopyThreads) dst[i] = src[i];
   } else if (((mix | (uintptr_t)n) & 3) == 0) {
@@ -304,16 +316,17 @@ __device__ inline void copy_span(uint8_t* dst, const uint8_t* src, int64_t n) {
 
 // chunk `part` of the first `rows` rows of page src copied to page dst, in layer `layer`: the parts
 // below `parts` cover the first pool in kCopyChunk pieces, part `parts` the second pool (if any)
+template <bool NT>
 __device__ inline void copy_item(const Pool& p0, const Pool& p1, int layer, int64_t src, int64_t dst, int64_t rows,
                                  int64_t part, int64_t parts) {
   if (part < parts) {
     const int64_t all = rows * p0.row_bytes, from = part * kCopyChunk;
     if (from >= all) return;
     uint8_t* b = p0.base + layer * p0.layer_bytes + from;
-    copy_span(b + dst * p0.page_bytes, b + src * p0.page_bytes, all - from < kCopyChunk ? all - from : kCopyChunk);
+    copy_span<NT>(b + dst * p0.page_bytes, b + src * p0.page_bytes, all - from < kCopyChunk ? all - from : kCopyChunk);
   } else {
     uint8_t* b = p1.base + layer * p1.layer_bytes;
-    copy_span(b + dst * p1.page_bytes, b + src * p1.page_bytes, rows * p1.row_bytes);
+    copy_span<NT>(b + dst * p1.page_bytes, b + src * p1.page_bytes, rows * p1.row_bytes);
   }
 }
 
@@ -376,7 +389,7 @@ __device__ inline int slot_entry(const PageArgs& a, int s, int c, const SlotPlan
 __device__ inline void copy_tail(const PageArgs& a, const SlotPlan& n, int64_t dst, int layer, int64_t part) {
   const int64_t src = a.table[n.parent * a.ld_table + n.full];
   if (src < 0 || src >= a.n_pages || src == dst) return;
-  copy_item(a.p0, a.p1, layer, src, dst, n.tail, part, a.parts);
+  copy_item<false>(a.p0, a.p1, layer, src, dst, n.tail, part, a.parts);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -582,7 +595,7 @@ __global__ __launch_bounds__(kPlanThreads) void compact_one_kernel(const PageArg
   constexpr int kGroups = kPlanThreads / kCopyThreads;
   for (int64_t i = (int64_t)blockIdx.x * kGroups + tid / kCopyThreads; i < items; i += (int64_t)gridDim.x * kGroups) {
     const int64_t cl = i / a.items_per_copy, at = cl / a.layers;
-    copy_item(a.p0, a.p1, (int)(cl % a.layers), l.movers[at], l.holes[at], a.P, i - cl * a.items_per_copy, a.parts);
+    copy_item<true>(a.p0, a.p1, (int)(cl % a.layers), l.movers[at], l.holes[at], a.P, i - cl * a.items_per_copy, a.parts);
   }
   __syncthreads();
   const int64_t n = (int64_t)a.S * a.M;
@@ -680,7 +693,7 @@ __global__ __launch_bounds__(kCopyThreads) void compact_apply_kernel(const PageA
   for (int64_t i = (int64_t)blockIdx.x - row_blocks; i < items; i += (int64_t)gridDim.x - row_blocks) {
     const int64_t cl = i / a.items_per_copy, part = i - cl * a.items_per_copy;
     const int64_t m = cl / a.layers;
-    copy_item(a.p0, a.p1, (int)(cl % a.layers), movers[m], holes[m], a.P, part, a.parts);
+    copy_item<true>(a.p0, a.p1, (int)(cl % a.layers), movers[m], holes[m], a.P, part, a.parts);
   }
 }
 
