@@ -516,6 +516,30 @@ def test_append_without_rotation_and_past_the_tables(dev):
     _run_append(dev, [3, 2], [30, 2], 2, 128, 8, torch.float32, "bf16", True, True, n_pos=29, seed=7)
 
 
+@pytest.mark.parametrize("xdt,T,kv", [(torch.bfloat16, 4100, "bf16"), (torch.float32, 2100, "fp8")])
+def test_append_of_a_long_prompt(dev, xdt, T, kv):
+    """More than 256 MiB of projections in one call: the bits of the same tokens in three calls."""
+    from smla import paged
+    announce(f"paged_append {T} tokens of 64 heads, {xdt} {kv}")
+    H, D, P = 64, 512, 64
+    g = torch.Generator().manual_seed(T)
+    q = torch.randn(T, H, D, generator=g).to(xdt).to(dev)
+    x = torch.randn(T, D, generator=g).to(xdt).to(dev)
+    cos, sin = _to(dev, *_tables(dev, T, 64))
+    cols = -(-T // P)
+    table = torch.randperm(cols, generator=g).to(torch.int32)[None].to(dev)
+    pools = []
+    for cuts in ([0, T], [0, T // 3, 2 * T // 3, T]):
+        pages = torch.zeros(cols, P, D, dtype=torch.uint8 if kv == "fp8" else torch.bfloat16, device=dev)
+        scales = torch.zeros(cols, P, D // 64, device=dev) if kv == "fp8" else None
+        out = [paged.paged_append(q[a:b], x[a:b], pages, table, _i32([b], dev), _i32([0, b - a], dev), cos, sin, kv_norm=True,
+                                  q_norm=True, page_scales=scales) for a, b in zip(cuts, cuts[1:])]
+        pools.append((torch.cat(out), pages, scales))
+    for one, three in zip(*pools):
+        assert one is None or torch.equal(one, three)
+    assert pools[0][0].isfinite().all() and (pools[0][0] != 0).any(-1).all()
+
+
 def test_append_many_sequences(dev):
     r = random.Random(4)
     n = [r.choice([0, 1, 2]) for _ in range(200)]
