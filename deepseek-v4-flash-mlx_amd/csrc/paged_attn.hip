@@ -26,8 +26,8 @@
 // NB = 2 (64 q rows) where that makes no more tiles (tile_blocks).
 //
 // What bounds it, measured: a 2048-token chunk at 32 K (64 heads, D 576) 7.6 to 8.0 ms = 1130 to 1190 TFLOP/s, the matrix
-// pipes (a large library product reaches 1261 on the card); a decode step of 32 sequences of 2 K to 32 K rows 156 us =
-// 5.0 TB/s, HBM; drafts of 64 sequences over fp8 rows 110 us, the conversion to bf16 beside the products; a 4096-token
+// pipes (a large library product reaches 1261 on the card); a decode step of 32 sequences of 2 K to 32 K rows 149 us =
+// 5.3 TB/s, HBM; drafts of 64 sequences over fp8 rows 110 us, the conversion to bf16 beside the products; a 4096-token
 // prompt in a 128-row window 200 us, five row tiles an item behind Q's arrival and before the output's leaving (Q and
 // out alone are 113 us of HBM); one token over 4 K rows 11 us and 6 us for the join, latencies.
 //
@@ -273,6 +273,7 @@ struct Work {
   int m0, p0, p_lo, p_hi;  // the first one's number in its sequence; positions of the sequence's first token, the tile's first and last
   int lo, nf;  // entry e < nf: row e; e >= nf: row lo + e - nf
   int e_begin, e_end, ntiles;
+  bool once;  // the sequence's only tile: nobody else reads its rows in this call
 };
 
 // ---- row copies of one tile, dealt to the value waves (one instruction a row for columns 0..511, one per 8 rows for the
@@ -298,21 +299,28 @@ __device__ inline void copy_row(uint32_t lds_dst, uint64_t row, int x, int lane,
   else
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_dst), "v"(at), "s"(row) : "memory", "m0");
 }
-template <class G>
-__device__ inline void issue_tile(const PagedArgs& a, uint32_t lds_base, const RowIds& id, int vi, int lane, int tl) {
+// NT: past the caches, where nobody else reads the rows in this call (a decode step of 32 sequences 149 us against 156; the
+// 128-byte tails too: 151; rows that tiles share, a prompt's window: 210 against 200).
+template <class G, bool NT>
+__device__ inline void issue_copies(const PagedArgs& a, uint32_t lds_base, const RowIds& id, int vi, int lane, int tl) {
   const uint32_t tbase = lds_base + (uint32_t)((tl % G::NBUF) * G::TILE_BYTES);
 #pragma unroll
   for (int k = 0; k < (G::NDMA + kValueWaves - 1) / kValueWaves; k++) {
     const int x = dealt(vi, k);
     if (x < kTileRows) {
       const uint64_t row = (uint64_t)(uintptr_t)a.pages + (uint64_t)(uint32_t)__builtin_amdgcn_readlane(id.mine, x) * G::ROWB;
-      copy_row(tbase + x * 1024, row, x, lane, false);
+      copy_row(tbase + x * 1024, row, x, lane, NT);
     } else if (x < G::NDMA) {
       const int r0 = (x - kTileRows) * 8, r = r0 + (lane >> 3);
       dma16((const uint8_t*)a.pages + (int64_t)id.tail * G::ROWB + 1024 + 16 * ((lane & 7) ^ (r & 7)),
             __builtin_amdgcn_readfirstlane(tbase + G::MAIN_BYTES + r0 * 128));
     }
   }
+}
+template <class G>
+__device__ inline void issue_tile(const PagedArgs& a, uint32_t lds_base, const RowIds& id, int vi, int lane, int tl, bool once) {
+  if (once) issue_copies<G, true>(a, lds_base, id, vi, lane, tl);
+  else issue_copies<G, false>(a, lds_base, id, vi, lane, tl);
 }
 // the same for 32 rows whose addresses `rowp` gives
 template <class G, class F>
@@ -677,7 +685,7 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
     if constexpr (DEEP) f8_load<D>(a, ids_s, x0, kValueWaves, lane, min(2, last), f8_next);
   } else {
     for (int tl = 0; tl < min(w.ntiles, EARLY); tl++)
-      issue_tile<G>(a, lds_base, read_ids<G>(ids_s, vi, lane, tl), vi, lane, tl);
+      issue_tile<G>(a, lds_base, read_ids<G>(ids_s, vi, lane, tl), vi, lane, tl, w.once);
   }
   // Q and tile 0 are there
   if (FP8 || w.ntiles <= 1) {
@@ -690,7 +698,7 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
   lds_barrier();  // the score waves have read Q
   if constexpr (!FP8) {
     for (int tl = EARLY; tl < min(w.ntiles, G::NBUF); tl++)
-      issue_tile<G>(a, lds_base, read_ids<G>(ids_s, vi, lane, tl), vi, lane, tl);
+      issue_tile<G>(a, lds_base, read_ids<G>(ids_s, vi, lane, tl), vi, lane, tl, w.once);
     if (G::NBUF < w.ntiles) ids = read_ids<G>(ids_s, vi, lane, G::NBUF);
   }
   // Iteration i: the score waves finish tile i - 1 and begin tile i, tile i - 2 is consumed here, and tile i + 1 goes
@@ -701,7 +709,7 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
       f8_load<D>(a, ids_s, x0, kValueWaves, lane, min(i + 2 + DEEP, last), f);
     } else {
       if (i >= 3 && i + 1 < w.ntiles) {
-        issue_tile<G>(a, lds_base, ids, vi, lane, i + 1);
+        issue_tile<G>(a, lds_base, ids, vi, lane, i + 1, w.once);
         if (i + 2 < w.ntiles) ids = read_ids<G>(ids_s, vi, lane, i + 2);
       }
     }
@@ -901,6 +909,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedArgs
   Work w;
   const int rows_b = it.s.n * a.H;
   w.m0 = it.tile * G::TILEQ;
+  w.once = it.s.tiles == 1;
   w.slot = it.nsplit > 1 ? it.slot + it.split : -1;
   w.nh = min(G::TILEQ, rows_b - w.m0);
   w.row0 = (int64_t)it.s.beg * a.H + w.m0;
