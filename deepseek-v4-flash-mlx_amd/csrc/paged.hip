@@ -16,7 +16,6 @@ namespace {
 
 // ---------------------------------------------------------------------------------------------
 // append
-constexpr int64_t kMemorySideCache = 256 << 20;  // bytes
 struct AppendArgs {
   const void* q;   // [T, H, D], tokens ldq elements apart
   const void* kv;  // [T, D], tokens ldkv elements apart
@@ -63,17 +62,12 @@ __device__ inline bool token_position(const AppendArgs& a, int t, int lane, int&
   return pos >= 0;
 }
 
-template <class T, bool NT>
-__device__ inline T load_once(const T* p) {
-  if constexpr (NT) return __builtin_nontemporal_load(p);
-  else return *p;
-}
-template <int XDT, bool NT>
+template <int XDT>
 __device__ inline f32x4_t load4(const void* p, int64_t i) {
   if constexpr (XDT == SMLA_F32) {
-    return load_once<f32x4_t, NT>((const f32x4_t*)((const float*)p + i));
+    return *(const f32x4_t*)((const float*)p + i);
   } else {
-    const u32x2_t w = load_once<u32x2_t, NT>((const u32x2_t*)((const uint16_t*)p + i));
+    const u32x2_t w = *(const u32x2_t*)((const uint16_t*)p + i);
     return f32x4_t{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16),
                    __uint_as_float(w[1] & 0xffff0000u)};
   }
@@ -82,10 +76,8 @@ __device__ inline f32x4_t load4(const void* p, int64_t i) {
 // Lane l of a wave owns channels 256 c + 4 l .. + 3 of chunk c: every access of a wave is one contiguous
 // run, a rotation pair and a lane's norm weights stay in the lane, and a 64-channel quantisation block
 // is one 16-lane row.  Sums and the rotation are fp32; a result is rounded once, to its stored type.
-// Bound by HBM: 4096 tokens of 64 heads and a row (fp32 in, bf16 out, 818 MB) 135 us = 6.1 TB/s; 8 tokens 3.6 us, latency.
-// NT: projections that the 256 MiB memory-side cache cannot hold are read past the caches (135 us against 141); smaller ones
-// may still be there from the product that wrote them.
-template <int XDT, int NCH, bool NT>
+// Bound by HBM: 4096 tokens of 64 heads and a row (fp32 in, bf16 out, 818 MB) 142 us = 5.8 TB/s; 8 tokens 3.6 us, latency.
+template <int XDT, int NCH>
 __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
   const int lane = threadIdx.x & 63;
   const uint32_t r = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
@@ -101,7 +93,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
 #pragma unroll
     for (int c = 0; c < NCH; c++) {
       const int ch = 256 * c + 4 * lane;
-      v[c] = ch < D ? load4<XDT, NT>(src, at + ch) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+      v[c] = ch < D ? load4<XDT>(src, at + ch) : f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
   }
   int seq;
@@ -896,12 +888,7 @@ extern "C" int smla_paged_append(const void* q, int64_t ldq, const void* kv, int
   a.cu = cu;
   const dim3 grid((unsigned)((T * (H + 1) + 3) / 4)), block(256);
   const hipStream_t st = (hipStream_t)stream;
-  const bool nt = T * (H + 1) * D * (x_dtype == SMLA_F32 ? 4 : 2) > kMemorySideCache;
-#define SMLA_APPEND(X, N)                                                                   \
-  do {                                                                                      \
-    if (nt) hipLaunchKernelGGL((paged_append_kernel<X, N, true>), grid, block, 0, st, a);    \
-    else hipLaunchKernelGGL((paged_append_kernel<X, N, false>), grid, block, 0, st, a);      \
-  } while (0)
+#define SMLA_APPEND(X, N) hipLaunchKernelGGL((paged_append_kernel<X, N>), grid, block, 0, st, a)
 #define SMLA_APPEND_D(X)                 \
   do {                                   \
     if (D <= 512) SMLA_APPEND(X, 2);      \

@@ -518,7 +518,7 @@ def test_append_without_rotation_and_past_the_tables(dev):
 
 @pytest.mark.parametrize("xdt,T,kv", [(torch.bfloat16, 4100, "bf16"), (torch.float32, 2100, "fp8")])
 def test_append_of_a_long_prompt(dev, xdt, T, kv):
-    """More than 256 MiB of projections in one call: the bits of the same tokens in three calls."""
+    """A call of a long prompt gives the bits of the same tokens in three calls."""
     from smla import paged
     announce(f"paged_append {T} tokens of 64 heads, {xdt} {kv}")
     H, D, P = 64, 512, 64
