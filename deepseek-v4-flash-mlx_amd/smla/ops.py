@@ -1015,7 +1015,11 @@ def _check_batch(table, lens, cu):
     """table, lens, cu, sequences, the table's columns and row stride."""
     table = _i32_rows(table, "table")
     B, cols = table.shape
-    return table, _i32(lens, (B,), "lens"), _i32(cu, (B + 1,), "cu"), B, cols, table.stride(0) if B > 1 else cols
+    # (one test where all is as it should be; else the one that names what is not)
+    if not (lens.dtype == cu.dtype == torch.int32 and lens.shape == (B,) and cu.shape == (B + 1,) and lens.is_contiguous()
+            and cu.is_contiguous()):
+        lens, cu = _i32(lens, (B,), "lens"), _i32(cu, (B + 1,), "cu")
+    return table, lens, cu, B, cols, table.stride(0) if B > 1 else cols
 
 
 def _paged_attn_(q: torch.Tensor, pages: torch.Tensor, page_scales: Optional[torch.Tensor], table: torch.Tensor,
@@ -1023,9 +1027,12 @@ def _paged_attn_(q: torch.Tensor, pages: torch.Tensor, page_scales: Optional[tor
                  first: int, fill: bool, out: torch.Tensor) -> None:
     """``smla_paged_attn`` into out [T, H, DV] (see ``paged.paged_attn``)."""
     dev = _one_device(q, pages, page_scales, table, lens, cu, attn_sink, out)
-    if q.dim() != 3 or out.dim() != 3 or out.shape[:2] != q.shape[:2]:
-        raise ValueError(f"expected q [T,H,D] and out [T,H,dv], got {list(q.shape)} and {list(out.shape)}")
+    shape = out.shape
+    if q.dim() != 3 or len(shape) != 3:
+        raise ValueError(f"expected q [T,H,D] and out [T,H,dv], got {list(q.shape)} and {list(shape)}")
     T, H, D = q.shape
+    if shape[0] != T or shape[1] != H:
+        raise ValueError(f"expected q [T,H,D] and out [T,H,dv], got {list(q.shape)} and {list(shape)}")
     code = _check_pool(pages, page_scales, (3,))
     n_pages, P, dp = pages.shape
     if dp != D:
@@ -1046,7 +1053,7 @@ def _paged_attn_(q: torch.Tensor, pages: torch.Tensor, page_scales: Optional[tor
     wsb = _lib.lib().smla_paged_attn_workspace(T, H, B, cols * P, window, first)
     ws = torch.empty(wsb, dtype=torch.uint8, device=q.device)
     _launch(dev, "smla_paged_attn", q.data_ptr(), _lib.BF16, pages.data_ptr(), code, _p(page_scales), n_pages, P,
-            table.data_ptr(), ld, cols, lens.data_ptr(), cu.data_ptr(), B, T, H, D, out.shape[2], scale, _p(attn_sink), window, first, _lib.PAGED_FILL if fill else 0, out.data_ptr(), _lib.BF16,
+            table.data_ptr(), ld, cols, lens.data_ptr(), cu.data_ptr(), B, T, H, D, shape[2], scale, _p(attn_sink), window, first, _lib.PAGED_FILL if fill else 0, out.data_ptr(), _lib.BF16,
             ws.data_ptr(), wsb)
 
 
@@ -1091,11 +1098,12 @@ def _paged_append_(q: Optional[torch.Tensor], kv: torch.Tensor, pages: torch.Ten
         ldkv = D
     H = ldq = 0
     if q is not None:
-        if q.dim() != 3 or q.shape[0] != T or q.shape[2] != D or q.dtype != kv.dtype:
-            raise ValueError(f"expected q [{T}, H, {D}] {kv.dtype}, got {list(q.shape)} {q.dtype}")
-        if q_out.shape != q.shape or q_out.dtype != torch.bfloat16 or not q_out.is_contiguous() or q_out.data_ptr() & 7:
+        shape = q.shape
+        if len(shape) != 3 or shape[0] != T or shape[2] != D or q.dtype != kv.dtype:
+            raise ValueError(f"expected q [{T}, H, {D}] {kv.dtype}, got {list(shape)} {q.dtype}")
+        if q_out.shape != shape or q_out.dtype != torch.bfloat16 or not q_out.is_contiguous() or q_out.data_ptr() & 7:
             raise ValueError("q_out must be contiguous, 8-byte aligned bf16 of q's shape")
-        H = q.shape[1]
+        H = shape[1]
         ldq, s1, s2 = q.stride()
         if H and (s2 != 1 or s1 != D or ldq < H * D or ldq % 4 or q.data_ptr() & unit):
             q = q.clone(memory_format=torch.contiguous_format)
@@ -1149,7 +1157,10 @@ def _update_pages(pages: torch.Tensor, page_scales: Optional[torch.Tensor], tabl
     n_pages, P, pool, scales = _pool_args(pages, page_scales)
     table = _i32_rows(table, "table")
     S, M = table.shape
-    lens, parent, grow = _i32(lens, (S,), "lens"), _i32(parent, (S,), "parent"), _i32(grow, (S,), "grow")
+    want = (S,)
+    if not (lens.dtype == parent.dtype == grow.dtype == torch.int32 and lens.shape == parent.shape == grow.shape == want
+            and lens.is_contiguous() and parent.is_contiguous() and grow.is_contiguous()):
+        lens, parent, grow = _i32(lens, want, "lens"), _i32(parent, want, "parent"), _i32(grow, want, "grow")
     refs = _i32(refs, (n_pages,), "refs")
     # (a table with its rows apart gives a dense one)
     table2 = torch.empty_like(table) if table.is_contiguous() else table.new_empty((S, M))
