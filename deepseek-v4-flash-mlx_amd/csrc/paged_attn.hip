@@ -29,7 +29,7 @@
 // pipes (a large library product reaches 1261 on the card); a decode step of 32 sequences of 2 K to 32 K rows 149 us =
 // 5.3 TB/s, HBM; drafts of 64 sequences over fp8 rows 110 us, the conversion to bf16 beside the products; a 4096-token
 // prompt in a 128-row window 200 us, five row tiles an item behind Q's arrival and before the output's leaving (Q and
-// out alone are 113 us of HBM); one token over 4 K rows 11 us and 6 us for the join, latencies.
+// out alone are 113 us of HBM); one token over 4 K rows 11.4 us and 5.5 us for the join, latencies.
 //
 // Rows come HBM -> LDS by DMA into a ring of four tiles, copies issued by the value waves (fp8 rows: loaded,
 // converted, written).  Row numbers go through an LDS ring of 8 tiles that score wave 0 fills six tiles
@@ -958,19 +958,20 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedArgs
 }
 
 // ---------------------------------------------------------------------------------------------
-// Joins the states of split tiles, in pieces of 1 KB (8 values of 32 q rows, twice).  A workgroup of 4 waves takes GROUP
-// pieces of a tile at a time.  One piece by all four: wave w the splits w, w + 4, .. with a running maximum, the waves'
-// sums then through LDS in a fixed order.  Where there are pieces enough (GROUP 4) and a tile has at most kAlone splits,
+// Joins the states of split tiles, in pieces of 1 KB (8 values of 32 q rows, twice).  A workgroup takes GROUP pieces of a tile
+// at a time.  One piece by all its waves: wave w the splits w, w + WAVES, .. with a running maximum, the waves' sums then
+// through LDS in a fixed order (kFewWaves: one tile of 65 splits 5.5 us, with four waves 6.5, with 16 8.3).
+// Where there are pieces enough (GROUP 4, four waves) and a tile has at most kAlone splits,
 // a piece a wave, which needs no LDS and no barriers: 1366 tiles of 2 or 3 splits 106 us against 254 (4.2 TB/s), 64 tiles of
 // 3 to 6 8.5 against 13.9, 32 tiles of 8 9.6 against 12.9.
 // Workgroups walk the pieces of all split tiles; with `fill` they also clear the tokens of no sequence.
-constexpr int kMergeWaves = 4, kMergeBatch = 8, kAlone = 16;
+constexpr int kFewWaves = 8, kMergeBatch = 8, kAlone = 16;
 
-template <int D, int NB, int GROUP>
-__global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const PagedArgs a) {
+template <int D, int NB, int GROUP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void paged_merge_kernel(const PagedArgs a) {
   using G = GeoP<D, NB>;
   constexpr int kPieces = kUnits * NB * 2;
-  __shared__ float red[kMergeWaves][64][10];
+  __shared__ float red[WAVES][64][10];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const Seq s0 = load_seq<G::TILEQ>(a, lane);
   const int rps = __builtin_amdgcn_readfirstlane(*(const int*)a.ws);
@@ -1046,13 +1047,13 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
       for (int j = 0; j < 4; j++) o[j] = pack2(t.acc[2 * j] * inv, t.acc[2 * j + 1] * inv);
       *(u32x4_t*)(a.out + ((int64_t)it.s.beg * a.H + m0 + row) * 512 + 32 * u + 16 * half + 8 * (lane >> 5)) = o;
     };
-    if constexpr (GROUP == kMergeWaves)
+    if constexpr (GROUP > 1)
       if (it.nsplit <= kAlone) {
         finish((int)piece0 + wave, gather((int)piece0 + wave, 0, 1));
         continue;
       }
     for (int piece = (int)piece0; piece < (int)piece0 + GROUP; piece++) {
-      const Sum t = gather(piece, wave, kMergeWaves);
+      const Sum t = gather(piece, wave, WAVES);
       __syncthreads();  // the last piece's sums are read
       red[wave][lane][0] = t.m;
       red[wave][lane][1] = t.l;
@@ -1063,12 +1064,12 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const Pag
         Sum y;
         y.m = t.m;
 #pragma unroll
-        for (int k = 1; k < kMergeWaves; k++) y.m = fmaxf(y.m, red[k][lane][0]);
+        for (int k = 1; k < WAVES; k++) y.m = fmaxf(y.m, red[k][lane][0]);
         y.l = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; j++) y.acc[j] = 0.f;
 #pragma unroll
-        for (int k = 0; k < kMergeWaves; k++) {
+        for (int k = 0; k < WAVES; k++) {
           const float mk = red[k][lane][0], e = mk > -SMLA_INF ? __builtin_amdgcn_exp2f(mk - y.m) : 1.f;
           y.l += red[k][lane][1] * e;
 #pragma unroll
@@ -1123,9 +1124,11 @@ int launch_paged(const PagedArgs& a, int64_t tiles, hipStream_t st) {
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * kWaves), G::LDS_BYTES, st, a);
   SMLA_HIP_CHECK_LAUNCH();
   const int64_t pieces = tiles * kUnits * NB * 2, most = 8 * (int64_t)a.cus;
-  const dim3 grid2((unsigned)(pieces < most ? pieces : most)), block2(64 * kMergeWaves);
-  if (pieces >= kMergeWaves * (int64_t)a.cus) hipLaunchKernelGGL((paged_merge_kernel<D, NB, kMergeWaves>), grid2, block2, 0, st, a);
-  else hipLaunchKernelGGL((paged_merge_kernel<D, NB, 1>), grid2, block2, 0, st, a);
+  const dim3 grid2((unsigned)(pieces < most ? pieces : most));
+  if (pieces >= 4 * (int64_t)a.cus)
+    hipLaunchKernelGGL((paged_merge_kernel<D, NB, 4, 4>), grid2, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((paged_merge_kernel<D, NB, 1, kFewWaves>), grid2, dim3(64 * kFewWaves), 0, st, a);
   SMLA_HIP_CHECK_LAUNCH();
   return SMLA_OK;
 }
