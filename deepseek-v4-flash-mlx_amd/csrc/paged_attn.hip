@@ -319,7 +319,8 @@ __device__ inline void issue_copies(const PagedArgs& a, uint32_t lds_base, const
 }
 template <class G>
 __device__ inline void issue_tile(const PagedArgs& a, uint32_t lds_base, const RowIds& id, int vi, int lane, int tl, bool once) {
-  if (once) issue_copies<G, true>(a, lds_base, id, vi, lane, tl);
+  // (at NB = 3 few sequences make one tile, and the choice alone costs a chunk 2 %)
+  if (G::NB == 2 && once) issue_copies<G, true>(a, lds_base, id, vi, lane, tl);
   else issue_copies<G, false>(a, lds_base, id, vi, lane, tl);
 }
 // the same for 32 rows whose addresses `rowp` gives
