@@ -25,7 +25,7 @@
 // wave) read 8.4 KB a row for two thirds of the products and was 11.6 ms where this one is 7.9.
 // NB = 2 (64 q rows) where that makes no more tiles (tile_blocks).
 //
-// What bounds it, measured: a 2048-token chunk at 32 K (64 heads, D 576) 7.6 to 8.2 ms = 1100 to 1190 TFLOP/s, the matrix
+// What bounds it, measured: a 2048-token chunk at 32 K (64 heads, D 576) 7.6 to 8.1 ms = 1120 to 1200 TFLOP/s, the matrix
 // pipes (a large library product reaches 1261 on the card); a decode step of 32 sequences of 2 K to 32 K rows 149 us =
 // 5.3 TB/s, HBM; drafts of 64 sequences over fp8 rows 110 us, the conversion to bf16 beside the products; a 4096-token
 // prompt in a 128-row window 200 us, five row tiles an item behind Q's arrival and before the output's leaving (Q and
