@@ -89,15 +89,16 @@ __device__ inline void wait_vm(int n) {
 }
 
 // 16-byte HBM -> LDS copy for every lane: lane l's bytes land at lds_dst + 16*l.  Untracked by the
-// compiler (inline asm); callers wait with wait_vm().
+// compiler (inline asm); callers wait with wait_vm().  The write of M0 needs a wait state before the copy
+// that reads it, which the compiler does not put inside an asm block: the s_nop.
 __device__ inline void dma16(const void* gsrc, uint32_t lds_dst_uniform) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_dst_uniform), "v"(gsrc)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_dst_uniform), "v"(gsrc)
                : "memory", "m0");
 }
 // the same copy with the non-temporal hint: data read once (a query's own Q rows) should not push
 // reused rows out of the L2
 __device__ inline void dma16_nt(const void* gsrc, uint32_t lds_dst_uniform) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds_dst_uniform), "v"(gsrc)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds_dst_uniform), "v"(gsrc)
                : "memory", "m0");
 }
 

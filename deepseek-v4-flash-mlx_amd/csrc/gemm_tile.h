@@ -35,9 +35,9 @@ struct Int {
 };
 
 // 16-byte HBM -> LDS copy for every lane (lane l lands at lds_dst + 16 l): 32-bit lane offsets from
-// a wave-uniform base, so a K step advances scalars only
+// a wave-uniform base, so a K step advances scalars only (the s_nop: M0 is read one wait state after its write at the earliest)
 __device__ inline void dma16_s(const uint8_t* base, uint32_t off, uint32_t lds_dst) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_dst), "v"(off), "s"(base) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_dst), "v"(off), "s"(base) : "memory", "m0");
 }
 
 // BM tokens x BN outputs by waves of WM x WN; D stages of 64 k in LDS

@@ -291,13 +291,13 @@ __device__ inline RowIds read_ids(const lds_i32_t* ids_s, int vi, int lane, int 
   const int t = (dealt(vi, 0) + 3) % kValueWaves;
   return RowIds{max(id[lane & 31], 0), G::TAIL && t < 4 ? max(id[8 * t + (lane >> 3)], 0) : 0};
 }
-// 1 KB from a row at a scalar address, chunks swizzled; nt: not kept in the L2
+// 1 KB from a row at a scalar address, chunks swizzled (the s_nop as in dma16); nt: not kept in the L2
 __device__ inline void copy_row(uint32_t lds_dst, uint64_t row, int x, int lane, bool nt) {
   const int at = 16 * (lane ^ row_swizzle(x));
   if (nt)
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds_dst), "v"(at), "s"(row) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds_dst), "v"(at), "s"(row) : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_dst), "v"(at), "s"(row) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_dst), "v"(at), "s"(row) : "memory", "m0");
 }
 // NT: past the caches, where nobody else reads the rows in this call (a decode step of 32 sequences 149 us against 156; the
 // 128-byte tails too: 151; rows that tiles share, a prompt's window: 210 against 200).
