@@ -919,10 +919,10 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attn_kernel(const PagedArgs
   w.p_hi = w.p0 + (int)((uint32_t)(w.m0 + w.nh - 1) / (uint32_t)a.H);
   const int w_lo = w.p_lo - a.window + 1;
   w.lo = a.window > 0 && w_lo > 0 ? w_lo : 0;
-  w.nf = min(a.first, w.lo);
-  const int64_t cap = (int64_t)a.cols * a.P;
+  const int64_t cap = (int64_t)a.cols * a.P;  // rows from it on are not in the table, nor are first rows
   const int top = (int)min((int64_t)w.p_hi + 1, cap);  // rows below it
-  const int entries = max(0, top - w.lo + w.nf);
+  w.nf = (int)min((int64_t)min(a.first, w.lo), cap);
+  const int entries = w.nf + max(0, top - w.lo);  // (the window may start past the table: its first rows are seen still)
   const int part = ceil_div(ceil_div(it.s.span, it.nsplit), kTileRows) * kTileRows;
   w.e_begin = (int)min((int64_t)it.split * part, (int64_t)entries);
   w.e_end = min(entries, w.e_begin + part);
