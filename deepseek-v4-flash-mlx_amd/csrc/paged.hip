@@ -30,22 +30,23 @@ struct AppendArgs {
   float* scales;
   int n_pages, P, cols, B;
   int64_t ld_table;
-  const int32_t *table, *lens, *cu;
+  const int32_t *table, *lens, *cu, *granted;  // granted null: every sequence
 };
 
 // Sequence of token t (the number of sequences that end at or before it; B: behind the last) and its
 // position, by one wave: every lane reads one boundary and one length, in one round trip per 64
-// sequences.
+// sequences.  false: a token of no sequence, or of one that was not granted its rows.
 __device__ inline bool token_position(const AppendArgs& a, int t, int lane, int& seq, int64_t& pos) {
   seq = 0;
-  int beg = 0, end = 0, len = 0;
+  int beg = 0, end = 0, len = 0, has = 1;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
-    int c0 = 0, c1 = 0x7fffffff, n = 0;
+    int c0 = 0, c1 = 0x7fffffff, n = 0, g = 1;
     if (b < a.B) {
       c0 = a.cu[b];
       c1 = a.cu[b + 1];
       n = a.lens[b];
+      if (a.granted) g = a.granted[b];
     }
     const uint64_t done = __builtin_amdgcn_ballot_w64(c1 <= t);
     const int k = (int)__builtin_popcountll(done);
@@ -54,10 +55,11 @@ __device__ inline bool token_position(const AppendArgs& a, int t, int lane, int&
       beg = __builtin_amdgcn_readlane(c0, k);
       end = __builtin_amdgcn_readlane(c1, k);
       len = __builtin_amdgcn_readlane(n, k);
+      has = __builtin_amdgcn_readlane(g, k);
       break;
     }
   }
-  if (seq >= a.B || beg > t || beg < 0) return false;
+  if (seq >= a.B || beg > t || beg < 0 || has == 0) return false;
   pos = (int64_t)len - ((int64_t)end - beg) + (t - beg);
   return pos >= 0;
 }
@@ -827,12 +829,13 @@ extern "C" int smla_compact_pages(const int32_t* table, int64_t ld_table, int64_
   return SMLA_OK;
 }
 
-extern "C" int smla_paged_append(const void* q, int64_t ldq, const void* kv, int64_t ldkv, int x_dtype, int64_t T,
-                                 int64_t H, int64_t D, int64_t norm_dims, const float* q_w, const float* kv_w,
-                                 const float* cos_t, const float* sin_t, int64_t n_pos, int64_t rd, float eps, int sim,
-                                 int flags, void* q_out, void* pages, int page_dtype, float* scales, int64_t n_pages,
-                                 int64_t P, const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* lens,
-                                 const int32_t* cu, int64_t B, void* stream) {
+extern "C" int smla_paged_append_granted(const void* q, int64_t ldq, const void* kv, int64_t ldkv, int x_dtype, int64_t T,
+                                         int64_t H, int64_t D, int64_t norm_dims, const float* q_w, const float* kv_w,
+                                         const float* cos_t, const float* sin_t, int64_t n_pos, int64_t rd, float eps,
+                                         int sim, int flags, void* q_out, void* pages, int page_dtype, float* scales,
+                                         int64_t n_pages, int64_t P, const int32_t* table, int64_t ld_table, int64_t cols,
+                                         const int32_t* lens, const int32_t* cu, const int32_t* granted, int64_t B,
+                                         void* stream) {
   if (!kv || !pages || !table || !lens || !cu || (H > 0 && (!q || !q_out)) || (rd > 0 && (!cos_t || !sin_t)))
     return SMLA_E_NULL;
   if (T < 0 || H < 0 || D <= 0 || B <= 0 || n_pages <= 0 || P <= 0 || cols <= 0 || ld_table < cols || rd < 0 ||
@@ -886,6 +889,7 @@ extern "C" int smla_paged_append(const void* q, int64_t ldq, const void* kv, int
   a.table = table;
   a.lens = lens;
   a.cu = cu;
+  a.granted = granted;
   const dim3 grid((unsigned)((T * (H + 1) + 3) / 4)), block(256);
   const hipStream_t st = (hipStream_t)stream;
 #define SMLA_APPEND(X, N) hipLaunchKernelGGL((paged_append_kernel<X, N>), grid, block, 0, st, a)
@@ -901,4 +905,15 @@ extern "C" int smla_paged_append(const void* q, int64_t ldq, const void* kv, int
 #undef SMLA_APPEND
   SMLA_HIP_CHECK_LAUNCH();
   return SMLA_OK;
+}
+
+extern "C" int smla_paged_append(const void* q, int64_t ldq, const void* kv, int64_t ldkv, int x_dtype, int64_t T,
+                                 int64_t H, int64_t D, int64_t norm_dims, const float* q_w, const float* kv_w,
+                                 const float* cos_t, const float* sin_t, int64_t n_pos, int64_t rd, float eps, int sim,
+                                 int flags, void* q_out, void* pages, int page_dtype, float* scales, int64_t n_pages,
+                                 int64_t P, const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* lens,
+                                 const int32_t* cu, int64_t B, void* stream) {
+  return smla_paged_append_granted(q, ldq, kv, ldkv, x_dtype, T, H, D, norm_dims, q_w, kv_w, cos_t, sin_t, n_pos, rd, eps,
+                                   sim, flags, q_out, pages, page_dtype, scales, n_pages, P, table, ld_table, cols, lens,
+                                   cu, nullptr, B, stream);
 }

@@ -60,7 +60,7 @@ struct PagedArgs {
   const uint16_t* q;
   const void* pages;
   const float* page_scales;
-  const int32_t *table, *lens, *cu;
+  const int32_t *table, *lens, *cu, *granted;  // granted null: every sequence
   const float* sink;
   uint16_t* out;
   uint8_t* ws;
@@ -120,9 +120,9 @@ template <int TILEQ>
 __device__ inline Seq load_seq(const PagedArgs& a, int b) {
   Seq s{0, 0, 0, 0, 0};
   if (b < a.B) {
-    const int c0 = a.cu[b], c1 = a.cu[b + 1], len = a.lens[b];
+    const int c0 = a.cu[b], c1 = a.cu[b + 1], len = a.lens[b], has = a.granted ? a.granted[b] : 1;
     s.beg = min(max(c0, 0), a.T);
-    s.n = max(min(c1, a.T) - s.beg, 0);
+    s.n = has ? max(min(c1, a.T) - s.beg, 0) : 0;
     s.len = max(len, 0);
     s.tiles = (int)(((uint32_t)s.n * (uint32_t)a.H + TILEQ - 1) / TILEQ);
     const int64_t cap = (int64_t)a.cols * a.P;
@@ -1084,8 +1084,23 @@ __global__ __launch_bounds__(64 * WAVES) void paged_merge_kernel(const PagedArgs
     // 16-byte pieces of the tokens before the first sequence and behind the last
     const int64_t tok = (int64_t)a.H * 64, to = a.T * tok, first = min(max(a.cu[0], 0), a.T) * tok;
     const int64_t gap = max(min(max(a.cu[a.B], 0), a.T) * tok - first, (int64_t)0);
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < to - gap; i += (int64_t)gridDim.x * blockDim.x)
-      *(u32x4_t*)(a.out + (i < first ? i : i + gap) * 8) = u32x4_t{0u, 0u, 0u, 0u};
+    const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = at; i < to - gap; i += step) *(u32x4_t*)(a.out + (i < first ? i : i + gap) * 8) = u32x4_t{0u, 0u, 0u, 0u};
+    // and of the sequences that were not granted theirs
+    for (int b0 = 0; a.granted && b0 < a.B; b0 += 64) {
+      const int b = b0 + lane;
+      int c0 = 0, c1 = 0;
+      if (b < a.B && a.granted[b] == 0) {
+        c0 = min(max(a.cu[b], 0), a.T);
+        c1 = min(max(a.cu[b + 1], 0), a.T);
+      }
+      for (uint64_t left = __builtin_amdgcn_ballot_w64(c0 < c1); left; left &= left - 1) {
+        const int k = (int)__builtin_ctzll(left);
+        const int64_t end = __builtin_amdgcn_readlane(c1, k) * tok;
+        for (int64_t i = __builtin_amdgcn_readlane(c0, k) * tok + at; i < end; i += step)
+          *(u32x4_t*)(a.out + i * 8) = u32x4_t{0u, 0u, 0u, 0u};
+      }
+    }
   }
 }
 
@@ -1147,11 +1162,12 @@ extern "C" size_t smla_paged_attn_workspace(int64_t T, int64_t H, int64_t B, int
   return (size_t)(kHeader + plan_slots(most_tiles(T, H, B, nb), smla_num_cus(), most_entries(rows, window, first, H)) * state);
 }
 
-extern "C" int smla_paged_attn(const void* q, int q_dtype, const void* pages, int page_dtype, const float* page_scales,
-                               int64_t n_pages, int64_t P, const int32_t* table, int64_t ld_table, int64_t cols,
-                               const int32_t* lens, const int32_t* cu, int64_t B, int64_t T, int64_t H, int64_t D,
-                               int64_t DV, float scale, const float* attn_sink, int64_t window, int64_t first, int flags,
-                               void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int smla_paged_attn_granted(const void* q, int q_dtype, const void* pages, int page_dtype,
+                                       const float* page_scales, int64_t n_pages, int64_t P, const int32_t* table,
+                                       int64_t ld_table, int64_t cols, const int32_t* lens, const int32_t* cu,
+                                       const int32_t* granted, int64_t B, int64_t T, int64_t H, int64_t D, int64_t DV,
+                                       float scale, const float* attn_sink, int64_t window, int64_t first, int flags,
+                                       void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace smla_attn;
   if (!q || !pages || !table || !lens || !cu || !out) return SMLA_E_NULL;
   if (T < 0 || H <= 0 || B <= 0 || n_pages <= 0 || P <= 0 || cols <= 0 || ld_table < cols || D <= 0 || DV <= 0 || DV > D)
@@ -1176,6 +1192,7 @@ extern "C" int smla_paged_attn(const void* q, int q_dtype, const void* pages, in
   a.table = table;
   a.lens = lens;
   a.cu = cu;
+  a.granted = granted;
   a.sink = attn_sink;
   a.out = (uint16_t*)out;
   a.ws = (uint8_t*)workspace;
@@ -1204,4 +1221,14 @@ extern "C" int smla_paged_attn(const void* q, int q_dtype, const void* pages, in
   if (D == 576) SMLA_PAGED(576, 3);
   SMLA_PAGED(512, 3);
 #undef SMLA_PAGED
+}
+
+extern "C" int smla_paged_attn(const void* q, int q_dtype, const void* pages, int page_dtype, const float* page_scales,
+                               int64_t n_pages, int64_t P, const int32_t* table, int64_t ld_table, int64_t cols,
+                               const int32_t* lens, const int32_t* cu, int64_t B, int64_t T, int64_t H, int64_t D,
+                               int64_t DV, float scale, const float* attn_sink, int64_t window, int64_t first, int flags,
+                               void* out, int out_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  return smla_paged_attn_granted(q, q_dtype, pages, page_dtype, page_scales, n_pages, P, table, ld_table, cols, lens, cu,
+                                 nullptr, B, T, H, D, DV, scale, attn_sink, window, first, flags, out, out_dtype,
+                                 workspace, workspace_bytes, stream);
 }

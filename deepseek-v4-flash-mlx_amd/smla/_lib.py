@@ -80,6 +80,11 @@ _SIGNATURES = {
     "smla_paged_attn_workspace": (_sz, [_i64] * 6),
     "smla_paged_attn": (_int, [_vp, _int, _vp, _int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
                                _i64, _f32, _vp, _i64, _i64, _int, _vp, _int, _vp, _sz, _vp]),
+    "smla_paged_attn_granted": (_int, [_vp, _int, _vp, _int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64,
+                                       _i64, _i64, _i64, _f32, _vp, _i64, _i64, _int, _vp, _int, _vp, _sz, _vp]),
+    "smla_paged_append_granted": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64,
+                                         _f32, _int, _int, _vp, _vp, _int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
+                                         _i64, _vp]),
     "smla_paged_append": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _f32,
                                  _int, _int, _vp, _vp, _int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp]),
     "smla_update_pages_workspace": (_sz, [_i64] * 3),

@@ -1011,22 +1011,24 @@ def _check_pool(pages, page_scales, dims):
     return _lib.FP8_E4M3 if fp8 else _lib.BF16
 
 
-def _check_batch(table, lens, cu):
-    """table, lens, cu, sequences, the table's columns and row stride."""
+def _check_batch(table, lens, cu, granted=None):
+    """table, lens, cu, sequences, the table's columns and row stride (a granted that is given is checked only)."""
     table = _i32_rows(table, "table")
     B, cols = table.shape
     # (one test where all is as it should be; else the one that names what is not)
     if not (lens.dtype == cu.dtype == torch.int32 and lens.shape == (B,) and cu.shape == (B + 1,) and lens.is_contiguous()
             and cu.is_contiguous()):
         lens, cu = _i32(lens, (B,), "lens"), _i32(cu, (B + 1,), "cu")
+    if granted is not None and not (granted.dtype == torch.int32 and granted.shape == (B,) and granted.is_contiguous()):
+        raise ValueError(f"granted must be dense int32 [{B}], got {granted.dtype} {list(granted.shape)}")
     return table, lens, cu, B, cols, table.stride(0) if B > 1 else cols
 
 
 def _paged_attn_(q: torch.Tensor, pages: torch.Tensor, page_scales: Optional[torch.Tensor], table: torch.Tensor,
                  lens: torch.Tensor, cu: torch.Tensor, attn_sink: Optional[torch.Tensor], scale: float, window: int,
-                 first: int, fill: bool, out: torch.Tensor) -> None:
-    """``smla_paged_attn`` into out [T, H, DV] (see ``paged.paged_attn``)."""
-    dev = _one_device(q, pages, page_scales, table, lens, cu, attn_sink, out)
+                 first: int, fill: bool, out: torch.Tensor, granted: Optional[torch.Tensor] = None) -> None:
+    """``smla_paged_attn_granted`` into out [T, H, DV] (see ``paged.paged_attn``)."""
+    dev = _one_device(q, pages, page_scales, table, lens, cu, attn_sink, out, granted)
     shape = out.shape
     if q.dim() != 3 or len(shape) != 3:
         raise ValueError(f"expected q [T,H,D] and out [T,H,dv], got {list(q.shape)} and {list(shape)}")
@@ -1045,23 +1047,23 @@ def _paged_attn_(q: torch.Tensor, pages: torch.Tensor, page_scales: Optional[tor
         if tuple(attn_sink.shape) != (H,):
             raise ValueError(f"attn_sink {list(attn_sink.shape)} must be [{H}]")
         attn_sink = _f32(attn_sink)
-    table, lens, cu, B, cols, ld = _check_batch(table, lens, cu)
+    table, lens, cu, B, cols, ld = _check_batch(table, lens, cu, granted)
     if T == 0:
         return
     if not q.is_contiguous() or q.data_ptr() & 15:     # rows are copied 16 bytes at a time
         q = q.clone(memory_format=torch.contiguous_format)
     wsb = _lib.lib().smla_paged_attn_workspace(T, H, B, cols * P, window, first)
     ws = torch.empty(wsb, dtype=torch.uint8, device=q.device)
-    _launch(dev, "smla_paged_attn", q.data_ptr(), _lib.BF16, pages.data_ptr(), code, _p(page_scales), n_pages, P,
-            table.data_ptr(), ld, cols, lens.data_ptr(), cu.data_ptr(), B, T, H, D, shape[2], scale, _p(attn_sink), window, first, _lib.PAGED_FILL if fill else 0, out.data_ptr(), _lib.BF16,
-            ws.data_ptr(), wsb)
+    _launch(dev, "smla_paged_attn_granted", q.data_ptr(), _lib.BF16, pages.data_ptr(), code, _p(page_scales), n_pages, P,
+            table.data_ptr(), ld, cols, lens.data_ptr(), cu.data_ptr(), _p(granted), B, T, H, D, shape[2], scale,
+            _p(attn_sink), window, first, _lib.PAGED_FILL if fill else 0, out.data_ptr(), _lib.BF16, ws.data_ptr(), wsb)
 
 
 paged_attn_op_ = torch.library.custom_op("smla::paged_attn_", mutates_args=("out",), device_types="cuda")(_paged_attn_)
 
 
 @paged_attn_op_.register_fake
-def _(q, pages, page_scales, table, lens, cu, attn_sink, scale, window, first, fill, out):
+def _(q, pages, page_scales, table, lens, cu, attn_sink, scale, window, first, fill, out, granted=None):
     return None
 
 
@@ -1077,9 +1079,9 @@ def _norm_weights(w, n, name):
 def _paged_append_(q: Optional[torch.Tensor], kv: torch.Tensor, pages: torch.Tensor, page_scales: Optional[torch.Tensor],
                    table: torch.Tensor, lens: torch.Tensor, cu: torch.Tensor, cos_t: torch.Tensor, sin_t: torch.Tensor,
                    q_norm: Optional[torch.Tensor], kv_norm: Optional[torch.Tensor], norm_dims: int, fp8_sim: bool,
-                   eps: float, flags: int, q_out: Optional[torch.Tensor]) -> None:
-    """``smla_paged_append`` (see ``paged.paged_append``)."""
-    dev = _one_device(kv, q, pages, page_scales, table, lens, cu, cos_t, sin_t, q_norm, kv_norm, q_out)
+                   eps: float, flags: int, q_out: Optional[torch.Tensor], granted: Optional[torch.Tensor] = None) -> None:
+    """``smla_paged_append_granted`` (see ``paged.paged_append``)."""
+    dev = _one_device(kv, q, pages, page_scales, table, lens, cu, cos_t, sin_t, q_norm, kv_norm, q_out, granted)
     if kv.dim() != 2:
         raise ValueError("expected kv [T,D]")
     T, D = kv.shape
@@ -1116,15 +1118,15 @@ def _paged_append_(q: Optional[torch.Tensor], kv: torch.Tensor, pages: torch.Ten
         raise ValueError("rotation tables must be [n_pos, rd/2]")
     cos_t, sin_t = _f32(cos_t), _f32(sin_t)
     n_pos, rd2 = cos_t.shape
-    table, lens, cu, B, cols, ld = _check_batch(table, lens, cu)
+    table, lens, cu, B, cols, ld = _check_batch(table, lens, cu, granted)
     if T == 0:
         return
     if T == 1:
         ldq, ldkv = H * D, D
-    _launch(dev, "smla_paged_append", _p(q), ldq, kv.data_ptr(), ldkv, xdt, T, H, D, norm_dims, _p(q_norm), _p(kv_norm),
+    _launch(dev, "smla_paged_append_granted", _p(q), ldq, kv.data_ptr(), ldkv, xdt, T, H, D, norm_dims, _p(q_norm), _p(kv_norm),
             cos_t.data_ptr(), sin_t.data_ptr(), n_pos, 2 * rd2, eps, _lib.SIM_FP8 if fp8_sim else _lib.SIM_NONE, flags,
             _p(q_out), pages.data_ptr(), code, _p(page_scales), n_pages, P, table.data_ptr(), ld, cols, lens.data_ptr(),
-            cu.data_ptr(), B)
+            cu.data_ptr(), _p(granted), B)
 
 
 paged_append_op_ = torch.library.custom_op("smla::paged_append_", mutates_args=("pages", "page_scales", "q_out"),
@@ -1132,7 +1134,8 @@ paged_append_op_ = torch.library.custom_op("smla::paged_append_", mutates_args=(
 
 
 @paged_append_op_.register_fake
-def _(q, kv, pages, page_scales, table, lens, cu, cos_t, sin_t, q_norm, kv_norm, norm_dims, fp8_sim, eps, flags, q_out):
+def _(q, kv, pages, page_scales, table, lens, cu, cos_t, sin_t, q_norm, kv_norm, norm_dims, fp8_sim, eps, flags, q_out,
+      granted=None):
     return None
 
 

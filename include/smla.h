@@ -42,6 +42,7 @@
  *   smla_q_up                 oracle/decode_engine.py:78-80    q_up, per-head norm and RoPE of a prompt
  *   smla_paged_attn           oracle/decode_engine.py:107-117  the attention of a ragged batch over pages of rows
  *   smla_paged_append         oracle/decode_engine.py:78-84    q / kv norms, RoPE, quantisation, write to pages
+ *   smla_paged_attn_granted, smla_paged_append_granted          the same, but for sequences without rows for them
  *   smla_update_pages         oracle/v4_fast.py:150-159        copies of sequences' caches (clone_states), as pages
  *   smla_compact_pages        (none: the reference's caches are contiguous)
  *   smla_o_proj, _ws          oracle/decode_engine.py:118-119  inverse RoPE of o's rope dims + o_grouped
@@ -528,12 +529,16 @@ int smla_o_proj_ws(const void* o, int o_dtype, const int32_t* pos, const float* 
  * All integers are int32 on the device and none is read by the host, so a captured call follows
  * them.  A page id outside [0, n_pages) is no page: such rows are not read, written or counted.
  * Several sequences may share a page; rows are then appended only past the rows they share
- * (smla_update_pages keeps it so).  n_pages * P < 2^31.
+ * (smla_update_pages keeps it so, for the slots that it granted).  n_pages * P < 2^31.
  *
  * A batch is ragged: B sequences with lens[b] rows in the cache, the last cu[b+1] - cu[b] of them those
  * of the tokens cu[b] .. cu[b+1]-1 (cu [B+1], cu[0] = 0, not decreasing, cu[B] <= T); token t sits at position
  * lens[b] - (cu[b+1] - cu[b]) + t - cu[b].  What belongs to tokens of no sequence is left as it was, or, with
- * SMLA_PAGED_FILL, set to 0. */
+ * SMLA_PAGED_FILL, set to 0.
+ *
+ * The _granted forms take granted [B] beside cu (NULL: as the others), what smla_update_pages returns: where it is 0 the
+ * tokens of cu[b] .. cu[b+1]-1 are tokens of no sequence.  A slot whose growth was refused has no rows for its
+ * new tokens: without granted they would be written over its last rows, which it may share. */
 enum { SMLA_PAGED_NORM_Q = 1, SMLA_PAGED_NORM_KV = 2, SMLA_PAGED_FILL = 4 };
 
 /* smla_paged_attn: attention of those tokens over their sequences' rows, after the rows are in the cache.
@@ -553,6 +558,12 @@ int smla_paged_attn(const void* q, int q_dtype, const void* pages, int page_dtyp
                     const int32_t* lens, const int32_t* cu, int64_t B, int64_t T, int64_t H, int64_t D, int64_t DV,
                     float scale, const float* attn_sink, int64_t window, int64_t first, int flags, void* out,
                     int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
+int smla_paged_attn_granted(const void* q, int q_dtype, const void* pages, int page_dtype, const float* page_scales,
+                            int64_t n_pages, int64_t P, const int32_t* table, int64_t ld_table, int64_t cols,
+                            const int32_t* lens, const int32_t* cu, const int32_t* granted, int64_t B, int64_t T,
+                            int64_t H, int64_t D, int64_t DV, float scale, const float* attn_sink, int64_t window,
+                            int64_t first, int flags, void* out, int out_dtype, void* workspace, size_t workspace_bytes,
+                            void* stream);
 
 /* smla_paged_append: the tokens' queries and latent rows from their projections, in one launch.
  *   q [T, H, D] (tokens ldq elements apart; H = 0: none) and kv [T, D] (ldkv apart), both F32 or BF16
@@ -569,6 +580,12 @@ int smla_paged_append(const void* q, int64_t ldq, const void* kv, int64_t ldkv, 
                       const float* sin_t, int64_t n_pos, int64_t rd, float eps, int sim, int flags, void* q_out,
                       void* pages, int page_dtype, float* scales, int64_t n_pages, int64_t P, const int32_t* table,
                       int64_t ld_table, int64_t cols, const int32_t* lens, const int32_t* cu, int64_t B, void* stream);
+int smla_paged_append_granted(const void* q, int64_t ldq, const void* kv, int64_t ldkv, int x_dtype, int64_t T, int64_t H,
+                              int64_t D, int64_t norm_dims, const float* q_w, const float* kv_w, const float* cos_t,
+                              const float* sin_t, int64_t n_pos, int64_t rd, float eps, int sim, int flags, void* q_out,
+                              void* pages, int page_dtype, float* scales, int64_t n_pages, int64_t P,
+                              const int32_t* table, int64_t ld_table, int64_t cols, const int32_t* lens,
+                              const int32_t* cu, const int32_t* granted, int64_t B, void* stream);
 
 /* smla_update_pages: what happens to S slots between two steps, all at once.  Slot s becomes a copy of slot
  * parent[s] as it was before the call (s: itself, -1: an empty slot) with grow[s] >= 0 more rows:
@@ -576,7 +593,7 @@ int smla_paged_append(const void* q, int64_t ldq, const void* kv, int64_t ldkv, 
  *     fresh page, unless the slot keeps its own (parent[s] == s);
  *   - fresh pages are the free ones (refs 0) in ascending order, taken by the slots in order;
  *   - granted[s] = 1 if parent[s] and grow[s] are valid, the rows fit M pages and the pages that slots 0 .. s ask
- *     for are at most the free ones; else 0, and the slot stays as it was.
+ *     for are at most the free ones; else 0, and the slot stays as it was (its new tokens: see the _granted forms).
  * In: table [S, M] (ld_table), lens [S], refs [n_pages] (how many entries name each page).  Out, all other
  * buffers than the inputs: table_out [S, M] dense (-1 past a slot's pages), lens_out, refs_out, granted [S].
  * Pages given up by the call are free from refs_out on.  Rows are copied within `layers` pools that share the table

@@ -38,3 +38,127 @@ def test_attn_window_past_the_table_split(dev, window, first, length):
     out = paged.paged_attn(dq, dp, dt, _i32([length], dev), _i32([0, 2], dev), 576 ** -0.5, None, window, first)
     torch.cuda.synchronize()
     _check_attn(out, q, pages, None, table, [length], [0, 2], None, window, first)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("capture", [False, True])
+def test_refused_slots_leave_every_row(dev, kv, capture):
+    """update -> append -> attn over a pool that runs out while slots share a full last page: the tokens of a refused slot
+    write nothing and give 0, every older row keeps its bits, the granted slots go on, and a refused one does so
+    once there are pages again."""
+    from smla import paged
+    announce(f"a step with refused slots, {kv}, {'captured' if capture else 'eager'}")
+    S, M, P, n_pages, H, D, T = 4, 6, 8, 8, 16, 512, 52
+    g = torch.Generator().manual_seed(31)
+    cos, sin = _to(dev, *_tables(dev, M * P, 64))
+    pages = torch.full((n_pages, P, D), float("nan"), dtype=torch.bfloat16, device=dev)
+    scales = None
+    if kv == "fp8":
+        pages = torch.full((n_pages, P, D), 0x7f, dtype=torch.uint8, device=dev)
+        scales = torch.full((n_pages, P, D // 64), float("nan"), device=dev)
+    zeros = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)  # noqa: E731
+    table, lens, refs = torch.full((S, M), -1, dtype=torch.int32, device=dev), zeros(S), zeros(n_pages)
+    parent, grow, cu = zeros(S), zeros(S), zeros(S + 1)
+    q, x = torch.zeros(T, H, D, device=dev), torch.zeros(T, D, device=dev)
+    mine, mine_q = [torch.zeros(T, H, D, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+    res = {}
+
+    def step():
+        t, n, f, ok = paged.update_pages(pages, table, lens, refs, parent, grow, page_scales=scales)
+        kw = dict(page_scales=scales, granted=ok)
+        qs = paged.paged_append(q, x, pages, t, n, cu, cos, sin, kv_norm=True, q_norm=True, **kw)
+        o = paged.paged_attn(qs, pages, t, n, cu, D ** -0.5, **kw)
+        paged.paged_append(q, x, pages, t, n, cu, cos, sin, kv_norm=True, q_norm=True, q_out=mine_q, **kw)
+        paged.paged_attn(qs, pages, t, n, cu, D ** -0.5, out=mine, **kw)
+        table.copy_(t), lens.copy_(n), refs.copy_(f)
+        res.update(q=qs, o=o, ok=ok)
+
+    graph = None
+    if capture:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+    dense = [[] for _ in range(S)]
+    # (parents, growth, what is granted): slots 0 and 1 share the two whole pages of a prompt of 16, slots 2 and 3 take
+    # five of the other six; the last goes to slot 0, then there are none until slot 0 is emptied
+    plan = [([-1, -1, -1, -1], [16, 0, 17, 16], [1, 1, 1, 1]), ([0, 0, 2, 3], [0, 0, 0, 0], [1, 1, 1, 1]),
+            ([0, 1, 2, 3], [1, 1, 1, 1], [1, 0, 0, 0]), ([0, 1, 2, 3], [7, 0, 2, 0], [1, 1, 1, 1]),
+            ([0, 1, 2, 3], [0, 3, 1, 1], [1, 0, 0, 0]), ([0, 0, 2, 3], [0, 3, 0, 0], [1, 0, 0, 0]),
+            ([-1, 1, 2, 3], [0, 1, 0, 0], [1, 0, 0, 0]), ([0, 1, 2, 3], [0, 3, 1, 1], [1, 1, 1, 0])]
+    for k, (ps, gs, want_ok) in enumerate(plan):
+        c = _cu(gs)
+        for dst, v in ((parent, ps), (grow, gs), (cu, c)):
+            dst.copy_(_i32(v, dev))
+        q.copy_(torch.randn(T, H, D, generator=g))
+        x.copy_(torch.randn(T, D, generator=g))
+        mine.fill_(7.0), mine_q.fill_(7.0)
+        t_want, l_want, r_want, ok_want, copies = op.update_pages((P, n_pages), table.tolist(), lens.tolist(), refs.tolist(), ps, gs)
+        assert ok_want == want_ok
+        before = pages.clone().view(torch.uint8).cpu()
+        step() if graph is None else graph.replay()
+        torch.cuda.synchronize()
+        assert (res["ok"].tolist(), table.tolist(), lens.tolist(), refs.tolist()) == (ok_want, t_want, l_want, r_want)
+        dense = [(list(dense[p]) if p >= 0 else []) if ok else dense[s] for s, (p, ok) in enumerate(zip(ps, ok_want))]
+        host, hs = pages.cpu(), None if scales is None else scales.cpu()
+        hp = host if scales is None else host.view(torch.float8_e4m3fn)
+        new = set()
+        for s in range(S):
+            rows = [hp[t_want[s][j // P], j % P].double() * (1.0 if hs is None else hs[t_want[s][j // P], j % P].double().repeat_interleave(64))
+                    for j in range(l_want[s])]
+            for j, old in enumerate(dense[s]):
+                assert torch.equal(rows[j], old), (k, s, j)
+            new |= {(t_want[s][j // P], j % P) for j in range(len(dense[s]), l_want[s])}
+            dense[s] = rows
+        new |= {(b, j) for _, b, n in copies for j in range(n)}
+        changed = (host.view(torch.uint8) != before).flatten(2).any(-1).nonzero().tolist()
+        assert {tuple(i) for i in changed} <= new, k
+        seen = [n if ok else -1 for n, ok in zip(l_want, ok_want)]     # a refused slot's tokens see nothing
+        if c[-1]:
+            _check_attn(res["o"], res["q"].cpu(), hp, hs, torch.tensor(t_want), seen, c, None, 0, 0)
+        for s in range(S):
+            of = slice(c[s], c[s + 1])
+            if ok_want[s]:
+                assert torch.equal(mine[of], res["o"][of]) and torch.equal(mine_q[of], res["q"][of])
+                assert c[s] == c[s + 1] or (res["q"][of] != 0).any(-1).all()
+            else:
+                assert (mine[of] == 7).all() and (mine_q[of] == 7).all() and not res["o"][of].any() and not res["q"][of].any()
+        assert not res["o"][c[-1]:].any() and (mine[c[-1]:] == 7).all()
+
+
+def test_refused_slots_among_many(dev):
+    """Sequences past a wave's lanes, every third refused, tiles split and whole: as with their tokens taken out."""
+    from smla import paged
+    announce("paged_attn and paged_append of 150 sequences, every third refused")
+    r = random.Random(2)
+    n = [r.choice([0, 1, 1, 3]) for _ in range(150)]
+    lens = [k + r.randint(0, 60) for k in n]
+    lens[70], n[70] = 3000, 2
+    lens[69], n[69] = 900, 1
+    granted = [int(b % 3 != 0) for b in range(150)]
+    pages, _, table = _cache(209, lens, 16, 512)
+    cu = _cu(n)
+    q = torch.randn(cu[-1] + 3, 16, 512, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    dq, dp, dt = _to(dev, q, pages, table)
+    ok = _i32(granted, dev)
+    out = paged.paged_attn(dq, dp, dt, _i32(lens, dev), _i32(cu, dev), 512 ** -0.5, granted=ok)
+    all_ = paged.paged_attn(dq, dp, dt, _i32(lens, dev), _i32(cu, dev), 512 ** -0.5, granted=torch.ones_like(ok))
+    assert torch.equal(all_, paged.paged_attn(dq, dp, dt, _i32(lens, dev), _i32(cu, dev), 512 ** -0.5))
+    seen = [k if ok else -1 for k, ok in zip(lens, granted)]
+    _check_attn(out, q, pages, None, table, seen, cu, None, 0, 0)
+    assert not out[cu[-1]:].any()
+    before, cos, sin = dp.clone(), *_to(dev, *_tables(dev, 3000, 64))
+    mine = torch.full_like(dq, 7.0)
+    paged.paged_append(dq, dq[:, 0], dp, dt, _i32(lens, dev), _i32(cu, dev), cos, sin, q_out=mine, granted=ok)
+    wrote = (dp != before).any(-1).cpu()
+    for b, ok in enumerate(granted):
+        for i in range(n[b]):
+            j = lens[b] - n[b] + i
+            assert bool(wrote[table[b, j // 16], j % 16]) == bool(ok) and bool((mine[cu[b] + i] == 7).all()) != bool(ok)
+            wrote[table[b, j // 16], j % 16] = False
+    assert not wrote.any()
