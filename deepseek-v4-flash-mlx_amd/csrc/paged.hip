@@ -171,15 +171,16 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
 #pragma unroll
   for (int c = 0; c < NCH; c++) {
     const int ch = 256 * c + 4 * lane;
-    // per 64 channels: s = 2^ceil(log2(max(|y|, 1e-4) / 448)), code = e4m3(y / s) to nearest even
+    // per 64 channels: s = 2^ceil(log2(max(|y|, 1e-4) / 448)), code = e4m3(y / s) to nearest even (NaN, as the whole block's
+    // value, where the largest is not finite: the page shows what a bf16 page would)
     const bool coded = a.page_dtype == SMLA_FP8_E4M3 || (a.sim == SMLA_SIM_FP8 && ch < nope);
     f32x4_t y = v[c];
-    float m = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
-    m = fmaxf(m, dpp_f<0xB1>(m));
-    m = fmaxf(m, dpp_f<0x4E>(m));
-    m = fmaxf(m, dpp_f<0x141>(m));
-    m = fmaxf(m, dpp_f<0x140>(m));
-    const float s = pow2_ceil(fmaxf(m, 1e-4f) / 448.0f);
+    uint32_t m = max(max(mag_bits(y[0]), mag_bits(y[1])), max(mag_bits(y[2]), mag_bits(y[3])));
+    m = max(m, dpp_u<0xB1>(m));
+    m = max(m, dpp_u<0x4E>(m));
+    m = max(m, dpp_u<0x141>(m));
+    m = max(m, dpp_u<0x140>(m));
+    const float s = fp8_scale(m);
     if (ch >= D || !stored) continue;
     if (coded) {
       float z[4];
@@ -187,6 +188,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
       for (int k = 0; k < 4; k++) z[k] = fminf(fmaxf(y[k] / s, -448.f), 448.f);
       int code = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
       code = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], code, true);
+      if (m >= kNotFinite) code = kNanCodes;
       if (a.page_dtype == SMLA_FP8_E4M3) {
         *(int*)((uint8_t*)a.pages + row * D + ch) = code;
         if ((lane & 15) == 0) a.scales[row * (D / 64) + ch / 64] = s;

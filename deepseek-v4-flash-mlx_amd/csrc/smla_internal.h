@@ -107,6 +107,16 @@ __host__ __device__ inline float pow2_ceil(float v) {
   return f;
 }
 
+// Scales of e4m3 blocks.  A block's largest magnitude is taken over bits (finite < infinite < NaN; fmaxf would drop a
+// NaN): s = 2^ceil(log2(max(m, 1e-4) / 448)), or m itself where it is not finite, and the block's codes are NaN then.
+constexpr uint32_t kNotFinite = 0x7f800000u;
+constexpr int kNanCodes = 0x7f7f7f7f;  // four e4m3 NaNs
+__device__ inline uint32_t mag_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ inline float fp8_scale(uint32_t m) {
+  const float a = __uint_as_float(max(m, 0x38d1b717u));  // 1e-4
+  return m < kNotFinite ? pow2_ceil(a / 448.0f) : a;
+}
+
 // ---------------------------------------------------------------------------------------------
 // fp4 e2m1 (grid 0, 0.5, 1, 1.5, 2, 3, 4, 6; bit 3 the sign) with power-of-two block scales.
 // Round to nearest, ties to the even code: the magnitude code counts the decision points passed,
@@ -180,6 +190,10 @@ __device__ inline int dpp_i(int v) {
 template <int CTRL>
 __device__ inline float dpp_f(float v) {
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+template <int CTRL>
+__device__ inline uint32_t dpp_u(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, false);
 }
 // wave-wide max / min (every lane gets the result)
 __device__ inline float wave_max_dpp(float v) {

@@ -571,7 +571,7 @@ int smla_paged_attn_granted(const void* q, int q_dtype, const void* pages, int p
  * RMS-normed (eps; weights q_w / kv_w [norm_dims] fp32, NULL: none); then the last rd channels are rotated to
  * the token's position as in smla_rope (cos_t, sin_t [n_pos, rd/2] fp32).  Queries go to q_out [T, H, D] BF16,
  * the row to its page: BF16 (sim SMLA_SIM_FP8: its first D - rd channels fp8 round-tripped) or e4m3 codes and
- * scales, quantised as smla_quant_fp8_pow2 does.  A token at a position outside [0, n_pos) (rd > 0) writes
+ * scales, quantised as smla_quant_fp8_pow2 does; a 64-channel block with a value that is not finite is NaN in all of it.  A token at a position outside [0, n_pos) (rd > 0) writes
  * nothing (SMLA_PAGED_FILL: zero queries); a row past the table's columns or whose entry is no
  * page is not stored.  D a multiple of 64 up to 1024, rd and norm_dims multiples of 4, ldq and ldkv too; rd a
  * multiple of 64 with SMLA_SIM_FP8; q and kv aligned to four of their elements, q_out and pages to 8 bytes. */

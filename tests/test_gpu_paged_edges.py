@@ -162,3 +162,48 @@ def test_refused_slots_among_many(dev):
             assert bool(wrote[table[b, j // 16], j % 16]) == bool(ok) and bool((mine[cu[b] + i] == 7).all()) != bool(ok)
             wrote[table[b, j // 16], j % 16] = False
     assert not wrote.any()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("xdt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kv,kv_norm", [("bf16", True), ("bf16", None), ("sim", True), ("sim", None), ("fp8", True), ("fp8", None)])
+def test_append_keeps_what_is_not_finite(dev, bad, xdt, kv, kv_norm):
+    """A channel that is not finite shows in the stored row, whatever the pages hold: as it is in bf16, as NaN over its
+    64-channel block where that is scaled by its largest magnitude; other blocks, rows and queries are as without it."""
+    from smla import paged
+    announce(f"paged_append of {bad} {xdt} {kv} norm={kv_norm}")
+    D, P, H, rd, lens = 576, 8, 3, 64, [9]
+    pages, scales, table = _cache(204, lens, P, D, "fp8" if kv == "fp8" else "bf16")
+    g = torch.Generator().manual_seed(4)
+    q, x = torch.randn(4, H, D, generator=g).to(xdt), torch.randn(4, D, generator=g).to(xdt)
+    x[1, 70], x[3, 5], x[3, 575] = bad, bad, bad
+    q[2, 1, 130] = bad
+    cos, sin = _tables(dev, 9, rd)
+    cu, nd = [0, 4], 512
+    args = _to(dev, q, x, pages, table)
+    dc, dsn, ds = _to(dev, cos, sin, scales)
+    out = paged.paged_append(*args[:3], args[3], _i32(lens, dev), _i32(cu, dev), dc, dsn, kv_norm=kv_norm, q_norm=True, norm_dims=nd,
+                             page_scales=ds, fp8_sim=kv == "sim").double().cpu()
+    got = args[2].cpu() if kv != "fp8" else args[2].cpu().view(torch.float8_e4m3fn)
+    for t, p in enumerate(range(5, 9)):
+        y = op.norm_rope(q[t], None, True, nd, cos[p], sin[p], 1e-6)
+        assert torch.equal(out[t].isnan(), y.isnan())
+        ok = ~y.isnan()
+        assert ((out[t] - y).abs() <= BF16 * y.abs() + 2.0 ** -16)[ok].all()
+        y = op.norm_rope(x[t, None], None, bool(kv_norm), nd, cos[p], sin[p], 1e-6)[0]
+        page = int(table[0, p // P])
+        val = got[page, p % P].double()
+        coded = {"bf16": 0, "sim": D - rd, "fp8": D}[kv]
+        if kv == "fp8":
+            val = val * ds.cpu()[page, p % P].double().repeat_interleave(64)
+        want = y.clone()
+        blocks = want[:coded].unflatten(0, (-1, 64))
+        blocks[~blocks.isfinite().all(-1)] = float("nan")
+        assert torch.equal(val.isnan(), want.isnan()), t
+        inf = want.isinf()
+        assert torch.equal(val[inf], want[inf])
+        ok = want.isfinite()
+        rel = torch.full((D,), BF16, dtype=torch.float64)
+        rel[:coded] = 2.0 ** -4
+        # (blocks of ordinary values: the largest is at most 2^3, so a subnormal half step is under 2^-10 * 2^-5)
+        assert ((val - want).abs() <= rel * want.abs() + 2.0 ** -14)[ok].all(), t
