@@ -145,16 +145,16 @@ __device__ inline f32x2_t epilogue_values(float v0, float v1, int d, int rd, flo
   }
   if (sim == SMLA_SIM_FP8 && c0 < nope) {
     // 64-channel blocks = 32 consecutive threads (half a wave)
-    float a = fmaxf(fabsf(y0), fabsf(y1));
+    uint32_t m = max(mag_bits(y0), mag_bits(y1));
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
-    a = fmaxf(a, 1e-4f);
-    float s = pow2_ceil(a / 448.0f);
+    for (int o = 16; o >= 1; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+    const float s = fp8_scale(m);
     float z0 = fminf(fmaxf(y0 / s, -448.f), 448.f);
     float z1 = fminf(fmaxf(y1 / s, -448.f), 448.f);
     // e4m3 round trip by the gfx950 converters (round-to-nearest-even encode of the clamped
     // values, exact decode): the codes of f32_to_e4m3
-    const f32x2_t q = __builtin_amdgcn_cvt_pk_f32_fp8(__builtin_amdgcn_cvt_pk_fp8_f32(z0, z1, 0, false), false);
+    const int code = __builtin_amdgcn_cvt_pk_fp8_f32(z0, z1, 0, false);
+    const f32x2_t q = __builtin_amdgcn_cvt_pk_f32_fp8(m < kNotFinite ? code : kNanCodes, false);
     y0 = q[0] * s;
     y1 = q[1] * s;
   } else if (sim == SMLA_SIM_ROTATE_FP4) {
@@ -410,13 +410,12 @@ __global__ __launch_bounds__(256) void quant_kernel(const void* __restrict__ x, 
       v[3] = bf16_bits_to_f32((uint16_t)(w[1] >> 16));
     }
   }
-  float a = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-  a = fmaxf(a, dpp_f<0xB1>(a));
-  a = fmaxf(a, dpp_f<0x4E>(a));
-  a = fmaxf(a, dpp_f<0x141>(a));
-  a = fmaxf(a, dpp_f<0x140>(a));  // every lane of the 16-lane row: the block's abs-max
-  a = fmaxf(a, 1e-4f);
-  const float s = pow2_ceil(a / 448.0f);
+  uint32_t m = max(max(mag_bits(v[0]), mag_bits(v[1])), max(mag_bits(v[2]), mag_bits(v[3])));
+  m = max(m, dpp_u<0xB1>(m));
+  m = max(m, dpp_u<0x4E>(m));
+  m = max(m, dpp_u<0x141>(m));
+  m = max(m, dpp_u<0x140>(m));  // every lane of the 16-lane row: the block's abs-max
+  const float s = fp8_scale(m);
   const float inv = 1.0f / s;
   if (!ok) return;
   // the gfx950 converter encodes OCP e4m3 with round-to-nearest-even; on the clamped values it
@@ -427,6 +426,7 @@ __global__ __launch_bounds__(256) void quant_kernel(const void* __restrict__ x, 
   for (int by = 0; by < 4; by++) z[by] = fminf(fmaxf(v[by] * inv, -448.f), 448.f);
   int word = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
   word = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], word, true);
+  if (m >= kNotFinite) word = kNanCodes;
   *(uint32_t*)(codes + e0) = (uint32_t)word;
   if (sub == 0) scales[blk] = s;
 }

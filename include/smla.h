@@ -310,6 +310,7 @@ int smla_block_mean_pool(const void* x, int x_dtype, int64_t B, int64_t N, int64
  * and smla_ring_step):
  *   SMLA_SIM_NONE        none (ref_torch/compressor.py:21-50);
  *   SMLA_SIM_FP8         the d-rd non-rope channels fp8 round-tripped with pow2 block-64 scales
+ *                        (NaN in all of a block with a value that is not finite)
  *                        (v4mlx/compressor.py:60-62, apply_sim=True);
  *   SMLA_SIM_ROTATE_FP4  all d channels Hadamard-rotated, then fp4 round-tripped with pow2
  *                        block-32 scales (v4mlx/compressor.py:57-59, rotate=True: the indexer
@@ -425,7 +426,8 @@ int smla_decode_ids(const int32_t* pos, int64_t B, int64_t window, int64_t ratio
                     int32_t* ids, int64_t T, const float* comp32, uint16_t* comp_out, int64_t d, void* stream);
 
 /* smla_quant_fp8_pow2: per 64-element block, s = 2^ceil(log2(max(|x|,1e-4)/448)),
- * code = e4m3(clip(x/s, +-448)) (round to nearest even).  x [rows, D] F32|BF16 (D % 64 == 0),
+ * code = e4m3(clip(x/s, +-448)) (round to nearest even); a block with a value that is not finite is NaN in all of
+ * its codes, its scale that magnitude.  x [rows, D] F32|BF16 (D % 64 == 0),
  * codes [rows, D] uint8, scales [rows, D/64] fp32.  The stored form of act_quant_sim,
  * v4mlx/compressor.py:11-20. */
 int smla_quant_fp8_pow2(const void* x, int x_dtype, int64_t rows, int64_t D, uint8_t* codes,

@@ -243,3 +243,45 @@ def test_gated_pool_unaligned_output(dev):
     call(out[1].data_ptr() + 4)
     assert torch.equal(out[0, :n], out[1, 1:n + 1])
     assert out[1, 0] == 7.0 and out[1, n + 1] == 7.0 and bool((out[0, n:] == 7.0).all())
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("xdt", [torch.float32, torch.bfloat16])
+def test_quant_fp8_of_what_is_not_finite(dev, bad, xdt):
+    """A block with a value that is not finite decodes to NaN in all of it; the others are as without it."""
+    from smla import ops
+    announce(f"quant fp8 of {bad} {xdt}")
+    x = torch.randn(70, 256, generator=torch.Generator().manual_seed(9)).to(xdt)
+    y = x.clone()
+    y[3, 64], y[3, 255], y[69, 130] = bad, bad, bad
+    hit = torch.zeros(70, 4, dtype=torch.bool)
+    hit[3, 1], hit[3, 3], hit[69, 2] = True, True, True
+    want_codes, want_scales = [t.cpu() for t in ops.quant_fp8_pow2_op(x.to(dev))]
+    codes, scales = [t.cpu() for t in ops.quant_fp8_pow2_op(y.to(dev))]
+    value = codes.view(torch.float8_e4m3fn).float().unflatten(-1, (-1, 64)) * scales[..., None]
+    assert value[hit].isnan().all()
+    assert torch.equal(scales[~hit], want_scales[~hit])
+    assert torch.equal(codes.unflatten(-1, (-1, 64))[~hit], want_codes.unflatten(-1, (-1, 64))[~hit])
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_row_epilogue_fp8_keeps_what_is_not_finite(dev, bad):
+    """A row whose norm is not finite is NaN behind the fp8 round trip too: its channels that the rotation leaves are 0 or
+    NaN as without the round trip, by blocks of 64."""
+    from smla import norm_rope as snr
+    from smla import ops
+    announce(f"row epilogue, fp8 round trip of {bad}")
+    d, rd = 512, 64
+    x = torch.randn(6, d, generator=torch.Generator().manual_seed(10)).to(dev)
+    w, pos = torch.rand(d, device=dev) + 0.5, torch.arange(6, dtype=torch.int32, device=dev)
+    cos_t, sin_t = snr.rope_tables(rd, 16, device=dev)
+    run = lambda v, sim: ops.row_epilogue(v, w, pos, cos_t, sin_t, rd, sim, torch.empty(6, d, device=dev))  # noqa: E731
+    y = x.clone()
+    y[1, 200], y[4, 510] = bad, bad
+    want, got, plain = [run(*a).cpu() for a in ((x, 1), (y, 1), (y, 0))]
+    keep = torch.tensor([0, 2, 3, 5])
+    assert torch.equal(got[keep], want[keep])
+    for r in (1, 4):
+        blocks = plain[r, :d - rd].unflatten(0, (-1, 64)).isnan().any(-1, keepdim=True).expand(-1, 64).flatten()
+        assert torch.equal(got[r, :d - rd].isnan(), blocks) and torch.equal(got[r, d - rd:].isnan(), plain[r, d - rd:].isnan())
+        assert blocks.any() or r == 4
