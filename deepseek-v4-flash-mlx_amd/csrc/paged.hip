@@ -8,7 +8,7 @@
 //  * paged_append_kernel : per new token, the per-head RMS norm and RoPE of its query heads and the norm,
 //                          RoPE and quantisation of its latent row, written to the row's page.  One wave
 //                          per (token, head) row; nothing is read twice.
-//  * update_one / update_plan + update_apply : slot s becomes a copy of slot parent[s] plus grow[s] rows.
+//  * update_one / update_plan + update_apply : slot s becomes a copy of slot parent[s] plus (or less) grow[s] rows.
 //  * compact_one / compact_plan + compact_apply : live pages moved to the pool's first ids.
 #include "smla_internal.h"
 
@@ -344,25 +344,28 @@ struct PageArgs {
   int32_t* ws;
 };
 
-// What slot s asks for: rows of its parent, rows after growing, its whole pages taken from the parent,
-// pages after growing; false: an argument out of range.
+// What slot s asks for: rows taken from its parent (all, or those that a negative grow leaves), rows afterwards, entries
+// taken from the parent as they are, pages afterwards; false: an argument out of range.
 struct SlotNeed {
-  int have, next, full, pages, parent;
-  bool keep;
+  int rows, next, full, pages, parent;
 };
 __device__ inline bool slot_need(const PageArgs& a, int s, SlotNeed& n) {
   const int p = a.parent[s], g = a.grow[s];
-  if (p < -1 || p >= a.S || g < 0) return false;
-  n.have = p >= 0 ? a.lens[p] : 0;
-  n.keep = p == s;
+  if (p < -1 || p >= a.S) return false;
+  const int have = p >= 0 ? a.lens[p] : 0;
   n.parent = p;
-  if (n.have < 0 || (int64_t)n.have + g > 0x7fffffff) return false;
-  n.next = n.have + g;
+  const int64_t next = (int64_t)have + g;
+  if (have < 0 || next < 0 || next > 0x7fffffff) return false;
+  n.next = (int)next;
+  n.rows = min(have, n.next);
   const uint32_t P = (uint32_t)a.P;
-  const int64_t pages = ((int64_t)n.next + P - 1) / P;
+  const int64_t pages = (next + P - 1) / P;
   n.pages = (int)pages;
-  n.full = n.keep ? (int)(((int64_t)n.have + P - 1) / P) : (int)((uint32_t)n.have / P);
+  n.full = p == s ? (int)(((int64_t)n.rows + P - 1) / P) : (int)((uint32_t)n.rows / P);
   return pages <= a.M;
+}
+__device__ inline int tail_rows(const PageArgs& a, const SlotNeed& n) {
+  return (int)max((int64_t)n.rows - (int64_t)n.full * a.P, (int64_t)0);
 }
 
 // What becomes of slot s: its first fresh rank (-1: refused), the slot it copies, entries it shares with that, entries
@@ -373,7 +376,7 @@ struct SlotPlan {
 __device__ inline SlotPlan slot_plan(const PageArgs& a, int s, int at, const SlotNeed& n) {
   const int len = a.lens[s];
   return SlotPlan{at, n.parent, n.full, n.pages, len > 0 ? (int)(((uint32_t)len + (uint32_t)a.P - 1) / (uint32_t)a.P) : 0,
-                  n.keep ? 0 : n.have - n.full * a.P};
+                  tail_rows(a, n)};
 }
 // Entry c of slot s after the update, fresh(k) the fresh page of rank k; count(page, by) for every change of a page's holders.
 template <class Fresh, class Count>
@@ -381,9 +384,7 @@ __device__ inline int slot_entry(const PageArgs& a, int s, int c, const SlotPlan
   const int old = a.table[s * a.ld_table + c];
   if (n.at < 0) return old;
   const int now = c < n.full ? a.table[n.parent * a.ld_table + c] : c < n.pages ? fresh(n.at + c - n.full) : -1;
-  if (n.parent == s) {
-    if (c >= n.full && c < n.pages) count(now, 1);
-  } else {
+  if (n.parent != s || c >= n.full) {  // (a kept slot's first entries stay as they are)
     if (c < n.held) count(old, -1);
     if (c < n.pages) count(now, 1);
   }
@@ -428,7 +429,7 @@ __global__ __launch_bounds__(kPlanThreads) void update_one_kernel(const PageArgs
     free += (int)__builtin_popcountll(m[k]);
   }
   ok = ok && at + ask <= found;
-  const bool copy = ok && !n.keep && n.have > n.full * a.P;
+  const bool copy = ok && tail_rows(a, n) > 0;
   const int slot = block_excl(copy, l.red, ncopy);
   if (tid < a.S) l.slot[tid] = ok ? slot_plan(a, tid, at, n) : SlotPlan{-1};
   if (copy) l.copies[slot] = (uint16_t)tid;
@@ -519,7 +520,7 @@ __global__ __launch_bounds__(kPlanThreads) void update_plan_kernel(const PageArg
     if (!ok) rank[s] = -1;
     a.granted[s] = ok;
     a.lens_out[s] = ok ? n.next : a.lens[s];
-    if (ok && !n.keep && n.have > n.full * a.P) copies[atomicAdd(&ncopy, 1)] = s;
+    if (ok && tail_rows(a, n) > 0) copies[atomicAdd(&ncopy, 1)] = s;
   }
   __syncthreads();
   if (tid == 0) a.ws[0] = ncopy;

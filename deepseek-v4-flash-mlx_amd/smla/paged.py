@@ -75,13 +75,15 @@ def paged_append(q, kv, pages, table, lens, cu, cos_t, sin_t, kv_norm=None, q_no
 
 def update_pages(pages, table, lens, refs, parent, grow, page_scales=None):
     """Every slot's next state at once: slot s becomes a copy of slot parent[s] as before the call (s: itself, -1: an
-    empty slot) and grows by grow[s] rows.  Whole pages are shared, a copied slot's partly filled last page is
-    copied to a fresh one, fresh pages are the free ones (refs 0) in ascending order.  pages [n_pages, P, D] or
-    [layers, n_pages, P, D] (layers under one table), table [S, M], lens / parent / grow [S], refs [n_pages] int32.
-    Returns new (table, lens, refs, granted); granted[s] = 0 marks a slot left as it was (arguments out of
-    range, more than M pages, or not enough free pages for slots 0 .. s): it has no rows for its new tokens, so pass
-    granted on to ``paged_append`` and ``paged_attn``.  Freeing is parent -1, grow 0; beam
-    reordering any map; a new sequence of n rows parent -1, grow n."""
+    empty slot) and grows by grow[s] rows, or gives its last -grow[s] rows back.  Whole pages are shared, a copied
+    slot's partly filled last page is copied to a fresh one, fresh pages are the free ones (refs 0) in ascending order.
+    pages [n_pages, P, D] or [layers, n_pages, P, D] (layers under one table), table [S, M], lens / parent / grow [S],
+    refs [n_pages] int32.  Returns new (table, lens, refs, granted), the state of the next call (lengths change here
+    only); granted[s] = 0 marks a slot left as it was (arguments out of range, more than M pages, or not enough free
+    pages for slots 0 .. s): it has no rows for its new tokens, so pass granted on to ``paged_append`` and
+    ``paged_attn``.  Freeing is parent -1, grow 0; beam reordering any map; a new sequence of n rows parent -1, grow n;
+    a step after rejected drafts grow = new tokens - rejected ones (given back by a call of their own, grow < 0, where
+    another slot was made a copy of this one since they were written)."""
     return ops.update_pages_op(pages, page_scales, table, lens, refs, parent, grow)
 
 

@@ -590,16 +590,22 @@ int smla_paged_append_granted(const void* q, int64_t ldq, const void* kv, int64_
                               const int32_t* cu, const int32_t* granted, int64_t B, void* stream);
 
 /* smla_update_pages: what happens to S slots between two steps, all at once.  Slot s becomes a copy of slot
- * parent[s] as it was before the call (s: itself, -1: an empty slot) with grow[s] >= 0 more rows:
+ * parent[s] as it was before the call (s: itself, -1: an empty slot) with grow[s] more rows, or -grow[s] fewer
+ * (the last rows, those of rejected drafts, are given back and not copied):
  *   - its parent's whole pages are shared; of a partly filled last page the rows in use are copied to a
  *     fresh page, unless the slot keeps its own (parent[s] == s);
  *   - fresh pages are the free ones (refs 0) in ascending order, taken by the slots in order;
- *   - granted[s] = 1 if parent[s] and grow[s] are valid, the rows fit M pages and the pages that slots 0 .. s ask
- *     for are at most the free ones; else 0, and the slot stays as it was (its new tokens: see the _granted forms).
+ *   - granted[s] = 1 if parent[s] is valid, the parent's rows and grow[s] make 0 rows or more, they fit M pages and
+ *     the pages that slots 0 .. s ask for are at most the free ones; else 0, and the slot stays as it was (its new
+ *     tokens: see the _granted forms).
  * In: table [S, M] (ld_table), lens [S], refs [n_pages] (how many entries name each page).  Out, all other
  * buffers than the inputs: table_out [S, M] dense (-1 past a slot's pages), lens_out, refs_out, granted [S].
- * Pages given up by the call are free from refs_out on.  Rows are copied within `layers` pools that share the table
- * (layer l at pages + l layer_bytes; row_bytes a row), and likewise within scales (NULL: none).
+ * Pages given up by the call are free from refs_out on.  A slot holds the pages of its lens[s] rows, so lengths change
+ * by this call only: one lowered by hand leaves pages counted that no entry names.  Without forks one call with
+ * grow = new tokens - rejected rows does both, and the append writes over the latter; where another slot was made a copy of
+ * the slot since they were written, they are given back by a call before the one that grows.
+ * Rows are copied within `layers` pools that share the table (layer l at pages + l layer_bytes; row_bytes a row),
+ * and likewise within scales (NULL: none).
  * workspace: smla_update_pages_workspace(S, M, n_pages) bytes, 4-byte aligned; none (0, NULL is taken) where one
  * launch does all. */
 size_t smla_update_pages_workspace(int64_t S, int64_t M, int64_t n_pages);

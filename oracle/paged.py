@@ -89,13 +89,14 @@ def update_pages(pages, table, lens, refs, parent, grow):
     asked = 0
     for s in range(S):
         p, g = parent[s], grow[s]
-        if not -1 <= p < S or g < 0:
+        if not -1 <= p < S:
             continue
         have = lens[p] if p >= 0 else 0
-        if have < 0 or have + g >= 1 << 31 or -(-(have + g) // P) > M:
+        if have < 0 or not 0 <= have + g < 1 << 31 or -(-(have + g) // P) > M:
             continue
         pages_now = -(-(have + g) // P)
-        kept = -(-have // P) if p == s else have // P
+        rows_kept = min(have, have + g)     # a negative growth gives rows back
+        kept = -(-rows_kept // P) if p == s else rows_kept // P
         at = asked
         asked += pages_now - kept
         if asked > len(free):
@@ -104,8 +105,8 @@ def update_pages(pages, table, lens, refs, parent, grow):
         fresh = free[at:asked]
         new_t[s] = (list(table[p][:kept]) if p >= 0 else []) + fresh
         new_t[s] += [-1] * (M - len(new_t[s]))
-        if p not in (s, -1) and have % P and 0 <= table[p][kept] < n_pages:
-            copies.append((table[p][kept], fresh[0], have % P))
+        if p not in (s, -1) and rows_kept % P and 0 <= table[p][kept] < n_pages:
+            copies.append((table[p][kept], fresh[0], rows_kept % P))
     new_r = list(refs)
     for s in range(S):
         if granted[s]:

@@ -207,3 +207,107 @@ def test_append_keeps_what_is_not_finite(dev, bad, xdt, kv, kv_norm):
         rel[:coded] = 2.0 ** -4
         # (blocks of ordinary values: the largest is at most 2^3, so a subnormal half step is under 2^-10 * 2^-5)
         assert ((val - want).abs() <= rel * want.abs() + 2.0 ** -14)[ok].all(), t
+
+
+def _held(table, lens, refs, P):
+    """The state is sound: every entry of a slot's rows names a page, no other entry does, refs counts them."""
+    count = [0] * len(refs)
+    for row, n in zip(table, lens):
+        used = -(-n // P)
+        assert all(p >= 0 for p in row[:used]) and all(p == -1 for p in row[used:])
+        for p in row[:used]:
+            count[p] += 1
+    assert count == refs
+
+
+@pytest.mark.parametrize("S,M,P,n_pages,D,kv", [(5, 8, 4, 30, 64, "bf16"), (64, 12, 16, 400, 64, "fp8"), (1030, 5, 4, 5000, 64, "bf16"),
+                                                (9, 4000, 2, 20000, 64, "bf16")])
+def test_rows_given_back(dev, S, M, P, n_pages, D, kv):
+    """Growth of either sign over forked slots: pages past the shorter lengths are free again, whichever path the pool takes."""
+    from smla import paged
+    r = random.Random(S)
+    table, lens, refs = [[-1] * M for _ in range(S)], [0] * S, [0] * n_pages
+    g = torch.Generator().manual_seed(S)
+    pool = torch.randint(0, 256, (n_pages, P, D * (1 if kv == "fp8" else 2)), generator=g, dtype=torch.uint8)
+    pool = pool if kv == "fp8" else pool.view(torch.bfloat16)
+    sc = torch.randn(n_pages, P, D // 64, generator=g) if kv == "fp8" else None
+    dp, ds = _to(dev, pool, sc)
+    for k in range(8):
+        announce(f"update_pages with rows given back, S={S} M={M} P={P} n_pages={n_pages} {kv} step {k}")
+        parent = [r.choice([s, s, s, r.randrange(S), -1]) for s in range(S)]
+        have = [lens[p] if p >= 0 else 0 for p in parent]
+        most = max(1, min(M * P, n_pages * P // S) // 2)
+        grow = [r.choice([0, 1, r.randint(0, most), -1, -r.randint(0, h), -h, -h - 1 if r.random() < 0.1 else 0, -r.randint(0, 2 * P)])
+                for h in have]
+        t2, l2, r2, ok, copies = op.update_pages((P, n_pages), table, lens, refs, parent, grow)
+        got = paged.update_pages(dp, *[_i32(v, dev) for v in (table, lens, refs, parent, grow)], page_scales=ds)
+        torch.cuda.synchronize()
+        assert [x.tolist() for x in got] == [t2, l2, r2, ok], k
+        pool, sc = _apply(pool, copies, P), _apply(sc, copies, P)
+        assert torch.equal(dp.cpu().view(torch.uint8), pool.view(torch.uint8)) and (sc is None or torch.equal(ds.cpu(), sc))
+        table, lens, refs = t2, l2, r2
+        _held(table, lens, refs, P)
+    paged_empty = paged.update_pages(dp, *[_i32(v, dev) for v in (table, lens, refs, list(range(S)), [-n for n in lens])], page_scales=ds)
+    assert not paged_empty[1].any() and not paged_empty[2].any() and (paged_empty[0] == -1).all() and paged_empty[3].all()
+
+
+@pytest.mark.parametrize("capture", [False, True])
+def test_drafts_rolled_back(dev, capture):
+    """Steps of four draft tokens of which some are rejected, past page ends: the pool never loses a page, and the attention is
+    that over the accepted rows."""
+    from smla import paged
+    announce(f"drafts rolled back, {'captured' if capture else 'eager'}")
+    S, M, P, n_pages, H, D, n = 3, 8, 4, 18, 16, 512, 4
+    r, g = random.Random(5), torch.Generator().manual_seed(5)
+    cos, sin = _to(dev, *_tables(dev, M * P, 64))
+    pages = torch.full((n_pages, P, D), float("nan"), dtype=torch.bfloat16, device=dev)
+    state = [torch.full((S, M), -1, dtype=torch.int32, device=dev), _i32([0] * S, dev), _i32([0] * n_pages, dev)]
+    parent, grow, cu = _i32(list(range(S)), dev), _i32([n] * S, dev), _i32(_cu([n] * S), dev)
+    q, x = torch.zeros(S * n, H, D, device=dev), torch.zeros(S * n, D, device=dev)
+    res = {}
+
+    def step():
+        t, l, f, ok = paged.update_pages(pages, *state, parent, grow)
+        qs = paged.paged_append(q, x, pages, t, l, cu, cos, sin, kv_norm=True, q_norm=True, granted=ok)
+        o = paged.paged_attn(qs, pages, t, l, cu, D ** -0.5, granted=ok)
+        for a, b in zip(state, (t, l, f)):
+            a.copy_(b)
+        res.update(q=qs, o=o, ok=ok)
+
+    if capture:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        for a, v in zip(state, (-1, 0, 0)):
+            a.fill_(v)
+    lens, granted = [0] * S, 0
+    for k in range(20):
+        rejected = [r.randint(0, min(n, m)) if k else 0 for m in lens]
+        base = [m - b for m, b in zip(lens, rejected)]
+        parent.copy_(_i32([s if m + n <= M * P else -1 for s, m in enumerate(base)], dev))
+        give = [n - b if p >= 0 else n for b, p in zip(rejected, parent.tolist())]
+        base = [m if p >= 0 else 0 for m, p in zip(base, parent.tolist())]
+        grow.copy_(_i32(give, dev))
+        q.copy_(torch.randn(S * n, H, D, generator=g))
+        x.copy_(torch.randn(S * n, D, generator=g))
+        t_want, l_want, r_want, ok, _ = op.update_pages((P, n_pages), *[t.tolist() for t in state], parent.tolist(), give)
+        base = [m if a else n for m, a, n in zip(base, ok, lens)]      # (the pool may run out: such a slot stays as it was)
+        old = [pages[state[0][s].clamp(min=0).long()].reshape(-1, D)[:base[s]].clone() for s in range(S)]
+        graph.replay() if capture else step()
+        torch.cuda.synchronize()
+        lens = [m + n if a else m for m, a in zip(base, ok)]
+        granted += sum(ok)
+        assert res["ok"].tolist() == ok and [t.tolist() for t in state] == [t_want, lens, r_want] and l_want == lens
+        _held(t_want, lens, r_want, P)
+        for s in range(S):
+            now = pages[state[0][s].clamp(min=0).long()].reshape(-1, D)
+            assert torch.equal(now[:base[s]], old[s])
+        seen = [m if a else -1 for m, a in zip(lens, ok)]
+        _check_attn(res["o"], res["q"].cpu(), pages.cpu(), None, state[0].cpu(), seen, _cu([n] * S), None, 0, 0)
+    assert 20 < granted < 20 * S      # both happened

@@ -102,3 +102,31 @@ def test_updates_keep_the_tables_sound():
             assert all(x > 0 for x in refs[:live]) and not any(refs[live:])
             _check_state(table, lens, refs, P)
     assert seen == {0, 1}
+
+
+def test_rows_given_back_free_their_pages():
+    """Growth of either sign: a draft's pages past the accepted rows are free again, and refs counts what the tables name."""
+    r = random.Random(4)
+    P, S, M, n_pages = 4, 6, 8, 30
+    table, lens, refs = [[-1] * M for _ in range(S)], [0] * S, [0] * n_pages
+    shorter = 0
+    for _ in range(400):
+        parent = [r.choice([s, s, s, r.randrange(S), -1]) for s in range(S)]
+        grow = [r.choice([0, 1, 5, -1, -5, -40, r.randrange(12)]) for _ in range(S)]
+        before = lens
+        table, lens, refs, granted, copies = op.update_pages((P, n_pages), table, lens, refs, parent, grow)
+        for s, p in enumerate(parent):
+            have = before[p] if p >= 0 else 0
+            assert lens[s] == (have + grow[s] if granted[s] else before[s])
+            shorter += granted[s] and grow[s] < 0 and p == s and -(-lens[s] // P) < -(-before[s] // P)
+        count = [0] * n_pages
+        for row, n in zip(table, lens):
+            used = -(-n // P)
+            assert all(p >= 0 for p in row[:used]) and all(p == -1 for p in row[used:])
+            for p in row[:used]:
+                count[p] += 1
+        assert count == refs
+        assert all(refs[b] == 1 and 0 < k < P for _, b, k in copies)
+    assert shorter > 20
+    t, n, f, ok, _ = op.update_pages((P, n_pages), table, lens, refs, list(range(S)), [-x for x in lens])
+    assert not any(n) and not any(f) and all(ok)
