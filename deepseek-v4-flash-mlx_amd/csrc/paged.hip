@@ -361,8 +361,16 @@ __device__ inline bool slot_need(const PageArgs& a, int s, SlotNeed& n) {
   const uint32_t P = (uint32_t)a.P;
   const int64_t pages = (next + P - 1) / P;
   n.pages = (int)pages;
-  n.full = p == s ? (int)(((int64_t)n.rows + P - 1) / P) : (int)((uint32_t)n.rows / P);
-  return pages <= a.M;
+  const uint32_t whole = (uint32_t)n.rows / P;
+  n.full = (int)whole;
+  if (pages > a.M) return false;
+  if (p == s && (uint32_t)n.rows % P) {
+    // its own partly filled page stays, unless rows change in one that others hold too (a slot that gave rows back past a
+    // fork): that is copied like another slot's
+    const int page = g != 0 ? a.table[s * a.ld_table + whole] : -1;
+    if (page < 0 || page >= a.n_pages || a.refs[page] <= 1) n.full++;
+  }
+  return true;
 }
 __device__ inline int tail_rows(const PageArgs& a, const SlotNeed& n) {
   return (int)max((int64_t)n.rows - (int64_t)n.full * a.P, (int64_t)0);

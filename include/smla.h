@@ -593,7 +593,8 @@ int smla_paged_append_granted(const void* q, int64_t ldq, const void* kv, int64_
  * parent[s] as it was before the call (s: itself, -1: an empty slot) with grow[s] more rows, or -grow[s] fewer
  * (the last rows, those of rejected drafts, are given back and not copied):
  *   - its parent's whole pages are shared; of a partly filled last page the rows in use are copied to a
- *     fresh page, unless the slot keeps its own (parent[s] == s);
+ *     fresh page, unless the slot keeps its own (parent[s] == s; where grow[s] is not 0 also its own is copied if
+ *     refs is above 1 there: a slot that gave back rows of a page shared since);
  *   - fresh pages are the free ones (refs 0) in ascending order, taken by the slots in order;
  *   - granted[s] = 1 if parent[s] is valid, the parent's rows and grow[s] make 0 rows or more, they fit M pages and
  *     the pages that slots 0 .. s ask for are at most the free ones; else 0, and the slot stays as it was (its new

@@ -96,7 +96,10 @@ def update_pages(pages, table, lens, refs, parent, grow):
             continue
         pages_now = -(-(have + g) // P)
         rows_kept = min(have, have + g)     # a negative growth gives rows back
-        kept = -(-rows_kept // P) if p == s else rows_kept // P
+        kept = rows_kept // P
+        tail = table[p][kept] if p >= 0 and rows_kept % P else -1
+        if p == s and rows_kept % P and (g == 0 or not 0 <= tail < n_pages or refs[tail] <= 1):
+            kept, tail = kept + 1, -1   # keeps its own partly filled page, which no other slot holds
         at = asked
         asked += pages_now - kept
         if asked > len(free):
@@ -105,8 +108,8 @@ def update_pages(pages, table, lens, refs, parent, grow):
         fresh = free[at:asked]
         new_t[s] = (list(table[p][:kept]) if p >= 0 else []) + fresh
         new_t[s] += [-1] * (M - len(new_t[s]))
-        if p not in (s, -1) and rows_kept % P and 0 <= table[p][kept] < n_pages:
-            copies.append((table[p][kept], fresh[0], rows_kept % P))
+        if 0 <= tail < n_pages:
+            copies.append((tail, fresh[0], rows_kept % P))
     new_r = list(refs)
     for s in range(S):
         if granted[s]:

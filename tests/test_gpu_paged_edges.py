@@ -311,3 +311,52 @@ def test_drafts_rolled_back(dev, capture):
         seen = [m if a else -1 for m, a in zip(lens, ok)]
         _check_attn(res["o"], res["q"].cpu(), pages.cpu(), None, state[0].cpu(), seen, _cu([n] * S), None, 0, 0)
     assert 20 < granted < 20 * S      # both happened
+
+
+@pytest.mark.parametrize("n_pages", [20, 20000])
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("net", [False, True])
+def test_rows_given_back_past_a_fork(dev, n_pages, kv, net):
+    """A slot that gives back rows of a page another slot holds, and appends: the other slot's rows keep their bits."""
+    from smla import paged
+    announce(f"rows given back past a fork, {n_pages} pages, {kv}, {'one call' if net else 'two calls'}")
+    S, M, P, D = 3, 4, 8, 512
+    cos, sin = _to(dev, *_tables(dev, M * P, 64))
+    g = torch.Generator().manual_seed(3)
+    pages = torch.zeros(n_pages, P, D, dtype=torch.uint8 if kv == "fp8" else torch.bfloat16, device=dev)
+    scales = torch.zeros(n_pages, P, D // 64, device=dev) if kv == "fp8" else None
+    state = torch.full((S, M), -1, dtype=torch.int32, device=dev), _i32([0] * S, dev), _i32([0] * n_pages, dev)
+
+    def step(state, parent, grow, new):
+        *state, ok = paged.update_pages(pages, *state, _i32(parent, dev), _i32(grow, dev), page_scales=scales)
+        assert ok.tolist() == [1] * S
+        if sum(new):
+            x = torch.randn(sum(new), D, generator=g).to(dev)
+            paged.paged_append(None, x, pages, state[0], state[1], _i32(_cu(new), dev), cos, sin, kv_norm=True, page_scales=scales,
+                               granted=ok)
+        torch.cuda.synchronize()
+        return state
+
+    def rows(state, s, n):
+        at = state[0][s].clamp(min=0).long()
+        return [t[at].flatten(0, 1)[:n].clone() for t in (pages, scales) if t is not None]
+
+    same = lambda a, b: all(torch.equal(x, y) for x, y in zip(a, b))  # noqa: E731
+    state = step(state, [-1, -1, -1], [16, 0, 3], [16, 0, 3])
+    state = step(state, [0, 0, 2], [0, 0, 0], [0, 0, 0])
+    first, other, r0 = rows(state, 0, 16), rows(state, 2, 3), rows(state, 1, 12)
+    assert state[0][0].tolist() == state[0][1].tolist() and state[2][:4].tolist() == [2, 2, 1, 0]
+    if net:     # four rows back, one new
+        state = step(state, [0, 1, 2], [0, -3, 0], [0, 1, 0])
+    else:
+        state = step(state, [0, 1, 2], [0, -4, 0], [0, 0, 0])
+        state = step(state, [0, 1, 2], [0, 1, 0], [0, 1, 0])
+    assert state[1].tolist() == [16, 13, 3]
+    assert same(rows(state, 0, 16), first) and same(rows(state, 1, 12), r0) and same(rows(state, 2, 3), other)
+    assert not same(rows(state, 1, 13), [t[:13] for t in first])
+    assert int(state[0][0, 0]) == int(state[0][1, 0]) and int(state[0][0, 1]) != int(state[0][1, 1])
+    _held(state[0].tolist(), state[1].tolist(), state[2].tolist(), P)
+    # the page is its own now: it grows in place
+    page = state[0][1].tolist()
+    state = step(state, [0, 1, 2], [0, 2, 0], [0, 2, 0])
+    assert state[0][1].tolist() == page and same(rows(state, 0, 16), first)

@@ -130,3 +130,31 @@ def test_rows_given_back_free_their_pages():
     assert shorter > 20
     t, n, f, ok, _ = op.update_pages((P, n_pages), table, lens, refs, list(range(S)), [-x for x in lens])
     assert not any(n) and not any(f) and all(ok)
+
+
+def test_rows_given_back_past_a_fork_stay_the_other_slots():
+    """Random forks, growth and rows given back: each slot's rows are its own however its pages are shared."""
+    r = random.Random(5)
+    P, S, M, n_pages = 4, 6, 8, 40
+    table, lens, refs = [[-1] * M for _ in range(S)], [0] * S, [0] * n_pages
+    data, want, own = [[None] * P for _ in range(n_pages)], [[] for _ in range(S)], 0
+    for step in range(600):
+        parent = [r.choice([s, s, s, r.randrange(S), -1 if r.random() < 0.3 else s]) for s in range(S)]
+        grow = [r.choice([0, 1, 1, -1, -2, r.randrange(9), -r.randrange(9)]) for _ in range(S)]
+        before = [list(w) for w in want]
+        table, lens, refs, granted, copies = op.update_pages((P, n_pages), table, lens, refs, parent, grow)
+        moved = [(b, k, list(data[a])) for a, b, k in copies]
+        for b, k, was in moved:
+            data[b][:k] = was[:k]
+        for s in range(S):
+            if granted[s]:
+                have = before[parent[s]] if parent[s] >= 0 else []
+                want[s] = list(have[:min(len(have), len(have) + grow[s])])
+                for j in range(len(want[s]), lens[s]):
+                    want[s].append((step, s, j))
+                    data[table[s][j // P]][j % P] = (step, s, j)
+        own += sum(granted[s] and parent[s] == s and any(table[s][len(want[s]) // P] == b for _, b, _ in copies)
+                   for s in range(S) if len(want[s]) < M * P)
+        for s in range(S):
+            assert [data[table[s][j // P]][j % P] for j in range(lens[s])] == want[s], (step, s)
+    assert own > 5
