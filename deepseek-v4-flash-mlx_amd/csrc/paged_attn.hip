@@ -36,8 +36,9 @@
 // ahead, so a row list of any length costs one table read per row.
 //
 // Rows masked for some of a tile's q rows may hold anything (rows not yet written, pages of id -1 read as
-// row 0): their probability is 0, and where a masked score is not finite the value waves take the tile's
-// values with their infinities and NaN as 0 (a row that sees such a value has a NaN sum already).
+// row 0): their probability is 0, and where a score of the tile is not finite the value waves take its
+// values with their infinities and NaN as 0.  So a row seen with a score of -inf counts for nothing, whatever else
+// is in its tile; one seen with +inf or NaN makes its q row's sum NaN.
 #include "attn_common.h"
 
 namespace smla_attn {
@@ -502,7 +503,7 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
       if (e < w.e_end) page = trow[col];
     }
   };
-  // scores of a tile of which some q row does not see some row: scaled, -inf there; whether a masked one is not finite
+  // scores of a tile of which some q row does not see some row: scaled, -inf there; whether one, seen or not, is not finite
   // (0 x it is not 0).  The rows that the q row sees as bits: those whose row number is there (a ballot), below eh, and
   // from `past` on or below first; then per score a bit spread to a word, and bitwise selects.
   auto mask = [&](f32x16_t& s, int i) -> bool {
@@ -514,7 +515,7 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
 #pragma unroll
     for (int k = 0; k < 16; k++) {
       const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)mine, 8 * (k >> 2) + (k & 3), 1);
-      z = __builtin_fmaf(__uint_as_float(__float_as_uint(s[k]) & ~m), 0.f, z);
+      z = __builtin_fmaf(s[k], 0.f, z);
       s[k] = __uint_as_float((__float_as_uint(s[k] * c2) & m) | (__float_as_uint(-SMLA_INF) & ~m));
     }
     return !(z == 0.f);
@@ -554,7 +555,9 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
     const float cm = open ? c2 : 1.f;  // what turns tile i - 1's scores to base 2 (1: masked, and scaled, already)
     float alpha = 1.f;                 // e^(old - new reference)
     bool odd = false;
-    if (!open) odd = mask(old, i - 1);
+    const bool masked = !open;
+    if (masked) odd = mask(old, i - 1);
+    float least = 0.f;  // of the scores; -inf where a seen row counts for nothing (masked: known already)
     auto look = [&]() {  // the reference moves to the tile's maximum where that is past it
       float x = fmaxf(old[0], old[1]);
 #pragma unroll
@@ -570,7 +573,10 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
         }
       }
     };
-    auto expo = [&](int k) { old[k] = __builtin_amdgcn_exp2f(old[k] * cm - m_ref); };
+    auto expo = [&](int k) {
+      if ((k & 1) == 0) least = fminf(fminf(least, old[k]), old[k + 1]);
+      old[k] = __builtin_amdgcn_exp2f(old[k] * cm - m_ref);
+    };
     auto put = [&](int q) {
       l_lane += (old[4 * q] + old[4 * q + 1]) + (old[4 * q + 2] + old[4 * q + 3]);
       *(lds_u32x2_t*)(lds + G::P_OFF + ((i - 1) & 1) * G::PBUF + p_at(r, q) + 8 * h) =
@@ -578,7 +584,7 @@ __device__ inline void score_role(const PagedArgs& a, const Work& w, const int32
     };
     auto put_alpha = [&]() {
       al_s[((i - 1) & 1) * G::TILEQ + r] = alpha;
-      const uint64_t any = __builtin_amdgcn_ballot_w64(odd);
+      const uint64_t any = __builtin_amdgcn_ballot_w64(odd | (!masked & (least == -SMLA_INF)));
       if (lane == 0) *(lds_i32_t*)(lds + G::FLAG_OFF + 16 * ((i - 1) & 1) + 4 * wave) = any != 0;
     };
     if (more) {

@@ -548,7 +548,7 @@ enum { SMLA_PAGED_NORM_Q = 1, SMLA_PAGED_NORM_KV = 2, SMLA_PAGED_FILL = 4 };
  * Token at position p attends rows j <= p; with window > 0 those with j > p - window or j < first (a
  * sliding window and the first rows).  scale multiplies q.row; the sink adds exp(sink) to the
  * denominator.  A token that sees no row gives 0.  Rows a token does not see may hold anything,
- * infinities and NaN too; a row it sees that scores NaN or +inf gives NaN.
+ * infinities and NaN too; a row it sees that scores NaN or +inf gives NaN, one that scores -inf counts for nothing.
  * flags: 0 or SMLA_PAGED_FILL.  q, pages, out and workspace 16-byte aligned; out apart from q.  Sums and softmax
  * statistics are fp32; probabilities are rounded to bf16 before their products, the partial sums of tokens whose rows are
  * split over workgroups to fp16 times a power of two (taken so that the largest of 64 is below 2) before they are joined.  The result does not depend on the order in which

@@ -360,3 +360,32 @@ def test_rows_given_back_past_a_fork(dev, n_pages, kv, net):
     page = state[0][1].tolist()
     state = step(state, [0, 1, 2], [0, 2, 0], [0, 2, 0])
     assert state[0][1].tolist() == page and same(rows(state, 0, 16), first)
+
+
+@pytest.mark.parametrize("length,n,D", [(45, 1, 512), (45, 4, 512), (128, 1, 576), (128, 9, 576), (1500, 1, 576), (1500, 5, 512)])
+def test_attn_minus_infinity_counts_for_nothing(dev, length, n, D):
+    """A row seen with a score of -inf has no share, whichever tokens are in the tile beside the one that sees it; where the
+    same row scores +inf the token is NaN."""
+    from smla import paged
+    announce(f"paged_attn a row of +inf, {n} tokens at {length}, D={D}")
+    pages, _, table = _cache(206, [length], 16, D)
+    row = min(43, length - 2)
+    pages[table[0, row // 16], row % 16, 5] = float("inf")
+    q = torch.randn(n, 64, D, generator=torch.Generator().manual_seed(6)).to(torch.bfloat16)
+    dq, dp, dt = _to(dev, q, pages, table)
+    lens = _i32([length], dev)
+    out = paged.paged_attn(dq, dp, dt, lens, _i32([0, n], dev), D ** -0.5)
+    kv, _ = op.rows(pages, None, table[0], length)
+    kv[row] = 0.0
+    for t in range(n):
+        end = length - n + t + 1
+        alone = paged.paged_attn(dq[t:t + 1], dp, dt, _i32([end], dev), _i32([0, 1], dev), D ** -0.5)[0].double().cpu()
+        up = (q[t, :, 5] > 0) & (row < end)     # (an earlier token does not see it)
+        assert alone[up].isnan().all() and out[t].cpu()[up].isnan().all()
+        s = q[t].double() @ kv[:end].T * D ** -0.5
+        if row < end:
+            s[:, row] = float("-inf")
+        want = torch.softmax(s, dim=-1) @ kv[:end, :512]
+        for x in (alone, out[t].double().cpu()):
+            err = (x - want).norm(dim=-1)[~up]
+            assert (err <= 3 * BF16 * want.norm(dim=-1)[~up]).all(), (t, err)
