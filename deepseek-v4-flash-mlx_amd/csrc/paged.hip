@@ -869,6 +869,14 @@ extern "C" int smla_paged_append_granted(const void* q, int64_t ldq, const void*
       T * (H + 1) > 0x7fffffff)
     return SMLA_E_RANGE;
   if (T == 0) return SMLA_OK;
+  // rows of q and kv are read while others of q_out are written; a row is read whole before it is written, so q itself
+  // (dense, bf16) may be q_out
+  const uintptr_t es = x_dtype == SMLA_F32 ? 4 : 2, o0 = (uintptr_t)q_out, o1 = o0 + (uintptr_t)T * H * D * 2;
+  auto over = [&](const void* p, int64_t ld, int64_t w) {
+    return o0 < (uintptr_t)p + ((uintptr_t)(T - 1) * ld + w) * es && (uintptr_t)p < o1;
+  };
+  const bool same = q == q_out && x_dtype == SMLA_BF16 && (T == 1 || ldq == H * D);
+  if (H > 0 && ((!same && over(q, ldq, H * D)) || over(kv, ldkv, D))) return SMLA_E_UNSUPPORTED;
   AppendArgs a{};
   a.q = q;
   a.kv = kv;

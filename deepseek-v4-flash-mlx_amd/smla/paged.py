@@ -47,7 +47,7 @@ def paged_append(q, kv, pages, table, lens, cu, cos_t, sin_t, kv_norm=None, q_no
     The rows go to their pages: bf16 (``fp8_sim``: the channels before the rotated ones fp8
     round-tripped first) or, with fp8 pages, e4m3 codes and ``page_scales``.  Returns the queries [T, H, D] bf16
     (``q_out`` when given: tokens of no sequence or at positions past the rotation tables are left as
-    they were; else 0 there), None without q.  ``granted`` [B] int32 (``update_pages``): the tokens of a sequence
+    they were; else 0 there; apart from q and kv, or q itself where that is dense bf16), None without q.  ``granted`` [B] int32 (``update_pages``): the tokens of a sequence
     where it is 0 are tokens of no sequence; without it they are written over the refused slot's last rows."""
     fill = q is not None and q_out is None
     if fill:

@@ -576,7 +576,8 @@ int smla_paged_attn_granted(const void* q, int q_dtype, const void* pages, int p
  * scales, quantised as smla_quant_fp8_pow2 does; a 64-channel block with a value that is not finite is NaN in all of it.  A token at a position outside [0, n_pos) (rd > 0) writes
  * nothing (SMLA_PAGED_FILL: zero queries); a row past the table's columns or whose entry is no
  * page is not stored.  D a multiple of 64 up to 1024, rd and norm_dims multiples of 4, ldq and ldkv too; rd a
- * multiple of 64 with SMLA_SIM_FP8; q and kv aligned to four of their elements, q_out and pages to 8 bytes. */
+ * multiple of 64 with SMLA_SIM_FP8; q and kv aligned to four of their elements, q_out and pages to 8 bytes.  q_out is
+ * apart from q and kv, or q itself (BF16, ldq = H * D). */
 int smla_paged_append(const void* q, int64_t ldq, const void* kv, int64_t ldkv, int x_dtype, int64_t T, int64_t H,
                       int64_t D, int64_t norm_dims, const float* q_w, const float* kv_w, const float* cos_t,
                       const float* sin_t, int64_t n_pos, int64_t rd, float eps, int sim, int flags, void* q_out,

@@ -389,3 +389,23 @@ def test_attn_minus_infinity_counts_for_nothing(dev, length, n, D):
         for x in (alone, out[t].double().cpu()):
             err = (x - want).norm(dim=-1)[~up]
             assert (err <= 3 * BF16 * want.norm(dim=-1)[~up]).all(), (t, err)
+
+
+def test_append_in_place(dev):
+    """Dense bf16 queries may be their own output; a q_out over other parts of the inputs is refused."""
+    from smla import _lib, paged
+    announce("paged_append with q_out = q")
+    T, H, D = 37, 5, 512
+    g = torch.Generator().manual_seed(7)
+    q = torch.randn(T, H, D, generator=g).to(torch.bfloat16).to(dev)
+    kv = torch.randn(T, D, generator=g).to(torch.bfloat16).to(dev)
+    cos, sin = _to(dev, *_tables(dev, 64, 64))
+    table, lens, cu = _i32([[0, 1, 2, 3, 4]], dev), _i32([T], dev), _i32([0, T], dev)
+    call = lambda q, out: paged.paged_append(q, kv, pages, table, lens, cu, cos, sin, q_norm=True, q_out=out)  # noqa: E731
+    pages = torch.zeros(5, 8, D, dtype=torch.bfloat16, device=dev)
+    want = call(q, None)
+    mine = q.clone()
+    assert call(mine, mine) is mine and torch.equal(mine, want)
+    flat = torch.zeros((T + 1) * H * D, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(_lib.SmlaError):
+        call(flat[:T * H * D].view(T, H, D), flat[H * D:].view(T, H, D))

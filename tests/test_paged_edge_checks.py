@@ -1,8 +1,10 @@
 """CPU tier: refusals and traces of the paged cache's calls beside those of ``test_paged_checks``."""
+import ctypes
+
 import pytest
 import torch
 
-from test_paged_checks import APPEND, APPEND_OK, ATTN, ATTN_OK, FAKE, NULL, OK, RANGE, SHAPE, UNSUP, _call
+from test_paged_checks import APPEND, APPEND_OK, ATTN, ATTN_OK, BF16, F32, FAKE, NULL, OK, RANGE, SHAPE, UNSUP, _call
 
 
 def _with_granted(names, defaults):
@@ -48,3 +50,20 @@ def test_calls_with_granted_trace_as_their_ops():
     program = torch.export.export(Call(), a, strict=False)
     called = [str(n.target) for n in program.graph.nodes if n.op == "call_function"]
     assert "smla.paged_append_.default" in called and "smla.paged_attn_.default" in called
+
+
+def _at(n):
+    return ctypes.c_void_p(1 << 20 | n)
+
+
+# a bf16 q of 2 tokens of 16 heads of 512 at 0 (32768 bytes), kv behind it with 512 spare elements a row (2048 + 1024 bytes)
+OVER = dict(T=2, x_dtype=BF16, q=_at(0), ldq=16 * 512, kv=_at(32768), ldkv=1024, B=1)
+
+
+@pytest.mark.parametrize("change", [
+    dict(q_out=_at(8)), dict(q_out=_at(32768 - 8)), dict(q_out=_at(32768)), dict(q_out=_at(32768 + 3072 - 8)),
+    dict(x_dtype=F32, q_out=_at(0), kv=_at(1 << 19)),                           # fp32 q: written rows lie over others
+    dict(q=_at(0), ldq=16 * 512 + 4, q_out=_at(0), kv=_at(1 << 19)),            # rows apart
+])
+def test_paged_append_refuses_queries_over_its_inputs(change):
+    assert _call("smla_paged_append", APPEND, APPEND_OK | OVER, **change) == UNSUP
