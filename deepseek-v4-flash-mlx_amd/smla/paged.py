@@ -3,7 +3,8 @@
 The reference keeps one contiguous buffer a sequence and clones it whole
 (``oracle/v4_fast.py:93-96,150-159``); a server that batches sequences keeps their rows in pages
 instead.  Row j of sequence b is row j % P of page ``table[b, j // P]`` of ``pages`` [n_pages, P, D]
-(bf16, or e4m3 codes with ``page_scales`` [n_pages, P, D/64]).  A step is
+(bf16, or e4m3 codes with ``page_scales`` [n_pages, P, D/64], whose products with the codes the attention takes as bf16:
+exactly where they are powers of two, as the append makes them).  A step is
 
 * ``update_pages``   slots forked, freed and grown (new ``table``, ``lens``, ``refs``);
 * ``paged_append``   the new tokens' queries normed and rotated, their rows written to the pages;

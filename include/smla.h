@@ -526,7 +526,8 @@ int smla_o_proj_ws(const void* o, int o_dtype, const int32_t* pos, const float* 
 
 /* ---------------------------------------------------------------------------------------------
  * Paged latent cache.  A pool is n_pages pages of P rows of D channels (pages [n_pages, P, D]: BF16, or
- * FP8_E4M3 codes with page_scales [n_pages, P, D/64] fp32, row value = decode(code) * scale).  Row j of
+ * FP8_E4M3 codes with page_scales [n_pages, P, D/64] fp32, row value = decode(code) * scale; smla_paged_attn rounds it
+ * to bf16 for its products, which is exact for the powers of two that smla_paged_append writes).  Row j of
  * sequence b is row j % P of page table[b, j / P] (table: B rows of cols entries, ld_table elements apart).
  * All integers are int32 on the device and none is read by the host, so a captured call follows
  * them.  A page id outside [0, n_pages) is no page: such rows are not read, written or counted.

@@ -409,3 +409,27 @@ def test_append_in_place(dev):
     flat = torch.zeros((T + 1) * H * D, dtype=torch.bfloat16, device=dev)
     with pytest.raises(_lib.SmlaError):
         call(flat[:T * H * D].view(T, H, D), flat[H * D:].view(T, H, D))
+
+
+@pytest.mark.parametrize("H,n", [(16, [1, 4, 3]), (64, [1, 40, 2])])
+def test_attn_scales_of_any_value(dev, H, n):
+    """e4m3 rows with scales that are no powers of two, beside such that are, negative and 0: rows are decode(code) * scale
+    rounded to bf16, over which the oracle computes."""
+    from smla import paged
+    announce(f"paged_attn e4m3 rows of any scale, {H} heads")
+    lens, D = [70, 333, 64], 576
+    pages, scales, table = _cache(208, lens, 16, D, "fp8")
+    g = torch.Generator().manual_seed(H)
+    pick = torch.randint(0, 5, scales.shape, generator=g)
+    scales = torch.where(pick == 0, scales, scales * (0.5 + torch.rand(scales.shape, generator=g)))
+    scales[pick == 2] *= -1.0
+    scales[(pick == 3) & (torch.rand(scales.shape, generator=g) < 0.1)] = 0.0
+    rows = (pages.float() * scales.repeat_interleave(64, dim=-1)).to(torch.bfloat16)
+    cu = _cu(n)
+    q = torch.randn(cu[-1], H, D, generator=g).to(torch.bfloat16)
+    dq, dp, ds, dt = _to(dev, q, pages, scales, table)
+    out = paged.paged_attn(dq, dp, dt, _i32(lens, dev), _i32(cu, dev), D ** -0.5, page_scales=ds)
+    torch.cuda.synchronize()
+    _check_attn(out, q, rows, None, table, lens, cu, None, 0, 0)
+    only = paged.paged_attn(dq, rows.to(dev), dt, _i32(lens, dev), _i32(cu, dev), D ** -0.5)
+    assert torch.equal(out, only)
