@@ -102,13 +102,4 @@ __device__ inline void dma16_nt(const void* gsrc, uint32_t lds_dst_uniform) {
                : "memory", "m0");
 }
 
-// 16-byte vector load that the compiler does not track (covered by a later wait_vm)
-__device__ inline u32x4_t load16_untracked(const void* p) {
-  u32x4_t r;
-  asm volatile("global_load_dwordx4 %0, %1, off" : "=v"(r) : "v"(p) : "memory");
-  return r;
-}
-
-
-
 }  // namespace smla_attn
