@@ -968,12 +968,10 @@ def _one_device(t, *rest):
 def _launch(dev, name, *args):
     """``_lib.call`` with GPU dev current (a launch goes to a stream of the current device)."""
     if _current_device() == dev:
-        status = getattr(_lib._LIB or _lib.lib(), name)(*args, _raw_stream(dev))
+        _lib.call(name, *args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            status = getattr(_lib.lib(), name)(*args, _raw_stream(dev))
-    if status != 0:
-        _lib.check(name, status)
+            _lib.call(name, *args, _raw_stream(dev))
 
 
 def _f32(t):
