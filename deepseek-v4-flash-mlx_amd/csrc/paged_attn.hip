@@ -16,7 +16,9 @@
 // A workgroup is 8 waves of up to 256 registers, two per SIMD, and walks its entries in tiles of 32 rows, two
 // roles with one barrier a tile between:
 //   * score waves 0 .. NB-1: S^T = K Q^T of 32 q rows (v_mfma_f32_32x32x16_bf16, rows as M; the 32 q rows' Q^T
-//     stays in 144 registers), online softmax with a lazy maximum, P in bf16 and the rescale factor to LDS;
+//     stays in 144 registers), online softmax with a lazy maximum, P in bf16 and the rescale factor to LDS (the products
+//     take rows and probabilities of one type, and the rows are bf16: against 64 bits a result is off by 1.7e-3 to 2.2e-3
+//     of its 2-norm, 1.7e-3 of that its own rounding);
 //   * value waves 3 .. 7: O^T += V^T P^T (v_mfma_f32_32x32x16_bf16) of 3 or 4 blocks of 32 value columns and all
 //     the tile's q rows, so each V^T fragment (ds_read_b64_tr_b16) is read by one wave and serves NB products.
 //     Wave 3 shares its SIMD with value wave 7 instead of a score wave and takes four blocks, the others three.
@@ -274,7 +276,7 @@ struct Work {
   int m0, p0, p_lo, p_hi;  // the first one's number in its sequence; positions of the sequence's first token, the tile's first and last
   int lo, nf;  // entry e < nf: row e; e >= nf: row lo + e - nf
   int e_begin, e_end, ntiles;
-  bool once;  // the sequence's only tile: nobody else reads its rows in this call
+  bool once;  // the sequence's only tile: nobody else reads its rows in this call, but sequences that share its pages
 };
 
 // ---- row copies of one tile, dealt to the value waves (one instruction a row for columns 0..511, one per 8 rows for the
@@ -300,8 +302,10 @@ __device__ inline void copy_row(uint32_t lds_dst, uint64_t row, int x, int lane,
   else
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_dst), "v"(at), "s"(row) : "memory", "m0");
 }
-// NT: past the caches, where nobody else reads the rows in this call (a decode step of 32 sequences 149 us against 156; the
-// 128-byte tails too: 151; rows that tiles share, a prompt's window: 210 against 200).
+// NT: past the caches, where no other tile of the sequence reads the rows (a decode step of 32 sequences 149 us against 156,
+// 32 of 8192 rows 68 / 74, 256 of 8192 458 / 466; the 128-byte tails too: 151; rows that tiles share, a prompt's window:
+// 210 against 200).  Sequences that share pages are not told apart, which costs little: 32 over one prefix of 8192 rows
+// 57.8 / 57.2, 128 over 16384 311 / 308, 64 over 2048 with 300 rows each of their own 43.2 / 42.4; 8 over 8192 37.5 / 33.0.
 template <class G, bool NT>
 __device__ inline void issue_copies(const PagedArgs& a, uint32_t lds_base, const RowIds& id, int vi, int lane, int tl) {
   const uint32_t tbase = lds_base + (uint32_t)((tl % G::NBUF) * G::TILE_BYTES);
@@ -816,7 +820,7 @@ __device__ inline void value_role(const PagedArgs& a, const Work& w, lds_u8_t* l
     // O^T of block u: register k holds column 8 (k >> 2) + 4 (lane >> 5) + (k & 3) of q row r; one lane swap per
     // pair of packed registers gives each lane 8 columns in a row, 16 h + 8 (lane >> 5) .. + 7
     if (w.slot >= 0) {
-      // the lane's largest magnitude sets its scale: fp16 keeps 11 bits of every value that matters beside it
+      // the largest magnitude of the lane pair's 32 NU columns sets their scale: fp16 keeps 11 bits of those down to 2^-14 of it
       float top = 0.f;
 #pragma unroll
       for (int u = 0; u < NU; u++)

@@ -535,7 +535,7 @@ int smla_o_proj_ws(const void* o, int o_dtype, const int32_t* pos, const float* 
  * (smla_update_pages keeps it so, for the slots that it granted).  n_pages * P < 2^31.
  *
  * A batch is ragged: B sequences with lens[b] rows in the cache, the last cu[b+1] - cu[b] of them those
- * of the tokens cu[b] .. cu[b+1]-1 (cu [B+1], cu[0] = 0, not decreasing, cu[B] <= T); token t sits at position
+ * of the tokens cu[b] .. cu[b+1]-1 (cu [B+1], cu[0] >= 0, not decreasing, cu[B] <= T); token t sits at position
  * lens[b] - (cu[b+1] - cu[b]) + t - cu[b].  What belongs to tokens of no sequence is left as it was, or, with
  * SMLA_PAGED_FILL, set to 0.
  *
@@ -551,10 +551,12 @@ enum { SMLA_PAGED_NORM_Q = 1, SMLA_PAGED_NORM_KV = 2, SMLA_PAGED_FILL = 4 };
  * denominator.  A token that sees no row gives 0.  Rows a token does not see may hold anything,
  * infinities and NaN too; a row it sees that scores NaN or +inf gives NaN, one that scores -inf counts for nothing.
  * flags: 0 or SMLA_PAGED_FILL.  q, pages, out and workspace 16-byte aligned; out apart from q.  Sums and softmax
- * statistics are fp32; probabilities are rounded to bf16 before their products, the partial sums of tokens whose rows are
- * split over workgroups to fp16 times a power of two (taken so that the largest of 64 is below 2) before they are joined.  The result does not depend on the order in which
- * workgroups run.  workspace: smla_paged_attn_workspace(T, H, B, rows, window, first) bytes, rows = cols * P, not shared
- * by calls that overlap. */
+ * statistics are fp32; probabilities are rounded to bf16 before their products, the partial sums of tokens whose rows
+ * are split over workgroups to fp16 before they are joined: times a power of two that puts the largest of the 128
+ * (columns 0 .. 127) or 96 columns of a head that share it between 1 and 2, so columns over 2^14 smaller than that
+ * keep fewer than fp16's 11 bits.  The result does not depend on the order in which workgroups run.
+ * workspace: smla_paged_attn_workspace(T, H, B, rows, window, first) bytes, rows = cols * P, not shared by calls
+ * that overlap. */
 size_t smla_paged_attn_workspace(int64_t T, int64_t H, int64_t B, int64_t rows, int64_t window, int64_t first);
 int smla_paged_attn(const void* q, int q_dtype, const void* pages, int page_dtype, const float* page_scales,
                     int64_t n_pages, int64_t P, const int32_t* table, int64_t ld_table, int64_t cols,
