@@ -84,7 +84,7 @@ def update_pages(pages, table, lens, refs, parent, grow, page_scales=None):
     pages for slots 0 .. s): it has no rows for its new tokens, so pass granted on to ``paged_append`` and
     ``paged_attn``.  Freeing is parent -1, grow 0; beam reordering any map; a new sequence of n rows parent -1, grow n;
     a step after rejected drafts grow = new tokens - rejected ones (given back by a call of their own, grow < 0, where
-    another slot was made a copy of this one since they were written)."""
+    another slot was made a copy of this one since they were written, in the same call too)."""
     return ops.update_pages_op(pages, page_scales, table, lens, refs, parent, grow)
 
 

@@ -607,8 +607,8 @@ int smla_paged_append_granted(const void* q, int64_t ldq, const void* kv, int64_
  * buffers than the inputs: table_out [S, M] dense (-1 past a slot's pages), lens_out, refs_out, granted [S].
  * Pages given up by the call are free from refs_out on.  A slot holds the pages of its lens[s] rows, so lengths change
  * by this call only: one lowered by hand leaves pages counted that no entry names.  Without forks one call with
- * grow = new tokens - rejected rows does both, and the append writes over the latter; where another slot was made a copy of
- * the slot since they were written, they are given back by a call before the one that grows.
+ * grow = new tokens - rejected rows does both, and the append writes over the latter; where another slot was made a copy
+ * of the slot since they were written, in this call too, they are given back by a call before the append's.
  * Rows are copied within `layers` pools that share the table (layer l at pages + l layer_bytes; row_bytes a row),
  * and likewise within scales (NULL: none).
  * workspace: smla_update_pages_workspace(S, M, n_pages) bytes, 4-byte aligned; none (0, NULL is taken) where one
