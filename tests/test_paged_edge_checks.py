@@ -56,12 +56,12 @@ def _at(n):
     return ctypes.c_void_p(1 << 20 | n)
 
 
-# a bf16 q of 2 tokens of 16 heads of 512 at 0 (32768 bytes), kv behind it with 512 spare elements a row (2048 + 1024 bytes)
-OVER = dict(T=2, x_dtype=BF16, q=_at(0), ldq=16 * 512, kv=_at(32768), ldkv=1024, B=1)
+# a bf16 q of 2 tokens of 16 heads of 512 at 0 (32768 bytes), kv behind it with 488 spare elements a row (2000 + 1024 bytes)
+OVER = dict(T=2, x_dtype=BF16, q=_at(0), ldq=16 * 512, kv=_at(32768), ldkv=1000, B=1)
 
 
 @pytest.mark.parametrize("change", [
-    dict(q_out=_at(8)), dict(q_out=_at(32768 - 8)), dict(q_out=_at(32768)), dict(q_out=_at(32768 + 3072 - 8)),
+    dict(q_out=_at(8)), dict(q_out=_at(32768 - 8)), dict(q_out=_at(32768)), dict(q_out=_at(32768 + 3024 - 8)),
     dict(x_dtype=F32, q_out=_at(0), kv=_at(1 << 19)),                           # fp32 q: written rows lie over others
     dict(q=_at(0), ldq=16 * 512 + 4, q_out=_at(0), kv=_at(1 << 19)),            # rows apart
 ])
