@@ -10,6 +10,7 @@ in libsmla.so (C ABI: include/smla.h):
 * ``smla.norm_rope``    — ``ref_torch/norm_rope.py`` (tables for the kernels)
 * ``smla.mla``          — ``v4mlx/mla.py`` projections
 * ``smla.paged``        — the paged latent cache: attention, append, slots forked and grown, compaction
+* ``smla.moe``          — the expert network: routing, the experts, weights packed to 4 bits
 * ``smla.workloads``    — seeded synthetic inputs of the benchmark configurations
 """
 from . import _lib  # noqa: F401

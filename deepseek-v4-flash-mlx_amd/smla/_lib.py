@@ -9,13 +9,14 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsmla.so")
 
-F32, BF16, FP8_E4M3, F16, I32 = 0, 1, 2, 3, 4
+F32, BF16, FP8_E4M3, F16, I32, FP4_E2M1 = 0, 1, 2, 3, 4, 5
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
 _int = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _sz = ctypes.c_size_t
 
 # name -> (restype, argtypes)
@@ -93,6 +94,12 @@ _SIGNATURES = {
     "smla_compact_pages_workspace": (_sz, [_i64]),
     "smla_compact_pages": (_int, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp,
                                   _i64, _i64, _vp, _sz, _vp]),
+    "smla_route": (_int, [_vp, _int, _i64, _vp, _i64, _i64, _i64, _int, _i64, _i64, _int, _f64, _i64, _vp, _vp, _vp, _vp]),
+    "smla_linear_fp4_workspace": (_sz, [_i64] * 3),
+    "smla_linear_fp4": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _int, _vp, _sz, _vp]),
+    "smla_experts_workspace": (_sz, [_i64] * 5),
+    "smla_experts": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _int, _f32, _vp,
+                            _vp, _sz, _vp]),
 }
 
 # sim modes of smla_gated_pool / smla_ring_step, flags of smla_rotate_fp4
@@ -104,6 +111,8 @@ ATTN_SPLIT, ATTN_MERGE = 1, 2
 # flags of smla_paged_append and smla_paged_attn (FILL)
 PAGED_NORM_Q, PAGED_NORM_KV, PAGED_FILL = 1, 2, 4
 INDEX_EXACT = 1
+# scores of smla_route
+SCORES = {"softmax": 0, "sigmoid": 1, "sqrtsoftplus": 2}
 
 
 class SmlaLibraryError(RuntimeError):

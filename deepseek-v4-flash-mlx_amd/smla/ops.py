@@ -961,7 +961,7 @@ def _one_device(t, *rest):
         _on_gpu(t)
     for r in rest:
         if r is not None and r.get_device() != dev:
-            raise RuntimeError(f"smla paged ops run on one GPU: got tensors on {t.device} and {r.device}")
+            raise RuntimeError(f"smla ops run on one GPU: got tensors on {t.device} and {r.device}")
     return dev
 
 
@@ -1213,3 +1213,155 @@ def _(pages, page_scales, table, refs):
 
 
 compact_pages_op = _with_eager_route(compact_pages_op, _compact_pages)
+
+
+# ----------------------------------------------------------------------------------------------
+# The expert network (smla.moe) and products with 4-bit weights.
+def _rows(x, K, name):
+    """x [T, K] bf16 as a tensor whose rows are 16-byte aligned, and the elements between them."""
+    if x.dim() != 2 or x.shape[1] != K or x.dtype != torch.bfloat16:
+        raise ValueError(f"{name} must be bf16 [T, {K}], got {x.dtype} {list(x.shape)}")
+    ld, s1 = x.stride()
+    if x.shape[0] <= 1:
+        ld = K
+    if s1 != 1 or ld < K or ld % 8 or x.data_ptr() & 15:
+        return x.clone(memory_format=torch.contiguous_format), K
+    return x, ld
+
+
+def _check_fp4(codes, scales, lead, name):
+    """K of codes [*lead, K/2] and scales [*lead, K/32]; dense, because the kernels address whole tensors."""
+    n = len(lead)
+    if codes.dtype != torch.uint8 or codes.dim() != n + 1 or codes.shape[:n] != lead or not codes.is_contiguous():
+        raise ValueError(f"{name} must be dense uint8 codes {[*lead, 'K/2']}, got {codes.dtype} {list(codes.shape)}")
+    K = 2 * codes.shape[n]
+    if scales is None or scales.dtype != torch.uint8 or scales.shape != (*lead, K // 32) or not scales.is_contiguous():
+        got = None if scales is None else (scales.dtype, list(scales.shape))
+        raise ValueError(f"{name} scales must be dense uint8 {[*lead, K // 32]}, got {got}")
+    if K % 32 or K == 0:
+        raise ValueError(f"{name} rows must hold a multiple of 32 weights, got {K}")
+    return K
+
+
+def _route(logits: torch.Tensor, bias: Optional[torch.Tensor], k: int, score: int, groups: int, topk_groups: int, renorm: bool,
+           scale: float, shared: int, given: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+    """``smla_route`` (see ``moe.route``): ids [T, k + shared] int32 and weights of the same shape, fp32."""
+    dev = _one_device(logits, bias, given)
+    if logits.dim() != 2:
+        raise ValueError(f"expected logits [T, E], got {list(logits.shape)}")
+    dt = _YDT.get(logits.dtype)
+    if dt is None:
+        raise TypeError("route takes fp32 or bf16 logits")
+    T, E = logits.shape
+    ld, s1 = logits.stride()
+    if T <= 1:
+        ld = E
+    if (s1 != 1 and E > 1) or ld < E:
+        logits, ld = logits.contiguous(), E
+    if bias is not None:
+        if bias.shape != (E,):
+            raise ValueError(f"bias must be [{E}], got {list(bias.shape)}")
+        bias = _f32(bias)
+    if given is not None:
+        given = _i32(given, (T, k), "ids")
+    ids = torch.empty(T, k + shared, dtype=torch.int32, device=logits.device)
+    weights = torch.empty(T, k + shared, dtype=torch.float32, device=logits.device)
+    _launch(dev, "smla_route", logits.data_ptr(), dt, ld, _p(bias), T, E, k, score, groups, topk_groups, renorm, scale, shared,
+            _p(given), ids.data_ptr(), weights.data_ptr())
+    return ids, weights
+
+
+route_op = torch.library.custom_op("smla::route", mutates_args=(), device_types="cuda")(_route)
+
+
+@route_op.register_fake
+def _(logits, bias, k, score, groups, topk_groups, renorm, scale, shared, given):
+    shape = (logits.shape[0], k + shared)
+    return logits.new_empty(shape, dtype=torch.int32), logits.new_empty(shape, dtype=torch.float32)
+
+
+route_op = _with_eager_route(route_op, _route)
+
+
+def _linear_fp4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:
+    """``smla_linear_fp4`` (see ``mla.linear_fp4``): x [T, K] bf16, codes [N, K/2], scales [N, K/32] -> [T, N]."""
+    dev = _one_device(x, codes, scales)
+    if codes.dim() != 2:
+        raise ValueError(f"expected codes [N, K/2], got {list(codes.shape)}")
+    N = codes.shape[0]
+    K = _check_fp4(codes, scales, (N,), "linear_fp4's weights")
+    x, ld = _rows(x, K, "x")
+    T = x.shape[0]
+    ydt = _YDT.get(out_dtype)
+    if ydt is None:
+        raise TypeError("linear_fp4 gives fp32 or bf16")
+    if codes.data_ptr() & 15:
+        codes = codes.clone()
+    y = torch.empty(T, N, dtype=out_dtype, device=x.device)
+    wsb = _lib.lib().smla_linear_fp4_workspace(T, N, K)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=x.device) if wsb else None
+    _launch(dev, "smla_linear_fp4", x.data_ptr(), ld, codes.data_ptr(), scales.data_ptr(), T, N, K, y.data_ptr(), ydt, _p(ws),
+            wsb)
+    return y
+
+
+linear_fp4_op = torch.library.custom_op("smla::linear_fp4", mutates_args=(), device_types="cuda")(_linear_fp4)
+
+
+@linear_fp4_op.register_fake
+def _(x, codes, scales, out_dtype):
+    return x.new_empty(x.shape[0], codes.shape[0], dtype=out_dtype)
+
+
+linear_fp4_op = _with_eager_route(linear_fp4_op, _linear_fp4)
+
+
+def _experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: torch.Tensor, up: torch.Tensor,
+             down: torch.Tensor, gate_scales: Optional[torch.Tensor], up_scales: Optional[torch.Tensor],
+             down_scales: Optional[torch.Tensor], limit: float) -> torch.Tensor:
+    """``smla_experts`` (see ``moe.experts``): -> [T, K] bf16."""
+    dev = _one_device(x, ids, weights, gate, up, down, gate_scales, up_scales, down_scales)
+    if gate.dim() != 3 or x.dim() != 2 or ids.dim() != 2:
+        raise ValueError("expected x [T, K], ids [T, k] and gate [E, I, K]")
+    E, inner = gate.shape[:2]
+    fp4 = gate.dtype == torch.uint8
+    if fp4:
+        K = _check_fp4(gate, gate_scales, (E, inner), "gate")
+        if _check_fp4(up, up_scales, (E, inner), "up") != K or _check_fp4(down, down_scales, (E, K), "down") != inner:
+            raise ValueError(f"gate and up are [E, I, K] and down is [E, K, I]: got K = {K} and I = {inner} from gate")
+    else:
+        K = gate.shape[2]
+        for w, name, want in ((gate, "gate", (E, inner, K)), (up, "up", (E, inner, K)), (down, "down", (E, K, inner))):
+            if w.dtype != torch.bfloat16 or w.shape != want or not w.is_contiguous():
+                raise ValueError(f"{name} must be dense bf16 {list(want)} or fp4 codes, got {w.dtype} {list(w.shape)}")
+        if gate_scales is not None or up_scales is not None or down_scales is not None:
+            raise ValueError("scales go with fp4 codes, and only with them")
+    if (gate.data_ptr() | up.data_ptr() | down.data_ptr()) & 15:
+        raise ValueError("the experts' weights must be 16-byte aligned")
+    x, ld = _rows(x, K, "x")
+    T = x.shape[0]
+    k = ids.shape[1]
+    ids = _i32(ids, (T, k), "ids")
+    if weights.shape != (T, k):
+        raise ValueError(f"weights must be [{T}, {k}], got {list(weights.shape)}")
+    weights = _f32(weights)
+    y = torch.empty(T, K, dtype=torch.bfloat16, device=x.device)
+    if T == 0:
+        return y
+    wsb = _lib.lib().smla_experts_workspace(T, k, E, K, inner)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=x.device) if wsb else None
+    _launch(dev, "smla_experts", x.data_ptr(), ld, ids.data_ptr(), weights.data_ptr(), T, k, E, K, inner, gate.data_ptr(),
+            _p(gate_scales), up.data_ptr(), _p(up_scales), down.data_ptr(), _p(down_scales),
+            _lib.FP4_E2M1 if fp4 else _lib.BF16, limit, y.data_ptr(), _p(ws), wsb)
+    return y
+
+
+experts_op = torch.library.custom_op("smla::experts", mutates_args=(), device_types="cuda")(_experts)
+
+
+@experts_op.register_fake
+def _(x, ids, weights, gate, up, down, gate_scales, up_scales, down_scales, limit):
+    return x.new_empty(x.shape[0], x.shape[1])
+
+
+experts_op = _with_eager_route(experts_op, _experts)

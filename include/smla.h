@@ -45,6 +45,9 @@
  *   smla_paged_attn_granted, smla_paged_append_granted          the same, but for sequences without rows for them
  *   smla_update_pages         oracle/v4_fast.py:150-159        copies of sequences' caches (clone_states), as pages
  *   smla_compact_pages        (none: the reference's caches are contiguous)
+ *   smla_route                oracle/decode_engine.py:122-128  the router's scores, choice of experts, weights
+ *   smla_linear_fp4           ref_torch/quant.py:19-45         a product with 4-bit weights, without unpacking them
+ *   smla_experts              oracle/decode_engine.py:122-133  the chosen experts' networks, weighted and summed
  *   smla_o_proj, _ws          oracle/decode_engine.py:118-119  inverse RoPE of o's rope dims + o_grouped
  *                             v4mlx/mla.py:42-56               o_grouped(o, wo_a, wo_b)
  */
@@ -66,7 +69,8 @@ enum {
   SMLA_BF16 = 1,
   SMLA_FP8_E4M3 = 2, /* OCP e4m3fn (max 448), one byte per element */
   SMLA_F16 = 3,
-  SMLA_I32 = 4
+  SMLA_I32 = 4,
+  SMLA_FP4_E2M1 = 5 /* weights only: packed e2m1 codes with ue8m0 scales per 32 (smla_rotate_fp4's stored form) */
 };
 
 /* status codes */
@@ -630,6 +634,46 @@ int smla_compact_pages(const int32_t* table, int64_t ld_table, int64_t S, int64_
                        int64_t n_pages, int64_t P, int32_t* table_out, int32_t* refs_out, int32_t* live, void* pages,
                        int64_t layers, int64_t layer_bytes, int64_t row_bytes, void* scales, int64_t scale_layer_bytes,
                        int64_t scale_row_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * The expert network (oracle/decode_engine.py:122-133): routing, products with 4-bit weights, the experts.
+ *
+ * smla_route: each token's k experts of E (E <= 1024, k + shared <= 64) and their weights.
+ *   logits [T, E] F32 or BF16, ld elements between rows;  s = softmax over the row, sigmoid or sqrt(softplus) of
+ *   each (SMLA_SCORE_*);  r = s + bias (bias [E] fp32 or NULL: none);
+ *   groups > 1 (E a multiple): a group of E / groups consecutive experts is worth the sum of its two largest r,
+ *   and only experts of the topk_groups best take part (k <= topk_groups E / groups);
+ *   ids = the k largest r in that order, all ties to the lower index (groups and experts), -inf and NaN last by
+ *   index; the order is the exact values' (without a bias, the logits');
+ *   weights = s[ids], divided by their sum if `renorm` (0 where that is 0), times scale;
+ *   `shared` more columns follow: ids E, E + 1, .., weight 1.
+ *   given [T, k] or NULL: these ids instead of a choice (a table's, as the first layers have); bias and groups play
+ *   no part then, an id outside 0 .. E-1 has weight 0.
+ *   ids, weights [T, k + shared].  A row of -inf under softmax has scores 0; a row with a NaN, NaN.
+ *
+ * smla_linear_fp4: y[t, n] = sum_k x[t, k] W[n, k], W[n, k] = e2m1(codes) 2^(scales[n, k / 32] - 127).
+ *   x [T, K] BF16, ldx elements between rows (a multiple of 8; K a multiple of 32); codes [N, K / 2], scales [N, K / 32]
+ *   as smla_rotate_fp4 writes them; y [T, N] F32 or BF16; fp32 sums of exact products; x and codes 16-byte aligned.
+ *   workspace: smla_linear_fp4_workspace bytes (may be 0), 16-byte aligned; with less the product runs without it, slower.
+ *
+ * smla_experts: y[t] = sum_j down_e(h_tj), h_tj = weights[t, j] silu(min(g, limit)) clamp(u, -limit, limit),
+ *   g = gate_e x[t], u = up_e x[t], e = ids[t, j]; an id outside 0 .. E-1 adds nothing (a token without any gives 0).
+ *   x [T, K] BF16 (ldx as above), ids [T, k] int32, weights [T, k] fp32; gate, up [E, I, K] and down [E, K, I], all BF16
+ *   (scales NULL) or all SMLA_FP4_E2M1 (codes, and scale bytes per 32); K and I multiples of 32, E <= 1024, k <= 64;
+ *   y [T, K] BF16; limit > 0, infinity for none.  fp32 sums; h is rounded to bf16.  Tensors but the scales, ids and weights
+ *   16-byte aligned.  workspace: smla_experts_workspace bytes, 16-byte aligned (SMLA_E_WORKSPACE otherwise). */
+enum { SMLA_SCORE_SOFTMAX = 0, SMLA_SCORE_SIGMOID = 1, SMLA_SCORE_SQRTSOFTPLUS = 2 };
+int smla_route(const void* logits, int dtype, int64_t ld, const float* bias, int64_t T, int64_t E, int64_t k, int score,
+               int64_t groups, int64_t topk_groups, int renorm, double scale, int64_t shared, const int32_t* given,
+               int32_t* ids, float* weights, void* stream);
+size_t smla_linear_fp4_workspace(int64_t T, int64_t N, int64_t K);
+int smla_linear_fp4(const void* x, int64_t ldx, const uint8_t* codes, const uint8_t* scales, int64_t T, int64_t N, int64_t K,
+                    void* y, int y_dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t smla_experts_workspace(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I);
+int smla_experts(const void* x, int64_t ldx, const int32_t* ids, const float* weights, int64_t T, int64_t k, int64_t E,
+                 int64_t K, int64_t I, const void* gate, const uint8_t* gate_scales, const void* up, const uint8_t* up_scales,
+                 const void* down, const uint8_t* down_scales, int w_dtype, float limit, void* y, void* workspace,
+                 size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
