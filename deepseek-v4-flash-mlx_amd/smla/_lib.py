@@ -97,7 +97,7 @@ _SIGNATURES = {
     "smla_route": (_int, [_vp, _int, _i64, _vp, _i64, _i64, _i64, _int, _i64, _i64, _int, _f64, _i64, _vp, _vp, _vp, _vp]),
     "smla_linear_fp4_workspace": (_sz, [_i64] * 3),
     "smla_linear_fp4": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _int, _vp, _sz, _vp]),
-    "smla_experts_workspace": (_sz, [_i64] * 5),
+    "smla_experts_workspace": (_sz, [_i64] * 5 + [_int]),
     "smla_experts": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _int, _f32, _vp,
                             _vp, _sz, _vp]),
 }

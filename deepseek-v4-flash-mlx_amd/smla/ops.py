@@ -1348,11 +1348,11 @@ def _experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: to
     y = torch.empty(T, K, dtype=torch.bfloat16, device=x.device)
     if T == 0:
         return y
-    wsb = _lib.lib().smla_experts_workspace(T, k, E, K, inner)
+    wdt = _lib.FP4_E2M1 if fp4 else _lib.BF16
+    wsb = _lib.lib().smla_experts_workspace(T, k, E, K, inner, wdt)
     ws = torch.empty(wsb, dtype=torch.uint8, device=x.device) if wsb else None
     _launch(dev, "smla_experts", x.data_ptr(), ld, ids.data_ptr(), weights.data_ptr(), T, k, E, K, inner, gate.data_ptr(),
-            _p(gate_scales), up.data_ptr(), _p(up_scales), down.data_ptr(), _p(down_scales),
-            _lib.FP4_E2M1 if fp4 else _lib.BF16, limit, y.data_ptr(), _p(ws), wsb)
+            _p(gate_scales), up.data_ptr(), _p(up_scales), down.data_ptr(), _p(down_scales), wdt, limit, y.data_ptr(), _p(ws), wsb)
     return y
 
 

@@ -654,7 +654,7 @@ int smla_compact_pages(const int32_t* table, int64_t ld_table, int64_t S, int64_
  * smla_linear_fp4: y[t, n] = sum_k x[t, k] W[n, k], W[n, k] = e2m1(codes) 2^(scales[n, k / 32] - 127).
  *   x [T, K] BF16, ldx elements between rows (a multiple of 8; K a multiple of 32); codes [N, K / 2], scales [N, K / 32]
  *   as smla_rotate_fp4 writes them; y [T, N] F32 or BF16; fp32 sums of exact products; x and codes 16-byte aligned.
- *   workspace: smla_linear_fp4_workspace bytes (may be 0), 16-byte aligned; with less the product runs without it, slower.
+ *   workspace: smla_linear_fp4_workspace bytes (may be 0), 16-byte aligned; SMLA_E_WORKSPACE where there is less.
  *
  * smla_experts: y[t] = sum_j down_e(h_tj), h_tj = weights[t, j] silu(min(g, limit)) clamp(u, -limit, limit),
  *   g = gate_e x[t], u = up_e x[t], e = ids[t, j]; an id outside 0 .. E-1 adds nothing (a token without any gives 0).
@@ -669,7 +669,7 @@ int smla_route(const void* logits, int dtype, int64_t ld, const float* bias, int
 size_t smla_linear_fp4_workspace(int64_t T, int64_t N, int64_t K);
 int smla_linear_fp4(const void* x, int64_t ldx, const uint8_t* codes, const uint8_t* scales, int64_t T, int64_t N, int64_t K,
                     void* y, int y_dtype, void* workspace, size_t workspace_bytes, void* stream);
-size_t smla_experts_workspace(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I);
+size_t smla_experts_workspace(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I, int w_dtype);
 int smla_experts(const void* x, int64_t ldx, const int32_t* ids, const float* weights, int64_t T, int64_t k, int64_t E,
                  int64_t K, int64_t I, const void* gate, const uint8_t* gate_scales, const void* up, const uint8_t* up_scales,
                  const void* down, const uint8_t* down_scales, int w_dtype, float limit, void* y, void* workspace,

@@ -75,7 +75,7 @@ def test_workspaces_of_bad_sizes_are_empty():
     from smla import _lib
     lib = _lib.lib()
     assert lib.smla_linear_fp4_workspace(0, 16, 64) == 0 and lib.smla_linear_fp4_workspace(64, 16, 33) == 0
-    assert lib.smla_experts_workspace(1, 1, 2000, 64, 64) == 0 and lib.smla_experts_workspace(0, 1, 20, 64, 64) == 0
+    assert lib.smla_experts_workspace(1, 1, 2000, 64, 64, 5) == 0 and lib.smla_experts_workspace(0, 1, 20, 64, 64, 5) == 0
 
 
 def _u8(*shape):
