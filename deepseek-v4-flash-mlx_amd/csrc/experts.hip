@@ -11,6 +11,8 @@
 #include "fp4.h"
 #include "smla_internal.h"
 
+#include <algorithm>
+
 namespace {
 
 using smla_fp4::scale_of;
@@ -24,83 +26,127 @@ struct Matrix {
   const uint8_t* s;
 };
 
-// 32 weights of a row, and their 8 values j = 0 .. 3
+// The kernels for few tokens know a third type: codes of rows that are no multiple of 128 weights.  Scales of whole steps
+// of 128 come through LDS, 16 bytes of a row a request (a step's four bytes of 16 rows are 16 requests, as its codes are, and
+// took as long: eight tokens' up products 115 against 70 us); the others byte by byte.
+constexpr int kFp4Odd = 2;
+
+using smla_attn::lds_u32x4_t;
+using smla_attn::lds_u8_t;
+
+// 32 weights of a row, and their 8 values j = 0 .. 3.  at: the first row of 16 (the same for the wave), row: this lane's.
 template <int WT>
 struct Block;
-template <>
-struct Block<kFp4> {
+template <int WT>
+struct BlockFp4 {
   u32x4_t c;
   uint32_t s;
-  __device__ void load(const Matrix& m, int64_t row, int K, int kb) {
-    c = *(const u32x4_t*)(m.w + row * (K / 2) + 16 * kb);
-    s = m.s[row * (K / 32) + kb];
+  __device__ void load(const Matrix& at, uint32_t row, uint32_t K, uint32_t kb) {
+    c = *(const u32x4_t*)(at.w + (row * (K / 2) + 16 * kb));
+    s = WT == kFp4Odd ? at.s[row * (K / 32) + kb] : 0;
   }
-  __device__ void zero() { c = u32x4_t{0, 0, 0, 0}, s = 127; }
+  // the scale of step s's block from LDS (scales: this lane's byte at step 0, 64 bytes a step)
+  __device__ void scale(const lds_u8_t* scales, int step) {
+    if constexpr (WT == kFp4) s = scales[64 * step];
+  }
+  __device__ void keep(bool k) { c = k ? c : u32x4_t{0, 0, 0, 0}, s = k ? s : 127; }
+  // waits for the loads, and with them for every copy that was requested before: LDS is read behind it
+  __device__ void arrived() { asm volatile("" : "+v"(c), "+v"(s) : : "memory"); }
   __device__ bf16x8_t frag(int j) const { return to_bf16(c[j], scale_of(s)); }
+  static __device__ Matrix rows(const Matrix& m, int64_t row, int K) { return {m.w + row * (K / 2), m.s + row * (K / 32)}; }
 };
+template <>
+struct Block<kFp4> : BlockFp4<kFp4> {};
+template <>
+struct Block<kFp4Odd> : BlockFp4<kFp4Odd> {};
 template <>
 struct Block<kBf16> {
   u32x4_t c[4];
-  __device__ void load(const Matrix& m, int64_t row, int K, int kb) {
-    const uint8_t* p = m.w + (row * K + 32 * kb) * 2;
+  __device__ void load(const Matrix& at, uint32_t row, uint32_t K, uint32_t kb) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) c[j] = *(const u32x4_t*)(p + 16 * j);
+    for (int j = 0; j < 4; j++) c[j] = *(const u32x4_t*)(at.w + (row * (2 * K) + 64 * kb + 16 * j));
   }
-  __device__ void zero() {
+  __device__ void scale(const lds_u8_t*, int) {}
+  __device__ void keep(bool k) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) c[j] = u32x4_t{0, 0, 0, 0};
+    for (int j = 0; j < 4; j++) c[j] = k ? c[j] : u32x4_t{0, 0, 0, 0};
   }
+  __device__ void arrived() { asm volatile("" : "+v"(c[0]), "+v"(c[1]), "+v"(c[2]), "+v"(c[3]) : : "memory"); }
   __device__ bf16x8_t frag(int j) const { return as_bf16x8(c[j]); }
+  static __device__ Matrix rows(const Matrix& m, int64_t row, int K) { return {m.w + row * (2 * (int64_t)K), nullptr}; }
 };
 
 // ---- few tokens (up to 16): the weights are streamed once, a 16-row block of W (A of the product) against all tokens
 // (B: column m of lane 16 q + m is token m).  A step is 128 k: lane group q takes the 32 of block 4 s + q on both
-// sides, 16 bytes of codes a lane.  The K range is cut over the waves of a workgroup, kAhead steps' loads are in flight.
+// sides, 16 bytes of codes a lane.  The K range is cut over the waves of a workgroup, and a wave keeps the loads of the
+// next steps in flight: as a step is multiplied the one that takes its registers is requested (a batch at a time, each
+// waited for whole, took half as long again).
 
 constexpr int kFew = 16;
-template <int WT>
-constexpr int kAhead = WT == kFp4 ? 4 : 2;
-
 __device__ inline void add4(f32x4_t& a, const f32x4_t& b) {
 #pragma unroll
   for (int i = 0; i < 4; i++) a[i] += b[i];
 }
 
-// acc[r] (rows 4 q .. +3 of matrix r's 16, column m) = the sums over steps s0 .. s1-1 for R matrices' rows; x: this
-// lane's column, null where there is none.
-template <int WT, int R>
-__device__ inline void products(const Matrix (&m)[R], int64_t row, const uint16_t* x, int K, int s0, int s1, f32x4_t (&acc)[R]) {
-  constexpr int U = kAhead<WT>;
-  const int q = (threadIdx.x >> 4) & 3, nb = K / 32;
+// Steps s0 .. s1-1 in order, U in flight: load(slot, s) in order, use(slot, s).  First what U does not divide, as one batch,
+// so that no load of the rest stands under a condition: the waits are for one step then (a conditional load has the
+// compiler wait for all; requesting the last step again instead costs what a step costs).  A step's reads of LDS are not
+// to be gathered ahead of the step before: the registers are the loads'. 
+template <int U, class L, class F>
+__device__ __attribute__((always_inline)) inline void rolling(int s0, int s1, L&& load, F&& use) {
+  const int rest = (s1 - s0) % U;
+  if (rest) {
 #pragma unroll
-  for (int r = 0; r < R; r++) acc[r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int s = s0; s < s1; s += U) {
-    Block<WT> w[U][R];
-    u32x4_t xv[U][4];
+    for (int u = 0; u < U - 1; u++)
+      if (u < rest) load(u, s0 + u);
+#pragma unroll
+    for (int u = 0; u < U - 1; u++)
+      if (u < rest) use(u, s0 + u);
+    s0 += rest;
+  }
+  if (s0 >= s1) return;
+#pragma unroll
+  for (int u = 0; u < U; u++) load(u, s0 + u);
+  for (; s0 + U < s1; s0 += U)
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int kb = 4 * (s + u) + q;
-#pragma unroll
-      for (int r = 0; r < R; r++) w[u][r].zero();
-#pragma unroll
-      for (int j = 0; j < 4; j++) xv[u][j] = u32x4_t{0, 0, 0, 0};
-      if (s + u < s1 && kb < nb) {
-#pragma unroll
-        for (int r = 0; r < R; r++) w[u][r].load(m[r], row, K, kb);
-        if (x) {
-#pragma unroll
-          for (int j = 0; j < 4; j++) xv[u][j] = *(const u32x4_t*)(x + 32 * kb + 8 * j);
-        }
-      }
+      use(u, s0 + u);
+      load(u, s0 + u + U);
+      __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-#pragma unroll
-        for (int r = 0; r < R; r++)
-          acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[u][r].frag(j), as_bf16x8(xv[u][j]), acc[r], 0, 0, 0);
+  for (int u = 0; u < U; u++) {
+    use(u, s0 + u);
+    __builtin_amdgcn_sched_barrier(0);
   }
+}
+
+// the block of step s and lane group q: clamped to the last (a step's blocks past K are dropped by `keep`)
+__device__ inline int block_of(int s, int q, int nb) { return min(4 * s + q, nb - 1); }
+
+// The steps s0 .. s1-1 of a row of K bf16 to LDS (256 bytes a step, contiguous), by this wave for itself: lane l's 16 bytes of
+// every 1 KB.  Bytes past the row are not copied.
+__device__ inline void copy_steps(const uint16_t* row, int K, int s0, int s1, uint32_t lds) {
+  const int lane = threadIdx.x & 63, end = min(256 * s1, 2 * K);
+  for (int b = 256 * s0; b < end; b += 1024)
+    if (b + 16 * lane < end) smla_attn::dma16((const uint8_t*)row + b + 16 * lane, lds + b - 256 * s0);
+}
+
+// The scales of steps s0 .. s1-1 of 16 rows (last: the last that exists) to LDS, 64 bytes a step, four steps a request; room
+// for whole fours.
+template <int WT>
+__device__ inline void copy_scales(const Matrix& at, int last, int K, int s0, int s1, uint32_t lds) {
+  if constexpr (WT == kFp4) {
+    const int lane = threadIdx.x & 63, row = min(lane & 15, last) * (K / 32);
+    for (int s = s0; s < s1; s += 4) smla_tile::dma4_s(at.s, row + 4 * min(s + (lane >> 4), s1 - 1), lds + 64 * (s - s0));
+  }
+}
+
+// the x operand j of step s from LDS (x: this lane's column at step 0, 64 bytes a lane group), 0 past K
+__device__ inline bf16x8_t operand(const lds_u8_t* x, int s, int j, bool drop) {
+  u32x4_t v = *(const lds_u32x4_t*)(x + 256 * s + 16 * j);
+  if (drop) v = u32x4_t{0, 0, 0, 0};
+  return as_bf16x8(v);
 }
 
 // the waves' sums, in wave order, in wave 0
@@ -118,13 +164,39 @@ __device__ inline void join(f32x4_t (&acc)[R]) {
     for (int r = 0; r < R; r++) add4(acc[r], red[v][r][lane]);
 }
 
-template <int NW, int YDT>
+constexpr int kRowPad = 16;  // bytes between the rows of a wave in LDS: 16 rows' columns fall in distinct banks
+
+// bytes of LDS of a wave of nw: n rows of K, scales of r matrices
+__host__ __device__ inline int few_steps(int K, int nw) { return ((K + 127) / 128 + nw - 1) / nw; }
+__host__ __device__ inline int few_scales(int K, int nw) { return (few_steps(K, nw) + 3) / 4 * 256; }
+__host__ __device__ inline int few_lds(int n, int K, int nw, int r) { return n * (few_steps(K, nw) * 256 + kRowPad) + r * few_scales(K, nw); }
+
+template <int WT, int NW, int YDT>
 __global__ __launch_bounds__(64 * NW) void linear_few_kernel(const uint16_t* __restrict__ x, int64_t ldx, Matrix w, int T, int N,
                                                              int K, void* __restrict__ y) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, q = lane >> 4, steps = (K + 127) / 128;
-  const int n0 = blockIdx.x * 16;
-  f32x4_t acc[1];
-  products<kFp4, 1>({w}, min(n0 + m, N - 1), m < T ? x + (int64_t)m * ldx : nullptr, K, steps * wave / NW, steps * (wave + 1) / NW, acc);
+  constexpr int U = 8;
+  extern __shared__ __align__(16) uint8_t lds_x[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, q = lane >> 4;
+  const int nb = K / 32, steps = (nb + 3) / 4, s0 = steps * wave / NW, s1 = steps * (wave + 1) / NW, n0 = blockIdx.x * 16;
+  lds_u8_t* mine = (lds_u8_t*)lds_x + wave * few_lds(T, K, NW, 1);
+  const int ld = few_lds(1, K, NW, 0), row = min(m, N - 1 - n0);
+  const Matrix at = Block<WT>::rows(w, n0, K);
+  copy_scales<WT>(at, N - 1 - n0, K, s0, s1, (uint32_t)(uintptr_t)mine + T * ld);
+  for (int t = 0; t < T; t++) copy_steps(x + (int64_t)t * ldx, K, s0, s1, (uint32_t)(uintptr_t)mine + t * ld);
+  const lds_u8_t* xl = mine + min(m, T - 1) * ld + 64 * q - 256 * s0;  // (columns past the last token are not stored)
+  const lds_u8_t* sl = mine + T * ld + 4 * m + q - 64 * s0;
+  Block<WT> b[U];
+  f32x4_t acc[1] = {f32x4_t{0.f, 0.f, 0.f, 0.f}};
+  rolling<U>(s0, s1, [&](int u, int s) __attribute__((always_inline)) { b[u].load(at, row, K, block_of(s, q, nb)); },
+             [&](int u, int s) __attribute__((always_inline)) {
+               b[u].arrived();  // and the copies, which went out before
+               b[u].scale(sl, s);
+               const bool drop = 4 * s + 4 > nb && 4 * s + q >= nb;
+               if (4 * s + 4 > nb) b[u].keep(!drop);  // uniform
+#pragma unroll
+               for (int j = 0; j < 4; j++)
+                 acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[u].frag(j), operand(xl, s, j, drop), acc[0], 0, 0, 0);
+             });
   join<NW>(acc);
   if (wave != 0 || m >= T) return;
 #pragma unroll
@@ -163,112 +235,223 @@ __device__ inline float gated(float g, float u, float lim) {
   return g / (1.f + __expf(-g)) * u;
 }
 
-// Workgroup (i, p): 16 hidden rows' gate and up products of the expert of pair p, where p is its first pair, for
-// every token that has it.  A token that has it twice has the sum of its weights.
-constexpr int kUpWaves = 8;
+// Workgroup (i, p): 16 hidden rows' gate and up products of the expert of pair p, where p is its first pair, for the
+// tokens that have it: column m is the m-th of them.  A token that has it twice has the sum of its weights.  A wave has its
+// K range of the tokens' rows of x in LDS (in registers they would take three times the weights' and leave one workgroup a
+// CU), room for `cap` of them; an expert of more streams its weights again for the others.
+constexpr int kUpWaves = 4;
 template <int WT>
-__global__ __launch_bounds__(64 * kUpWaves) void few_up_kernel(const ExpertArgs a) {
-  const int p = blockIdx.y, e = a.ids[p], lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, q = lane >> 4;
-  if (e < 0 || e >= a.E) return;
-  bool seen = false;
-  for (int o = lane; o < p; o += 64) seen |= a.ids[o] == e;
-  if (__any(seen)) return;
+constexpr int kUpAhead = WT == kBf16 ? 2 : WT == kFp4Odd ? 6 : 8;
+template <int WT>
+__global__ __launch_bounds__(64 * kUpWaves) __attribute__((amdgpu_waves_per_eu(4))) void few_up_kernel(const ExpertArgs a, int cap) {
+  constexpr int U = kUpAhead<WT>;
+  extern __shared__ __align__(16) uint8_t lds_x[];
+  const int p = blockIdx.y, e = __builtin_amdgcn_readfirstlane(a.ids[p]), lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, q = lane >> 4;
+  // lane t < T: token t's first place with this expert, and its weight; eight loads at a time (one after the other they
+  // took longer than the weights)
   int pair = -1;
-  float w = 0.f;
-  if (m < a.T)
-    for (int j = a.k - 1; j >= 0; j--)
-      if (a.ids[m * a.k + j] == e) pair = m * a.k + j, w += a.weights[pair];
-  const int i0 = blockIdx.x * 16, steps = (a.K + 127) / 128;
-  f32x4_t acc[2];
-  products<WT, 2>({a.gate, a.up}, (int64_t)e * a.I + i0 + m, pair >= 0 ? a.x + m * a.ldx : nullptr, a.K, steps * wave / kUpWaves,
-                  steps * (wave + 1) / kUpWaves, acc);
-  join<kUpWaves>(acc);
-  if (wave != 0 || pair < 0) return;
-  float h[4];
+  float wt = 0.f;
+  for (int j0 = 0; j0 < a.k; j0 += 8) {
+    int id[8];
+    float w[8];
+    const int base = min(lane, a.T - 1) * a.k;
 #pragma unroll
-  for (int i = 0; i < 4; i++) h[i] = w * gated(acc[0][i], acc[1][i], a.limit);
-  *(u32x2_t*)(a.h + (int64_t)pair * a.I + i0 + 4 * q) = u32x2_t{pack_bf16x2(h[0], h[1]), pack_bf16x2(h[2], h[3])};
+    for (int j = 0; j < 8; j++) {
+      id[j] = a.ids[base + min(j0 + j, a.k - 1)];
+      w[j] = a.weights[base + min(j0 + j, a.k - 1)];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (lane < a.T && j0 + j < a.k && id[j] == e) {
+        if (pair < 0) pair = base + j0 + j;
+        wt += w[j];
+      }
+  }
+  if (e < 0 || e >= a.E || __any(pair >= 0 && pair < p)) return;
+  uint32_t has = __builtin_amdgcn_readfirstlane((uint32_t)__ballot(pair >= 0));
+  const int i0 = blockIdx.x * 16, nb = a.K / 32, steps = (nb + 3) / 4;
+  const int s0 = steps * wave / kUpWaves, s1 = steps * (wave + 1) / kUpWaves, ld = few_lds(1, a.K, kUpWaves, 0);
+  lds_u8_t* mine = (lds_u8_t*)lds_x + wave * few_lds(cap, a.K, kUpWaves, 2);
+  const Matrix gate = Block<WT>::rows(a.gate, (int64_t)e * a.I + i0, a.K), up = Block<WT>::rows(a.up, (int64_t)e * a.I + i0, a.K);
+  const int s_up = few_scales(a.K, kUpWaves);
+  copy_scales<WT>(gate, 15, a.K, s0, s1, (uint32_t)(uintptr_t)mine + cap * ld);
+  copy_scales<WT>(up, 15, a.K, s0, s1, (uint32_t)(uintptr_t)mine + cap * ld + s_up);
+  const lds_u8_t* sl = mine + cap * ld + 4 * m + q - 64 * s0;
+  while (has) {
+    int col = 0, nt = 0;  // lane m < nt: its token
+    for (; has && nt < cap; nt++) {
+      const int t = __ffs((int)has) - 1;
+      has &= has - 1;
+      if (m == nt) col = t;
+      copy_steps(a.x + t * a.ldx, a.K, s0, s1, (uint32_t)(uintptr_t)mine + nt * ld);
+    }
+    const lds_u8_t* xl = mine + min(m, nt - 1) * ld + 64 * q - 256 * s0;
+    uint32_t wr = m, wq = q;  // (not known to be the same in every pass: else the addresses of all loads are kept, and spilled)
+    asm volatile("" : "+v"(wr), "+v"(wq));
+    Block<WT> w[U][2];
+    f32x4_t acc[2];
+    acc[0] = acc[1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    rolling<U>(s0, s1, [&](int u, int s) __attribute__((always_inline)) {
+      const int kb = block_of(s, wq, nb);
+      w[u][0].load(gate, wr, a.K, kb);
+      w[u][1].load(up, wr, a.K, kb);
+    }, [&](int u, int s) __attribute__((always_inline)) {
+      w[u][0].arrived();  // and the copies, which went out before
+      w[u][1].arrived();
+      w[u][0].scale(sl, s);
+      w[u][1].scale(sl + s_up, s);
+      const bool drop = 4 * s + 4 > nb && 4 * s + q >= nb;
+      if (4 * s + 4 > nb) {  // uniform
+        w[u][0].keep(!drop);
+        w[u][1].keep(!drop);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const bf16x8_t x = operand(xl, s, j, drop);
+#pragma unroll
+        for (int r = 0; r < 2; r++) acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[u][r].frag(j), x, acc[r], 0, 0, 0);
+      }
+    });
+    join<kUpWaves>(acc);
+    const int to = __shfl(pair, col, 64);
+    const float weight = __shfl(wt, col, 64);
+    if (wave == 0 && m < nt) {
+      float h[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) h[i] = weight * gated(acc[0][i], acc[1][i], a.limit);
+      *(u32x2_t*)(a.h + (int64_t)to * a.I + i0 + 4 * q) = u32x2_t{pack_bf16x2(h[0], h[1]), pack_bf16x2(h[2], h[3])};
+    }
+    if (has) __syncthreads();  // the sums are read before the next pass writes its own
+  }
 }
 
 // Workgroup i: 16 columns of y for every token, over all experts that any token has: the waves share out the K
-// ranges of all of them.  A wave adds an expert's sums to a token's only where the token has it (0 times an infinite
-// weight of another token's expert would be NaN).
-constexpr int kDownWaves = 16;
+// ranges of all of them.  An item is an expert and up to kItemTokens tokens that have it, whose hidden rows go to the
+// wave's LDS a step ahead of the step's weights (256 bytes a token; as operands from memory they are four loads of 1 KB
+// a step, against one of the weights).  Column m is token m: a wave adds an item's sums to a token's only where the item
+// has it (0 times an infinite weight of another token's expert would be NaN).
+constexpr int kDownWaves = 16, kItemTokens = 4;
+template <int WT>
+constexpr int kDownAhead = WT == kBf16 ? 3 : 4;
+template <int WT>
+constexpr int kDownRing = kDownAhead<WT> * kItemTokens * 256;
+template <int WT>
+constexpr int kDownScales = WT == kFp4 ? (kDownAhead<WT> + 2) * 256 : 0;
+template <int WT>
+constexpr int kDownLds = kDownWaves * (kDownRing<WT> + kDownScales<WT>);
+
 template <int WT>
 __global__ __launch_bounds__(64 * kDownWaves) void few_down_kernel(const ExpertArgs a) {
-  constexpr int U = kAhead<WT>;
-  __shared__ int32_t ids[kFew * kMaxChoices], act[kFew * kMaxChoices];
-  __shared__ int16_t pairs[kFew * kMaxChoices][kFew];
-  __shared__ int cnt[kDownWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, q = lane >> 4;
-  const int e0 = tid < a.P ? a.ids[tid] : -1;
-  ids[tid] = e0;
+  constexpr int U = kDownAhead<WT>;
+  extern __shared__ __align__(16) uint8_t lds_x[];
+  __shared__ int32_t slot[kMaxExperts];                // an expert's first pair, then its number
+  __shared__ int32_t item[kFew * kMaxChoices];         // first the ids, then expert | tokens << 10
+  __shared__ __align__(16) int16_t pairs[kFew * kMaxChoices][kFew];  // of an expert and a token: the first pair
+  __shared__ int cnt[2][kDownWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, q = lane >> 4;
+  const int e = tid < a.P ? a.ids[tid] : -1, t = (uint32_t)tid / (uint32_t)a.k;
+  const bool real = e >= 0 && e < a.E;
+  slot[tid] = 0x7fffffff;
+  item[tid] = e;
+  for (int i = tid; i < a.P * kFew / 2; i += 64 * kDownWaves) ((int32_t*)pairs)[i] = -1;
   __syncthreads();
-  bool first = e0 >= 0 && e0 < a.E;
-  for (int o = 0; first && o < tid; o++) first = ids[o] != e0;
+  if (real) atomicMin(&slot[e], tid);
+  __syncthreads();
+  const bool first = real && slot[e] == tid;
   const uint64_t mask = __ballot(first);
-  if (lane == 0) cnt[wave] = __popcll(mask);
+  if (lane == 0) cnt[0][wave] = __popcll(mask);
   __syncthreads();
-  int at = 0, n = 0;
+  int at = __popcll(mask & ((1ull << lane) - 1));  // the expert's number
+  for (int v = 0; v < wave; v++) at += cnt[0][v];
+  if (first) slot[e] = at;
+  __syncthreads();
+  // the first of a token's choices of the same expert
+  if (real) {
+    bool again = false;
+    for (int o = t * a.k; o < tid; o++) again |= item[o] == e;
+    if (!again) pairs[slot[e]][t] = (int16_t)tid;
+  }
+  __syncthreads();
+  int experts = 0;
+  for (int v = 0; v < kDownWaves; v++) experts += cnt[0][v];
+  // items of up to kItemTokens tokens
+  uint32_t tokens = 0;
+  if (first)
+    for (int o = 0; o < a.T; o++) tokens |= (uint32_t)(pairs[at][o] >= 0) << o;
+  const int need = ((int)__popc(tokens) + kItemTokens - 1) / kItemTokens;
+  int sum_before = need;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const int u = __shfl_up(sum_before, o, 64);
+    if (lane >= o) sum_before += u;
+  }
+  if (lane == 63) cnt[1][wave] = sum_before;
+  __syncthreads();
+  int it = sum_before - need, items = 0;
   for (int v = 0; v < kDownWaves; v++) {
-    if (v < wave) at += cnt[v];
-    n += cnt[v];
+    if (v < wave) it += cnt[1][v];
+    items += cnt[1][v];
   }
-  if (first) act[at + __popcll(mask & ((1ull << lane) - 1))] = e0;
-  __syncthreads();
-  for (int i = tid; i < n * kFew; i += 64 * kDownWaves) {
-    const int t = i % kFew, e = act[i / kFew];
-    int pair = -1;
-    if (t < a.T)
-      for (int j = a.k - 1; j >= 0; j--)
-        if (ids[t * a.k + j] == e) pair = t * a.k + j;
-    pairs[i / kFew][t] = (int16_t)pair;
+  for (; tokens; it++) {
+    uint32_t some = 0;
+    for (int o = 0; o < kItemTokens && tokens; o++) some |= tokens & -tokens, tokens &= tokens - 1;
+    item[it] = e | some << 10;
   }
   __syncthreads();
-  const int n0 = blockIdx.x * 16, nb = a.I / 32, per = (nb + 3) / 4, steps = n * per;
+  items = __builtin_amdgcn_readfirstlane(items);
+
+  const int n0 = blockIdx.x * 16, nb = a.I / 32, per = (nb + 3) / 4, steps = items * per;
   const int s0 = steps * wave / kDownWaves, s1 = steps * (wave + 1) / kDownWaves;
+  lds_u8_t *ring = (lds_u8_t*)lds_x + wave * kDownRing<WT>, *scales = (lds_u8_t*)lds_x + kDownWaves * kDownRing<WT> + wave * kDownScales<WT>;
   f32x4_t sum = {0.f, 0.f, 0.f, 0.f}, acc = sum;
-  int cur = s0 / per, k0 = s0 - cur * per;  // expert and its step, of the loads
-  int has = -1, of = cur;
-  if (s0 < s1) has = pairs[cur][m];
-  for (int s = s0; s < s1; s += U) {
-    Block<WT> w[U];
-    u32x4_t xv[U][4];
-    int ex[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int kb = 4 * k0 + q;
-      ex[u] = cur;
-      w[u].zero();
-#pragma unroll
-      for (int j = 0; j < 4; j++) xv[u][j] = u32x4_t{0, 0, 0, 0};
-      if (s + u < s1) {
-        if (kb < nb) {
-          w[u].load(a.down, (int64_t)act[cur] * a.K + n0 + m, a.I, kb);
-          const int pair = pairs[cur][m];
-          if (pair >= 0) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) xv[u][j] = *(const u32x4_t*)(a.h + (int64_t)pair * a.I + 32 * kb + 8 * j);
-          }
-        }
-        if (++k0 == per) k0 = 0, cur++;
+  int lk = s0 % per, uk = lk, li = s0 / per, ui = li;  // an item's step, and the item, of the loads and of the products
+  auto get = [&](int i) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(i < items ? item[i] : 0); };
+  int lit = get(li), uit = lit;
+  auto rows_of = [&](int it) __attribute__((always_inline)) { return items > 0 ? (int)pairs[slot[it & 1023]][m] : -1; };
+  // scales: a request for each four steps of an item that the wave has any of, in a ring of slots of 256 bytes
+  constexpr int SLOTS = U + 2;
+  int ls = -1, us = -1;  // slots of the loads' and the products' step
+  auto next = [&](int slot) __attribute__((always_inline)) { return slot + 1 == SLOTS ? 0 : slot + 1; };
+  int lp = rows_of(lit);  // lane m: token m's row of h, of the loads' item
+  Block<WT> w[U];
+  rolling<U>(s0, s1, [&](int u, int s) __attribute__((always_inline)) {
+    const int ex = lit & 1023;
+    const Matrix at = Block<WT>::rows(a.down, (int64_t)ex * a.K + n0, a.I);
+    uint32_t has = (uint32_t)lit >> 10;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot's last reads are done
+    for (int c = 0; has; c++) {  // uniform
+      const int pair = __builtin_amdgcn_readlane(lp, __ffs((int)has) - 1);
+      has &= has - 1;
+      const int b = min(256 * lk + 4 * lane, 2 * a.I - 4);  // (past the row: any, dropped)
+      smla_tile::dma4_s((const uint8_t*)a.h + 2 * (int64_t)pair * a.I, b, (uint32_t)(uintptr_t)ring + (u * kItemTokens + c) * 256);
+    }
+    if constexpr (WT == kFp4) {
+      if (lk % 4 == 0 || s == s0) {  // uniform
+        ls = next(ls);
+        smla_tile::dma4_s(at.s, m * (a.I / 32) + 4 * min((lk & ~3) + q, per - 1), (uint32_t)(uintptr_t)scales + 256 * ls);
       }
     }
+    w[u].load(at, m, a.I, block_of(lk, q, nb));
+    if (++lk == per) lk = 0, lit = get(++li), lp = rows_of(lit);
+  }, [&](int u, int s) __attribute__((always_inline)) {
+    w[u].arrived();  // and the copies, which went out before
+    if (uk % 4 == 0 || s == s0) us = next(us);
+    w[u].scale(scales + 256 * us + 4 * m + q, uk & 3);
+    const bool drop = 4 * uk + 4 > nb && 4 * uk + q >= nb;
+    if (4 * uk + 4 > nb) w[u].keep(!drop);  // uniform
+    const uint32_t has = (uint32_t)uit >> 10;
+    const lds_u8_t* x = ring + (u * kItemTokens + min((int)__popc(has & ((1u << m) - 1)), kItemTokens - 1)) * 256 + 64 * q;
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      if (s + u >= s1) break;
-      if (ex[u] != of) {
-        if (has >= 0) add4(sum, acc);
-        acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        of = ex[u];
-        has = pairs[of][m];
-      }
-#pragma unroll
-      for (int j = 0; j < 4; j++) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[u].frag(j), as_bf16x8(xv[u][j]), acc, 0, 0, 0);
+    for (int j = 0; j < 4; j++) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[u].frag(j), operand(x, 0, j, drop), acc, 0, 0, 0);
+    if (++uk == per || s + 1 == s1) {
+      if (has >> m & 1) add4(sum, acc);
+      acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      uk = 0, uit = get(++ui);
     }
-  }
-  if (has >= 0) add4(sum, acc);
+  });
   f32x4_t all[1] = {sum};
+  __syncthreads();
   join<kDownWaves>(all);
   if (wave != 0 || m >= a.T) return;
   *(u32x2_t*)(a.y + (int64_t)m * a.K + n0 + 4 * q) = u32x2_t{pack_bf16x2(all[0][0], all[0][1]), pack_bf16x2(all[0][2], all[0][3])};
@@ -518,12 +701,18 @@ int launch_pad(const uint8_t* s, int64_t rows, int64_t K, uint8_t* out, hipStrea
 
 // ---- y = x W^T
 
+constexpr int kMaxFewLds = 144 * 1024;  // the tokens' rows (and up to 16 KB of sums)
+
 struct LinearPlan {
   int form, splits;  // form -1: few tokens
 };
 
+// waves of the kernel for few tokens: about four steps of 128 k each
+int few_waves(int64_t K) { return K <= 2048 ? 4 : K <= 4096 ? 8 : 16; }
+
 LinearPlan linear_plan(int64_t T, int64_t N, int64_t K) {
-  if (T <= kFew) return {-1, 1};
+  const int nw = few_waves(K);
+  if (T <= kFew && K <= (1 << 20) && nw * (int64_t)few_lds((int)T, (int)K, nw, 1) <= kMaxFewLds) return {-1, 1};
   const int64_t cus = smla_num_cus(), steps = (K + 127) / 128;
   const int form = T <= 32 ? 0 : T <= 64 ? 1 : T * N >= 128 * 512 * cus ? 3 : 2;
   const int64_t tiles = (T + kFormBM[form] - 1) / kFormBM[form] * ((N + kFormBN[form] - 1) / kFormBN[form]);
@@ -547,10 +736,15 @@ int check_linear_fp4(int64_t T, int64_t N, int64_t K) {
   return SMLA_OK;
 }
 
-template <int NW>
+
+template <int WT, int NW>
 int launch_linear_few(const void* x, int64_t ldx, const Matrix& w, int64_t T, int64_t N, int64_t K, void* y, int y_dtype, hipStream_t st) {
-  auto kern = y_dtype == SMLA_BF16 ? linear_few_kernel<NW, SMLA_BF16> : linear_few_kernel<NW, SMLA_F32>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)((N + 15) / 16)), dim3(64 * NW), 0, st, (const uint16_t*)x, ldx, w, (int)T, (int)N, (int)K, y);
+  const bool bf = y_dtype == SMLA_BF16;
+  auto kern = bf ? linear_few_kernel<WT, NW, SMLA_BF16> : linear_few_kernel<WT, NW, SMLA_F32>;
+  static std::atomic<uint64_t> attr[2] = {{0}, {0}};
+  if (hipError_t e = smla_set_dynamic_lds((const void*)kern, kMaxFewLds, attr[bf]); e != hipSuccess) return (int)e;
+  hipLaunchKernelGGL(kern, dim3((unsigned)((N + 15) / 16)), dim3(64 * NW), NW * few_lds((int)T, (int)K, NW, 1), st, (const uint16_t*)x, ldx, w,
+                     (int)T, (int)N, (int)K, y);
   SMLA_HIP_CHECK_LAUNCH();
   return SMLA_OK;
 }
@@ -565,8 +759,8 @@ int check_experts(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I) {
 }
 
 // the tile form by the pairs an expert has on average (-1: few tokens)
-int expert_form(int64_t T, int64_t k, int64_t E) {
-  if (T <= kFew) return -1;
+int expert_form(int64_t T, int64_t k, int64_t E, int64_t K) {
+  if (T <= kFew && kUpWaves * (int64_t)few_lds((int)T, (int)K, kUpWaves, 2) <= kMaxFewLds) return -1;
   const int64_t P = T * k, per = P / (E < P ? E : P);
   return per <= 24 ? 0 : per <= 48 ? 1 : 2;
 }
@@ -578,19 +772,36 @@ struct ExpertBytes {
 };
 ExpertBytes expert_bytes(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I, bool fp4) {
   const int64_t P = T * k;
-  const int form = expert_form(T, k, E);
+  const int form = expert_form(T, k, E, K);
   if (form < 0) return {0, 0, up16(2 * P * I), 0, 0, 0};
   return {up16(4 * P), up16(4 + 12 * max_tiles(P, E, kFormBM[form])), up16(2 * P * I), up16(4 * P * K),
           fp4 && K % 128 ? up16(E * I * padded_row(K)) : 0, fp4 && I % 128 ? up16(E * K * padded_row(I)) : 0};
 }
 
 template <int WT>
-int launch_few(const ExpertArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(few_up_kernel<WT>, dim3(a.I / 16, a.P), dim3(64 * kUpWaves), 0, st, a);
-  SMLA_HIP_CHECK_LAUNCH();
-  hipLaunchKernelGGL(few_down_kernel<WT>, dim3(a.K / 16), dim3(64 * kDownWaves), 0, st, a);
+int launch_few_up(const ExpertArgs& a, hipStream_t st) {
+  // rows for four times the tokens that an expert has on average, and two more
+  const int cap = (int)std::min<int64_t>(a.T, 4 * a.P / a.E + 2), lds = kUpWaves * few_lds(cap, a.K, kUpWaves, 2);
+  static std::atomic<uint64_t> attr{0};
+  if (hipError_t e = smla_set_dynamic_lds((const void*)few_up_kernel<WT>, kMaxFewLds, attr); e != hipSuccess) return (int)e;
+  hipLaunchKernelGGL(few_up_kernel<WT>, dim3(a.I / 16, a.P), dim3(64 * kUpWaves), lds, st, a, cap);
   SMLA_HIP_CHECK_LAUNCH();
   return SMLA_OK;
+}
+
+template <int WT>
+int launch_few_down(const ExpertArgs& a, hipStream_t st) {
+  static std::atomic<uint64_t> attr2{0};
+  if (hipError_t e = smla_set_dynamic_lds((const void*)few_down_kernel<WT>, kDownLds<WT>, attr2); e != hipSuccess) return (int)e;
+  hipLaunchKernelGGL(few_down_kernel<WT>, dim3(a.K / 16), dim3(64 * kDownWaves), kDownLds<WT>, st, a);
+  SMLA_HIP_CHECK_LAUNCH();
+  return SMLA_OK;
+}
+
+int launch_few(const ExpertArgs& a, bool fp4, hipStream_t st) {
+  int rc = !fp4 ? launch_few_up<kBf16>(a, st) : a.K % 128 ? launch_few_up<kFp4Odd>(a, st) : launch_few_up<kFp4>(a, st);
+  if (rc) return rc;
+  return !fp4 ? launch_few_down<kBf16>(a, st) : a.I % 128 ? launch_few_down<kFp4Odd>(a, st) : launch_few_down<kFp4>(a, st);
 }
 
 template <class L>
@@ -646,10 +857,13 @@ extern "C" int smla_linear_fp4(const void* x, int64_t ldx, const uint8_t* codes,
   const LinearPlan p = linear_plan(T, N, K);
   const Matrix w{codes, scales};
   if (p.form < 0) {
-    const int64_t steps = (K + 127) / 128;
-    return steps <= 16   ? launch_linear_few<4>(x, ldx, w, T, N, K, y, y_dtype, st)
-           : steps <= 32 ? launch_linear_few<8>(x, ldx, w, T, N, K, y, y_dtype, st)
-                         : launch_linear_few<16>(x, ldx, w, T, N, K, y, y_dtype, st);
+    const int nw = few_waves(K);
+#define SMLA_FEW(WT)                                                              \
+  (nw == 4   ? launch_linear_few<WT, 4>(x, ldx, w, T, N, K, y, y_dtype, st)     \
+   : nw == 8 ? launch_linear_few<WT, 8>(x, ldx, w, T, N, K, y, y_dtype, st)     \
+             : launch_linear_few<WT, 16>(x, ldx, w, T, N, K, y, y_dtype, st))
+    return K % 128 ? SMLA_FEW(kFp4Odd) : SMLA_FEW(kFp4);
+#undef SMLA_FEW
   }
   const LinearBytes b = linear_bytes(T, N, K);
   if (!usable_workspace(workspace, workspace_bytes, (size_t)(b.part + b.scales)) && b.part + b.scales > 0) return SMLA_E_WORKSPACE;
@@ -710,8 +924,8 @@ extern "C" int smla_experts(const void* x, int64_t ldx, const int32_t* ids, cons
   a.list = (int32_t*)take(b.list), a.at = (int32_t*)take(b.list), a.tiles = (int32_t*)take(b.tiles);
   a.h = (uint16_t*)take(b.h), a.part = (float*)take(b.part);
   hipStream_t st = (hipStream_t)stream;
-  const int form = expert_form(T, k, E);
-  if (form < 0) return fp4 ? launch_few<kFp4>(a, st) : launch_few<kBf16>(a, st);
+  const int form = expert_form(T, k, E, K);
+  if (form < 0) return launch_few(a, fp4, st);
   a.tile = kFormBM[form];
   if (b.up_scales) {
     for (Matrix* m : {&a.gate, &a.up}) {

@@ -1,5 +1,5 @@
 // Routing of tokens to experts (oracle/decode_engine.py:122-128: scores, the balance bias, the top-k, its
-// weights), one wave a token.
+// weights).
 //
 //   s_e = softmax | sigmoid | sqrt(softplus) of the logits;  r_e = s_e + bias_e
 //   a group of E / groups experts is worth the sum of its two largest r; the topk_groups best stay
@@ -7,7 +7,17 @@
 //
 // Ties go to the lowest id, and the order is that of the values and not of their fp32 roundings: two scores an
 // fp32 step apart would otherwise trade places with the formula's rounding.  Without a bias the scores' order
-// is the logits', which needs no scores.  A NaN ranks below everything.
+// is the logits', which needs no scores.  -inf and NaN rank last.
+//
+// route_kernel: 16 lanes a token, four tokens a wave, lane l holds experts l, l + 16, ..  A pick is a maximum over a lane's
+// values and four lane moves inside the row of 16 (DPP).  It ranks fp32 scores, whose error is below 2^-21 (1 + |r|)
+// (score32).  Where two neighbours of the order are closer than twice that (1 row in 300 of 256 random experts; never without
+// a bias), the k and the next one are put in the order of their float64 values; where that does not settle it, the last
+// group in and the first one out are as close, or anything is not finite, the whole wave ranks the token in float64
+// (rank_f64).  The weights are of float64 scores, of the k picked alone (softmax: the sum over the row is of fp32
+// exponentials).
+// What bounds it is issue: about 1300 instructions for four tokens of 256 experts.
+// route_f64_kernel: one token a wave in float64 throughout, for what the first does not take.
 #include "smla_internal.h"
 
 namespace {
@@ -36,30 +46,15 @@ __device__ inline double wave_max_f64(double v) {
 }
 
 template <int SCORE>
-__device__ inline double score_of(double x) {
+__device__ inline double score_f64(double x) {
   if constexpr (SCORE == SMLA_SCORE_SIGMOID) return 1.0 / (1.0 + exp(-x));
   else return sqrt(fmax(x, 0.0) + log1p(exp(-fabs(x))));
 }
 
-// the largest of the lanes' values v[0 .. V) (id lane + 64 i) and the lowest id that has it; NaN was replaced
-template <int V>
-__device__ inline int wave_argmax(const double (&v)[V], double& top) {
-  const int lane = threadIdx.x & 63;
-  double m = v[0];
-#pragma unroll
-  for (int i = 1; i < V; i++) m = fmax(m, v[i]);
-  top = wave_max_f64(m);
-  int id = 0x7fffffff;
-#pragma unroll
-  for (int i = V - 1; i >= 0; i--)
-    if (v[i] == top) id = lane + 64 * i;
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) id = min(id, __shfl_xor(id, o, 64));
-  return id;
-}
+constexpr double kOut = -__builtin_inf();  // not in the running
 
 // lane j < k: the j-th id and its score; then the shared experts
-__device__ inline void finish(const RouteArgs& a, int64_t t, int id, double w) {
+__device__ inline void finish_f64(const RouteArgs& a, int64_t t, int id, double w) {
   const int lane = threadIdx.x & 63, n = a.k + a.shared;
   if (a.renorm) {
     const double total = wave_sum_f64(lane < a.k ? w : 0.0);
@@ -71,36 +66,32 @@ __device__ inline void finish(const RouteArgs& a, int64_t t, int id, double w) {
   }
 }
 
-constexpr double kOut = -__builtin_inf();  // not in the running
-
+// One token in float64 by the whole wave: lane j < k gets the j-th id and its score.  lds: 128 V doubles.
 template <int XDT, int SCORE, int V>
-__global__ __launch_bounds__(64) void route_kernel(const RouteArgs a) {
-  const int lane = threadIdx.x;
-  const int64_t t = blockIdx.x;
-  double s[V], r[V];  // scores; ranking values
+__device__ inline void rank_f64(const RouteArgs& a, int64_t t, double* lds, int& mine, double& w) {
+  const int lane = threadIdx.x & 63;
+  double s[V], r[V];  // scores; logits
   bool have[V];
 #pragma unroll
   for (int i = 0; i < V; i++) {
     const int e = lane + 64 * i;
     have[i] = e < a.E;
-    const float x = have[i] ? load_as_f32(a.logits, t * a.ld + e, XDT) : -SMLA_INF;
-    s[i] = x;
+    r[i] = have[i] ? load_as_f32(a.logits, t * a.ld + e, XDT) : -SMLA_INF;
   }
   if constexpr (SCORE == SMLA_SCORE_SOFTMAX) {
-    double m = s[0];
+    double m = r[0];
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      m = fmax(m, s[i]);
-      nan |= s[i] != s[i];
+      m = fmax(m, r[i]);
+      nan |= r[i] != r[i];
     }
     m = wave_max_f64(m);
     nan = __any(nan);
     double sum = 0;
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      r[i] = s[i];
-      s[i] = m == kOut ? 0.0 : exp(s[i] - m);  // a row of -inf: every score 0
+      s[i] = m == kOut ? 0.0 : exp(r[i] - m);  // a row of -inf: every score 0
       sum += s[i];
     }
     sum = wave_sum_f64(sum);
@@ -108,31 +99,24 @@ __global__ __launch_bounds__(64) void route_kernel(const RouteArgs a) {
     for (int i = 0; i < V; i++) s[i] = nan ? __builtin_nan("") : sum > 0 ? s[i] / sum : sum;
   } else {
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-      r[i] = s[i];
-      s[i] = score_of<SCORE>(s[i]);
-    }
+    for (int i = 0; i < V; i++) s[i] = score_f64<SCORE>(r[i]);
   }
-  if (a.given) {  // no choice: the weights of these ids (0 outside 0 .. E-1)
-    __shared__ double sc[64 * V];
-#pragma unroll
-    for (int i = 0; i < V; i++) sc[lane + 64 * i] = s[i];
+  if (a.given) {
     __syncthreads();
-    const int id = lane < a.k ? a.given[t * a.k + lane] : -1;
-    finish(a, t, id, id >= 0 && id < a.E ? sc[id] : 0.0);
+#pragma unroll
+    for (int i = 0; i < V; i++) lds[lane + 64 * i] = s[i];
+    __syncthreads();
+    mine = lane < a.k ? a.given[t * a.k + lane] : -1;
+    w = mine >= 0 && mine < a.E ? lds[mine] : 0.0;
     return;
   }
-  // ranking values; NaN and what does not exist last
   double v[V];
 #pragma unroll
-  for (int i = 0; i < V; i++) {
-    const int e = lane + 64 * i;
-    v[i] = a.bias && have[i] ? s[i] + (double)a.bias[e] : s[i];
-    if (!a.bias && a.groups == 1) v[i] = r[i];
-  }
-  __shared__ double gv[1024], rank[1024];
+  for (int i = 0; i < V; i++) v[i] = a.bias && have[i] ? s[i] + (double)a.bias[lane + 64 * i] : s[i];
   if (a.groups > 1) {
+    double *rank = lds, *gv = lds + 64 * V;
     const int per = a.E / a.groups;
+    __syncthreads();  // (a workgroup is one wave)
 #pragma unroll
     for (int i = 0; i < V; i++)
       if (have[i]) rank[lane + 64 * i] = v[i] != v[i] ? kOut : v[i];
@@ -140,9 +124,9 @@ __global__ __launch_bounds__(64) void route_kernel(const RouteArgs a) {
     for (int g = lane; g < a.groups; g += 64) {
       double b0 = kOut, b1 = kOut;
       for (int j = 0; j < per; j++) {
-        const double w = rank[g * per + j];
-        if (w > b0) b1 = b0, b0 = w;
-        else if (w > b1) b1 = w;
+        const double x = rank[g * per + j];
+        if (x > b0) b1 = b0, b0 = x;
+        else if (x > b1) b1 = x;
       }
       const double sum = per > 1 ? b0 + b1 : b0;
       gv[g] = sum != sum ? kOut : sum;
@@ -150,35 +134,32 @@ __global__ __launch_bounds__(64) void route_kernel(const RouteArgs a) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      const int e = lane + 64 * i;
       if (!have[i]) continue;
-      const int g = e / per;
+      const int g = (lane + 64 * i) / per;
       int before = 0;  // groups ahead of this one
       for (int o = 0; o < a.groups; o++) before += gv[o] > gv[g] || (gv[o] == gv[g] && o < g);
-      if (!a.bias) v[i] = r[i];
       if (before >= a.topk_groups) have[i] = false;
     }
   }
-  // three classes: in the running, NaN or -inf in the running, out
-  bool low[V];
+  bool low[V];  // in the running, but -inf or NaN
 #pragma unroll
   for (int i = 0; i < V; i++) {
+    if (!a.bias) v[i] = r[i];
     low[i] = have[i] && !(v[i] > kOut);
     if (!have[i] || low[i]) v[i] = kOut;
   }
-  int mine = -1;        // lane j: the j-th id
-  double w = 0;
+  mine = -1, w = 0;
   for (int j = 0; j < a.k; j++) {
-    double top;
-    int id = wave_argmax<V>(v, top);
-    if (top == kOut) {  // only -inf and NaN are left: by id, -inf before NaN
-      id = 0x7fffffff;
+    double top = v[0];
 #pragma unroll
-      for (int i = V - 1; i >= 0; i--)
-        if (low[i]) id = lane + 64 * i;
+    for (int i = 1; i < V; i++) top = fmax(top, v[i]);
+    top = wave_max_f64(top);
+    int id = 0x7fffffff;
 #pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) id = min(id, __shfl_xor(id, o, 64));
-    }
+    for (int i = V - 1; i >= 0; i--)
+      if (top == kOut ? low[i] : v[i] == top) id = lane + 64 * i;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) id = min(id, __shfl_xor(id, o, 64));
     double sj = 0;
 #pragma unroll
     for (int i = 0; i < V; i++)
@@ -190,14 +171,258 @@ __global__ __launch_bounds__(64) void route_kernel(const RouteArgs a) {
     sj = __shfl(sj, id & 63, 64);
     if (lane == j) mine = id, w = sj;
   }
-  finish(a, t, mine, w);
+}
+
+template <int XDT, int SCORE, int V>
+__global__ __launch_bounds__(64) void route_f64_kernel(const RouteArgs a) {
+  __shared__ double lds[128 * V];
+  int id;
+  double w;
+  rank_f64<XDT, SCORE, V>(a, blockIdx.x, lds, id, w);
+  finish_f64(a, blockIdx.x, id, w);
+}
+
+// ---- 16 lanes a token
+
+// row-of-16 reductions, every lane gets the result
+template <class F>
+__device__ inline float row_reduce(float v, F&& f) {
+  v = f(v, dpp_f<0xB1>(v));
+  v = f(v, dpp_f<0x4E>(v));
+  v = f(v, dpp_f<0x141>(v));
+  return f(v, dpp_f<0x140>(v));
+}
+__device__ inline float row_max(float v) { return row_reduce(v, [](float x, float y) { return fmaxf(x, y); }); }
+__device__ inline float row_min(float v) { return row_reduce(v, [](float x, float y) { return fminf(x, y); }); }
+__device__ inline int row_min_i(int v) {
+  v = min(v, (int)dpp_u<0xB1>((uint32_t)v));
+  v = min(v, (int)dpp_u<0x4E>((uint32_t)v));
+  v = min(v, (int)dpp_u<0x141>((uint32_t)v));
+  return min(v, (int)dpp_u<0x140>((uint32_t)v));
+}
+__device__ inline double row_sum_f64(double v) {
+#pragma unroll
+  for (int o = 8; o >= 1; o >>= 1) v += __shfl_xor(v, o, 16);
+  return v;
+}
+
+// fp32 score, off by less than 2^-21 (1 + s): exp(-|x|) is off by (|x| + 4) 2^-23 of it (the argument's product, the
+// instruction), which times its share in s (at most s (1 - s) |x| < 1/4 for the sigmoid, e^(-|x|/2) |x| < 3/4 for the root)
+// stays below 2^-22; the quotient, the series and the root add a few 2^-24 of s.
+template <int SCORE>
+__device__ inline float score32(float x) {
+  const float t = __expf(-fabsf(x));
+  if constexpr (SCORE == SMLA_SCORE_SIGMOID) {
+    return (x >= 0.f ? 1.f : t) * __builtin_amdgcn_rcpf(1.f + t);
+  } else {
+    // log(1 + t) = 2 (z + z^3 / 3 + z^5 / 5 + ..), z = t / (2 + t) <= 1/3: the first term left out is below 2^-27
+    const float z = t * __builtin_amdgcn_rcpf(2.f + t), q = z * z;
+    float p = 1.f / 15.f;
+    p = fmaf(p, q, 1.f / 13.f);
+    p = fmaf(p, q, 1.f / 11.f);
+    p = fmaf(p, q, 1.f / 9.f);
+    p = fmaf(p, q, 1.f / 7.f);
+    p = fmaf(p, q, 1.f / 5.f);
+    p = fmaf(p, q, 1.f / 3.f);
+    p = fmaf(p, q, 1.f);
+    return __builtin_amdgcn_sqrtf(fmaf(2.f * z, p, fmaxf(x, 0.f)));
+  }
+}
+
+constexpr float kTol = 0x1p-20f;  // twice a score's error
+
+template <int XDT, int SCORE, int V>
+__global__ __launch_bounds__(64) void route_kernel(const RouteArgs a) {
+  constexpr int V64 = (V + 3) / 4;
+  __shared__ double lds[128 * V64];
+  const int lane = threadIdx.x, l = lane & 15;
+  const int64_t t0 = (int64_t)blockIdx.x * 4, row = min(t0 + (lane >> 4), a.T - 1);  // rows past the last repeat it
+  const int64_t at = row * a.ld;
+  float x[V], v[V];  // logits; ranking values
+#pragma unroll
+  for (int i = 0; i < V; i++) x[i] = load_as_f32(a.logits, at + min(l + 16 * i, a.E - 1), XDT);
+  float b[V];  // (read with the logits; clamped indexes and selects: a guard would put a branch around every load)
+  const bool add = a.bias && !a.given;
+  if (add) {
+#pragma unroll
+    for (int i = 0; i < V; i++) b[i] = a.bias[min(l + 16 * i, a.E - 1)];
+  }
+#pragma unroll
+  for (int i = 0; i < V; i++) x[i] = l + 16 * i < a.E ? x[i] : -SMLA_INF;
+  bool bad = false;  // this token is ranked in float64
+  float m = -SMLA_INF;
+  double sum = 1.0;
+  if constexpr (SCORE == SMLA_SCORE_SOFTMAX) {
+#pragma unroll
+    for (int i = 0; i < V; i++) m = fmaxf(m, x[i]);
+    m = row_max(m);
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      v[i] = expf(x[i] - m);
+      sum += v[i];
+    }
+    sum = row_sum_f64(sum);
+    bad = !(sum < SMLA_INF);  // a NaN, an infinite maximum
+    const float inv = (float)(1.0 / sum);
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] *= inv;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i++) bad |= x[i] != x[i];
+    if (a.bias || a.groups > 1) {
+#pragma unroll
+      for (int i = 0; i < V; i++) v[i] = score32<SCORE>(x[i]);
+    }
+  }
+  int mine = -1;
+  if (a.given) {
+    if (l < a.k) mine = a.given[row * a.k + l];
+    bad = __any(bad) && SCORE == SMLA_SCORE_SOFTMAX ? bad : false;  // else each id's score stands alone
+  } else {
+    if (add) {
+#pragma unroll
+      for (int i = 0; i < V; i++) v[i] = l + 16 * i < a.E ? v[i] + b[i] : -SMLA_INF;
+    }
+    uint32_t kept = 0xffffffffu;
+    const int spg = a.groups > 1 ? a.E / a.groups / 16 : V;  // values a lane holds of a group
+    if (a.groups > 1) {
+      float gv = -SMLA_INF, b0 = gv, b1 = gv;  // lane g: group g
+      int g = 0, left = spg;
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        b1 = fmaxf(b1, fminf(b0, v[i]));
+        b0 = fmaxf(b0, v[i]);
+        if (--left == 0) {  // uniform
+          float c0 = b0, c1 = b1;
+          auto merge = [&](float d0, float d1) {
+            c1 = fmaxf(fmaxf(c1, d1), fminf(c0, d0));
+            c0 = fmaxf(c0, d0);
+          };
+          merge(dpp_f<0xB1>(c0), dpp_f<0xB1>(c1));
+          merge(dpp_f<0x4E>(c0), dpp_f<0x4E>(c1));
+          merge(dpp_f<0x141>(c0), dpp_f<0x141>(c1));
+          merge(dpp_f<0x140>(c0), dpp_f<0x140>(c1));
+          if (l == g && g < a.groups) gv = c0 + c1;
+          g++, left = spg;
+          b0 = b1 = -SMLA_INF;
+        }
+      }
+      int before = 0;
+      auto beside = [&](float o, int og) { before += o > gv || (o == gv && og < l); };
+#define SMLA_ROR(n) beside(dpp_f<0x120 + n>(gv), (int)dpp_u<0x120 + n>((uint32_t)l));
+      SMLA_ROR(1) SMLA_ROR(2) SMLA_ROR(3) SMLA_ROR(4) SMLA_ROR(5) SMLA_ROR(6) SMLA_ROR(7) SMLA_ROR(8)
+      SMLA_ROR(9) SMLA_ROR(10) SMLA_ROR(11) SMLA_ROR(12) SMLA_ROR(13) SMLA_ROR(14) SMLA_ROR(15)
+#undef SMLA_ROR
+      const bool in = l < a.groups && before < a.topk_groups;
+      const float last = row_min(in ? gv : SMLA_INF), next = row_max(in ? -SMLA_INF : gv);
+      // (a group's value is the sum of two: twice the error)
+      if (a.topk_groups < a.groups) bad |= !(last - next > 2.f * kTol * (1.f + fabsf(last))) || !(last > -SMLA_INF);
+      kept = (uint32_t)(__ballot(in) >> (lane & 48)) & 0xffffu;
+    }
+    {
+      int left = spg;
+      uint32_t k = kept;
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        if (!a.bias) v[i] = x[i];
+        if (a.groups > 1) {
+          if (!(k & 1)) v[i] = -SMLA_INF;
+          if (--left == 0) k >>= 1, left = spg;
+        }
+      }
+    }
+    auto best = [&]() __attribute__((always_inline)) {
+      float top = v[0];
+#pragma unroll
+      for (int i = 1; i < V; i++) top = fmaxf(top, v[i]);
+      return row_max(top);
+    };
+    auto pick = [&](float top, int j) __attribute__((always_inline)) {  // its lowest id to lane j, out of the running
+      int id = 0x7fffffff;
+#pragma unroll
+      for (int i = V - 1; i >= 0; i--)
+        if (v[i] == top) id = l + 16 * i;
+      id = row_min_i(id);
+#pragma unroll
+      for (int i = 0; i < V; i++)
+        if (l + 16 * i == id) v[i] = -SMLA_INF;
+      if (l == j) mine = id;
+    };
+    bool close = false;  // neighbours in the order that fp32 cannot tell apart
+    float prev = SMLA_INF, top;
+    for (int j = 0;; j++) {
+      top = best();
+      if (a.bias && j > 0) close |= !(prev - top > kTol * (1.f + fabsf(prev)));
+      if (j == a.k) break;
+      bad |= !(top > -SMLA_INF);
+      pick(top, j);
+      prev = top;
+    }
+    if (__any(close)) {
+      // the k and the next one in the order of their float64 values, a lane each; the one after it has to be apart
+      if (SCORE != SMLA_SCORE_SOFTMAX && a.k < 16) {
+        pick(top, a.k);
+        const float after = best();
+        if (close) bad |= !(prev - after > kTol * (1.f + fabsf(prev))) || !(top > -SMLA_INF);
+        double r = kOut;
+        if (l <= a.k && mine < a.E) r = score_f64<SCORE>(load_as_f32(a.logits, at + mine, XDT)) + (double)a.bias[mine];
+        int place = 0;
+#pragma unroll
+        for (int o = 1; o < 16; o++) {
+          const int from = (lane & 48) + ((l + o) & 15), oid = __shfl(mine, from, 64);
+          const double other = __shfl(r, from, 64);
+          place += ((l + o) & 15) <= a.k && (other > r || (other == r && oid < mine));
+        }
+        int* ids = (int*)lds;
+        if (l <= a.k) ids[(lane & 48) + place] = mine;
+        __syncthreads();  // (one wave)
+        if (l <= a.k) mine = ids[lane];
+      } else {
+        bad |= close;
+      }
+    }
+  }
+  double w = 0;
+  if (l < a.k && mine >= 0 && mine < a.E) {
+    const float y = load_as_f32(a.logits, at + mine, XDT);
+    if constexpr (SCORE == SMLA_SCORE_SOFTMAX) w = exp((double)y - (double)m) / sum;
+    else w = score_f64<SCORE>(y);
+  }
+  if (a.renorm) {
+    const double total = row_sum_f64(l < a.k ? w : 0.0);
+    w = total > 0 ? w / total : total;  // all 0: 0
+  }
+  uint64_t again = __ballot(bad);
+  const int n = a.k + a.shared;
+  if (l < n && t0 + (lane >> 4) < a.T && !(again >> (lane & 48) & 0xffffu)) {
+    a.ids[row * n + l] = l < a.k ? mine : a.E + l - a.k;
+    a.weights[row * n + l] = l < a.k ? (float)(w * a.scale) : 1.f;
+  }
+  while (again) {
+    const int g = (__ffsll((unsigned long long)again) - 1) / 16;
+    again &= ~(0xffffull << (16 * g));
+    const int64_t t = t0 + g;
+    if (t >= a.T) break;
+    int id;
+    double ww;
+    rank_f64<XDT, SCORE, V64>(a, t, lds, id, ww);
+    finish_f64(a, t, id, ww);
+  }
 }
 
 template <int XDT, int SCORE>
 int launch_route(const RouteArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)a.T), blk(64);
-  if (a.E <= 256) hipLaunchKernelGGL((route_kernel<XDT, SCORE, 4>), grid, blk, 0, st, a);
-  else hipLaunchKernelGGL((route_kernel<XDT, SCORE, 16>), grid, blk, 0, st, a);
+  // 16 lanes a token: up to 32 values a lane, a lane for every group and every column, whole 16s in a group
+  const bool rows16 = a.E <= 512 && a.k + a.shared <= 16 &&
+                      (a.groups == 1 || a.given || (a.groups <= 16 && a.E / a.groups % 16 == 0));
+  const dim3 blk(64), grid((unsigned)(rows16 ? (a.T + 3) / 4 : a.T));
+  if (rows16 && a.E <= 64) hipLaunchKernelGGL((route_kernel<XDT, SCORE, 4>), grid, blk, 0, st, a);
+  else if (rows16 && a.E <= 128) hipLaunchKernelGGL((route_kernel<XDT, SCORE, 8>), grid, blk, 0, st, a);
+  else if (rows16 && a.E <= 256) hipLaunchKernelGGL((route_kernel<XDT, SCORE, 16>), grid, blk, 0, st, a);
+  else if (rows16) hipLaunchKernelGGL((route_kernel<XDT, SCORE, 32>), grid, blk, 0, st, a);
+  else if (a.E <= 256) hipLaunchKernelGGL((route_f64_kernel<XDT, SCORE, 4>), grid, blk, 0, st, a);
+  else hipLaunchKernelGGL((route_f64_kernel<XDT, SCORE, 16>), grid, blk, 0, st, a);
   SMLA_HIP_CHECK_LAUNCH();
   return SMLA_OK;
 }
