@@ -32,25 +32,28 @@ using smla_gemm::Int;
 
 constexpr int kFp4 = 0, kBf16 = 1;
 
-template <int WT_, int BM_, int BN_, int WM_, int WN_, int D_>
+template <int WT_, int BM_, int BN_, int WM_, int WN_, int D_, int KB_>
 struct Tile {
-  static constexpr int WT = WT_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, D = D_;
-  static constexpr int KB = WT == kFp4 ? 128 : 64, SUB = KB / 16;
+  static constexpr int WT = WT_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, D = D_, KB = KB_, SUB = KB / 16;
   static constexpr int XROW = 2 * KB, WROW = WT == kFp4 ? KB / 2 : 2 * KB;  // bytes of a row per step
   static constexpr int XC = XROW / 16, WC = WROW / 16;                        // chunks
   static constexpr int NWN = BN / WN, NW = (BM / WM) * NWN, MB = WM / 32, NB = WN / 32;
-  static constexpr int XB = BM * XROW, WB = BN * WROW, SB = WT == kFp4 ? BN * 4 : 0, STAGE = XB + WB + SB;
-  static constexpr int CX = XB / 1024 / NW, CW = WB / 1024 / NW, CP = CX + CW, CS = WT == kFp4 ? 1 : 0, CT = CP + CS;  // copies a wave and step
-  static constexpr int LDS = D * STAGE;
+  static constexpr int XB = BM * XROW, WB = BN * WROW, STAGE = XB + WB;
+  static constexpr int SG = WT == kFp4 ? BN * 16 : 0;  // a group of scales, 512 k
+  static constexpr int CX = XB / 1024 / NW, CW = WB / 1024 / NW, CP = CX + CW;  // copies a wave and step
+  static constexpr int GS = WT == kFp4 ? 512 / KB : 1, CS = WT == kFp4 ? 4 / GS : 0, CT = CP + CS;  // steps of a group of scales
+  static constexpr int LDS = D * STAGE + 3 * SG;
   static constexpr int THREADS = 64 * NW;
-  static_assert(CX * NW * 1024 == XB && CW * NW * 1024 == WB && BN % 128 == 0 && BN / 64 <= NW && (WN == 64 || WN == 128), "whole copies per wave");
-  static __device__ int swx(int r) { return WT == kFp4 ? r & 15 : (r >> 1) & 7; }
-  static __device__ int sww(int r) { return WT == kFp4 ? (r >> 2) & 3 : (r >> 1) & 7; }
+  static_assert(CX * NW * 1024 == XB && CW * NW * 1024 == WB && BN % 64 == 0 && (WN == 64 || (WN == 128 && BM == 2 * WM)), "whole copies per wave");
+  static_assert((WT == kFp4 ? KB == 128 || KB == 256 : KB == 64) && D >= 2, "a step");
+  static __device__ int swx(int r) { return XROW >= 256 ? r & 15 : (r >> 1) & 7; }
+  static __device__ int sww(int r) { return WROW == 64 ? (r >> 2) & 3 : (r >> 1) & 7; }
 };
 
-// 4-byte copy for every lane (lane l lands at lds_dst + 4 l), addresses as dma16_s
+// 4-byte copy for every lane (lane l lands at lds_dst + 4 l), addresses as dma16_s (the s_nop: a base that a vector
+// instruction has just written, v_readfirstlane, is read five wait states later at the earliest)
 __device__ inline void dma4_s(const uint8_t* base, uint32_t off, uint32_t lds_dst) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_dst), "v"(off), "s"(base) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_dst), "v"(off), "s"(base) : "memory", "m0");
 }
 
 // a value that every lane of the wave has, in a scalar register (the copies' addresses need one)
@@ -77,7 +80,6 @@ template <class L, int MBV, class XO, class WR, class WH>
 __device__ __attribute__((always_inline)) inline void tile_loop(lds_u8_t* lds, const Source& src, int steps, XO&& xoff, WR&& wrow,
                                                                 WH&& whalf, f32x16_t (&acc)[MBV > 0 ? MBV : 1][L::NB]) {
   constexpr int NB = L::NB, NM = MBV * NB, D = L::D, SUB = L::SUB, CT = L::CT;
-  constexpr int CQ = (CT + 3) / 4;  // copies a sub-step: a step's go out in sub-step SUB - 1 and the three after
   const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / L::NWN, wn = wave % L::NWN;
@@ -100,12 +102,22 @@ __device__ __attribute__((always_inline)) inline void tile_loop(lds_u8_t* lds, c
     off[L::CX + i] = row + 16 * c;
     off0[L::CX + i] = row + max(16 * c, L::WT == kFp4 ? src.pad / 2 : 2 * src.pad);
   }
-  // scales: a wave copies those of 64 rows, 32 of each of two waves' and of one half (one base address); row r's stand
-  // at place 64 (2 (r / 128) + r / 32 mod 2) + 32 (r / 64 mod 2) + r mod 32 (wider waves: at r)
-  const int su = wave % (L::BN / 64);
-  const int sr = L::WN == 64 ? 128 * (su / 2) + 64 * (lane >> 5) + 32 * (su & 1) + (lane & 31) : 64 * su + lane;
-  const uint8_t* sb = uniform(L::WT == kFp4 ? (whalf(L::WN == 64 ? 32 * (su & 1) : 0) ? src.s[1] : src.s[0]) : src.x);
-  const uint32_t so = (uint32_t)wrow(sr) * src.lds;
+  // scales: 512 k of a row are 16 bytes (a step's four alone, 64 rows a request, took as many requests as all the
+  // weights).  With a step's copies a wave requests those of 16 (KB = 256: 32) of its rows for the group behind the
+  // step's, so that a group is there when its first step is; three groups in LDS.
+  const int su = L::WN == 64 ? 64 * wn : 64 * (2 * wn + wm);
+  uint32_t so0 = (uint32_t)wrow(su + (lane >> 2)) * src.lds, so1 = (uint32_t)wrow(su + 16 + (lane >> 2)) * src.lds,
+           so2 = (uint32_t)wrow(su + 32 + (lane >> 2)) * src.lds, so3 = (uint32_t)wrow(su + 48 + (lane >> 2)) * src.lds;
+  asm volatile("" : "+v"(so0), "+v"(so1), "+v"(so2), "+v"(so3));  // (four registers, not an array in scratch memory)
+  const uint8_t* sb[2] = {uniform(L::WT == kFp4 ? src.s[0] : src.x), uniform(L::WT == kFp4 ? src.s[1] : src.x)};
+  const uint32_t sl = lds_base + D * L::STAGE + 16 * su;
+  const int lack = src.pad / 128, words = nk * (L::KB / 128) - lack;  // a row's groups of 128 k: those of the pad are not there
+  auto copy_scales = [&](int part, int of) __attribute__((always_inline)) {
+    const int j = __builtin_amdgcn_readfirstlane(part), group = __builtin_amdgcn_readfirstlane(of);  // (scalar registers for the copy)
+    const int w = min(max(4 * group + (lane & 3) - lack, 0), words - 1);
+    const uint32_t o = (j == 0 ? so0 : j == 1 ? so1 : j == 2 ? so2 : so3) + 4 * w;
+    dma4_s(whalf(su + 16 * j) ? sb[1] : sb[0], o, sl + (group % 3) * L::SG + 256 * j);
+  };
   auto copy_to = [&](int ks, int stage, int i, bool head) __attribute__((always_inline)) {
     const uint32_t st = lds_base + stage * L::STAGE;
     if (i < L::CP) {
@@ -113,17 +125,17 @@ __device__ __attribute__((always_inline)) inline void tile_loop(lds_u8_t* lds, c
       const int q = i < L::CX ? wave * L::CX + i : L::XB / 1024 + wave * L::CW + i - L::CX;
       smla_gemm::dma16_s(base, head ? off0[i] : off[i], st + q * 1024);
     } else {
-      dma4_s(sb + (int64_t)ks * 4, so, st + L::XB + L::WB + 256 * su);
+      copy_scales(ks % L::GS * L::CS + i - L::CP, ks / L::GS + 1);
     }
   };
   auto copy = [&](int ks, int i) __attribute__((always_inline)) { copy_to(ks, ks % D, i, false); };
   // operands: a of this lane's row, chunks as above; raw: 32 codes and their scale, or nothing
   const int r32 = lane & 31, h = lane >> 5, sx = L::swx(r32), sw = L::sww(r32);
   const uint32_t xrow = (L::WM * wm + r32) * L::XROW, wrw = L::XB + (L::WN * wn + r32) * L::WROW,
-                 srow = L::XB + L::WB + (L::WN == 64 ? 128 * (wn / 2) + 32 * (wn % 2) + r32 : L::WN * wn + r32) * 4 + h;
+                 srow = D * L::STAGE + (L::WN * wn + r32) * 16;
   bf16x8_t a[2][MBV > 0 ? MBV : 1], b[2][NB];
   u32x4_t raw[2][NB];
-  uint32_t rs[2][NB];
+  uint32_t rs[2 * NB];  // a step's scale bytes, of its first 128 k and of its second
   auto read_a = [&](int ks, int kk, int m) __attribute__((always_inline)) {
     const lds_u8_t* p = lds + (ks % D) * L::STAGE + 16 * ((8 * (kk / 4) + 4 * h + kk % 4) ^ sx) + xrow + 32 * L::XROW * m;
     a[kk & 1][m] = as_bf16x8(*(const lds_u32x4_t*)p);
@@ -133,13 +145,18 @@ __device__ __attribute__((always_inline)) inline void tile_loop(lds_u8_t* lds, c
     if constexpr (L::WT == kFp4) {
       const int g = kk / 4;
       raw[g & 1][n] = *(const lds_u32x4_t*)(st + wrw + 32 * L::WROW * n + 16 * ((2 * g + h) ^ sw));
-      rs[g & 1][n] = *(st + srow + (L::WN == 64 ? 256 : 128) * n + 2 * g);
+      if (g == 0) {
+        const lds_u8_t* at = lds + srow + 512 * n + (ks / L::GS % 3) * L::SG + ks % L::GS * (16 / L::GS);
+        rs[n] = *(const smla_attn::lds_i32_t*)at;
+        if constexpr (L::KB == 256) rs[NB + n] = *(const smla_attn::lds_i32_t*)(at + 4);
+      }
     } else {
       b[kk & 1][n] = as_bf16x8(*(const lds_u32x4_t*)(st + wrw + 32 * L::WROW * n + 16 * ((4 * h + kk) ^ sw)));
     }
   };
   auto convert = [&](int kk, int n) __attribute__((always_inline)) {
-    if constexpr (L::WT == kFp4) b[kk & 1][n] = smla_fp4::to_bf16(raw[(kk / 4) & 1][n][kk % 4], smla_fp4::scale_of(rs[(kk / 4) & 1][n]));
+    if constexpr (L::WT == kFp4)
+      b[kk & 1][n] = smla_fp4::to_bf16(raw[(kk / 4) & 1][n][kk % 4], smla_fp4::scale_of(rs[kk / 8 * NB + n] >> (8 * h + kk / 4 % 2 * 16) & 255));
   };
   // the products of sub-step kk, with what comes between them: the operands of sub-step (ns, nkk) (nkk < 0: none), raw
   // codes of group (gs, gk) (gk < 0: none), copies i0 .. i1-1 of step `is`
@@ -171,22 +188,20 @@ __device__ __attribute__((always_inline)) inline void tile_loop(lds_u8_t* lds, c
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  constexpr int C0 = CQ < CT ? CQ : CT, C1 = 2 * CQ < CT ? 2 * CQ : CT, C2 = 3 * CQ < CT ? 3 * CQ : CT;
+  // copy i of a step goes out in part i NSP / CT of them: part 0 in sub-step SUB - 1, part p in sub-step p - 1 of the next step
+  constexpr int NSP = SUB >= 8 ? SUB / 2 : 4, C0 = CT / NSP;
   // step ks: MORE: the rest of step ks + D - 1's copies goes out; FIRST: the first part of step ks + D's; NEXT: a step follows
   auto step = [&](int ks, auto more_, auto first_, auto next_) __attribute__((always_inline)) {
     constexpr int more = decltype(more_)::value, first = decltype(first_)::value, next = decltype(next_)::value;
-    const int is = ks + D - 1;
-    sub(Int<0>{}, ks, Int<1>{}, ks, Int<SUB == 8 ? 4 : -1>{}, is, Int<C0>{}, Int<more ? C1 : C0>{});
-    sub(Int<1>{}, ks, Int<2>{}, 0, Int<-1>{}, is, Int<C1>{}, Int<more ? C2 : C1>{});
-    if constexpr (SUB == 4) {
-      sub(Int<2>{}, ks, Int<3>{}, 0, Int<-1>{}, is, Int<C2>{}, Int<more ? CT : C2>{});
-    } else {
-      sub(Int<2>{}, ks, Int<3>{}, 0, Int<-1>{}, is, Int<C2>{}, Int<more ? CT : C2>{});
-      sub(Int<3>{}, ks, Int<4>{}, 0, Int<-1>{}, 0, Int<0>{}, Int<0>{});
-      sub(Int<4>{}, ks, Int<5>{}, 0, Int<-1>{}, 0, Int<0>{}, Int<0>{});
-      sub(Int<5>{}, ks, Int<6>{}, 0, Int<-1>{}, 0, Int<0>{}, Int<0>{});
-      sub(Int<6>{}, ks, Int<7>{}, 0, Int<-1>{}, 0, Int<0>{}, Int<0>{});
-    }
+    auto subs = [&](auto self, auto kk_) __attribute__((always_inline)) {
+      constexpr int kk = decltype(kk_)::value, p = kk + 1;
+      if constexpr (kk < SUB - 1) {
+        constexpr int i0 = more && p < NSP ? p * CT / NSP : 0, i1 = more && p < NSP ? (p + 1) * CT / NSP : 0;
+        sub(Int<kk>{}, ks, Int<kk + 1>{}, ks, Int<kk % 4 == 0 && kk + 4 < SUB ? kk + 4 : -1>{}, ks + D - 1, Int<i0>{}, Int<i1>{});
+        self(self, Int<kk + 1>{});
+      }
+    };
+    subs(subs, Int<0>{});
     if constexpr (next) {
       wait_vm(more ? (D - 2) * CT : 0);  // this wave's copies of step ks + 1
       lds_barrier();                      // everyone's; and step ks is in every wave's registers
@@ -201,6 +216,8 @@ __device__ __attribute__((always_inline)) inline void tile_loop(lds_u8_t* lds, c
     for (int n = 0; n < NB; n++)
 #pragma unroll
       for (int r = 0; r < 16; r++) acc[m][n][r] = 0.f;
+#pragma unroll
+  for (int j = 0; j < (L::WT == kFp4 ? 4 : 0); j++) copy_scales(j, 0);
 #pragma unroll
   for (int s = 0; s < D; s++)
 #pragma unroll

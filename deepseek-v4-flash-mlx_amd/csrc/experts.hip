@@ -221,8 +221,8 @@ struct ExpertArgs {
   float limit;           // infinity: none
   int32_t* list;         // pairs by expert
   int32_t* at;           // a pair's place in it
-  int32_t* tiles;        // [0] their number, then (expert, first place, pairs) each
-  int tile;              // pairs of a tile at most
+  int32_t* tiles;        // [8] their numbers, then for each XCD `room` of (expert, first place, pairs)
+  int tile, room;        // pairs of a tile at most
   uint16_t* h;           // [P, I] hidden rows, by place (few tokens: by pair)
   float* part;           // [P, K] their products, by place
   uint16_t* y;
@@ -457,47 +457,83 @@ __global__ __launch_bounds__(64 * kDownWaves) void few_down_kernel(const ExpertA
   *(u32x2_t*)(a.y + (int64_t)m * a.K + n0 + 4 * q) = u32x2_t{pack_bf16x2(all[0][0], all[0][1]), pack_bf16x2(all[0][2], all[0][3])};
 }
 
-// ---- more tokens: the pairs (token, choice) sorted by expert, in tiles of one expert's.  The order within an expert is
-// as it comes; no result depends on it.
+// ---- more tokens: the pairs (token, choice) sorted by expert, in tiles of one expert's pairs.
+
+template <class F>
+__device__ inline void each_pair(const ExpertArgs& a, F&& f) {
+  constexpr int U = 12;  // ids in flight a thread (one after the other: 33 us for 4096 tokens of 6, against 24)
+  for (int p0 = threadIdx.x; p0 < a.P; p0 += 1024 * U) {
+    int e[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) e[u] = a.ids[min(p0 + 1024 * u, a.P - 1)];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (p0 + 1024 * u < a.P) f(p0 + 1024 * u, e[u]);
+  }
+}
+
+// An expert's pairs go to tiles by twos, which share its weights in an XCD's L2.  Such units go to the XCDs in turn, the
+// longest first: every XCD has as many of each length (tiles in the experts' order, an eighth of them an XCD, left one with
+// up to a sixth more to do than the others; the short ones last fill the end).  The order within an expert and among units of
+// a length is as it comes; no result depends on it.
+constexpr int kMaxPairs = 1 << 20;
+constexpr int kMaxUnits = kMaxPairs / 256 + kMaxExperts;  // (tiles of 32 pairs are taken for 32 an expert and less)
 __global__ __launch_bounds__(1024) void plan_kernel(const ExpertArgs a) {
-  __shared__ int cnt[kMaxExperts], at[kMaxExperts], tile[kMaxExperts];
-  const int tid = threadIdx.x;
+  __shared__ int cnt[kMaxExperts], part[16], length[16], units_of[16];
+  __shared__ int unit_at[kMaxUnits], unit[kMaxUnits];  // first place; expert | pairs << 10
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   cnt[tid] = 0;
+  if (tid < 16) length[tid] = units_of[tid] = 0;
   __syncthreads();
-  for (int p = tid; p < a.P; p += 1024) {
-    const int e = a.ids[p];
+  each_pair(a, [&](int, int e) {
     if (e >= 0 && e < a.E) atomicAdd(&cnt[e], 1);
+  });
+  __syncthreads();
+  const int n = cnt[tid], upto = wave_incl_scan(n);
+  if (lane == 63) part[wave] = upto;
+  // units by their length in 32s (1 .. most)
+  const int most = 2 * a.tile / 32, whole = n / (2 * a.tile), rest = n - whole * 2 * a.tile, of_rest = (rest + 31) / 32;
+  if (whole) atomicAdd(&length[most], whole);
+  if (rest) atomicAdd(&length[of_rest], 1);
+  __syncthreads();
+  int first = upto - n;
+  for (int v = 0; v < wave; v++) first += part[v];
+  auto place = [&](int len, int many) {
+    int at = atomicAdd(&units_of[len], many);
+    for (int l = len + 1; l <= most; l++) at += length[l];
+    return at;
+  };
+  if (whole) {
+    const int at = place(most, whole);
+    for (int i = 0; i < whole; i++) unit_at[at + i] = first + 2 * a.tile * i, unit[at + i] = tid | (2 * a.tile) << 10;
   }
-  __syncthreads();
-  const int n = cnt[tid], nt = (n + a.tile - 1) / a.tile;
-  at[tid] = n, tile[tid] = nt;
-  __syncthreads();
-  for (int o = 1; o < 1024; o *= 2) {  // inclusive sums
-    const int u = tid >= o ? at[tid - o] : 0, v = tid >= o ? tile[tid - o] : 0;
-    __syncthreads();
-    at[tid] += u, tile[tid] += v;
-    __syncthreads();
+  if (rest) {
+    const int at = place(of_rest, 1);
+    unit_at[at] = first + n - rest, unit[at] = tid | rest << 10;
   }
-  const int first = at[tid] - n, t0 = tile[tid] - nt;
-  if (tid == 1023) a.tiles[0] = tile[tid];
-  for (int i = 0; i < nt; i++) {
-    a.tiles[1 + 3 * (t0 + i)] = tid;
-    a.tiles[2 + 3 * (t0 + i)] = first + i * a.tile;
-    a.tiles[3 + 3 * (t0 + i)] = min(a.tile, n - i * a.tile);
-  }
+  cnt[tid] = first;
   __syncthreads();
-  at[tid] = first;
-  __syncthreads();
-  for (int p = tid; p < a.P; p += 1024) {
-    const int e = a.ids[p];
-    if (e >= 0 && e < a.E) {
-      const int i = atomicAdd(&at[e], 1);
-      a.list[i] = p;
-      a.at[p] = i;
-    } else {
-      a.at[p] = -1;
+  if (wave < kXcds) {  // an XCD's tiles
+    int units = 0, base = 0;
+    for (int l = 1; l <= most; l++) units += length[l];
+    for (int u0 = 0; kXcds * u0 < units; u0 += 64) {
+      const int u = kXcds * (u0 + lane) + wave;
+      const int what = u < units ? unit[u] : 0, pairs = what >> 10, tiles = (pairs + a.tile - 1) / a.tile;
+      const int to = base + wave_incl_scan(tiles) - tiles;
+      for (int i = 0; i < tiles; i++) {
+        int32_t* t = a.tiles + 8 + 3 * ((int64_t)wave * a.room + to + i);
+        t[0] = what & 1023, t[1] = unit_at[u] + i * a.tile, t[2] = min(a.tile, pairs - i * a.tile);
+      }
+      base = __shfl(to + tiles, 63, 64);
     }
+    if (lane == 0) a.tiles[wave] = base;
   }
+  each_pair(a, [&](int p, int e) {
+    const bool real = e >= 0 && e < a.E;
+    const int i = real ? atomicAdd(&cnt[e], 1) : -1;
+    if (real) a.list[i] = p;
+    a.at[p] = i;
+  });
 }
 
 // y[t] = the sum of its pairs' rows, in their order
@@ -552,20 +588,14 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ p
 template <int WT, int FORM>
 struct Form;
 template <>
-struct Form<kFp4, 0> : smla_tile::Tile<kFp4, 32, 256, 32, 64, 3> {};  // 75 KB, 4 waves: two workgroups a CU
+struct Form<kFp4, 0> : smla_tile::Tile<kFp4, 32, 256, 32, 64, 3, 256> {};  // 156 KB, 4 waves
 template <>
-struct Form<kFp4, 1> : smla_tile::Tile<kFp4, 64, 128, 32, 64, 3> {};  // 74 KB, 4 waves
+struct Form<kFp4, 1> : smla_tile::Tile<kFp4, 128, 512, 64, 128, 2, 128> {};  // 152 KB, 8 waves
 template <>
-struct Form<kFp4, 2> : smla_tile::Tile<kFp4, 128, 256, 64, 64, 3> {};  // 147 KB, 8 waves
+struct Form<kBf16, 0> : smla_tile::Tile<kBf16, 32, 256, 32, 64, 4, 64> {};  // 144 KB, 4 waves
 template <>
-struct Form<kFp4, 3> : smla_tile::Tile<kFp4, 128, 512, 64, 128, 2> {};  // 132 KB, 8 waves
-template <>
-struct Form<kBf16, 0> : smla_tile::Tile<kBf16, 32, 256, 32, 64, 4> {};  // 144 KB, 4 waves
-template <>
-struct Form<kBf16, 1> : smla_tile::Tile<kBf16, 64, 128, 32, 64, 3> {};  // 72 KB, 4 waves
-template <>
-struct Form<kBf16, 2> : smla_tile::Tile<kBf16, 128, 256, 64, 64, 3> {};  // 144 KB, 8 waves
-constexpr int kFormBM[4] = {32, 64, 128, 128}, kFormBN[4] = {256, 128, 256, 512};
+struct Form<kBf16, 1> : smla_tile::Tile<kBf16, 128, 256, 64, 64, 3, 64> {};  // 144 KB, 8 waves
+constexpr int kFormBM[2] = {32, 128}, kFormBN[2] = {256, 512}, kFormKB[2] = {256, 128};  // (kFp4)
 
 constexpr int kLinear = 0, kUp = 1, kDown = 2;
 
@@ -582,6 +612,7 @@ struct TileArgs {
   int vec;
   // kUp, kDown
   const int32_t* tiles;
+  int room;
   const int32_t* list;
   const float* weights;
   int k;
@@ -640,7 +671,7 @@ __global__ __launch_bounds__(L::THREADS) void tile_kernel(const TileArgs a) {
     nk = steps * (sp + 1) / a.splits - s0;
     const smla_tile::Source src{a.x + first * a.ldx + (int64_t)s0 * L::XROW - 2 * pad,
                                 {a.w[0].w + (int64_t)n0 * (a.K * L::WROW / L::KB) + (int64_t)s0 * L::WROW - pad * L::WROW / L::KB, nullptr},
-                                {a.w[0].s + (int64_t)n0 * a.lds + 4 * s0, nullptr},
+                                {a.w[0].s + (int64_t)n0 * a.lds + (s0 ? 4 * (s0 * (L::KB / 128) - pad / 128) : 0), nullptr},
                                 (uint32_t)(a.K * L::WROW / L::KB), (uint32_t)a.lds, s0 == 0 ? pad : 0};
     uint8_t* y = a.y + (sp * a.split_stride + first * a.ldy) * (YDT == SMLA_BF16 ? 2 : 4);
     const int mine = rows - L::WM * (wave / L::NWN);
@@ -648,10 +679,10 @@ __global__ __launch_bounds__(L::THREADS) void tile_kernel(const TileArgs a) {
     else if (mine <= 0) tile_body<L, MODE, YDT, 0>(a, lds, src, nk, rows, n0, y, tok, wt);
     else if constexpr (L::MB == 2) tile_body<L, MODE, YDT, 1>(a, lds, src, nk, rows, n0, y, tok, wt);
   } else {
-    const uint32_t ntn = (a.N + BNO - 1) / BNO, tot = a.tiles[0] * ntn, id = smla_tile::xcd_run(tot);
-    if (id >= tot) return;
-    const uint32_t tile = id / ntn;
-    const int32_t* tl = a.tiles + 1 + 3 * tile;
+    // workgroups are dealt to the XCDs in turn: this XCD's tiles, all of a tile's columns one after the other
+    const uint32_t ntn = (a.N + BNO - 1) / BNO, xcd = blockIdx.x % kXcds, id = blockIdx.x / kXcds, tile = id / ntn;
+    if (tile >= (uint32_t)a.tiles[xcd]) return;
+    const int32_t* tl = a.tiles + 8 + 3 * (xcd * a.room + tile);
     e = tl[0], first = tl[1], rows = tl[2];
     n0 = (id - tile * ntn) * BNO;
     if constexpr (MODE == kUp) {
@@ -713,8 +744,8 @@ int few_waves(int64_t K) { return K <= 2048 ? 4 : K <= 4096 ? 8 : 16; }
 LinearPlan linear_plan(int64_t T, int64_t N, int64_t K) {
   const int nw = few_waves(K);
   if (T <= kFew && K <= (1 << 20) && nw * (int64_t)few_lds((int)T, (int)K, nw, 1) <= kMaxFewLds) return {-1, 1};
-  const int64_t cus = smla_num_cus(), steps = (K + 127) / 128;
-  const int form = T <= 32 ? 0 : T <= 64 ? 1 : T * N >= 128 * 512 * cus ? 3 : 2;
+  const int form = T <= 32 ? 0 : 1;
+  const int64_t cus = smla_num_cus(), steps = (K + kFormKB[form] - 1) / kFormKB[form];
   const int64_t tiles = (T + kFormBM[form] - 1) / kFormBM[form] * ((N + kFormBN[form] - 1) / kFormBN[form]);
   int64_t splits = 1;
   while (splits < 8 && tiles * splits * 2 <= cus && steps / (splits * 2) >= 4) splits *= 2;
@@ -753,7 +784,7 @@ int launch_linear_few(const void* x, int64_t ldx, const Matrix& w, int64_t T, in
 
 int check_experts(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I) {
   if (T <= 0 || k <= 0 || E <= 0 || K <= 0 || I <= 0) return SMLA_E_SHAPE;
-  if (K % 32 != 0 || I % 32 != 0 || E > kMaxExperts || k > kMaxChoices || K > (1 << 20) || I > (1 << 20) || T > (1 << 20) / k)
+  if (K % 32 != 0 || I % 32 != 0 || E > kMaxExperts || k > kMaxChoices || K > (1 << 20) || I > (1 << 20) || T > kMaxPairs / k)
     return SMLA_E_UNSUPPORTED;
   return SMLA_OK;
 }
@@ -762,9 +793,10 @@ int check_experts(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I) {
 int expert_form(int64_t T, int64_t k, int64_t E, int64_t K) {
   if (T <= kFew && kUpWaves * (int64_t)few_lds((int)T, (int)K, kUpWaves, 2) <= kMaxFewLds) return -1;
   const int64_t P = T * k, per = P / (E < P ? E : P);
-  return per <= 24 ? 0 : per <= 48 ? 1 : 2;
+  return per <= 32 ? 0 : 1;
 }
-int64_t max_tiles(int64_t P, int64_t E, int tile) { return P / tile + (E < P ? E : P); }
+// an XCD's tiles at most: units of one length are shared out evenly (plan_kernel)
+int64_t room_of(int64_t P, int64_t E, int tile) { return (P / tile + (E < P ? E : P)) / kXcds + 3; }
 
 struct ExpertBytes {
   int64_t list, tiles, h, part, up_scales, down_scales;
@@ -774,7 +806,7 @@ ExpertBytes expert_bytes(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I, 
   const int64_t P = T * k;
   const int form = expert_form(T, k, E, K);
   if (form < 0) return {0, 0, up16(2 * P * I), 0, 0, 0};
-  return {up16(4 * P), up16(4 + 12 * max_tiles(P, E, kFormBM[form])), up16(2 * P * I), up16(4 * P * K),
+  return {up16(4 * P), up16(32 + 12 * kXcds * room_of(P, E, kFormBM[form])), up16(2 * P * I), up16(4 * P * K),
           fp4 && K % 128 ? up16(E * I * padded_row(K)) : 0, fp4 && I % 128 ? up16(E * K * padded_row(I)) : 0};
 }
 
@@ -806,24 +838,21 @@ int launch_few(const ExpertArgs& a, bool fp4, hipStream_t st) {
 
 template <class L>
 int launch_tiles(const ExpertArgs& a, int64_t up_lds, int64_t down_lds, hipStream_t st) {
-  const int64_t nt = max_tiles(a.P, a.E, a.tile);
+  const int64_t nt = kXcds * (int64_t)a.room;
   const TileArgs up{(const uint8_t*)a.x, 2 * a.ldx, {a.gate, a.up}, up_lds, a.K, a.I, 0, 0, 0, 0, (uint8_t*)a.h, a.I, 0, 1,
-                    a.tiles, a.list, a.weights, a.k, a.limit};
-  // (a run of workgroups a XCD: room for each XCD's share rounded up)
-  int rc = launch_tile<L, kUp, SMLA_BF16>(up, nt * ((a.I + L::BN / 2 - 1) / (L::BN / 2)) + kXcds, st);
+                    a.tiles, a.room, a.list, a.weights, a.k, a.limit};
+  const int rc = launch_tile<L, kUp, SMLA_BF16>(up, nt * ((a.I + L::BN / 2 - 1) / (L::BN / 2)), st);
   if (rc) return rc;
   const TileArgs down{(const uint8_t*)a.h, 2 * (int64_t)a.I, {a.down, a.down}, down_lds, a.I, a.K, 0, 0, 0, 0, (uint8_t*)a.part, a.K, 0, 1,
-                      a.tiles, a.list, a.weights, a.k, a.limit};
-  return launch_tile<L, kDown, SMLA_F32>(down, nt * ((a.K + L::BN - 1) / L::BN) + kXcds, st);
+                      a.tiles, a.room, a.list, a.weights, a.k, a.limit};
+  return launch_tile<L, kDown, SMLA_F32>(down, nt * ((a.K + L::BN - 1) / L::BN), st);
 }
 
 template <int WT>
 int launch_many(const ExpertArgs& a, int form, int64_t up_lds, int64_t down_lds, hipStream_t st) {
   hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, a);
   SMLA_HIP_CHECK_LAUNCH();
-  const int rc = form == 0   ? launch_tiles<Form<WT, 0>>(a, up_lds, down_lds, st)
-                 : form == 1 ? launch_tiles<Form<WT, 1>>(a, up_lds, down_lds, st)
-                             : launch_tiles<Form<WT, 2>>(a, up_lds, down_lds, st);
+  const int rc = form == 0 ? launch_tiles<Form<WT, 0>>(a, up_lds, down_lds, st) : launch_tiles<Form<WT, 1>>(a, up_lds, down_lds, st);
   if (rc) return rc;
   for (int64_t t0 = 0; t0 < a.T; t0 += 65535) {
     ExpertArgs c = a;
@@ -876,12 +905,12 @@ extern "C" int smla_linear_fp4(const void* x, int64_t ldx, const uint8_t* codes,
   const int64_t nt = (T + kFormBM[p.form] - 1) / kFormBM[p.form], nn = (N + kFormBN[p.form] - 1) / kFormBN[p.form];
   const int odt = p.splits > 1 ? SMLA_F32 : y_dtype;
   TileArgs a{(const uint8_t*)x, 2 * ldx, {{codes, scales}, {nullptr, nullptr}}, padded_row(K), (int)K, (int)N, (int)T, (int)nt, (int)nn,
-             p.splits, p.splits > 1 ? part : (uint8_t*)y, N, T * N, 0, nullptr, nullptr, nullptr, 1, 0.f};
+             p.splits, p.splits > 1 ? part : (uint8_t*)y, N, T * N, 0, nullptr, 0, nullptr, nullptr, 1, 0.f};
   a.vec = N % (odt == SMLA_BF16 ? 8 : 4) == 0 && ((uintptr_t)a.y & 15) == 0;
   const int64_t wgs = nt * nn * p.splits;
 #define SMLA_LINEAR(F) \
   (odt == SMLA_BF16 ? launch_tile<Form<kFp4, F>, kLinear, SMLA_BF16>(a, wgs, st) : launch_tile<Form<kFp4, F>, kLinear, SMLA_F32>(a, wgs, st))
-  rc = p.form == 0 ? SMLA_LINEAR(0) : p.form == 1 ? SMLA_LINEAR(1) : p.form == 2 ? SMLA_LINEAR(2) : SMLA_LINEAR(3);
+  rc = p.form == 0 ? SMLA_LINEAR(0) : SMLA_LINEAR(1);
 #undef SMLA_LINEAR
   if (rc || p.splits == 1) return rc;
   const int64_t n = T * N;
@@ -918,7 +947,7 @@ extern "C" int smla_experts(const void* x, int64_t ldx, const int32_t* ids, cons
   const int64_t P = T * k;
   ExpertArgs a{(const uint16_t*)x, ldx, ids, weights, (int)T, (int)k, (int)E, (int)K, (int)I, (int)P,
                {(const uint8_t*)gate, gate_scales}, {(const uint8_t*)up, up_scales}, {(const uint8_t*)down, down_scales}, limit,
-               nullptr, nullptr, nullptr, 0, nullptr, nullptr, (uint16_t*)y};
+               nullptr, nullptr, nullptr, 0, 0, nullptr, nullptr, (uint16_t*)y};
   uint8_t* ws = (uint8_t*)workspace;
   auto take = [&](int64_t n) { uint8_t* p = ws; ws += n; return p; };
   a.list = (int32_t*)take(b.list), a.at = (int32_t*)take(b.list), a.tiles = (int32_t*)take(b.tiles);
@@ -926,7 +955,7 @@ extern "C" int smla_experts(const void* x, int64_t ldx, const int32_t* ids, cons
   hipStream_t st = (hipStream_t)stream;
   const int form = expert_form(T, k, E, K);
   if (form < 0) return launch_few(a, fp4, st);
-  a.tile = kFormBM[form];
+  a.tile = kFormBM[form], a.room = (int)room_of(P, E, a.tile);
   if (b.up_scales) {
     for (Matrix* m : {&a.gate, &a.up}) {
       uint8_t* s = take(b.up_scales);
