@@ -16,7 +16,7 @@
 // group in and the first one out are as close, or anything is not finite, the whole wave ranks the token in float64
 // (rank_f64).  The weights are of float64 scores, of the k picked alone (softmax: the sum over the row is of fp32
 // exponentials).
-// What bounds it is issue: about 1300 instructions for four tokens of 256 experts.
+// What bounds it is issue: a pick is about 85 instructions for four tokens of 256 experts.
 // route_f64_kernel: one token a wave in float64 throughout, for what the first does not take.
 #include "smla_internal.h"
 
@@ -39,10 +39,27 @@ __device__ inline double wave_sum_f64(double v) {
   for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
-__device__ inline double wave_max_f64(double v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
-  return v;
+template <int CTRL>
+__device__ inline double dpp_f64(double v) {
+  return __hiloint2double(dpp_i<CTRL>(__double2hiint(v)), dpp_i<CTRL>(__double2loint(v)));
+}
+__device__ inline double readlane_f64(double v, int lane) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
+}
+__device__ inline double wave_max_f64(double v) {  // (lane moves: through LDS, ten steps a pick were most of a token's 10 us)
+  v = fmax(v, dpp_f64<0xB1>(v));
+  v = fmax(v, dpp_f64<0x4E>(v));
+  v = fmax(v, dpp_f64<0x141>(v));
+  v = fmax(v, dpp_f64<0x140>(v));
+  return fmax(fmax(readlane_f64(v, 0), readlane_f64(v, 16)), fmax(readlane_f64(v, 32), readlane_f64(v, 48)));
+}
+__device__ inline int wave_min_i(int v) {
+  v = min(v, dpp_i<0xB1>(v));
+  v = min(v, dpp_i<0x4E>(v));
+  v = min(v, dpp_i<0x141>(v));
+  v = min(v, dpp_i<0x140>(v));
+  return min(min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
 
 template <int SCORE>
@@ -121,15 +138,24 @@ __device__ inline void rank_f64(const RouteArgs& a, int64_t t, double* lds, int&
     for (int i = 0; i < V; i++)
       if (have[i]) rank[lane + 64 * i] = v[i] != v[i] ? kOut : v[i];
     __syncthreads();
-    for (int g = lane; g < a.groups; g += 64) {
+    int each = 1;  // lanes of a group: a power of two
+    while (2 * each * a.groups <= 64) each *= 2;
+    for (int g0 = 0; g0 < a.groups; g0 += 64 / each) {
+      const int g = g0 + lane / each;
       double b0 = kOut, b1 = kOut;
-      for (int j = 0; j < per; j++) {
-        const double x = rank[g * per + j];
-        if (x > b0) b1 = b0, b0 = x;
-        else if (x > b1) b1 = x;
+      auto add = [&](double x) {
+        b1 = fmax(b1, fmin(b0, x));
+        b0 = fmax(b0, x);
+      };
+      if (g < a.groups)
+        for (int j = lane % each; j < per; j += each) add(rank[g * per + j]);
+      for (int o = 1; o < each; o *= 2) {
+        const double c0 = __shfl_xor(b0, o, 64), c1 = __shfl_xor(b1, o, 64);
+        add(c0);
+        add(c1);
       }
       const double sum = per > 1 ? b0 + b1 : b0;
-      gv[g] = sum != sum ? kOut : sum;
+      if (g < a.groups && lane % each == 0) gv[g] = sum != sum ? kOut : sum;
     }
     __syncthreads();
 #pragma unroll
@@ -158,8 +184,7 @@ __device__ inline void rank_f64(const RouteArgs& a, int64_t t, double* lds, int&
 #pragma unroll
     for (int i = V - 1; i >= 0; i--)
       if (top == kOut ? low[i] : v[i] == top) id = lane + 64 * i;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) id = min(id, __shfl_xor(id, o, 64));
+    id = wave_min_i(id);
     double sj = 0;
 #pragma unroll
     for (int i = 0; i < V; i++)
@@ -168,7 +193,7 @@ __device__ inline void rank_f64(const RouteArgs& a, int64_t t, double* lds, int&
         low[i] = false;
         sj = s[i];
       }
-    sj = __shfl(sj, id & 63, 64);
+    sj = readlane_f64(sj, id & 63);
     if (lane == j) mine = id, w = sj;
   }
 }
@@ -193,13 +218,24 @@ __device__ inline float row_reduce(float v, F&& f) {
   return f(v, dpp_f<0x140>(v));
 }
 __device__ inline float row_max(float v) { return row_reduce(v, [](float x, float y) { return fmaxf(x, y); }); }
-__device__ inline float row_min(float v) { return row_reduce(v, [](float x, float y) { return fminf(x, y); }); }
-__device__ inline int row_min_i(int v) {
-  v = min(v, (int)dpp_u<0xB1>((uint32_t)v));
-  v = min(v, (int)dpp_u<0x4E>((uint32_t)v));
-  v = min(v, (int)dpp_u<0x141>((uint32_t)v));
-  return min(v, (int)dpp_u<0x140>((uint32_t)v));
+template <class F>
+__device__ inline int row_reduce_i(int v, F&& f) {
+  v = f(v, dpp_i<0xB1>(v));
+  v = f(v, dpp_i<0x4E>(v));
+  v = f(v, dpp_i<0x141>(v));
+  return f(v, dpp_i<0x140>(v));
 }
+__device__ inline int row_max_i(int v) { return row_reduce_i(v, [](int x, int y) { return max(x, y); }); }
+__device__ inline int row_min_i(int v) { return row_reduce_i(v, [](int x, int y) { return min(x, y); }); }
+
+// a float as an integer of the same order (-0 as 0; no NaN): integer maxima need no care for NaN and take their operand from
+// another lane as they are
+__device__ inline int to_key(float x) {
+  const int b = __float_as_int(x + 0.f);
+  return b ^ (b >> 31 & 0x7fffffff);
+}
+__device__ inline float of_key(int k) { return __int_as_float(k ^ (k >> 31 & 0x7fffffff)); }
+constexpr int kOutKey = -0x7fffffff - 1, kLowKey = (int)0x807fffff;  // not in the running; -inf
 __device__ inline double row_sum_f64(double v) {
 #pragma unroll
   for (int o = 8; o >= 1; o >>= 1) v += __shfl_xor(v, o, 16);
@@ -282,89 +318,94 @@ __global__ __launch_bounds__(64) void route_kernel(const RouteArgs a) {
   } else {
     if (add) {
 #pragma unroll
-      for (int i = 0; i < V; i++) v[i] = l + 16 * i < a.E ? v[i] + b[i] : -SMLA_INF;
+      for (int i = 0; i < V; i++) {
+        v[i] = l + 16 * i < a.E ? v[i] + b[i] : -SMLA_INF;
+        bad |= v[i] != v[i];
+      }
     }
-    uint32_t kept = 0xffffffffu;
-    const int spg = a.groups > 1 ? a.E / a.groups / 16 : V;  // values a lane holds of a group
+    int key[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) key[i] = to_key(a.bias ? v[i] : x[i]);
     if (a.groups > 1) {
-      float gv = -SMLA_INF, b0 = gv, b1 = gv;  // lane g: group g
+      const int spg = a.E / a.groups / 16;  // values a lane holds of a group
+      int gv = kOutKey, b0 = gv, b1 = gv;   // lane g: group g's value
       int g = 0, left = spg;
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        b1 = fmaxf(b1, fminf(b0, v[i]));
-        b0 = fmaxf(b0, v[i]);
+        const int r = a.bias ? key[i] : to_key(v[i]);
+        b1 = max(b1, min(b0, r));
+        b0 = max(b0, r);
         if (--left == 0) {  // uniform
-          float c0 = b0, c1 = b1;
-          auto merge = [&](float d0, float d1) {
-            c1 = fmaxf(fmaxf(c1, d1), fminf(c0, d0));
-            c0 = fmaxf(c0, d0);
+          int c0 = b0, c1 = b1;
+          auto merge = [&](auto other) __attribute__((always_inline)) {
+            const int low = min(c0, other(c0));
+            c1 = max(max(c1, other(c1)), low);
+            c0 = max(c0, other(c0));
           };
-          merge(dpp_f<0xB1>(c0), dpp_f<0xB1>(c1));
-          merge(dpp_f<0x4E>(c0), dpp_f<0x4E>(c1));
-          merge(dpp_f<0x141>(c0), dpp_f<0x141>(c1));
-          merge(dpp_f<0x140>(c0), dpp_f<0x140>(c1));
-          if (l == g && g < a.groups) gv = c0 + c1;
+          merge([](int q) { return dpp_i<0xB1>(q); });
+          merge([](int q) { return dpp_i<0x4E>(q); });
+          merge([](int q) { return dpp_i<0x141>(q); });
+          merge([](int q) { return dpp_i<0x140>(q); });
+          if (l == g) gv = g < a.groups ? to_key(of_key(c0) + of_key(c1)) : kOutKey;
           g++, left = spg;
-          b0 = b1 = -SMLA_INF;
+          b0 = b1 = kOutKey;
         }
       }
-      int before = 0;
-      auto beside = [&](float o, int og) { before += o > gv || (o == gv && og < l); };
-#define SMLA_ROR(n) beside(dpp_f<0x120 + n>(gv), (int)dpp_u<0x120 + n>((uint32_t)l));
+      int before = 0;  // groups ahead of this lane's
+#define SMLA_ROR(n) before += dpp_i<0x120 + n>(gv) > gv - (dpp_i<0x120 + n>(l) < l);
       SMLA_ROR(1) SMLA_ROR(2) SMLA_ROR(3) SMLA_ROR(4) SMLA_ROR(5) SMLA_ROR(6) SMLA_ROR(7) SMLA_ROR(8)
       SMLA_ROR(9) SMLA_ROR(10) SMLA_ROR(11) SMLA_ROR(12) SMLA_ROR(13) SMLA_ROR(14) SMLA_ROR(15)
 #undef SMLA_ROR
       const bool in = l < a.groups && before < a.topk_groups;
-      const float last = row_min(in ? gv : SMLA_INF), next = row_max(in ? -SMLA_INF : gv);
+      const int last = row_min_i(in ? gv : 0x7fffffff), next = row_max_i(in ? kOutKey : gv);
       // (a group's value is the sum of two: twice the error)
-      if (a.topk_groups < a.groups) bad |= !(last - next > 2.f * kTol * (1.f + fabsf(last))) || !(last > -SMLA_INF);
-      kept = (uint32_t)(__ballot(in) >> (lane & 48)) & 0xffffu;
-    }
-    {
-      int left = spg;
-      uint32_t k = kept;
+      if (a.topk_groups < a.groups)
+        bad |= !(of_key(last) - of_key(next) > 2.f * kTol * (1.f + fabsf(of_key(last)))) || last <= kLowKey;
+      uint32_t kept = (uint32_t)(__ballot(in) >> (lane & 48)) & 0xffffu;
+      left = spg;
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        if (!a.bias) v[i] = x[i];
-        if (a.groups > 1) {
-          if (!(k & 1)) v[i] = -SMLA_INF;
-          if (--left == 0) k >>= 1, left = spg;
-        }
+        if (!(kept & 1)) key[i] = kOutKey;
+        if (--left == 0) kept >>= 1, left = spg;
       }
     }
     auto best = [&]() __attribute__((always_inline)) {
-      float top = v[0];
+      int top = key[0];
 #pragma unroll
-      for (int i = 1; i < V; i++) top = fmaxf(top, v[i]);
-      return row_max(top);
+      for (int i = 1; i < V; i++) top = max(top, key[i]);
+      return row_max_i(top);
     };
-    auto pick = [&](float top, int j) __attribute__((always_inline)) {  // its lowest id to lane j, out of the running
-      int id = 0x7fffffff;
+    auto pick = [&](int top, int j) __attribute__((always_inline)) {  // its lowest id to lane j, out of the running
+      int slot = V;
 #pragma unroll
-      for (int i = V - 1; i >= 0; i--)
-        if (v[i] == top) id = l + 16 * i;
-      id = row_min_i(id);
+      for (int i = V - 1; i >= 0; i--) slot = key[i] == top ? i : slot;
+      const int id = row_min_i(slot * 16 + l);
+      slot = (id & 15) == l ? id >> 4 : V;
 #pragma unroll
-      for (int i = 0; i < V; i++)
-        if (l + 16 * i == id) v[i] = -SMLA_INF;
+      for (int i = 0; i < V; i++) key[i] = slot == i ? kOutKey : key[i];
       if (l == j) mine = id;
     };
     bool close = false;  // neighbours in the order that fp32 cannot tell apart
-    float prev = SMLA_INF, top;
+    float prev = SMLA_INF;
+    int top;
     for (int j = 0;; j++) {
       top = best();
-      if (a.bias && j > 0) close |= !(prev - top > kTol * (1.f + fabsf(prev)));
+      if (a.bias) {
+        const float now = of_key(top);
+        if (j > 0) close |= !(prev - now > kTol * (1.f + fabsf(prev))) && top != kOutKey;
+        prev = now;
+      }
       if (j == a.k) break;
-      bad |= !(top > -SMLA_INF);
+      bad |= top <= kLowKey;
       pick(top, j);
-      prev = top;
     }
     if (__any(close)) {
       // the k and the next one in the order of their float64 values, a lane each; the one after it has to be apart
       if (SCORE != SMLA_SCORE_SOFTMAX && a.k < 16) {
         pick(top, a.k);
-        const float after = best();
-        if (close) bad |= !(prev - after > kTol * (1.f + fabsf(prev))) || !(top > -SMLA_INF);
+        const int after = best();
+        // (prev is the next one's value: what is apart from it is apart from the k-th)
+        if (close) bad |= top <= kLowKey || !(prev - of_key(after) > kTol * (1.f + fabsf(prev)) || after == kOutKey);
         double r = kOut;
         if (l <= a.k && mine < a.E) r = score_f64<SCORE>(load_as_f32(a.logits, at + mine, XDT)) + (double)a.bias[mine];
         int place = 0;

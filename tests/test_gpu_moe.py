@@ -55,16 +55,17 @@ def test_route(dev, case):
 @pytest.mark.parametrize("score", ["softmax", "sigmoid", "sqrtsoftplus"])
 @pytest.mark.parametrize("groups", [1, 4])
 @pytest.mark.parametrize("bias", [False, True])
-def test_route_ties_and_values_out_of_range(dev, score, groups, bias):
+@pytest.mark.parametrize("E", [40, 64])
+def test_route_ties_and_values_out_of_range(dev, score, groups, bias, E):
     """Equal logits, whole rows of one value, logits of -inf, +inf, NaN and the type's lowest, alone and together."""
     from smla import moe
-    announce(f"route out of range {score} {groups} {bias}")
-    E, k = 40, 7
+    announce(f"route out of range {score} {groups} {bias} {E}")
+    k = 7
     r = random.Random(5)
     low, inf, nan = torch.finfo(torch.float32).min, math.inf, math.nan
     rows = [[0.0] * E, [low] * E, [-inf] * E, [nan] * E, [1.0, 2.0] * (E // 2), [-inf] * (E - 3) + [1.0, -2.0, 1.0],
-            [low] * (E - 2) + [3.0, 3.0], [nan] + [0.5] * (E - 1), [-inf, nan] * (E // 2), [-100.0] * 20 + [-101.0] * 20,
-            [80.0, 81.0] * 20, [0.0, -0.0] * 20]
+            [low] * (E - 2) + [3.0, 3.0], [nan] + [0.5] * (E - 1), [-inf, nan] * (E // 2), [-100.0] * 20 + [-101.0] * (E - 20),
+            [80.0, 81.0] * (E // 2), [0.0, -0.0] * (E // 2)]
     rows += [[r.choice([0.25, -1.0, 3.0, -inf, low]) for _ in range(E)] for _ in range(20)]
     if score != "softmax":
         rows += [[r.choice([0.25, -1.0, nan, -inf]) for _ in range(E)] for _ in range(20)]
@@ -74,6 +75,9 @@ def test_route_ties_and_values_out_of_range(dev, score, groups, bias):
     b = torch.tensor([(e % 5) / 8 for e in range(E)]) if bias else None
     kw = dict(score=score, groups=groups, topk_groups=max(1, groups // 2), scale=1.5)
     _check_route(moe.route(x.to(dev), k, bias=None if b is None else b.to(dev), **kw), om.route(x, k, bias=b, **kw))
+    if bias:
+        b[3], b[17], b[30] = -inf, nan, inf
+        _check_route(moe.route(x.to(dev), k, bias=b.to(dev), **kw), om.route(x, k, bias=b, **kw))
 
 
 def test_route_order_next_to_a_border(dev):
