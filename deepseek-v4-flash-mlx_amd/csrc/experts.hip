@@ -166,25 +166,34 @@ __device__ inline void join(f32x4_t (&acc)[R]) {
 
 constexpr int kRowPad = 16;  // bytes between the rows of a wave in LDS: 16 rows' columns fall in distinct banks
 
-// bytes of LDS of a wave of nw: n rows of K, scales of r matrices
-__host__ __device__ inline int few_steps(int K, int nw) { return ((K + 127) / 128 + nw - 1) / nw; }
-__host__ __device__ inline int few_scales(int K, int nw) { return (few_steps(K, nw) + 3) / 4 * 256; }
-__host__ __device__ inline int few_lds(int n, int K, int nw, int r) { return n * (few_steps(K, nw) * 256 + kRowPad) + r * few_scales(K, nw); }
+// LDS of a workgroup of nw waves: n rows of K, a wave's share of all of them together, then the scales of r matrices, each a
+// wave's share of whole fours of steps
+__host__ __device__ inline int few_steps(int K) { return (K + 127) / 128; }
+__host__ __device__ inline int few_scales(int K, int nw) { return ((few_steps(K) + nw - 1) / nw + 3) / 4 * 256; }
+__host__ __device__ inline int64_t few_lds(int64_t n, int K, int nw, int r) {
+  return n * (256 * (int64_t)few_steps(K) + kRowPad * nw) + nw * r * (int64_t)few_scales(K, nw);
+}
+// matrices whose scales go through LDS
+template <int WT>
+constexpr int kStaged = WT == kFp4 ? 1 : 0;
 
+// Workgroup (i, j): outputs 16 i .. of tokens 16 j .. .
 template <int WT, int NW, int YDT>
-__global__ __launch_bounds__(64 * NW) void linear_few_kernel(const uint16_t* __restrict__ x, int64_t ldx, Matrix w, int T, int N,
+__global__ __launch_bounds__(64 * NW) void linear_few_kernel(const uint16_t* __restrict__ x, int64_t ldx, Matrix w, int tokens, int N,
                                                              int K, void* __restrict__ y) {
   constexpr int U = 8;
   extern __shared__ __align__(16) uint8_t lds_x[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, q = lane >> 4;
   const int nb = K / 32, steps = (nb + 3) / 4, s0 = steps * wave / NW, s1 = steps * (wave + 1) / NW, n0 = blockIdx.x * 16;
-  lds_u8_t* mine = (lds_u8_t*)lds_x + wave * few_lds(T, K, NW, 1);
-  const int ld = few_lds(1, K, NW, 0), row = min(m, N - 1 - n0);
+  const int t0 = blockIdx.y * kFew, T = min(tokens - t0, kFew);
+  x += t0 * ldx;
+  lds_u8_t *mine = (lds_u8_t*)lds_x + T * (256 * s0 + kRowPad * wave), *scales = (lds_u8_t*)lds_x + few_lds(T, K, NW, 0) + wave * few_scales(K, NW);
+  const int ld = 256 * (s1 - s0) + kRowPad, row = min(m, N - 1 - n0);
   const Matrix at = Block<WT>::rows(w, n0, K);
-  copy_scales<WT>(at, N - 1 - n0, K, s0, s1, (uint32_t)(uintptr_t)mine + T * ld);
+  copy_scales<WT>(at, N - 1 - n0, K, s0, s1, (uint32_t)(uintptr_t)scales);
   for (int t = 0; t < T; t++) copy_steps(x + (int64_t)t * ldx, K, s0, s1, (uint32_t)(uintptr_t)mine + t * ld);
   const lds_u8_t* xl = mine + min(m, T - 1) * ld + 64 * q - 256 * s0;  // (columns past the last token are not stored)
-  const lds_u8_t* sl = mine + T * ld + 4 * m + q - 64 * s0;
+  const lds_u8_t* sl = scales + 4 * m + q - 64 * s0;
   Block<WT> b[U];
   f32x4_t acc[1] = {f32x4_t{0.f, 0.f, 0.f, 0.f}};
   rolling<U>(s0, s1, [&](int u, int s) __attribute__((always_inline)) { b[u].load(at, row, K, block_of(s, q, nb)); },
@@ -203,8 +212,8 @@ __global__ __launch_bounds__(64 * NW) void linear_few_kernel(const uint16_t* __r
   for (int i = 0; i < 4; i++) {
     const int n = n0 + 4 * q + i;
     if (n < N) {
-      if constexpr (YDT == SMLA_BF16) ((uint16_t*)y)[(int64_t)m * N + n] = bf16_rne(acc[0][i]);
-      else ((float*)y)[(int64_t)m * N + n] = acc[0][i];
+      if constexpr (YDT == SMLA_BF16) ((uint16_t*)y)[(int64_t)(t0 + m) * N + n] = bf16_rne(acc[0][i]);
+      else ((float*)y)[(int64_t)(t0 + m) * N + n] = acc[0][i];
     }
   }
 }
@@ -271,13 +280,14 @@ __global__ __launch_bounds__(64 * kUpWaves) __attribute__((amdgpu_waves_per_eu(4
   if (e < 0 || e >= a.E || __any(pair >= 0 && pair < p)) return;
   uint32_t has = __builtin_amdgcn_readfirstlane((uint32_t)__ballot(pair >= 0));
   const int i0 = blockIdx.x * 16, nb = a.K / 32, steps = (nb + 3) / 4;
-  const int s0 = steps * wave / kUpWaves, s1 = steps * (wave + 1) / kUpWaves, ld = few_lds(1, a.K, kUpWaves, 0);
-  lds_u8_t* mine = (lds_u8_t*)lds_x + wave * few_lds(cap, a.K, kUpWaves, 2);
-  const Matrix gate = Block<WT>::rows(a.gate, (int64_t)e * a.I + i0, a.K), up = Block<WT>::rows(a.up, (int64_t)e * a.I + i0, a.K);
+  const int s0 = steps * wave / kUpWaves, s1 = steps * (wave + 1) / kUpWaves, ld = 256 * (s1 - s0) + kRowPad;
   const int s_up = few_scales(a.K, kUpWaves);
-  copy_scales<WT>(gate, 15, a.K, s0, s1, (uint32_t)(uintptr_t)mine + cap * ld);
-  copy_scales<WT>(up, 15, a.K, s0, s1, (uint32_t)(uintptr_t)mine + cap * ld + s_up);
-  const lds_u8_t* sl = mine + cap * ld + 4 * m + q - 64 * s0;
+  lds_u8_t *mine = (lds_u8_t*)lds_x + cap * (256 * s0 + kRowPad * wave),
+           *scales = (lds_u8_t*)lds_x + few_lds(cap, a.K, kUpWaves, 0) + wave * 2 * s_up;
+  const Matrix gate = Block<WT>::rows(a.gate, (int64_t)e * a.I + i0, a.K), up = Block<WT>::rows(a.up, (int64_t)e * a.I + i0, a.K);
+  copy_scales<WT>(gate, 15, a.K, s0, s1, (uint32_t)(uintptr_t)scales);
+  copy_scales<WT>(up, 15, a.K, s0, s1, (uint32_t)(uintptr_t)scales + s_up);
+  const lds_u8_t* sl = scales + 4 * m + q - 64 * s0;
   while (has) {
     int col = 0, nt = 0;  // lane m < nt: its token
     for (; has && nt < cap; nt++) {
@@ -584,18 +594,25 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ p
 
 // ---- tiles (expert_tile.h)
 
-// tokens x outputs: waves of .. x .., stages
+// tokens x outputs, waves of .. x .., stages, k of a step.  Few tokens an expert stream the weights: 128 bytes of a row
+// a copy (64 bytes a step, with every row in turn, come at 4.9 TB/s, 128 at 6.2).  64 x 128 is for the sizes between, whose
+// large tiles are too few for the CUs.
 template <int WT, int FORM>
 struct Form;
 template <>
 struct Form<kFp4, 0> : smla_tile::Tile<kFp4, 32, 256, 32, 64, 3, 256> {};  // 156 KB, 4 waves
 template <>
-struct Form<kFp4, 1> : smla_tile::Tile<kFp4, 128, 512, 64, 128, 2, 128> {};  // 152 KB, 8 waves
+struct Form<kFp4, 1> : smla_tile::Tile<kFp4, 64, 128, 32, 64, 3, 128> {};  // 78 KB, 4 waves: two workgroups a CU
+template <>
+struct Form<kFp4, 2> : smla_tile::Tile<kFp4, 128, 512, 64, 128, 2, 128> {};  // 152 KB, 8 waves
 template <>
 struct Form<kBf16, 0> : smla_tile::Tile<kBf16, 32, 256, 32, 64, 4, 64> {};  // 144 KB, 4 waves
 template <>
-struct Form<kBf16, 1> : smla_tile::Tile<kBf16, 128, 256, 64, 64, 3, 64> {};  // 144 KB, 8 waves
-constexpr int kFormBM[2] = {32, 128}, kFormBN[2] = {256, 512}, kFormKB[2] = {256, 128};  // (kFp4)
+struct Form<kBf16, 1> : smla_tile::Tile<kBf16, 64, 128, 32, 64, 3, 64> {};  // 72 KB, 4 waves: two workgroups a CU
+template <>
+struct Form<kBf16, 2> : smla_tile::Tile<kBf16, 128, 256, 64, 64, 3, 64> {};  // 144 KB, 8 waves
+constexpr int kForms = 3;
+constexpr int kFormBM[kForms] = {32, 64, 128}, kFormBN[kForms] = {256, 128, 512}, kFormKB[kForms] = {256, 128, 128};  // (BN, KB: kFp4)
 
 constexpr int kLinear = 0, kUp = 1, kDown = 2;
 
@@ -742,14 +759,41 @@ struct LinearPlan {
 int few_waves(int64_t K) { return K <= 2048 ? 4 : K <= 4096 ? 8 : 16; }
 
 LinearPlan linear_plan(int64_t T, int64_t N, int64_t K) {
+  // A model of the launches in microseconds, its constants fitted to 112 products (T 17 .. 512, N 256 .. 16384, K 512 .. 4096):
+  // the plan it picks is 2 % off the fastest on average and 30 % at worst.  The kernel for few tokens: a workgroup's time
+  // goes with the bytes it reads (16 tokens and 16 outputs), those resident together overlap.  Tiles: a step takes kIdle when
+  // few CUs run, kOne with a workgroup on each, kBusy with as many as fit; a split adds the launch that sums and its
+  // fp32 partial sums, rows of scales that are no whole words another that lays them out.
+  constexpr double kIdle[kForms] = {0.95, 0.46, 2.2}, kOne[kForms] = {1.25, 0.66, 2.85}, kBusy[kForms] = {1.25, 1.08, 2.85};
+  const int64_t cus = smla_num_cus();
+  LinearPlan best{kForms - 1, 1};
+  double bt = 1e30;
   const int nw = few_waves(K);
-  if (T <= kFew && K <= (1 << 20) && nw * (int64_t)few_lds((int)T, (int)K, nw, 1) <= kMaxFewLds) return {-1, 1};
-  const int form = T <= 32 ? 0 : 1;
-  const int64_t cus = smla_num_cus(), steps = (K + kFormKB[form] - 1) / kFormKB[form];
-  const int64_t tiles = (T + kFormBM[form] - 1) / kFormBM[form] * ((N + kFormBN[form] - 1) / kFormBN[form]);
-  int64_t splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= cus && steps / (splits * 2) >= 4) splits *= 2;
-  return {form, (int)splits};
+  const int64_t cols = std::min<int64_t>(T, kFew), lds = few_lds(cols, (int)K, nw, K % 128 == 0);
+  if (lds <= kMaxFewLds) {
+    const int64_t tt = (T + kFew - 1) / kFew, wgs = (N + 15) / 16 * tt;
+    const double each = std::max(0.7, K * (2.0 * T / tt + 8.5) * 25.3e-6);
+    const bool alone = 2 * (lds + 1024 * nw) > 160 * 1024;  // on a CU
+    const double more = alone ? (double)((wgs + cus - 1) / cus - 1) : std::max(0.0, (double)wgs / cus - 1);
+    bt = 3.6 + 0.35 * K / 1024 + more * each;
+    best = {-1, 1};
+  }
+  for (int f = 0; f < kForms; f++) {
+    const int64_t tiles = (T + kFormBM[f] - 1) / kFormBM[f] * ((N + kFormBN[f] - 1) / kFormBN[f]), steps = (K + kFormKB[f] - 1) / kFormKB[f];
+    const int64_t cap = f == 1 ? 2 * cus : cus;
+    for (int s = 1; s <= 8 && (s == 1 || steps / s >= 2); s *= 2) {
+      const int64_t rest = tiles * s % cap;
+      double t = (double)(tiles * s / cap) * kBusy[f];
+      if (rest > cus) t += kOne[f] + (kBusy[f] - kOne[f]) * (double)(rest - cus) / (double)cus;
+      else if (rest > 0) t += kIdle[f] + (kOne[f] - kIdle[f]) * (double)rest / (double)cus;
+      t = 3.6 + t * (double)((steps + s - 1) / s);
+      t = std::max(t, 2.5 + N * (double)K * 0.53 / 5.5e6);
+      if (s > 1) t += 2.4 + s * (double)T * N * 8 / 4.3e6;
+      if (K % 128) t += 2.5;
+      if (t < bt) bt = t, best = {f, s};
+    }
+  }
+  return best;
 }
 
 struct LinearBytes {
@@ -774,7 +818,8 @@ int launch_linear_few(const void* x, int64_t ldx, const Matrix& w, int64_t T, in
   auto kern = bf ? linear_few_kernel<WT, NW, SMLA_BF16> : linear_few_kernel<WT, NW, SMLA_F32>;
   static std::atomic<uint64_t> attr[2] = {{0}, {0}};
   if (hipError_t e = smla_set_dynamic_lds((const void*)kern, kMaxFewLds, attr[bf]); e != hipSuccess) return (int)e;
-  hipLaunchKernelGGL(kern, dim3((unsigned)((N + 15) / 16)), dim3(64 * NW), NW * few_lds((int)T, (int)K, NW, 1), st, (const uint16_t*)x, ldx, w,
+  hipLaunchKernelGGL(kern, dim3((unsigned)((N + 15) / 16), (unsigned)((T + kFew - 1) / kFew)), dim3(64 * NW),
+                     few_lds(std::min<int64_t>(T, kFew), (int)K, NW, kStaged<WT>), st, (const uint16_t*)x, ldx, w,
                      (int)T, (int)N, (int)K, y);
   SMLA_HIP_CHECK_LAUNCH();
   return SMLA_OK;
@@ -789,11 +834,13 @@ int check_experts(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I) {
   return SMLA_OK;
 }
 
-// the tile form by the pairs an expert has on average (-1: few tokens)
-int expert_form(int64_t T, int64_t k, int64_t E, int64_t K) {
-  if (T <= kFew && kUpWaves * (int64_t)few_lds((int)T, (int)K, kUpWaves, 2) <= kMaxFewLds) return -1;
+// the tile form by the pairs an expert has on average (-1: few tokens).  4-bit weights in 64 x 128 tiles came out behind
+// one of the others at every number of pairs (48: 709 us, 128 x 512 696 up; 32: 640, 32 x 256 513).
+int expert_form(int64_t T, int64_t k, int64_t E, int64_t K, bool fp4) {
+  if (T <= kFew && few_lds(T, (int)K, kUpWaves, 2) <= kMaxFewLds) return -1;
   const int64_t P = T * k, per = P / (E < P ? E : P);
-  return per <= 32 ? 0 : 1;
+  if (fp4) return per <= 32 ? 0 : 2;
+  return per <= 24 ? 0 : per <= 64 ? 1 : 2;
 }
 // an XCD's tiles at most: units of one length are shared out evenly (plan_kernel)
 int64_t room_of(int64_t P, int64_t E, int tile) { return (P / tile + (E < P ? E : P)) / kXcds + 3; }
@@ -804,7 +851,7 @@ struct ExpertBytes {
 };
 ExpertBytes expert_bytes(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I, bool fp4) {
   const int64_t P = T * k;
-  const int form = expert_form(T, k, E, K);
+  const int form = expert_form(T, k, E, K, fp4);
   if (form < 0) return {0, 0, up16(2 * P * I), 0, 0, 0};
   return {up16(4 * P), up16(32 + 12 * kXcds * room_of(P, E, kFormBM[form])), up16(2 * P * I), up16(4 * P * K),
           fp4 && K % 128 ? up16(E * I * padded_row(K)) : 0, fp4 && I % 128 ? up16(E * K * padded_row(I)) : 0};
@@ -813,7 +860,7 @@ ExpertBytes expert_bytes(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I, 
 template <int WT>
 int launch_few_up(const ExpertArgs& a, hipStream_t st) {
   // rows for four times the tokens that an expert has on average, and two more
-  const int cap = (int)std::min<int64_t>(a.T, 4 * a.P / a.E + 2), lds = kUpWaves * few_lds(cap, a.K, kUpWaves, 2);
+  const int cap = (int)std::min<int64_t>(a.T, 4 * a.P / a.E + 2), lds = (int)few_lds(cap, a.K, kUpWaves, 2 * kStaged<WT>);
   static std::atomic<uint64_t> attr{0};
   if (hipError_t e = smla_set_dynamic_lds((const void*)few_up_kernel<WT>, kMaxFewLds, attr); e != hipSuccess) return (int)e;
   hipLaunchKernelGGL(few_up_kernel<WT>, dim3(a.I / 16, a.P), dim3(64 * kUpWaves), lds, st, a, cap);
@@ -852,7 +899,12 @@ template <int WT>
 int launch_many(const ExpertArgs& a, int form, int64_t up_lds, int64_t down_lds, hipStream_t st) {
   hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, a);
   SMLA_HIP_CHECK_LAUNCH();
-  const int rc = form == 0 ? launch_tiles<Form<WT, 0>>(a, up_lds, down_lds, st) : launch_tiles<Form<WT, 1>>(a, up_lds, down_lds, st);
+  int rc = SMLA_OK;
+  if (form == 0) rc = launch_tiles<Form<WT, 0>>(a, up_lds, down_lds, st);
+  if constexpr (WT == kBf16) {
+    if (form == 1) rc = launch_tiles<Form<WT, 1>>(a, up_lds, down_lds, st);
+  }
+  if (form == 2) rc = launch_tiles<Form<WT, 2>>(a, up_lds, down_lds, st);
   if (rc) return rc;
   for (int64_t t0 = 0; t0 < a.T; t0 += 65535) {
     ExpertArgs c = a;
@@ -910,7 +962,7 @@ extern "C" int smla_linear_fp4(const void* x, int64_t ldx, const uint8_t* codes,
   const int64_t wgs = nt * nn * p.splits;
 #define SMLA_LINEAR(F) \
   (odt == SMLA_BF16 ? launch_tile<Form<kFp4, F>, kLinear, SMLA_BF16>(a, wgs, st) : launch_tile<Form<kFp4, F>, kLinear, SMLA_F32>(a, wgs, st))
-  rc = p.form == 0 ? SMLA_LINEAR(0) : SMLA_LINEAR(1);
+  rc = p.form == 0 ? SMLA_LINEAR(0) : p.form == 1 ? SMLA_LINEAR(1) : SMLA_LINEAR(2);
 #undef SMLA_LINEAR
   if (rc || p.splits == 1) return rc;
   const int64_t n = T * N;
@@ -953,7 +1005,7 @@ extern "C" int smla_experts(const void* x, int64_t ldx, const int32_t* ids, cons
   a.list = (int32_t*)take(b.list), a.at = (int32_t*)take(b.list), a.tiles = (int32_t*)take(b.tiles);
   a.h = (uint16_t*)take(b.h), a.part = (float*)take(b.part);
   hipStream_t st = (hipStream_t)stream;
-  const int form = expert_form(T, k, E, K);
+  const int form = expert_form(T, k, E, K, fp4);
   if (form < 0) return launch_few(a, fp4, st);
   a.tile = kFormBM[form], a.room = (int)room_of(P, E, a.tile);
   if (b.up_scales) {
