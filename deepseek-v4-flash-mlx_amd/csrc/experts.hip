@@ -239,8 +239,9 @@ struct ExpertArgs {
 
 constexpr int kMaxExperts = 1024, kMaxChoices = 64;
 
+// (comparisons, not fminf: a NaN stays one)
 __device__ inline float gated(float g, float u, float lim) {
-  g = fminf(g, lim), u = fminf(fmaxf(u, -lim), lim);
+  g = g > lim ? lim : g, u = u > lim ? lim : u < -lim ? -lim : u;
   return g / (1.f + __expf(-g)) * u;
 }
 
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(64 * kDownWaves) void few_down_kernel(const ExpertA
   int lk = s0 % per, uk = lk, li = s0 / per, ui = li;  // an item's step, and the item, of the loads and of the products
   auto get = [&](int i) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(i < items ? item[i] : 0); };
   int lit = get(li), uit = lit;
-  auto rows_of = [&](int it) __attribute__((always_inline)) { return items > 0 ? (int)pairs[slot[it & 1023]][m] : -1; };
+  auto rows_of = [&](int it) __attribute__((always_inline)) { return it ? (int)pairs[slot[it & 1023]][m] : -1; };  // (0: no item, one has a token)
   // scales: a request for each four steps of an item that the wave has any of, in a ring of slots of 256 bytes
   constexpr int SLOTS = U + 2;
   int ls = -1, us = -1;  // slots of the loads' and the products' step
@@ -730,7 +731,7 @@ int launch_tile(const TileArgs& a, int64_t wgs, hipStream_t st) {
   static_assert(lds <= 160 * 1024, "fits a CU");
   static std::atomic<uint64_t> attr{0};
   if (hipError_t e = smla_set_dynamic_lds((const void*)kern, lds, attr); e != hipSuccess) return (int)e;
-  if (wgs > 0x7fffffff) return SMLA_E_UNSUPPORTED;
+  if (wgs * L::THREADS > 0xffffffff) return SMLA_E_UNSUPPORTED;
   hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(L::THREADS), lds, st, a);
   SMLA_HIP_CHECK_LAUNCH();
   return SMLA_OK;
@@ -741,7 +742,7 @@ int64_t padded_row(int64_t K) { return (K + 127) / 128 * 4; }  // bytes of a row
 
 int launch_pad(const uint8_t* s, int64_t rows, int64_t K, uint8_t* out, hipStream_t st) {
   const int64_t n = rows * (padded_row(K) / 4);
-  if ((n + 255) / 256 > 0x7fffffff) return SMLA_E_UNSUPPORTED;
+  if (n > 0xffffff00) return SMLA_E_UNSUPPORTED;
   hipLaunchKernelGGL(pad_scales_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, s, rows, (int)(K / 32), (int)padded_row(K), out);
   SMLA_HIP_CHECK_LAUNCH();
   return SMLA_OK;
@@ -770,8 +771,9 @@ LinearPlan linear_plan(int64_t T, int64_t N, int64_t K) {
   double bt = 1e30;
   const int nw = few_waves(K);
   const int64_t cols = std::min<int64_t>(T, kFew), lds = few_lds(cols, (int)K, nw, K % 128 == 0);
-  if (lds <= kMaxFewLds) {
-    const int64_t tt = (T + kFew - 1) / kFew, wgs = (N + 15) / 16 * tt;
+  const int64_t tt = (T + kFew - 1) / kFew;
+  if (lds <= kMaxFewLds && tt <= 65535) {  // (the grid's limit)
+    const int64_t wgs = (N + 15) / 16 * tt;
     const double each = std::max(0.7, K * (2.0 * T / tt + 8.5) * 25.3e-6);
     const bool alone = 2 * (lds + 1024 * nw) > 160 * 1024;  // on a CU
     const double more = alone ? (double)((wgs + cus - 1) / cus - 1) : std::max(0.0, (double)wgs / cus - 1);
@@ -781,7 +783,7 @@ LinearPlan linear_plan(int64_t T, int64_t N, int64_t K) {
   for (int f = 0; f < kForms; f++) {
     const int64_t tiles = (T + kFormBM[f] - 1) / kFormBM[f] * ((N + kFormBN[f] - 1) / kFormBN[f]), steps = (K + kFormKB[f] - 1) / kFormKB[f];
     const int64_t cap = f == 1 ? 2 * cus : cus;
-    for (int s = 1; s <= 8 && (s == 1 || steps / s >= 2); s *= 2) {
+    for (int s = 1; s <= (f == 2 ? 1 : 8) && (s == 1 || steps / s >= 2); s *= 2) {  // (large tiles are for many)
       const int64_t rest = tiles * s % cap;
       double t = (double)(tiles * s / cap) * kBusy[f];
       if (rest > cus) t += kOne[f] + (kBusy[f] - kOne[f]) * (double)(rest - cus) / (double)cus;
@@ -810,7 +812,6 @@ int check_linear_fp4(int64_t T, int64_t N, int64_t K) {
   if (K % 32 != 0 || T > (1 << 24) || N > (1 << 24) || K > (1 << 22)) return SMLA_E_UNSUPPORTED;
   return SMLA_OK;
 }
-
 
 template <int WT, int NW>
 int launch_linear_few(const void* x, int64_t ldx, const Matrix& w, int64_t T, int64_t N, int64_t K, void* y, int y_dtype, hipStream_t st) {
@@ -932,7 +933,7 @@ extern "C" int smla_linear_fp4(const void* x, int64_t ldx, const uint8_t* codes,
   if (T > 1 && ldx < K) return SMLA_E_SHAPE;
   if (T == 0) return SMLA_OK;
   if (!x || !codes || !scales || !y) return SMLA_E_NULL;
-  if (ldx % 8 != 0 || ((uintptr_t)x & 15) || ((uintptr_t)codes & 15) || (K % 128 == 0 && ((uintptr_t)scales & 3)) || ldx > (1 << 22))
+  if (ldx % 8 != 0 || (((uintptr_t)x | (uintptr_t)codes | (uintptr_t)y) & 15) || (K % 128 == 0 && ((uintptr_t)scales & 3)) || ldx > (1 << 22))
     return SMLA_E_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
   const LinearPlan p = linear_plan(T, N, K);
@@ -958,7 +959,7 @@ extern "C" int smla_linear_fp4(const void* x, int64_t ldx, const uint8_t* codes,
   const int odt = p.splits > 1 ? SMLA_F32 : y_dtype;
   TileArgs a{(const uint8_t*)x, 2 * ldx, {{codes, scales}, {nullptr, nullptr}}, padded_row(K), (int)K, (int)N, (int)T, (int)nt, (int)nn,
              p.splits, p.splits > 1 ? part : (uint8_t*)y, N, T * N, 0, nullptr, 0, nullptr, nullptr, 1, 0.f};
-  a.vec = N % (odt == SMLA_BF16 ? 8 : 4) == 0 && ((uintptr_t)a.y & 15) == 0;
+  a.vec = N % (odt == SMLA_BF16 ? 8 : 4) == 0;
   const int64_t wgs = nt * nn * p.splits;
 #define SMLA_LINEAR(F) \
   (odt == SMLA_BF16 ? launch_tile<Form<kFp4, F>, kLinear, SMLA_BF16>(a, wgs, st) : launch_tile<Form<kFp4, F>, kLinear, SMLA_F32>(a, wgs, st))

@@ -31,7 +31,6 @@ def linear_fp4(x, codes, scales, out_dtype=None):
     """y = x @ W^T with W [out, in] held as e2m1 codes [out, in/2] and ue8m0 scale bytes [out, in/32] (``moe.pack_fp4``;
     the reference unpacks such weights first, ``ref_torch/quant.py:19-45``): x [..., in] bf16 -> [..., out] in
     ``out_dtype``, bf16 (the default) or fp32.  The products are exact and summed in fp32."""
-    ops._on_gpu(x, codes, scales)
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if x.dim() == 2:
         return ops.linear_fp4_op(x, codes, scales, out_dtype)

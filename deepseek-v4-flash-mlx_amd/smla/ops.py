@@ -1231,10 +1231,10 @@ def _rows(x, K, name):
 
 def _check_fp4(codes, scales, lead, name):
     """K of codes [*lead, K/2] and scales [*lead, K/32]; dense, because the kernels address whole tensors."""
-    n = len(lead)
-    if codes.dtype != torch.uint8 or codes.dim() != n + 1 or codes.shape[:n] != lead or not codes.is_contiguous():
+    half = codes.shape[-1]
+    if codes.dtype != torch.uint8 or codes.shape != (*lead, half) or not codes.is_contiguous():
         raise ValueError(f"{name} must be dense uint8 codes {[*lead, 'K/2']}, got {codes.dtype} {list(codes.shape)}")
-    K = 2 * codes.shape[n]
+    K = 2 * half
     if scales is None or scales.dtype != torch.uint8 or scales.shape != (*lead, K // 32) or not scales.is_contiguous():
         got = None if scales is None else (scales.dtype, list(scales.shape))
         raise ValueError(f"{name} scales must be dense uint8 {[*lead, K // 32]}, got {got}")
@@ -1264,8 +1264,9 @@ def _route(logits: torch.Tensor, bias: Optional[torch.Tensor], k: int, score: in
         bias = _f32(bias)
     if given is not None:
         given = _i32(given, (T, k), "ids")
-    ids = torch.empty(T, k + shared, dtype=torch.int32, device=logits.device)
-    weights = torch.empty(T, k + shared, dtype=torch.float32, device=logits.device)
+    device = logits.device
+    ids = torch.empty(T, k + shared, dtype=torch.int32, device=device)
+    weights = torch.empty(T, k + shared, dtype=torch.float32, device=device)
     _launch(dev, "smla_route", logits.data_ptr(), dt, ld, _p(bias), T, E, k, score, groups, topk_groups, renorm, scale, shared,
             _p(given), ids.data_ptr(), weights.data_ptr())
     return ids, weights
@@ -1297,6 +1298,8 @@ def _linear_fp4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_
         raise TypeError("linear_fp4 gives fp32 or bf16")
     if codes.data_ptr() & 15:
         codes = codes.clone()
+    if scales.data_ptr() & 3:
+        scales = scales.clone()
     y = torch.empty(T, N, dtype=out_dtype, device=x.device)
     wsb = _lib.lib().smla_linear_fp4_workspace(T, N, K)
     ws = torch.empty(wsb, dtype=torch.uint8, device=x.device) if wsb else None
@@ -1338,6 +1341,8 @@ def _experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: to
             raise ValueError("scales go with fp4 codes, and only with them")
     if (gate.data_ptr() | up.data_ptr() | down.data_ptr()) & 15:
         raise ValueError("the experts' weights must be 16-byte aligned")
+    if fp4 and (gate_scales.data_ptr() | up_scales.data_ptr() | down_scales.data_ptr()) & 3:
+        raise ValueError("the experts' scales must be 4-byte aligned")
     x, ld = _rows(x, K, "x")
     T = x.shape[0]
     k = ids.shape[1]

@@ -131,6 +131,8 @@ LINEARS = [  # T, N, K
     (15, 31, 2048), (16, 48, 8192), (17, 130, 384), (24, 2048, 1024), (31, 257, 288), (32, 64, 4096), (33, 129, 512),
     (64, 256, 256), (65, 300, 1184), (77, 1000, 4128), (128, 128, 128), (129, 513, 320), (200, 96, 64), (255, 1030, 640),
     (256, 256, 1024), (300, 77, 992), (700, 384, 1536), (1025, 640, 416),
+    (16, 48, 4352), (5, 17, 14208), (6, 16, 12512), (6, 409, 11776), (20, 8383, 3296), (1722, 71, 2560), (3283, 66, 2240),
+    (37, 11078, 2240), (784, 10036, 32), (719, 11074, 128), (17, 12932, 160), (1, 6848, 128), (18, 11030, 32),
 ]
 
 
@@ -255,6 +257,55 @@ def test_experts(dev, case):
     y = moe.experts(x.to(dev), ids.to(dev), w.to(dev), *_on(dev, mats), limit=limit)
     assert y.dtype == torch.bfloat16 and y.shape == (T, K)
     _check_experts(y, want)
+
+
+@pytest.mark.parametrize("T", [1, 9, 40, 400])
+@pytest.mark.parametrize("kind", ["fp4", "bf16"])
+@pytest.mark.parametrize("limit", [None, 10.0])
+def test_experts_nan_and_infinity_stay(dev, T, kind, limit):
+    """A token whose products are NaN, and an expert whose scales are, give NaN with a clamp too, to nobody else."""
+    from smla import moe
+    announce(f"experts nan {T} {kind} {limit}")
+    E, k, K, I = 5, 2, 160, 96
+    x, _, w, mats = _experts_case(T, T, E, E, k, K, I, kind)
+    gate, up, down = _on(dev, mats)
+    ids = torch.arange(T * k, dtype=torch.int32).view(T, k) % (E - 1)      # none has the last expert
+    args = [w.to(dev), gate, up, down]
+    want = moe.experts(x.to(dev), ids.to(dev), *args, limit=limit)
+    assert want.isfinite().all()
+    bad = x.clone()
+    bad[T // 2, 7] = math.nan
+    got = moe.experts(bad.to(dev), ids.to(dev), *args, limit=limit)
+    assert got[T // 2].isnan().all()
+    others = torch.arange(T) != T // 2
+    assert torch.equal(got.cpu()[others], want.cpu()[others])
+    last = gate[1] if kind == "fp4" else gate
+    last[E - 1] = 255 if kind == "fp4" else math.nan
+    assert torch.equal(moe.experts(x.to(dev), ids.to(dev), *args, limit=limit), want)
+    ids[0, 1] = E - 1
+    got = moe.experts(x.to(dev), ids.to(dev), *args, limit=limit)
+    assert got[0].isnan().all() and got[1:].isfinite().all()   # (the sums' order goes with the ids)
+
+
+@pytest.mark.parametrize("T", [3, 70])
+def test_weights_that_begin_anywhere(dev, T):
+    """Codes and scales of a product are taken at any address; the experts' have to be aligned, and are refused if not."""
+    from smla import mla, moe
+    announce(f"weights anywhere {T}")
+    N, K = 40, 256
+    codes, scales, _ = _packed(2, N, K)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16).to(dev)
+
+    def moved(t, by):
+        at = torch.empty(t.numel() + 16, dtype=t.dtype, device=dev)[by:by + t.numel()].view(t.shape)
+        return at.copy_(t)
+    want = mla.linear_fp4(x, codes.to(dev), scales.to(dev))
+    assert torch.equal(mla.linear_fp4(x, moved(codes, 3), moved(scales, 5)), want)
+    c, s, _ = _packed(3, 2, 64, 64)
+    ids, w = torch.zeros(T, 1, dtype=torch.int32, device=dev), torch.ones(T, 1, device=dev)
+    for pair in ((moved(c, 1), s.to(dev)), (c.to(dev), moved(s, 1))):
+        with pytest.raises(ValueError, match="aligned"):
+            moe.experts(x[:, :64], ids, w, pair, pair, pair)
 
 
 @pytest.mark.parametrize("T", [1, 5, 16, 50, 300])
