@@ -607,8 +607,6 @@ struct Form<kFp4, 1> : smla_tile::Tile<kFp4, 64, 128, 32, 64, 3, 128> {};  // 78
 template <>
 struct Form<kFp4, 2> : smla_tile::Tile<kFp4, 128, 512, 64, 128, 2, 128> {};  // 152 KB, 8 waves
 template <>
-struct Form<kBf16, 0> : smla_tile::Tile<kBf16, 32, 256, 32, 64, 4, 64> {};  // 144 KB, 4 waves
-template <>
 struct Form<kBf16, 1> : smla_tile::Tile<kBf16, 64, 128, 32, 64, 3, 64> {};  // 72 KB, 4 waves: two workgroups a CU
 template <>
 struct Form<kBf16, 2> : smla_tile::Tile<kBf16, 128, 256, 64, 64, 3, 64> {};  // 144 KB, 8 waves
@@ -835,13 +833,14 @@ int check_experts(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I) {
   return SMLA_OK;
 }
 
-// the tile form by the pairs an expert has on average (-1: few tokens).  4-bit weights in 64 x 128 tiles came out behind
-// one of the others at every number of pairs (48: 709 us, 128 x 512 696 up; 32: 640, 32 x 256 513).
+// The tile form by the pairs an expert has on average (-1: few tokens).  4-bit weights in 64 x 128 tiles came out behind
+// one of the others at every number of pairs (256 experts of 4096 x 2048, the up products: 48 pairs 709 us, 128 x 512 696;
+// 32 pairs 640, 32 x 256 513).  bf16 in 32 x 256 tiles came out behind 64 x 128 at every number (24 experts of 4096 x 2048:
+// 8 pairs 247 us against 235, 48 pairs 271 against 247); 128 x 256 passes those between 48 (261) and 64 (256 against 278).
 int expert_form(int64_t T, int64_t k, int64_t E, int64_t K, bool fp4) {
   if (T <= kFew && few_lds(T, (int)K, kUpWaves, 2) <= kMaxFewLds) return -1;
   const int64_t P = T * k, per = P / (E < P ? E : P);
-  if (fp4) return per <= 32 ? 0 : 2;
-  return per <= 24 ? 0 : per <= 64 ? 1 : 2;
+  return fp4 ? per <= 32 ? 0 : 2 : per <= 56 ? 1 : 2;
 }
 // an XCD's tiles at most: units of one length are shared out evenly (plan_kernel)
 int64_t room_of(int64_t P, int64_t E, int tile) { return (P / tile + (E < P ? E : P)) / kXcds + 3; }
@@ -901,11 +900,8 @@ int launch_many(const ExpertArgs& a, int form, int64_t up_lds, int64_t down_lds,
   hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, a);
   SMLA_HIP_CHECK_LAUNCH();
   int rc = SMLA_OK;
-  if (form == 0) rc = launch_tiles<Form<WT, 0>>(a, up_lds, down_lds, st);
-  if constexpr (WT == kBf16) {
-    if (form == 1) rc = launch_tiles<Form<WT, 1>>(a, up_lds, down_lds, st);
-  }
-  if (form == 2) rc = launch_tiles<Form<WT, 2>>(a, up_lds, down_lds, st);
+  if (form < 2) rc = launch_tiles<Form<WT, WT == kFp4 ? 0 : 1>>(a, up_lds, down_lds, st);
+  else rc = launch_tiles<Form<WT, 2>>(a, up_lds, down_lds, st);
   if (rc) return rc;
   for (int64_t t0 = 0; t0 < a.T; t0 += 65535) {
     ExpertArgs c = a;
