@@ -228,6 +228,7 @@ struct ExpertArgs {
   int T, k, E, K, I, P;  // P = T k pairs
   Matrix gate, up, down;
   float limit;           // infinity: none
+  uint32_t* items;       // few tokens: [P][4], few_down_kernel's
   int32_t* list;         // pairs by expert
   int32_t* at;           // a pair's place in it
   int32_t* tiles;        // [8] their numbers, then for each XCD `room` of (expert, first place, pairs)
@@ -238,6 +239,7 @@ struct ExpertArgs {
 };
 
 constexpr int kMaxExperts = 1024, kMaxChoices = 64;
+constexpr int kItemTokens = 4;
 
 // (comparisons, not fminf: a NaN stays one)
 __device__ inline float gated(float g, float u, float lim) {
@@ -278,8 +280,28 @@ __global__ __launch_bounds__(64 * kUpWaves) __attribute__((amdgpu_waves_per_eu(4
         wt += w[j];
       }
   }
-  if (e < 0 || e >= a.E || __any(pair >= 0 && pair < p)) return;
   uint32_t has = __builtin_amdgcn_readfirstlane((uint32_t)__ballot(pair >= 0));
+  const bool real = e >= 0 && e < a.E;
+  if (blockIdx.x == 0 && wave == 0) {
+    // few_down_kernel's item of place p: {expert | tokens << 10, their places by 16 bits}, where p is the first place of each
+    // fourth token with the expert; 0: none
+    const int t = p / a.k;
+    uint32_t what = 0, places[2] = {0, 0};
+    if (real && __builtin_amdgcn_readlane(pair, t) == p && __popc(has & ((1u << t) - 1)) % kItemTokens == 0) {
+      uint32_t left = has >> t << t;
+#pragma unroll
+      for (int c = 0; c < kItemTokens; c++)
+        if (left) {
+          const int b = __ffs((int)left) - 1;
+          left &= left - 1;
+          what |= 1u << b;
+          places[c / 2] |= (uint32_t)__builtin_amdgcn_readlane(pair, b) << (16 * (c & 1));
+        }
+      what = (uint32_t)e | what << 10;
+    }
+    if (lane == 0) *(u32x4_t*)(a.items + 4 * p) = u32x4_t{what, places[0], places[1], 0};
+  }
+  if (!real || __any(pair >= 0 && pair < p)) return;
   const int i0 = blockIdx.x * 16, nb = a.K / 32, steps = (nb + 3) / 4;
   const int s0 = steps * wave / kUpWaves, s1 = steps * (wave + 1) / kUpWaves, ld = 256 * (s1 - s0) + kRowPad;
   const int s_up = few_scales(a.K, kUpWaves);
@@ -342,7 +364,7 @@ __global__ __launch_bounds__(64 * kUpWaves) __attribute__((amdgpu_waves_per_eu(4
 // wave's LDS a step ahead of the step's weights (256 bytes a token; as operands from memory they are four loads of 1 KB
 // a step, against one of the weights).  Column m is token m: a wave adds an item's sums to a token's only where the item
 // has it (0 times an infinite weight of another token's expert would be NaN).
-constexpr int kDownWaves = 16, kItemTokens = 4;
+constexpr int kDownWaves = 16;
 template <int WT>
 constexpr int kDownAhead = WT == kBf16 ? 3 : 4;
 template <int WT>
@@ -356,59 +378,21 @@ template <int WT>
 __global__ __launch_bounds__(64 * kDownWaves) void few_down_kernel(const ExpertArgs a) {
   constexpr int U = kDownAhead<WT>;
   extern __shared__ __align__(16) uint8_t lds_x[];
-  __shared__ int32_t slot[kMaxExperts];                // an expert's first pair, then its number
-  __shared__ int32_t item[kFew * kMaxChoices];         // first the ids, then expert | tokens << 10
-  __shared__ __align__(16) int16_t pairs[kFew * kMaxChoices][kFew];  // of an expert and a token: the first pair
-  __shared__ int cnt[2][kDownWaves];
+  __shared__ u32x4_t item[kFew * kMaxChoices];
+  __shared__ int cnt[kDownWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, q = lane >> 4;
-  const int e = tid < a.P ? a.ids[tid] : -1, t = (uint32_t)tid / (uint32_t)a.k;
-  const bool real = e >= 0 && e < a.E;
-  slot[tid] = 0x7fffffff;
-  item[tid] = e;
-  for (int i = tid; i < a.P * kFew / 2; i += 64 * kDownWaves) ((int32_t*)pairs)[i] = -1;
+  // the items, in the order of their places
+  u32x4_t mine = {0, 0, 0, 0};
+  if (tid < a.P) mine = *(const u32x4_t*)(a.items + 4 * tid);
+  const uint64_t mask = __ballot(mine[0] != 0);
+  if (lane == 0) cnt[wave] = __popcll(mask);
   __syncthreads();
-  if (real) atomicMin(&slot[e], tid);
-  __syncthreads();
-  const bool first = real && slot[e] == tid;
-  const uint64_t mask = __ballot(first);
-  if (lane == 0) cnt[0][wave] = __popcll(mask);
-  __syncthreads();
-  int at = __popcll(mask & ((1ull << lane) - 1));  // the expert's number
-  for (int v = 0; v < wave; v++) at += cnt[0][v];
-  if (first) slot[e] = at;
-  __syncthreads();
-  // the first of a token's choices of the same expert
-  if (real) {
-    bool again = false;
-    for (int o = t * a.k; o < tid; o++) again |= item[o] == e;
-    if (!again) pairs[slot[e]][t] = (int16_t)tid;
-  }
-  __syncthreads();
-  int experts = 0;
-  for (int v = 0; v < kDownWaves; v++) experts += cnt[0][v];
-  // items of up to kItemTokens tokens
-  uint32_t tokens = 0;
-  if (first)
-    for (int o = 0; o < a.T; o++) tokens |= (uint32_t)(pairs[at][o] >= 0) << o;
-  const int need = ((int)__popc(tokens) + kItemTokens - 1) / kItemTokens;
-  int sum_before = need;
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const int u = __shfl_up(sum_before, o, 64);
-    if (lane >= o) sum_before += u;
-  }
-  if (lane == 63) cnt[1][wave] = sum_before;
-  __syncthreads();
-  int it = sum_before - need, items = 0;
+  int to = __popcll(mask & ((1ull << lane) - 1)), items = 0;
   for (int v = 0; v < kDownWaves; v++) {
-    if (v < wave) it += cnt[1][v];
-    items += cnt[1][v];
+    if (v < wave) to += cnt[v];
+    items += cnt[v];
   }
-  for (; tokens; it++) {
-    uint32_t some = 0;
-    for (int o = 0; o < kItemTokens && tokens; o++) some |= tokens & -tokens, tokens &= tokens - 1;
-    item[it] = e | some << 10;
-  }
+  if (mine[0]) item[to] = mine;
   __syncthreads();
   items = __builtin_amdgcn_readfirstlane(items);
 
@@ -417,23 +401,22 @@ __global__ __launch_bounds__(64 * kDownWaves) void few_down_kernel(const ExpertA
   lds_u8_t *ring = (lds_u8_t*)lds_x + wave * kDownRing<WT>, *scales = (lds_u8_t*)lds_x + kDownWaves * kDownRing<WT> + wave * kDownScales<WT>;
   f32x4_t sum = {0.f, 0.f, 0.f, 0.f}, acc = sum;
   int lk = s0 % per, uk = lk, li = s0 / per, ui = li;  // an item's step, and the item, of the loads and of the products
-  auto get = [&](int i) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(i < items ? item[i] : 0); };
-  int lit = get(li), uit = lit;
-  auto rows_of = [&](int it) __attribute__((always_inline)) { return it ? (int)pairs[slot[it & 1023]][m] : -1; };  // (0: no item, one has a token)
+  auto get = [&](int i) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(i < items ? item[i][0] : 0); };
+  uint32_t lit = get(li), uit = lit;
+  auto places = [&](int i, int c) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(i < items ? item[i][1 + c] : 0); };
   // scales: a request for each four steps of an item that the wave has any of, in a ring of slots of 256 bytes
   constexpr int SLOTS = U + 2;
   int ls = -1, us = -1;  // slots of the loads' and the products' step
   auto next = [&](int slot) __attribute__((always_inline)) { return slot + 1 == SLOTS ? 0 : slot + 1; };
-  int lp = rows_of(lit);  // lane m: token m's row of h, of the loads' item
+  uint32_t lp0 = places(li, 0), lp1 = places(li, 1);  // the places of the loads' item
   Block<WT> w[U];
   rolling<U>(s0, s1, [&](int u, int s) __attribute__((always_inline)) {
-    const int ex = lit & 1023;
+    const uint32_t ex = lit & 1023;
     const Matrix at = Block<WT>::rows(a.down, (int64_t)ex * a.K + n0, a.I);
-    uint32_t has = (uint32_t)lit >> 10;
+    const int many = __popc(lit >> 10);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot's last reads are done
-    for (int c = 0; has; c++) {  // uniform
-      const int pair = __builtin_amdgcn_readlane(lp, __ffs((int)has) - 1);
-      has &= has - 1;
+    for (int c = 0; c < many; c++) {  // uniform
+      const uint32_t pair = (c < 2 ? lp0 : lp1) >> (16 * (c & 1)) & 0xffff;
       const int b = min(256 * lk + 4 * lane, 2 * a.I - 4);  // (past the row: any, dropped)
       smla_tile::dma4_s((const uint8_t*)a.h + 2 * (int64_t)pair * a.I, b, (uint32_t)(uintptr_t)ring + (u * kItemTokens + c) * 256);
     }
@@ -444,14 +427,14 @@ __global__ __launch_bounds__(64 * kDownWaves) void few_down_kernel(const ExpertA
       }
     }
     w[u].load(at, m, a.I, block_of(lk, q, nb));
-    if (++lk == per) lk = 0, lit = get(++li), lp = rows_of(lit);
+    if (++lk == per) lk = 0, lit = get(++li), lp0 = places(li, 0), lp1 = places(li, 1);
   }, [&](int u, int s) __attribute__((always_inline)) {
     w[u].arrived();  // and the copies, which went out before
     if (uk % 4 == 0 || s == s0) us = next(us);
     w[u].scale(scales + 256 * us + 4 * m + q, uk & 3);
     const bool drop = 4 * uk + 4 > nb && 4 * uk + q >= nb;
     if (4 * uk + 4 > nb) w[u].keep(!drop);  // uniform
-    const uint32_t has = (uint32_t)uit >> 10;
+    const uint32_t has = uit >> 10;
     const lds_u8_t* x = ring + (u * kItemTokens + min((int)__popc(has & ((1u << m) - 1)), kItemTokens - 1)) * 256 + 64 * q;
 #pragma unroll
     for (int j = 0; j < 4; j++) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[u].frag(j), operand(x, 0, j, drop), acc, 0, 0, 0);
@@ -846,14 +829,14 @@ int expert_form(int64_t T, int64_t k, int64_t E, int64_t K, bool fp4) {
 int64_t room_of(int64_t P, int64_t E, int tile) { return (P / tile + (E < P ? E : P)) / kXcds + 3; }
 
 struct ExpertBytes {
-  int64_t list, tiles, h, part, up_scales, down_scales;
-  int64_t total() const { return 2 * list + tiles + h + part + 2 * up_scales + down_scales; }
+  int64_t items, list, tiles, h, part, up_scales, down_scales;
+  int64_t total() const { return items + 2 * list + tiles + h + part + 2 * up_scales + down_scales; }
 };
 ExpertBytes expert_bytes(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I, bool fp4) {
   const int64_t P = T * k;
   const int form = expert_form(T, k, E, K, fp4);
-  if (form < 0) return {0, 0, up16(2 * P * I), 0, 0, 0};
-  return {up16(4 * P), up16(32 + 12 * kXcds * room_of(P, E, kFormBM[form])), up16(2 * P * I), up16(4 * P * K),
+  if (form < 0) return {16 * P, 0, 0, up16(2 * P * I), 0, 0, 0};
+  return {0, up16(4 * P), up16(32 + 12 * kXcds * room_of(P, E, kFormBM[form])), up16(2 * P * I), up16(4 * P * K),
           fp4 && K % 128 ? up16(E * I * padded_row(K)) : 0, fp4 && I % 128 ? up16(E * K * padded_row(I)) : 0};
 }
 
@@ -996,10 +979,10 @@ extern "C" int smla_experts(const void* x, int64_t ldx, const int32_t* ids, cons
   const int64_t P = T * k;
   ExpertArgs a{(const uint16_t*)x, ldx, ids, weights, (int)T, (int)k, (int)E, (int)K, (int)I, (int)P,
                {(const uint8_t*)gate, gate_scales}, {(const uint8_t*)up, up_scales}, {(const uint8_t*)down, down_scales}, limit,
-               nullptr, nullptr, nullptr, 0, 0, nullptr, nullptr, (uint16_t*)y};
+               nullptr, nullptr, nullptr, nullptr, 0, 0, nullptr, nullptr, (uint16_t*)y};
   uint8_t* ws = (uint8_t*)workspace;
   auto take = [&](int64_t n) { uint8_t* p = ws; ws += n; return p; };
-  a.list = (int32_t*)take(b.list), a.at = (int32_t*)take(b.list), a.tiles = (int32_t*)take(b.tiles);
+  a.items = (uint32_t*)take(b.items), a.list = (int32_t*)take(b.list), a.at = (int32_t*)take(b.list), a.tiles = (int32_t*)take(b.tiles);
   a.h = (uint16_t*)take(b.h), a.part = (float*)take(b.part);
   hipStream_t st = (hipStream_t)stream;
   const int form = expert_form(T, k, E, K, fp4);

@@ -4,6 +4,7 @@ Each op validates shapes/dtypes on the host, allocates its outputs (and workspac
 caching allocator, and launches on ``torch.cuda.current_stream()``.  Fake (meta) kernels give
 output shapes for tracing.
 """
+import functools
 from typing import Optional
 
 import torch
@@ -1217,6 +1218,13 @@ compact_pages_op = _with_eager_route(compact_pages_op, _compact_pages)
 
 # ----------------------------------------------------------------------------------------------
 # The expert network (smla.moe) and products with 4-bit weights.
+@functools.lru_cache(maxsize=512)
+def _workspace(dev, name, *sizes):
+    """Bytes that a call of these sizes needs on GPU dev (the plan goes by its CUs)."""
+    with torch.cuda.device(dev):
+        return getattr(_lib.lib(), name)(*sizes)
+
+
 def _rows(x, K, name):
     """x [T, K] bf16 as a tensor whose rows are 16-byte aligned, and the elements between them."""
     if x.dim() != 2 or x.shape[1] != K or x.dtype != torch.bfloat16:
@@ -1301,7 +1309,7 @@ def _linear_fp4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_
     if scales.data_ptr() & 3:
         scales = scales.clone()
     y = torch.empty(T, N, dtype=out_dtype, device=x.device)
-    wsb = _lib.lib().smla_linear_fp4_workspace(T, N, K)
+    wsb = _workspace(dev, "smla_linear_fp4_workspace", T, N, K)
     ws = torch.empty(wsb, dtype=torch.uint8, device=x.device) if wsb else None
     _launch(dev, "smla_linear_fp4", x.data_ptr(), ld, codes.data_ptr(), scales.data_ptr(), T, N, K, y.data_ptr(), ydt, _p(ws),
             wsb)
@@ -1354,7 +1362,7 @@ def _experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: to
     if T == 0:
         return y
     wdt = _lib.FP4_E2M1 if fp4 else _lib.BF16
-    wsb = _lib.lib().smla_experts_workspace(T, k, E, K, inner, wdt)
+    wsb = _workspace(dev, "smla_experts_workspace", T, k, E, K, inner, wdt)
     ws = torch.empty(wsb, dtype=torch.uint8, device=x.device) if wsb else None
     _launch(dev, "smla_experts", x.data_ptr(), ld, ids.data_ptr(), weights.data_ptr(), T, k, E, K, inner, gate.data_ptr(),
             _p(gate_scales), up.data_ptr(), _p(up_scales), down.data_ptr(), _p(down_scales), wdt, limit, y.data_ptr(), _p(ws), wsb)
