@@ -109,9 +109,12 @@ __device__ __attribute__((always_inline)) inline void rolling(int s0, int s1, L&
   for (int u = 0; u < U; u++) load(u, s0 + u);
   for (; s0 + U < s1; s0 += U)
 #pragma unroll
-    for (int u = 0; u < U; u++) {
+    for (int u = 0; u < U; u += 2) {
       use(u, s0 + u);
+      __builtin_amdgcn_sched_barrier(0);
+      if (u + 1 < U) use(u + 1, s0 + u + 1);
       load(u, s0 + u + U);
+      if (u + 1 < U) load(u + 1, s0 + u + 1 + U);
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
@@ -253,7 +256,7 @@ __device__ inline float gated(float g, float u, float lim) {
 // CU), room for `cap` of them; an expert of more streams its weights again for the others.
 constexpr int kUpWaves = 4;
 template <int WT>
-constexpr int kUpAhead = WT == kBf16 ? 2 : WT == kFp4Odd ? 6 : 8;
+constexpr int kUpAhead = WT == kBf16 ? 2 : 4;
 template <int WT>
 __global__ __launch_bounds__(64 * kUpWaves) __attribute__((amdgpu_waves_per_eu(4))) void few_up_kernel(const ExpertArgs a, int cap) {
   constexpr int U = kUpAhead<WT>;
@@ -397,7 +400,7 @@ __global__ __launch_bounds__(64 * kDownWaves) void few_down_kernel(const ExpertA
   items = __builtin_amdgcn_readfirstlane(items);
 
   const int n0 = blockIdx.x * 16, nb = a.I / 32, per = (nb + 3) / 4, steps = items * per;
-  const int s0 = steps * wave / kDownWaves, s1 = steps * (wave + 1) / kDownWaves;
+  const int s0 = steps * wave / kDownWaves & ~1, s1 = wave + 1 == kDownWaves ? steps : steps * (wave + 1) / kDownWaves & ~1;
   lds_u8_t *ring = (lds_u8_t*)lds_x + wave * kDownRing<WT>, *scales = (lds_u8_t*)lds_x + kDownWaves * kDownRing<WT> + wave * kDownScales<WT>;
   f32x4_t sum = {0.f, 0.f, 0.f, 0.f}, acc = sum;
   int lk = s0 % per, uk = lk, li = s0 / per, ui = li;  // an item's step, and the item, of the loads and of the products
