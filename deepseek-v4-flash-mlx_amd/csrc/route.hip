@@ -10,7 +10,7 @@
 // is the logits', which needs no scores.  -inf and NaN rank last.
 //
 // route_kernel: 16 lanes a token, four tokens a wave, lane l holds experts l, l + 16, ..  A pick is a maximum over a lane's
-// values and four lane moves inside the row of 16 (DPP).  It ranks fp32 scores, whose error is below 2^-21 (1 + |r|)
+// values and four lane moves inside the row of 16 (DPP).  It ranks fp32 scores, whose error is below 2^-21 (1 + s + |r|)
 // (score32).  Where two neighbours of the order are closer than twice that (1 row in 300 of 256 random experts; never without
 // a bias), the k and the next one are put in the order of their float64 values; where that does not settle it, the last
 // group in and the first one out are as close, or anything is not finite, the whole wave ranks the token in float64
@@ -316,7 +316,14 @@ __global__ __launch_bounds__(64) void route_kernel(const RouteArgs a) {
     if (l < a.k) mine = a.given[row * a.k + l];
     bad = __any(bad) && SCORE == SMLA_SCORE_SOFTMAX ? bad : false;  // else each id's score stands alone
   } else {
+    float scale = 1.f;  // 1 + the largest score: a bias may take most of one away, but not its error
     if (add) {
+      if constexpr (SCORE == SMLA_SCORE_SQRTSOFTPLUS) {  // (the others' are 1 at most)
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; i++) s = fmaxf(s, v[i]);
+        scale += row_max(s);
+      }
 #pragma unroll
       for (int i = 0; i < V; i++) {
         v[i] = l + 16 * i < a.E ? v[i] + b[i] : -SMLA_INF;
@@ -330,6 +337,7 @@ __global__ __launch_bounds__(64) void route_kernel(const RouteArgs a) {
       const int spg = a.E / a.groups / 16;  // values a lane holds of a group
       int gv = kOutKey, b0 = gv, b1 = gv;   // lane g: group g's value
       int g = 0, left = spg;
+      float parts = 0.f;                    // the magnitudes that its sum is of
 #pragma unroll
       for (int i = 0; i < V; i++) {
         const int r = a.bias ? key[i] : to_key(v[i]);
@@ -346,7 +354,10 @@ __global__ __launch_bounds__(64) void route_kernel(const RouteArgs a) {
           merge([](int q) { return dpp_i<0x4E>(q); });
           merge([](int q) { return dpp_i<0x141>(q); });
           merge([](int q) { return dpp_i<0x140>(q); });
-          if (l == g) gv = g < a.groups ? to_key(of_key(c0) + of_key(c1)) : kOutKey;
+          if (l == g && g < a.groups) {
+            gv = to_key(of_key(c0) + of_key(c1));
+            parts = gv > kLowKey ? fabsf(of_key(c0)) + fabsf(of_key(c1)) : 0.f;
+          }
           g++, left = spg;
           b0 = b1 = kOutKey;
         }
@@ -359,8 +370,7 @@ __global__ __launch_bounds__(64) void route_kernel(const RouteArgs a) {
       const bool in = l < a.groups && before < a.topk_groups;
       const int last = row_min_i(in ? gv : 0x7fffffff), next = row_max_i(in ? kOutKey : gv);
       // (a group's value is the sum of two: twice the error)
-      if (a.topk_groups < a.groups)
-        bad |= !(of_key(last) - of_key(next) > 2.f * kTol * (1.f + fabsf(of_key(last)))) || last <= kLowKey;
+      if (a.topk_groups < a.groups) bad |= !(of_key(last) - of_key(next) > 2.f * kTol * (scale + row_max(parts))) || last <= kLowKey;
       uint32_t kept = (uint32_t)(__ballot(in) >> (lane & 48)) & 0xffffu;
       left = spg;
 #pragma unroll
@@ -392,7 +402,7 @@ __global__ __launch_bounds__(64) void route_kernel(const RouteArgs a) {
       top = best();
       if (a.bias) {
         const float now = of_key(top);
-        if (j > 0) close |= !(prev - now > kTol * (1.f + fabsf(prev))) && top != kOutKey;
+        if (j > 0) close |= !(prev - now > kTol * (scale + fabsf(prev))) && top != kOutKey;
         prev = now;
       }
       if (j == a.k) break;
@@ -405,7 +415,7 @@ __global__ __launch_bounds__(64) void route_kernel(const RouteArgs a) {
         pick(top, a.k);
         const int after = best();
         // (prev is the next one's value: what is apart from it is apart from the k-th)
-        if (close) bad |= top <= kLowKey || !(prev - of_key(after) > kTol * (1.f + fabsf(prev)) || after == kOutKey);
+        if (close) bad |= top <= kLowKey || !(prev - of_key(after) > kTol * (scale + fabsf(prev)) || after == kOutKey);
         double r = kOut;
         if (l <= a.k && mine < a.E) r = score_f64<SCORE>(load_as_f32(a.logits, at + mine, XDT)) + (double)a.bias[mine];
         int place = 0;

@@ -97,6 +97,28 @@ def test_route_order_next_to_a_border(dev):
                      om.route(x, 9, score, bias=b, groups=8, topk_groups=3))
 
 
+@pytest.mark.parametrize("groups", [1, 2])
+def test_route_large_scores_that_the_bias_takes_away(dev, groups):
+    """Scores of 100, whose fp32 steps are 2^-17, and biases that leave differences about as large; groups whose two
+    largest values are large and opposite."""
+    from smla import moe
+    announce(f"route cancelled {groups}")
+    E, k = 32, 3
+    for seed in range(200):
+        g = torch.Generator().manual_seed(seed)
+        x = 10000 + torch.randn(1, E, generator=g)
+        s = torch.tensor(om.scores(x.double().tolist()[0], "sqrtsoftplus"), dtype=torch.float64)
+        b = -s.float()
+        if seed % 2:                     # a few experts left near 0, all others far below
+            b -= 1000.0 * (torch.arange(E) % 16 > 2 + seed % 3)
+        if groups > 1:                   # two values of -+5100 to a group, which all but cancel
+            b = -20000.0 - 100.0 * torch.arange(E)
+            b[::16] = 5000.0
+            b[1::16] = (-(s[::16] + 5000.0 + s[1::16])).float()
+        kw = dict(bias=b, groups=groups, topk_groups=1)
+        _check_route(moe.route(x.to(dev), k, "sqrtsoftplus", **{**kw, "bias": b.to(dev)}), om.route(x, k, "sqrtsoftplus", **kw))
+
+
 def test_route_given_ids_strides_empty(dev):
     from smla import moe
     announce("route given ids")
