@@ -180,7 +180,8 @@ __host__ __device__ inline int64_t few_lds(int64_t n, int K, int nw, int r) {
 template <int WT>
 constexpr int kStaged = WT == kFp4 ? 1 : 0;
 
-// Workgroup (i, j): outputs 16 i .. of tokens 16 j .. .
+// Workgroup (i, j): outputs 16 i .. of tokens 16 j .. .  One token by 4096 x 8192 (17.8 MB): 6.3-6.8 us, 2.8 TB/s: one round
+// of 256 workgroups, a launch, two dependent latencies (weights; the sums through LDS) and 2.9 us of bytes.
 template <int WT, int NW, int YDT>
 __global__ __launch_bounds__(64 * NW) void linear_few_kernel(const uint16_t* __restrict__ x, int64_t ldx, Matrix w, int tokens, int N,
                                                              int K, void* __restrict__ y) {
@@ -254,6 +255,9 @@ __device__ inline float gated(float g, float u, float lim) {
 // tokens that have it: column m is the m-th of them.  A token that has it twice has the sum of its weights.  A wave has its
 // K range of the tokens' rows of x in LDS (in registers they would take three times the weights' and leave one workgroup a
 // CU), room for `cap` of them; an expert of more streams its weights again for the others.
+// Bound by HBM: 8 tokens x 6 of 256 experts of 4096 x 2048 (390 MB) 71-75 us, 5.3 TB/s, where a bare read of such rows reaches
+// 6.2; one token 13 us.  Four, six or eight steps in flight and 2, 4 or 8 waves take the same; two blocks of 16 rows a
+// workgroup, one behind the other, 2 us longer.
 constexpr int kUpWaves = 4;
 template <int WT>
 constexpr int kUpAhead = WT == kBf16 ? 2 : 4;
@@ -367,6 +371,9 @@ __global__ __launch_bounds__(64 * kUpWaves) __attribute__((amdgpu_waves_per_eu(4
 // wave's LDS a step ahead of the step's weights (256 bytes a token; as operands from memory they are four loads of 1 KB
 // a step, against one of the weights).  Column m is token m: a wave adds an item's sums to a token's only where the item
 // has it (0 times an infinite weight of another token's expert would be NaN).
+// The items come from few_up_kernel, which has the tokens of each expert at hand: listing them here took 2 us of every
+// workgroup.  8 tokens x 6 experts (200 MB) 41-45 us, 4.7 TB/s (with each step requested alone, half a 128-byte line a row,
+// 45-46; three to five steps in flight are alike); one token 8.7 us.
 constexpr int kDownWaves = 16;
 template <int WT>
 constexpr int kDownAhead = WT == kBf16 ? 3 : 4;
@@ -533,7 +540,8 @@ __global__ __launch_bounds__(1024) void plan_kernel(const ExpertArgs a) {
   });
 }
 
-// y[t] = the sum of its pairs' rows, in their order
+// y[t] = the sum of its pairs' rows, in their order.  Bound by HBM: 24576 rows of 4096 (403 MB) 80 us, 5.4 TB/s with y.  The rows
+// are fp32: bf16 ones would halve that, and round each of a token's k products as coarsely as y.
 __global__ __launch_bounds__(256) void combine_kernel(const ExpertArgs a) {
   const int t = blockIdx.y, n = (blockIdx.x * 256 + threadIdx.x) * 4;
   if (n >= a.K) return;
@@ -651,6 +659,11 @@ __device__ __attribute__((always_inline)) inline void tile_body(const TileArgs& 
   }
 }
 
+// Figures.  4-bit, 128 x 512: 4096 x 4096 x 8192 in 186-196 us, 1.40-1.48 PFLOP/s (an 8192^3 bf16 library product: 1.29), bound by
+// the products; 256 experts of 4096 x 2048 with 96 pairs each, the up products 805 us, 1.02 PFLOP/s (128 each 1.17, 256 each 1.3:
+// what a tile lacks of its rows costs about as much as what is there).  32 x 256: 100 tokens x 6 of those experts, up 371-460
+// and down 195-239 us for 3.1 GB, bound by HBM at 5.2-5.4 TB/s over the call.  bf16: 24 experts of 2048 x 1408, 1000 pairs, up
+// 84 us and down 32 for 415 MB: 264 tiles leave 8 CUs with two.
 template <class L, int MODE, int YDT>
 __global__ __launch_bounds__(L::THREADS) void tile_kernel(const TileArgs a) {
   extern __shared__ __align__(16) uint8_t lds_t[];

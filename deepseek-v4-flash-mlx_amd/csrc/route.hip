@@ -16,7 +16,9 @@
 // group in and the first one out are as close, or anything is not finite, the whole wave ranks the token in float64
 // (rank_f64).  The weights are of float64 scores, of the k picked alone (softmax: the sum over the row is of fp32
 // exponentials).
-// What bounds it is issue: a pick is about 85 instructions for four tokens of 256 experts.
+// What bounds it is issue: a pick is about 85 instructions for four tokens of 256 experts.  16384 tokens of 256 experts in 8
+// groups, k = 8: 19-22 us (17.8 MB, 2.9 us of bytes); 1031 tokens of 100, k = 4: 4.2 us; one token 5.6 us (three dependent
+// latencies and float64 weights).
 // route_f64_kernel: one token a wave in float64 throughout, for what the first does not take.
 #include "smla_internal.h"
 

@@ -653,15 +653,16 @@ int smla_compact_pages(const int32_t* table, int64_t ld_table, int64_t S, int64_
  *
  * smla_linear_fp4: y[t, n] = sum_k x[t, k] W[n, k], W[n, k] = e2m1(codes) 2^(scales[n, k / 32] - 127).
  *   x [T, K] BF16, ldx elements between rows (a multiple of 8; K a multiple of 32); codes [N, K / 2], scales [N, K / 32]
- *   as smla_rotate_fp4 writes them; y [T, N] F32 or BF16; fp32 sums of exact products; x and codes 16-byte aligned.
+ *   as smla_rotate_fp4 writes them; y [T, N] F32 or BF16; fp32 sums of exact products; x, codes and y 16-byte aligned,
+ *   scales 4-byte aligned where K is a multiple of 128.  T and N <= 2^24, K and ldx <= 2^22 (SMLA_E_UNSUPPORTED past it).
  *   workspace: smla_linear_fp4_workspace bytes (may be 0), 16-byte aligned; SMLA_E_WORKSPACE where there is less.
  *
  * smla_experts: y[t] = sum_j down_e(h_tj), h_tj = weights[t, j] silu(min(g, limit)) clamp(u, -limit, limit),
  *   g = gate_e x[t], u = up_e x[t], e = ids[t, j]; an id outside 0 .. E-1 adds nothing (a token without any gives 0).
  *   x [T, K] BF16 (ldx as above), ids [T, k] int32, weights [T, k] fp32; gate, up [E, I, K] and down [E, K, I], all BF16
  *   (scales NULL) or all SMLA_FP4_E2M1 (codes, and scale bytes per 32); K and I multiples of 32, E <= 1024, k <= 64;
- *   y [T, K] BF16; limit > 0, infinity for none.  fp32 sums; h is rounded to bf16.  Tensors but the scales, ids and weights
- *   16-byte aligned.  workspace: smla_experts_workspace bytes, 16-byte aligned (SMLA_E_WORKSPACE otherwise). */
+ *   y [T, K] BF16; limit > 0, infinity for none.  fp32 sums; h is rounded to bf16.  x, y and the matrices 16-byte aligned,
+ *   scales 4-byte.  T k, K, I and ldx <= 2^20, T ldx < 2^30 (SMLA_E_UNSUPPORTED past it).  workspace: smla_experts_workspace bytes, 16-byte aligned (SMLA_E_WORKSPACE otherwise). */
 enum { SMLA_SCORE_SOFTMAX = 0, SMLA_SCORE_SIGMOID = 1, SMLA_SCORE_SQRTSOFTPLUS = 2 };
 int smla_route(const void* logits, int dtype, int64_t ld, const float* bias, int64_t T, int64_t E, int64_t k, int score,
                int64_t groups, int64_t topk_groups, int renorm, double scale, int64_t shared, const int32_t* given,
