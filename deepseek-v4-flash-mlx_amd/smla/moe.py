@@ -90,6 +90,8 @@ class ExpertLayer:
     def __call__(self, xn, tokens=None):
         """xn [..., K] bf16 -> [..., K] bf16.  ``tokens`` [...]: the token ids, which a layer with a table chooses by."""
         x = xn.reshape(-1, xn.shape[-1])
+        if x.shape[0] == 0:
+            return torch.empty_like(xn)
         ids = None
         if self.w.table is not None:
             if tokens is None:

@@ -239,6 +239,9 @@ EXPERTS = [  # T, E, of, k, K, I, weights, limit
     (40, 8, 16, 2, 288, 96, "fp4", None), (64, 3, 3, 2, 128, 128, "bf16", 10.0), (100, 40, 40, 6, 160, 64, "fp4", 10.0),
     (130, 2, 2, 1, 64, 96, "fp4", None), (257, 7, 9, 3, 192, 224, "bf16", None), (300, 1000, 1000, 4, 64, 32, "fp4", 2.0),
     (513, 4, 4, 2, 384, 64, "fp4", 10.0), (600, 16, 16, 1, 96, 288, "bf16", 10.0),
+    (16, 64, 64, 64, 64, 32, "fp4", None), (16, 1024, 1024, 64, 64, 32, "bf16", 10.0), (16, 2, 2, 2, 4096, 32, "fp4", 10.0),
+    (16, 2, 2, 1, 4352, 64, "fp4", None), (5, 3, 3, 2, 32, 4096, "fp4", 10.0), (300, 2, 2, 2, 416, 352, "fp4", 10.0),
+    (20, 64, 64, 64, 96, 64, "bf16", None), (900, 1024, 1024, 1, 128, 64, "fp4", None), (50, 2, 2, 1, 96, 4128, "bf16", 10.0),
 ]
 
 
@@ -429,6 +432,7 @@ def test_layer_by_token(dev):
     tokens = torch.randint(0, 50, (3, 7), generator=torch.Generator().manual_seed(10))
     y = layer(x.to(dev), tokens.to(dev))
     assert y.shape == x.shape
+    assert layer(x[:0].to(dev), tokens[:0].to(dev)).shape == (0, 7, K)
     flat = x.view(-1, K)
     ids, w = om.route(layer.logits(flat.to(dev)).cpu(), k, "sqrtsoftplus", ids=table[tokens.view(-1)], scale=1.5, shared=1)
     _check_experts(y.view(-1, K), om.experts(flat, ids, w.float(), *dense, 10.0))
