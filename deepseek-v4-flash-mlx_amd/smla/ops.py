@@ -35,8 +35,8 @@ def _stream(t):
 # The eager route of the ops below.  A torch.library op's dispatch (schema, autograd and python
 # fallback layers) costs more host time than a decode step's kernels take; plain tensors under
 # nothing that needs the op itself skip it and run the op's own body.  linear of one token: 17 -> 10 us.
-_PLAIN = (torch.Tensor, torch.nn.Parameter)
-_VALUES = (int, float, bool, type(None), torch.dtype)
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter))
+_VALUES = frozenset((int, float, bool, type(None), torch.dtype))
 try:
     _raw_stream = torch._C._cuda_getCurrentRawStream
 except AttributeError:      # a torch built without it
@@ -62,10 +62,10 @@ def _eager(args):
         return False
     grad = _grad_enabled()
     for a in args:
-        if type(a) in _PLAIN:
-            if not a.is_cuda or a.is_neg() or (grad and a.requires_grad):
-                return False
-        elif type(a) not in _VALUES:
+        t = type(a)
+        if t in _VALUES:
+            continue
+        if t not in _PLAIN or not a.is_cuda or a.is_neg() or (grad and a.requires_grad):
             return False
     return True
 
@@ -1227,10 +1227,11 @@ def _workspace(dev, name, *sizes):
 
 def _rows(x, K, name):
     """x [T, K] bf16 as a tensor whose rows are 16-byte aligned, and the elements between them."""
-    if x.dim() != 2 or x.shape[1] != K or x.dtype != torch.bfloat16:
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != K or x.dtype != torch.bfloat16:
         raise ValueError(f"{name} must be bf16 [T, {K}], got {x.dtype} {list(x.shape)}")
     ld, s1 = x.stride()
-    if x.shape[0] <= 1:
+    if shape[0] <= 1:
         ld = K
     if s1 != 1 or ld < K or ld % 8 or x.data_ptr() & 15:
         return x.clone(memory_format=torch.contiguous_format), K
