@@ -9,16 +9,17 @@
 // fp32 step apart would otherwise trade places with the formula's rounding.  Without a bias the scores' order
 // is the logits', which needs no scores.  -inf and NaN rank last.
 //
-// route_kernel: 16 lanes a token, four tokens a wave, lane l holds experts l, l + 16, ..  A pick is a maximum over a lane's
-// values and four lane moves inside the row of 16 (DPP).  It ranks fp32 scores, whose error is below 2^-21 (1 + s + |r|)
-// (score32).  Where two neighbours of the order are closer than twice that (1 row in 300 of 256 random experts; never without
-// a bias), the k and the next one are put in the order of their float64 values; where that does not settle it, the last
-// group in and the first one out are as close, or anything is not finite, the whole wave ranks the token in float64
-// (rank_f64).  The weights are of float64 scores, of the k picked alone (softmax: the sum over the row is of fp32
+// route_kernel: 16 lanes a token, four tokens a wave, lane l holds experts l, l + 16, .. as integers of the values' order, whose
+// last 4 (5) bits are the place in the lane.  Each lane sorts its own, and a pick is a maximum over the lanes' first ones (lane
+// moves inside the row of 16, DPP).  It ranks fp32 scores, whose error is below 2^-21 (1 + s + |r|) (score32).  Where two
+// neighbours of the order are closer than twice that and the last bits (1 row in some hundreds of 256 random experts; never
+// for bf16 logits without a bias), the k and the next one are put in the order of their float64 values; where that does not
+// settle it, the last group in and the first one out are as close, or anything is not finite, the whole wave ranks the token in
+// float64 (rank_f64).  The weights are of float64 scores, of the k picked alone (softmax: the sum over the row is of fp32
 // exponentials).
-// What bounds it is issue: a pick is about 85 instructions for four tokens of 256 experts.  16384 tokens of 256 experts in 8
-// groups, k = 8: 19-22 us (17.8 MB, 2.9 us of bytes); 1031 tokens of 100, k = 4: 4.2 us; one token 5.6 us (three dependent
-// latencies and float64 weights).
+// What bounds it is issue and latency: 16384 tokens of 256 experts in 8 groups, k = 8, 17.6-20 us (17.8 MB, 2.9 us of bytes;
+// 19-22 where each pick searched a lane's 16 values, about 85 instructions for four tokens against 35 and 130 for the sort);
+// 1031 tokens of 100, k = 4, 4.1 us; one token 4.5 us (three dependent latencies and float64 weights).
 // route_f64_kernel: one token a wave in float64 throughout, for what the first does not take.
 #include "smla_internal.h"
 
@@ -269,6 +270,21 @@ __device__ inline float score32(float x) {
 
 constexpr float kTol = 0x1p-20f;  // twice a score's error
 
+// a lane's keys, largest first (Batcher's odd-even merge sort)
+template <int V>
+__device__ inline void sort_keys(int (&key)[V]) {
+#pragma unroll
+  for (int p = 1; p < V; p *= 2)
+#pragma unroll
+    for (int d = p; d >= 1; d /= 2)
+#pragma unroll
+      for (int i = 0; i + d < V; i++)
+        if (i >= d % p && (i - d % p) / d % 2 == 0 && i / (2 * p) == (i + d) / (2 * p)) {
+          const int a = key[i], b = key[i + d];
+          key[i] = max(a, b), key[i + d] = min(a, b);
+        }
+}
+
 template <int XDT, int SCORE, int V>
 __global__ __launch_bounds__(64) void route_kernel(const RouteArgs a) {
   constexpr int V64 = (V + 3) / 4;
@@ -381,45 +397,52 @@ __global__ __launch_bounds__(64) void route_kernel(const RouteArgs a) {
         if (--left == 0) kept >>= 1, left = spg;
       }
     }
-    auto best = [&]() __attribute__((always_inline)) {
-      int top = key[0];
+    // A lane's values in order, the place among its 16 (32) instead of the last bits: a pick takes from the lanes' first ones
+    constexpr int kPlace = V <= 16 ? 15 : 31;
 #pragma unroll
-      for (int i = 1; i < V; i++) top = max(top, key[i]);
-      return row_max_i(top);
-    };
+    for (int i = 0; i < V; i++) key[i] = key[i] == kOutKey ? kOutKey : (key[i] & ~kPlace) | (kPlace - i);
+    sort_keys<V>(key);
+    auto best = [&]() __attribute__((always_inline)) { return row_max_i(key[0]); };
     auto pick = [&](int top, int j) __attribute__((always_inline)) {  // its lowest id to lane j, out of the running
-      int slot = V;
+      const int from = row_min_i(key[0] == top ? l : 16);
+      const bool pop = l == from;
 #pragma unroll
-      for (int i = V - 1; i >= 0; i--) slot = key[i] == top ? i : slot;
-      const int id = row_min_i(slot * 16 + l);
-      slot = (id & 15) == l ? id >> 4 : V;
-#pragma unroll
-      for (int i = 0; i < V; i++) key[i] = slot == i ? kOutKey : key[i];
-      if (l == j) mine = id;
+      for (int i = 0; i + 1 < V && i < 16; i++) key[i] = pop ? key[i + 1] : key[i];
+      if (V <= 16) key[V - 1] = pop ? kOutKey : key[V - 1];
+      if (l == j) mine = (kPlace - (top & kPlace)) * 16 + from;
     };
-    bool close = false;  // neighbours in the order that fp32 cannot tell apart
+    // Neighbours in the order that the keys cannot tell apart: the scores' error, and what the last bits were worth
+    // (bf16 logits have none there)
+    const bool exact = XDT == SMLA_BF16 && !a.bias;
+    const float lost = V <= 16 ? 0x1p-18f : 0x1p-17f, tol0 = a.bias ? kTol * scale : 0.f, tol1 = a.bias ? kTol + lost : lost;
+    bool close = false;
     float prev = SMLA_INF;
     int top;
     for (int j = 0;; j++) {
       top = best();
-      if (a.bias) {
-        const float now = of_key(top);
-        if (j > 0) close |= !(prev - now > kTol * (scale + fabsf(prev))) && top != kOutKey;
+      if (!exact) {
+        const float now = of_key(top & ~kPlace);
+        if (j > 0) close |= !(prev - now > fmaf(tol1, fabsf(prev), tol0)) && top != kOutKey;
         prev = now;
       }
       if (j == a.k) break;
-      bad |= top <= kLowKey;
+      bad |= (top | kPlace) <= kLowKey;
       pick(top, j);
     }
     if (__any(close)) {
       // the k and the next one in the order of their float64 values, a lane each; the one after it has to be apart
-      if (SCORE != SMLA_SCORE_SOFTMAX && a.k < 16) {
+      if ((SCORE != SMLA_SCORE_SOFTMAX || !a.bias) && a.k < 16) {
         pick(top, a.k);
         const int after = best();
         // (prev is the next one's value: what is apart from it is apart from the k-th)
-        if (close) bad |= top <= kLowKey || !(prev - of_key(after) > kTol * (scale + fabsf(prev)) || after == kOutKey);
+        if (close)
+          bad |= (top | kPlace) <= kLowKey || !(prev - of_key(after & ~kPlace) > fmaf(tol1, fabsf(prev), tol0) || after == kOutKey);
         double r = kOut;
-        if (l <= a.k && mine < a.E) r = score_f64<SCORE>(load_as_f32(a.logits, at + mine, XDT)) + (double)a.bias[mine];
+        if (l <= a.k && mine < a.E) {
+          const float y = load_as_f32(a.logits, at + mine, XDT);
+          if constexpr (SCORE == SMLA_SCORE_SOFTMAX) r = y;
+          else r = a.bias ? score_f64<SCORE>(y) + (double)a.bias[mine] : y;
+        }
         int place = 0;
 #pragma unroll
         for (int o = 1; o < 16; o++) {
