@@ -512,7 +512,7 @@ extern "C" int smla_route(const void* logits, int dtype, int64_t ld, const float
   if (T < 0 || E <= 0 || k <= 0 || groups <= 0 || topk_groups <= 0 || shared < 0 || (T > 1 && ld < E)) return SMLA_E_SHAPE;
   if (score < SMLA_SCORE_SOFTMAX || score > SMLA_SCORE_SQRTSOFTPLUS || !(scale == scale)) return SMLA_E_RANGE;
   if (!given && (E % groups != 0 || topk_groups > groups || k > topk_groups * (E / groups))) return SMLA_E_SHAPE;
-  if (E > 1024 || k + shared > 64 || T > 0x7fffffff) return SMLA_E_UNSUPPORTED;
+  if (E > 1024 || k + shared > 64 || T >= 1 << 26) return SMLA_E_UNSUPPORTED;  // (a grid holds 2^32 threads)
   if (T == 0) return SMLA_OK;
   if (!logits || !ids || !weights) return SMLA_E_NULL;
   const RouteArgs a{logits, ld, bias, ids, weights, T, given, (int)E, (int)k, (int)groups, (int)topk_groups, renorm != 0, (int)shared, scale};

@@ -638,7 +638,7 @@ int smla_compact_pages(const int32_t* table, int64_t ld_table, int64_t S, int64_
 /* ---------------------------------------------------------------------------------------------
  * The expert network (oracle/decode_engine.py:122-133): routing, products with 4-bit weights, the experts.
  *
- * smla_route: each token's k experts of E (E <= 1024, k + shared <= 64) and their weights.
+ * smla_route: each token's k experts of E (E <= 1024, k + shared <= 64, T < 2^26) and their weights.
  *   logits [T, E] F32 or BF16, ld elements between rows;  s = softmax over the row, sigmoid or sqrt(softplus) of
  *   each (SMLA_SCORE_*);  r = s + bias (bias [E] fp32 or NULL: none);
  *   groups > 1 (E a multiple): a group of E / groups consecutive experts is worth the sum of its two largest r,

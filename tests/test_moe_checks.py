@@ -29,7 +29,7 @@ ROUTE_OK = dict(logits=FAKE, dtype=F32, ld=64, bias=None, T=0, E=64, k=6, score=
     (dict(groups=16, topk_groups=1, k=5), SHAPE), (dict(k=65), SHAPE), (dict(k=60, shared=5), UNSUP),
     (dict(E=1025, ld=1025), UNSUP), (dict(score=3), RANGE), (dict(score=-1), RANGE), (dict(scale=float("nan")), RANGE),
     (dict(T=1, logits=None), NULL), (dict(T=1, ids=None), NULL), (dict(T=1, weights=None), NULL),
-    (dict(logits=None), OK), (dict(groups=7, given=FAKE), OK),
+    (dict(logits=None), OK), (dict(groups=7, given=FAKE), OK), (dict(T=1 << 26), UNSUP),
 ])
 def test_route_status(change, status):
     assert _call("smla_route", ROUTE, ROUTE_OK, **change) == status
@@ -44,6 +44,7 @@ LINEAR_OK = dict(x=FAKE, ldx=64, codes=FAKE, scales=FAKE, T=0, N=10, K=64, y=FAK
     (dict(y_dtype=F16), DTYPE), (dict(y_dtype=FP8), DTYPE),
     (dict(T=1, x=None), NULL), (dict(T=1, codes=None), NULL), (dict(T=1, scales=None), NULL), (dict(T=1, y=None), NULL),
     (dict(T=1, K=80, ldx=80), UNSUP), (dict(T=1, ldx=68), UNSUP), (dict(T=1, x=ODD), UNSUP), (dict(T=1, codes=ODD), UNSUP),
+    (dict(T=1, y=ODD), UNSUP), (dict(T=1, K=128, ldx=128, scales=ctypes.c_void_p(4097)), UNSUP),
     (dict(T=1 << 40), UNSUP), (dict(T=1, N=1 << 40), UNSUP), (dict(T=1, K=1 << 40, ldx=1 << 40), UNSUP),
 ])
 def test_linear_fp4_status(change, status):
@@ -63,6 +64,8 @@ EXPERTS_OK = dict(x=FAKE, ldx=64, ids=FAKE, weights=FAKE, T=0, k=2, E=8, K=64, I
     (dict(T=1, K=80, ldx=80), UNSUP), (dict(T=1, I=48), UNSUP), (dict(T=1, E=1025), UNSUP), (dict(T=1, k=65), UNSUP),
     (dict(T=1, ldx=68), UNSUP), (dict(T=1, x=ODD), UNSUP), (dict(T=1, gate=ODD), UNSUP), (dict(T=1, up=ODD), UNSUP),
     (dict(T=1, down=ODD), UNSUP), (dict(T=1, y=ODD), UNSUP), (dict(T=1 << 40), UNSUP),
+    *[(dict(T=1, **{n: ctypes.c_void_p(4097)}), UNSUP) for n in ("gate_scales", "up_scales", "down_scales")],
+    (dict(T=1 << 20, ldx=1024), UNSUP), (dict(T=1 << 19, k=1, ldx=2048), UNSUP),
     *[(dict(T=1, **{n: None}), NULL) for n in ("x", "ids", "weights", "gate", "up", "down", "y", "gate_scales", "up_scales", "down_scales")],
     (dict(T=1, limit=0.0), RANGE), (dict(T=1, limit=-1.0), RANGE), (dict(T=1, limit=float("nan")), RANGE),
     (dict(T=1, ws=None), WS), (dict(T=1, ws_bytes=15), WS), (dict(T=1, ws=ctypes.c_void_p(4104)), WS),
