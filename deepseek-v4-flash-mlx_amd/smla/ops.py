@@ -1225,15 +1225,16 @@ def _workspace(dev, name, *sizes):
         return getattr(_lib.lib(), name)(*sizes)
 
 
-def _rows(x, K, name):
-    """x [T, K] bf16 as a tensor whose rows are 16-byte aligned, and the elements between them."""
+def _rows(x, K, name, most=1 << 22, whole=1 << 62):
+    """x [T, K] bf16 as a tensor whose rows are 16-byte aligned, and the elements between them: up to ``most``, and less than
+    ``whole`` in all (what the kernels address); packed where it is not."""
     shape = x.shape
     if len(shape) != 2 or shape[1] != K or x.dtype != torch.bfloat16:
         raise ValueError(f"{name} must be bf16 [T, {K}], got {x.dtype} {list(x.shape)}")
     ld, s1 = x.stride()
     if shape[0] <= 1:
         ld = K
-    if s1 != 1 or ld < K or ld % 8 or x.data_ptr() & 15:
+    if s1 != 1 or ld < K or ld % 8 or x.data_ptr() & 15 or ld > K and (ld > most or shape[0] * ld >= whole):
         return x.clone(memory_format=torch.contiguous_format), K
     return x, ld
 
@@ -1331,7 +1332,8 @@ linear_fp4_op = _with_eager_route(linear_fp4_op, _linear_fp4)
 def _experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: torch.Tensor, up: torch.Tensor,
              down: torch.Tensor, gate_scales: Optional[torch.Tensor], up_scales: Optional[torch.Tensor],
              down_scales: Optional[torch.Tensor], limit: float) -> torch.Tensor:
-    """``smla_experts`` (see ``moe.experts``): -> [T, K] bf16."""
+    """``smla_experts`` (see ``moe.experts``): -> [T, K] bf16.  A call takes up to 2^20 choices and less than 2^30 elements of
+    x; more tokens are as many calls, one behind the other in one workspace (tokens do not see each other)."""
     dev = _one_device(x, ids, weights, gate, up, down, gate_scales, up_scales, down_scales)
     if gate.dim() != 3 or x.dim() != 2 or ids.dim() != 2:
         raise ValueError("expected x [T, K], ids [T, k] and gate [E, I, K]")
@@ -1352,7 +1354,7 @@ def _experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: to
         raise ValueError("the experts' weights must be 16-byte aligned")
     if fp4 and (gate_scales.data_ptr() | up_scales.data_ptr() | down_scales.data_ptr()) & 3:
         raise ValueError("the experts' scales must be 4-byte aligned")
-    x, ld = _rows(x, K, "x")
+    x, ld = _rows(x, K, "x", 1 << 20, 1 << 30)
     T = x.shape[0]
     k = ids.shape[1]
     ids = _i32(ids, (T, k), "ids")
@@ -1363,10 +1365,18 @@ def _experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: to
     if T == 0:
         return y
     wdt = _lib.FP4_E2M1 if fp4 else _lib.BF16
-    wsb = _workspace(dev, "smla_experts_workspace", T, k, E, K, inner, wdt)
+    n = T
+    if T * k > 1 << 20 or T * ld >= 1 << 30:
+        most = max(1, min((1 << 20) // max(k, 1), ((1 << 30) - 1) // ld))
+        n = -(-T // -(-T // most))      # as many tokens a call, the last one's rest aside
+    wsb = _workspace(dev, "smla_experts_workspace", n, k, E, K, inner, wdt)
+    if T % n:
+        wsb = max(wsb, _workspace(dev, "smla_experts_workspace", T % n, k, E, K, inner, wdt))
     ws = torch.empty(wsb, dtype=torch.uint8, device=x.device) if wsb else None
-    _launch(dev, "smla_experts", x.data_ptr(), ld, ids.data_ptr(), weights.data_ptr(), T, k, E, K, inner, gate.data_ptr(),
-            _p(gate_scales), up.data_ptr(), _p(up_scales), down.data_ptr(), _p(down_scales), wdt, limit, y.data_ptr(), _p(ws), wsb)
+    for t in range(0, T, n):
+        _launch(dev, "smla_experts", x.data_ptr() + 2 * ld * t, ld, ids.data_ptr() + 4 * k * t, weights.data_ptr() + 4 * k * t,
+                min(n, T - t), k, E, K, inner, gate.data_ptr(), _p(gate_scales), up.data_ptr(), _p(up_scales), down.data_ptr(),
+                _p(down_scales), wdt, limit, y.data_ptr() + 2 * K * t, _p(ws), wsb)
     return y
 
 

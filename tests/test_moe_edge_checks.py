@@ -1,0 +1,59 @@
+"""CPU tier: what the expert network's wrappers ask of the library, with the launches recorded instead of made."""
+import pytest
+import torch
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The arguments of every launch, from CPU tensors."""
+    from smla import _lib, ops
+    made = []
+    monkeypatch.setattr(ops, "_one_device", lambda t, *rest: 0)
+    monkeypatch.setattr(ops, "_launch", lambda dev, name, *args: made.append((name, args)))
+    monkeypatch.setattr(ops, "_workspace", lambda dev, name, *sizes: getattr(_lib.lib(), name)(*sizes))
+    return made
+
+
+def _bf16(*shape):
+    return torch.zeros(*shape, dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("T,k,K,ld", [
+    (1, 1, 32, 32), (16, 6, 64, 72), ((1 << 20) - 1, 1, 32, 32), (1 << 20, 1, 32, 32), ((1 << 20) + 1, 1, 32, 32), (174763, 6, 32, 32),
+    (300000, 7, 32, 40), (33, 64, 32, 32), (16385, 64, 32, 32), (1100, 2, 32, 1 << 20), (1023, 2, 32, 1 << 20), (3, 2, 32, (1 << 20) + 8),
+    (1 << 17, 1, 8192, 8192), ((1 << 17) - 1, 1, 8192, 8192), (300000, 1, 8192, 8192),
+])
+def test_experts_of_any_number_of_tokens(calls, T, k, K, ld):
+    """Every call is within the library's limits, in order, and together they are all tokens; x stays where it is unless its rows
+    lie too far apart."""
+    from smla import ops
+    inner, E = 32, 2
+    x = torch.empty_strided((T, K), (ld, 1), dtype=torch.bfloat16)       # (never written: no memory behind it)
+    ids, w = torch.zeros(T, k, dtype=torch.int32), torch.zeros(T, k)
+    y = ops._experts(x, ids, w, _bf16(E, inner, K), _bf16(E, inner, K), _bf16(E, K, inner), None, None, None, 1.0)
+    assert y.shape == (T, K)
+    at = 0
+    for name, a in calls:
+        xp, ldx, ip, wp, n, kk, ee, KK, ii = a[:9]
+        yp, _, wsb = a[-3:]
+        assert name == "smla_experts" and (kk, ee, KK, ii) == (k, E, K, inner)
+        assert 0 < n and n * k <= 1 << 20 and ldx <= 1 << 20 and ldx % 8 == 0 and (n == 1 or n * ldx < 1 << 30)
+        if T * ld < 1 << 30 and ld <= 1 << 20:
+            assert ldx == (ld if T > 1 else K) and xp == x.data_ptr() + 2 * ldx * at
+        assert ip == ids.data_ptr() + 4 * k * at and wp == w.data_ptr() + 4 * k * at and yp == y.data_ptr() + 2 * K * at
+        assert xp % 16 == yp % 16 == 0
+        from smla import _lib
+        assert wsb >= _lib.lib().smla_experts_workspace(n, k, E, K, inner, _lib.BF16)
+        at += n
+    assert at == T
+    fewest = max(-(-T * k // (1 << 20)), -(-T * K // ((1 << 30) - 1)))
+    assert len(calls) <= fewest + 1
+
+
+def test_products_of_rows_that_lie_far_apart(calls):
+    from smla import ops
+    codes, scales = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
+    for ld, want in (((1 << 22), 1 << 22), ((1 << 22) + 8, 64)):
+        x = torch.empty_strided((3, 64), (ld, 1), dtype=torch.bfloat16)
+        ops._linear_fp4(x, codes, scales, torch.float32)
+        assert calls[-1][1][1] == want
