@@ -88,7 +88,8 @@ class ExpertLayer:
         return ops.linear_op(xn if r.dtype == xn.dtype else xn.to(r.dtype), r, 1, torch.float32)
 
     def __call__(self, xn, tokens=None):
-        """xn [..., K] bf16 -> [..., K] bf16.  ``tokens`` [...]: the token ids, which a layer with a table chooses by."""
+        """xn [..., K] bf16 -> [..., K] bf16.  ``tokens`` [...]: the token ids, which a layer with a table chooses by; one outside
+        the table (a padded batch's) has the shared experts alone."""
         x = xn.reshape(-1, xn.shape[-1])
         if x.shape[0] == 0:
             return torch.empty_like(xn)
@@ -96,6 +97,9 @@ class ExpertLayer:
         if self.w.table is not None:
             if tokens is None:
                 raise ValueError("this layer chooses its experts by token: tokens are needed")
-            ids = self.w.table[tokens.reshape(-1).long()]
+            table = self.w.table
+            at = tokens.reshape(-1).to(table.device, torch.long)
+            row = at.clamp(0, table.shape[0] - 1)       # (no row is read that is not there)
+            ids = table[row].masked_fill_((row != at)[:, None], -1)
         ids, weights = route(self.logits(x), self.k, bias=self.w.bias, shared=self.shared, ids=ids, **self.choice)
         return experts(x, ids, weights, self.w.gate, self.w.up, self.w.down, self.limit).view(xn.shape)

@@ -6,7 +6,7 @@ import torch
 
 from conftest import announce
 from oracle import moe as om
-from test_gpu_moe import _check_experts, _experts_case, _on, _packed
+from test_gpu_moe import _check_experts, _experts_case, _layer, _on, _packed
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +44,30 @@ def test_rows_that_lie_far_apart(dev):
         near, i, v = x[:T].to(dev), ids[:T].to(dev), w[:T].to(dev)
         assert torch.equal(moe.experts(far, i, v, *on), moe.experts(near, i, v, *on))
         assert torch.equal(mla.linear_fp4(far, codes, scales), mla.linear_fp4(near, codes, scales))
+
+
+def test_layer_of_tokens_outside_the_table(dev):
+    """A padded batch's token ids (-1, the vocabulary's size, far past it) have the shared expert alone, the others their rows'
+    experts; eager and captured."""
+    announce("layer of tokens outside the table")
+    E, k, K, I, V = 16, 2, 128, 64, 50
+    table = torch.randint(0, E, (V, k), generator=torch.Generator().manual_seed(8), dtype=torch.int32)
+    layer, _, _, dense = _layer(dev, E, k, K, I, 1, "fp4", table)
+    x = torch.randn(2, 4, K, generator=torch.Generator().manual_seed(9)).to(torch.bfloat16)
+    tokens = torch.tensor([[0, V - 1, -1, V], [7, -V, 2 ** 31 - 1, -2 ** 31]])
+    flat, t = x.view(-1, K), tokens.view(-1)
+    inside = (t >= 0) & (t < V)
+    given = torch.where(inside[:, None], table[t.clamp(0, V - 1)], -1).to(torch.int32)
+    ids, w = om.route(layer.logits(flat.to(dev)).cpu(), k, "sqrtsoftplus", ids=given, scale=1.5, shared=1)
+    want = om.experts(flat, ids, w.float(), *dense, 10.0)
+    xd, td = x.to(dev), tokens.to(dev)
+    y = layer(xd, td)
+    _check_experts(y.view(-1, K), want)
+    assert torch.equal(layer(xd, td.int()), y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        z = layer(xd, td)
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(z, y)
+        torch.cuda.synchronize()

@@ -57,3 +57,21 @@ def test_products_of_rows_that_lie_far_apart(calls):
         x = torch.empty_strided((3, 64), (ld, 1), dtype=torch.bfloat16)
         ops._linear_fp4(x, codes, scales, torch.float32)
         assert calls[-1][1][1] == want
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
+def test_tokens_outside_the_table_choose_nothing(monkeypatch, dtype):
+    """A layer that chooses by token (a padded batch's -1, an id past the vocabulary): ids of -1, which add nothing, in place of a
+    row that is another token's or no row at all."""
+    from smla import moe, ops
+    seen = []
+    monkeypatch.setattr(ops, "linear_op", lambda x, w, groups, dt: torch.zeros(x.shape[0], w.shape[0], dtype=dt))
+    monkeypatch.setattr(moe, "route", lambda logits, k, ids=None, **kw: (seen.append(ids), (ids, None))[1])
+    monkeypatch.setattr(moe, "experts", lambda x, *rest: x.clone())
+    w = _bf16(3, 32, 64)
+    table = torch.arange(10, dtype=torch.int32).view(5, 2)
+    layer = moe.ExpertLayer(moe.ExpertWeights(_bf16(3, 64), w, w, w, table=table), k=2)
+    tokens = torch.tensor([[0, 4, -1, 3], [5, -5, 1, torch.iinfo(dtype).max]], dtype=dtype)
+    assert layer(_bf16(2, 4, 64), tokens).shape == (2, 4, 64)
+    assert seen[0].tolist() == [[0, 1], [8, 9], [-1, -1], [6, 7], [-1, -1], [-1, -1], [2, 3], [-1, -1]]
+    assert table.tolist() == [[0, 1], [2, 3], [4, 5], [6, 7], [8, 9]] and seen[0].dtype == torch.int32
