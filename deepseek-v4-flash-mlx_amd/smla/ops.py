@@ -482,7 +482,7 @@ def rotate_fp4_op(x: torch.Tensor, rotate: bool, fp4: bool, want_out: bool,
                   want_codes: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """x [..., n] fp32/bf16 (n a power of two, 32..1024) -> (out fp32 [..., n], packed e2m1 codes
     uint8 [..., n/2], ue8m0 scales uint8 [..., n/32]); outputs not asked for come back empty."""
-    _on_gpu(x)
+    dev = _one_device(x)
     if x.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("rotate_fp4 takes fp32 or bf16")
     if want_codes and not fp4:
@@ -494,8 +494,8 @@ def rotate_fp4_op(x: torch.Tensor, rotate: bool, fp4: bool, want_out: bool,
     codes = torch.empty((*x.shape[:-1], n // 2) if want_codes else (0,), dtype=torch.uint8, device=x.device)
     scales = torch.empty((*x.shape[:-1], n // 32) if want_codes else (0,), dtype=torch.uint8, device=x.device)
     flags = (_lib.QAT_ROTATE if rotate else 0) | (_lib.QAT_FP4 if fp4 else 0)
-    _lib.call("smla_rotate_fp4", _p(x), dtype_code(x), rows, n, flags, _p(out) if want_out else None,
-              _p(codes) if want_codes else None, _p(scales) if want_codes else None, _stream(x))
+    _launch(dev, "smla_rotate_fp4", _p(x), dtype_code(x), rows, n, flags, _p(out) if want_out else None,
+            _p(codes) if want_codes else None, _p(scales) if want_codes else None)
     return out, codes, scales
 
 
@@ -514,7 +514,7 @@ _YDT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 def _linear(x: torch.Tensor, w: torch.Tensor, groups: int, out_dtype: torch.dtype) -> torch.Tensor:
     """x [T, G*K], w [G*N, K] (both bf16 or both fp32) -> y [T, G*N]: y[:, gN:(g+1)N] = x[:, gK:(g+1)K] @ w_g^T
     (the weight-streaming kernel for few bf16 rows, the tiled MFMA GEMM otherwise)."""
-    _on_gpu(x, w)
+    dev = _one_device(x, w)
     x, w = x.contiguous(), w.contiguous()
     T = x.shape[0]
     K = w.shape[1]
@@ -526,8 +526,8 @@ def _linear(x: torch.Tensor, w: torch.Tensor, groups: int, out_dtype: torch.dtyp
     wsb = 0 if T <= 8 and x.dtype == torch.bfloat16 and K % 512 == 0 and N % 16 == 0 else \
         _lib.lib().smla_linear_workspace(T, groups, N, K, dtype_code(x))
     ws = torch.empty(wsb, dtype=torch.uint8, device=x.device) if wsb else None
-    _lib.call("smla_linear_ws", _p(x), dtype_code(x), _p(w), dtype_code(w), T, groups, N, K, _p(y), _YDT[out_dtype],
-              _p(ws), wsb, _stream(x))
+    _launch(dev, "smla_linear_ws", _p(x), dtype_code(x), _p(w), dtype_code(w), T, groups, N, K, _p(y), _YDT[out_dtype],
+            _p(ws), wsb)
     return y
 
 

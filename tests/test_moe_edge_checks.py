@@ -75,3 +75,33 @@ def test_tokens_outside_the_table_choose_nothing(monkeypatch, dtype):
     assert layer(_bf16(2, 4, 64), tokens).shape == (2, 4, 64)
     assert seen[0].tolist() == [[0, 1], [8, 9], [-1, -1], [6, 7], [-1, -1], [-1, -1], [2, 3], [-1, -1]]
     assert table.tolist() == [[0, 1], [2, 3], [4, 5], [6, 7], [8, 9]] and seen[0].dtype == torch.int32
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_a_layer_on_another_device(monkeypatch, current):
+    """Every launch of a layer and of the packing of its weights is made with the tensors' GPU current, on a stream of it."""
+    import contextlib
+    from smla import _lib, moe, ops
+    now, made = [current], []
+
+    @contextlib.contextmanager
+    def device(dev):
+        before, now[0] = now[0], dev
+        yield
+        now[0] = before
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(ops, "_current_device", lambda: now[0])
+    monkeypatch.setattr(ops, "_one_device", lambda t, *rest: 1)
+    monkeypatch.setattr(ops, "_on_gpu", lambda *ts: None)
+    monkeypatch.setattr(ops, "_raw_stream", lambda dev: ("stream", 1 if dev is None else dev))
+    monkeypatch.setattr(_lib, "call", lambda name, *args: made.append((name, now[0], args[-1])))
+    monkeypatch.setattr(ops, "linear_op", ops._linear)
+    monkeypatch.setattr(ops, "route_op", ops._route)
+    monkeypatch.setattr(ops, "experts_op", ops._experts)
+    monkeypatch.setattr(ops, "rotate_fp4_op", ops.rotate_fp4_op._init_fn)
+    gate, down = moe.pack_fp4(_bf16(3, 32, 64)), moe.pack_fp4(_bf16(3, 64, 32))
+    for T in (1, 8, 40):
+        for dt in (torch.bfloat16, torch.float32):
+            moe.ExpertLayer(moe.ExpertWeights(torch.zeros(2, 64, dtype=dt), gate, gate, down), k=2)(_bf16(T, 64))
+    assert [m[0] for m in made] == ["smla_rotate_fp4"] * 2 + ["smla_linear_ws", "smla_route", "smla_experts"] * 6
+    assert all(m[1:] == (1, ("stream", 1)) for m in made), made
