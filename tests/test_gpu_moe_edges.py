@@ -71,3 +71,66 @@ def test_layer_of_tokens_outside_the_table(dev):
         graph.replay()
         assert torch.equal(z, y)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("T", [1, 9, 60])
+def test_layer_with_a_router_in_fp32(dev, T):
+    """(The product of fp32 operands is within the bound that test_gpu_linear.py gives.)"""
+    from smla import moe
+    announce(f"layer with an fp32 router {T}")
+    E, k, K, I = 24, 4, 192, 64
+    layer, router, bias, dense = _layer(dev, E, k, K, I, 1, "fp4")
+    g = torch.Generator().manual_seed(T)
+    router = torch.randn(E, K, generator=g) * K ** -0.5
+    layer = moe.ExpertLayer(moe.ExpertWeights(router.to(dev), layer.w.gate, layer.w.up, layer.w.down, bias=bias.to(dev)), k=k)
+    x = torch.randn(T, K, generator=g).to(torch.bfloat16)
+    logits = layer.logits(x.to(dev)).cpu()
+    ref = x.double() @ router.double().T
+    assert ((logits.double() - ref).abs() <= (K + 8) * 2.0 ** -23 * (x.double().abs() @ router.double().abs().T)).all()
+    ids, w = om.route(logits, k, "sqrtsoftplus", bias=bias, scale=1.5, shared=1)
+    _check_experts(layer(x.to(dev)), om.experts(x, ids, w.float(), *dense, 10.0))
+
+
+def test_rows_up_to_the_last_that_a_call_addresses(dev):
+    """1023 rows 2^20 elements apart: offsets up to 2^31 bytes, in the tiles and, first and last 16 rows, in the kernels for few."""
+    from smla import mla, moe
+    announce("rows up to 2^31 bytes")
+    T, ld, E, k, K, I = 1023, 1 << 20, 4, 2, 64, 32
+    x, ids, w, mats = _experts_case(5, T, E, E, k, K, I, "fp4")
+    on = _on(dev, mats)
+    codes, scales, _ = _packed(6, 48, K)
+    codes, scales = codes.to(dev), scales.to(dev)
+    far = torch.empty(T * ld, dtype=torch.bfloat16, device=dev).as_strided((T, K), (ld, 1))
+    far.copy_(x)
+    near, ids, w = x.to(dev), ids.to(dev), w.to(dev)
+    for rows in (slice(0, T), slice(0, 16), slice(T - 16, T)):
+        assert torch.equal(moe.experts(far[rows], ids[rows], w[rows], *on), moe.experts(near[rows], ids[rows], w[rows], *on))
+        assert torch.equal(mla.linear_fp4(far[rows], codes, scales), mla.linear_fp4(near[rows], codes, scales))
+
+
+def test_two_threads(dev):
+    """Layers called from two threads at once, each on its own stream and with other sizes, give what they give alone."""
+    import threading
+    announce("two threads")
+    K = 192
+    layer, *_ = _layer(dev, 24, 4, K, 64, 1, "fp4")
+    xs = [torch.randn(T, K, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16).to(dev) for T in (3, 17, 61, 300)]
+    want = [layer(x) for x in xs]
+    torch.cuda.synchronize()
+    wrong, done = [], []
+
+    def work(mine):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                for i in mine:
+                    y = layer(xs[i])
+                    torch.cuda.current_stream().synchronize()
+                    if not torch.equal(y, want[i]):
+                        wrong.append(i)
+        done.append(mine)
+    threads = [threading.Thread(target=work, args=(m,)) for m in ((0, 2), (3, 1))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(done) == 2 and not wrong
