@@ -134,3 +134,25 @@ def test_two_threads(dev):
     for t in threads:
         t.join()
     assert len(done) == 2 and not wrong
+
+
+@pytest.mark.parametrize("T", [12, 40, 500])
+@pytest.mark.parametrize("kind", ["fp4", "bf16"])
+def test_experts_repeat_bit_for_bit(dev, T, kind):
+    """The same call gives the same bits, whatever order its pairs are sorted in; past 16 tokens a token's result does not
+    depend on the ids beside it either."""
+    from smla import moe
+    announce(f"experts repeat {T} {kind}")
+    E, k, K, I = 6, 3, 544, 416
+    x, ids, w, mats = _experts_case(T, T, E, E, k, K, I, kind)
+    on = _on(dev, mats)
+    xd, idd, wd = x.to(dev), ids.to(dev), w.to(dev)
+    y = moe.experts(xd, idd, wd, *on)
+    for _ in range(8):
+        assert torch.equal(moe.experts(xd, idd, wd, *on), y)
+    other = ids.clone()
+    other[1::2] = other[1::2].flip(0)
+    z = moe.experts(xd, other.to(dev), wd, *on)
+    if T > 16:
+        assert torch.equal(z[::2], y[::2])
+    _check_experts(z, om.experts(x, other, w, *[m[2] for m in mats]))
