@@ -6,7 +6,8 @@
 //
 // Products run on the bf16 matrix cores with fp32 sums; the weights are e2m1 codes (fp4.h) or bf16.  The hidden
 // row, its router weight in it, is rounded to bf16 once: it is an operand of the second product, and half a step of
-// its 8 bits is what y's own rounding costs again.
+// its 8 bits is what y's own rounding costs again (the norm of y's error 0.0023-0.0024 of y's; 0.0017 with fp32 hidden
+// rows, whose second product would be two or three bf16 ones).
 #include "expert_tile.h"
 #include "fp4.h"
 #include "smla_internal.h"
@@ -758,7 +759,8 @@ int few_waves(int64_t K) { return K <= 2048 ? 4 : K <= 4096 ? 8 : 16; }
 
 LinearPlan linear_plan(int64_t T, int64_t N, int64_t K) {
   // A model of the launches in microseconds, its constants fitted to 112 products (T 17 .. 512, N 256 .. 16384, K 512 .. 4096):
-  // the plan it picks is 2 % off the fastest on average and 30 % at worst.  The kernel for few tokens: a workgroup's time
+  // the plan it picks is 2 % off the fastest on average and 30 % at worst among those; larger sizes go by the same model,
+  // extrapolated.  The kernel for few tokens: a workgroup's time
   // goes with the bytes it reads (16 tokens and 16 outputs), those resident together overlap.  Tiles: a step takes kIdle when
   // few CUs run, kOne with a workgroup on each, kBusy with as many as fit; a split adds the launch that sums and its
   // fp32 partial sums, rows of scales that are no whole words another that lays them out.
@@ -836,6 +838,11 @@ int check_experts(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I) {
 // one of the others at every number of pairs (256 experts of 4096 x 2048, the up products: 48 pairs 709 us, 128 x 512 696;
 // 32 pairs 640, 32 x 256 513).  bf16 in 32 x 256 tiles came out behind 64 x 128 at every number (24 experts of 4096 x 2048:
 // 8 pairs 247 us against 235, 48 pairs 271 against 247); 128 x 256 passes those between 48 (261) and 64 (256 against 278).
+// The average is of all T k pairs over the E experts here, which the host knows without the ids: it is too high by the share of
+// ids outside 0 .. E-1 (24 of 48 experts here: 83 for 42, 128 x 256 in 126-131 us where 64 x 128 takes 117), and a shared expert's
+// pairs, T of them, count as any other's (1000 tokens of 256 + 1 experts: 32 x 256 throughout).  K, I and the number of CUs play no
+// part: 8 experts of 4096 x 1024 with 128 pairs each are 32 and 64 workgroups (79 and 27 us).
+// Few tokens: the LDS test is for T rows, though few_up_kernel holds `cap` of them.
 int expert_form(int64_t T, int64_t k, int64_t E, int64_t K, bool fp4) {
   if (T <= kFew && few_lds(T, (int)K, kUpWaves, 2) <= kMaxFewLds) return -1;
   const int64_t P = T * k, per = P / (E < P ? E : P);
@@ -858,7 +865,9 @@ ExpertBytes expert_bytes(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I, 
 
 template <int WT>
 int launch_few_up(const ExpertArgs& a, hipStream_t st) {
-  // rows for four times the tokens that an expert has on average, and two more
+  // rows for four times the tokens that an expert has on average, and two more; one that all tokens have (a shared one) is
+  // streamed once for each `cap` of them: 256 experts of 4096 x 2048 and a shared one, 6 + 1 a token, up and down: 8 tokens (cap 2) 94
+  // and 55 us, 16 (cap 3) 155 and 88
   const int cap = (int)std::min<int64_t>(a.T, 4 * a.P / a.E + 2), lds = (int)few_lds(cap, a.K, kUpWaves, 2 * kStaged<WT>);
   static std::atomic<uint64_t> attr{0};
   if (hipError_t e = smla_set_dynamic_lds((const void*)few_up_kernel<WT>, kMaxFewLds, attr); e != hipSuccess) return (int)e;

@@ -10,17 +10,20 @@
 // is the logits', which needs no scores.  -inf and NaN rank last.
 //
 // route_kernel: 16 lanes a token, four tokens a wave, lane l holds experts l, l + 16, .. as integers of the values' order, whose
-// last 4 (5) bits are the place in the lane.  Each lane sorts its own, and a pick is a maximum over the lanes' first ones (lane
-// moves inside the row of 16, DPP).  It ranks fp32 scores, whose error is below 2^-21 (1 + s + |r|) (score32).  Where two
-// neighbours of the order are closer than twice that and the last bits (1 row in some hundreds of 256 random experts; never
-// for bf16 logits without a bias), the k and the next one are put in the order of their float64 values; where that does not
-// settle it, the last group in and the first one out are as close, or anything is not finite, the whole wave ranks the token in
-// float64 (rank_f64).  The weights are of float64 scores, of the k picked alone (softmax: the sum over the row is of fp32
-// exponentials).
+// last 4 (5) bits are the place in the lane.  Each lane sorts its own, and a pick is a maximum over the lanes' first ones
+// (lane moves inside the row of 16, DPP).  It ranks fp32 scores, whose error is below 2^-21 (1 + s + |r|) (score32).  Where
+// two neighbours of the order are closer than twice that and the last bits (of 256 random experts 1 row in 320 to 640 with a
+// bias, in 2300 without one; never for bf16 logits without a bias), the k and the next one are put in the order of their
+// float64 values; where that does not settle it, the last group in and the first one out are as close (1 row in 9000, 4 of 8
+// groups), or anything is not finite, the whole wave ranks the token in float64 (rank_f64).  The weights are of float64
+// scores, of the k picked alone (softmax: the sum over the row is of fp32 exponentials).
 // What bounds it is issue and latency: 16384 tokens of 256 experts in 8 groups, k = 8, 17.6-20 us (17.8 MB, 2.9 us of bytes;
-// 19-22 where each pick searched a lane's 16 values, about 85 instructions for four tokens against 35 and 130 for the sort);
-// 1031 tokens of 100, k = 4, 4.1 us; one token 4.5 us (three dependent latencies and float64 weights).
-// route_f64_kernel: one token a wave in float64 throughout, for what the first does not take.
+// a wave is 1640 vector instructions, four waves a SIMD, which are active for 11 us; 19-22 where each pick searched a lane's
+// 16 values, about 85 instructions for four tokens against 35 and 130 for the sort); 1031 tokens of 100, k = 4, 4.1 us; one
+// token 4.5 us (three dependent latencies and float64 weights).
+// route_f64_kernel: one token a wave in float64 throughout, for what the first does not take (more than 16 columns or 512 experts,
+// groups of no whole 16): 16384 tokens of 160 experts in 8 groups, k = 6, 36 us; of 256, k = 16 and a shared one, 64 us; one token
+// 6.7 us.
 #include "smla_internal.h"
 
 namespace {

@@ -27,7 +27,8 @@ def route(logits, k, score="softmax", bias=None, groups=1, topk_groups=1, renorm
     values.  The weights are the scores of the ids, divided by their sum (``renorm``; 0 where it is 0), times
     ``scale``.  ``shared`` columns E, E + 1, .. of weight 1 follow: experts that every token uses, stored behind the E.
     ``ids`` [T, k] int32 are taken instead of a choice (a layer whose table gives every token its experts): those and
-    their weights are returned, 0 for one outside 0 .. E-1.  Logits of -inf and NaN rank last."""
+    their weights are returned, 0 for one outside 0 .. E-1.  Logits of -inf and NaN rank last.  E up to 1024, k + ``shared`` up to
+    64."""
     if score not in _lib.SCORES:
         raise ValueError(f"score must be one of {sorted(_lib.SCORES)}, got {score!r}")
     return ops.route_op(logits, bias, int(k), _lib.SCORES[score], int(groups), int(topk_groups), bool(renorm), float(scale),
@@ -39,7 +40,9 @@ def experts(x, ids, weights, gate, up, down, limit=None):
     u = up_e(x[t]), e = ids[t, j] (``limit`` None: no clamp).  x [T, K] bf16 (rows may lie apart), ids [T, k] int32,
     weights [T, k].  gate, up [E, I, K] and down [E, K, I]: dense bf16 tensors, or (codes, scales) pairs of ``pack_fp4``.
     An id outside 0 .. E-1 adds nothing: a device that holds some of the experts passes ids less its first one's.  The same
-    id twice counts twice.  Sums are fp32, the hidden row (its weight in it) and y are rounded to bf16."""
+    id twice counts twice.  Sums are fp32, the hidden row (its weight in it) and y are rounded to bf16.  The same call gives the same
+    bits; in a batch of up to 16 tokens the ids of the others may change the order of a token's fp32 sums.  E up to 1024, k up to 64;
+    any number of tokens."""
     (gate, gs), (up, us), (down, ds) = (w if isinstance(w, (tuple, list)) else (w, None) for w in (gate, up, down))
     return ops.experts_op(x, ids, weights, gate, up, down, gs, us, ds, float("inf") if limit is None else float(limit))
 
