@@ -1367,7 +1367,7 @@ def _experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate: to
     wdt = _lib.FP4_E2M1 if fp4 else _lib.BF16
     n = T
     if T * k > 1 << 20 or T * ld >= 1 << 30:
-        most = max(1, min((1 << 20) // max(k, 1), ((1 << 30) - 1) // ld))
+        most = max(1, min((1 << 20) // max(k, 1), ((1 << 30) - 1) // max(ld, 1)))
         n = -(-T // -(-T // most))      # as many tokens a call, the last one's rest aside
     wsb = _workspace(dev, "smla_experts_workspace", n, k, E, K, inner, wdt)
     if T % n:

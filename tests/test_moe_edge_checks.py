@@ -105,3 +105,16 @@ def test_a_layer_on_another_device(monkeypatch, current):
             moe.ExpertLayer(moe.ExpertWeights(torch.zeros(2, 64, dtype=dt), gate, gate, down), k=2)(_bf16(T, 64))
     assert [m[0] for m in made] == ["smla_rotate_fp4"] * 2 + ["smla_linear_ws", "smla_route", "smla_experts"] * 6
     assert all(m[1:] == (1, ("stream", 1)) for m in made), made
+
+
+def test_rows_and_choices_of_nothing_are_the_librarys_errors(calls, monkeypatch):
+    """Many tokens of no choices or of empty rows reach the library, which refuses them."""
+    import ctypes
+    from smla import _lib, ops
+    monkeypatch.setattr(ops, "_launch", lambda dev, name, *args: _lib.call(name, *args, ctypes.c_void_p(0)))
+    T = (1 << 20) + 1
+    for k, K in ((1, 0), (0, 32)):
+        x = torch.empty(T, K, dtype=torch.bfloat16)
+        with pytest.raises(_lib.SmlaError):
+            ops._experts(x, torch.zeros(T, k, dtype=torch.int32), torch.zeros(T, k), _bf16(2, 32, K), _bf16(2, 32, K),
+                         _bf16(2, K, 32), None, None, None, 1.0)
