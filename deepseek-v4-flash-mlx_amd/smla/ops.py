@@ -516,6 +516,8 @@ def _linear(x: torch.Tensor, w: torch.Tensor, groups: int, out_dtype: torch.dtyp
     (the weight-streaming kernel for few bf16 rows, the tiled MFMA GEMM otherwise)."""
     dev = _one_device(x, w)
     x, w = x.contiguous(), w.contiguous()
+    if x.data_ptr() & 15:       # (a dense view may begin anywhere)
+        x = x.clone()
     T = x.shape[0]
     K = w.shape[1]
     N = w.shape[0] // groups

@@ -156,3 +156,20 @@ def test_experts_repeat_bit_for_bit(dev, T, kind):
     if T > 16:
         assert torch.equal(z[::2], y[::2])
     _check_experts(z, om.experts(x, other, w, *[m[2] for m in mats]))
+
+
+@pytest.mark.parametrize("T", [1, 2, 40])
+@pytest.mark.parametrize("kind", ["fp4", "bf16"])
+def test_layer_of_inputs_that_begin_anywhere(dev, T, kind):
+    """A layer takes its inputs at any address, one token (whose row is dense wherever it begins) as many."""
+    announce(f"layer inputs anywhere {T} {kind}")
+    K = 192
+    layer, *_ = _layer(dev, 24, 4, K, 64, 1, kind)
+    x = torch.randn(T, K, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16).to(dev)
+    want = layer(x)
+    for wide, at in ((K + 8, 3), (K + 5, 1), (K + 16, 8)):
+        y = torch.full((T, wide), math.nan, dtype=torch.bfloat16, device=dev)[:, at:at + K]
+        y.copy_(x)
+        assert torch.equal(layer(y), want)
+    flat = torch.empty(T * K + 1, dtype=torch.bfloat16, device=dev)[1:].view(T, K).copy_(x)
+    assert torch.equal(layer(flat), want)
