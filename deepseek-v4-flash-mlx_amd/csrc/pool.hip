@@ -185,13 +185,13 @@ __device__ inline f32x2_t epilogue_values(float v0, float v1, int d, int rd, flo
     y0 *= hs;
     y1 *= hs;
     // fp4 round trip per 32-channel block = 16 threads (one DPP row), v4mlx/qat.py:23-31
-    float am = fmaxf(fabsf(y0), fabsf(y1));
-    am = fmaxf(am, dpp_f<0xB1>(am));
-    am = fmaxf(am, dpp_f<0x4E>(am));
-    am = fmaxf(am, dpp_f<0x141>(am));
-    am = fmaxf(am, dpp_f<0x140>(am));
+    float am = fp4_amax(fp4_amax(0.f, y0), y1);
+    am = fp4_amax(am, dpp_f<0xB1>(am));
+    am = fp4_amax(am, dpp_f<0x4E>(am));
+    am = fp4_amax(am, dpp_f<0x141>(am));
+    am = fp4_amax(am, dpp_f<0x140>(am));
     const int k = fp4_scale_exp(am);
-    const float si = exp2i_f32(-k), s = exp2i_f32(k);
+    const float si = exp2i_f32(-k), s = fp4_scale(k);
     y0 = e2m1_to_f32(f32_to_e2m1(fminf(fmaxf(y0 * si, -6.f), 6.f))) * s;
     y1 = e2m1_to_f32(f32_to_e2m1(fminf(fmaxf(y1 * si, -6.f), 6.f))) * s;
   }

@@ -7,7 +7,8 @@
 //      FP4   : v4mlx/qat.py:23-31 per block of 32: s = 2^ceil(log2(max(amax, 6*2^-126) / 6)),
 //              code = e2m1(clip(x / s, +-6)), round to nearest even; written as the round trip
 //              (code value * s, float32) and/or the stored form (packed codes, element 2i in the
-//              low nibble of byte i; one ue8m0 scale byte log2(s) + 127 per block).
+//              low nibble of byte i; one ue8m0 scale byte log2(s) + 127 per block); a block with a value
+//              that is not finite has scale 255 and is NaN in all of it.
 //    Layout: a lane holds 32 consecutive values (one fp4 block), a row spans L = N / 32 lanes of
 //    one wave, so 64 / L rows share a wave.  Butterfly stages h < 32 stay in registers; the
 //    others pair lane l with lane l ^ (h / 32) through DPP (h / 32 < 4) or ds_bpermute.  The
@@ -109,9 +110,9 @@ __global__ __launch_bounds__(kQatThreads) void rotate_fp4_kernel(const void* __r
   if (fp4) {
     float a = 0.f;
 #pragma unroll
-    for (int i = 0; i < E; i++) a = fmaxf(a, fabsf(v[i]));
+    for (int i = 0; i < E; i++) a = fp4_amax(a, v[i]);
     const int kexp = fp4_scale_exp(a);
-    const float inv = exp2i_f32(-kexp), s = exp2i_f32(kexp);
+    const float inv = exp2i_f32(-kexp), s = fp4_scale(kexp);
     // z = x * 2^-k (== x / 2^k, one rounding) in VALU arithmetic; the gfx950 conversion with
     // scale 1 then rounds z to e2m1 (nearest, ties to even, saturating at +-6), two per call,
     // element 2i into the low nibble of byte i

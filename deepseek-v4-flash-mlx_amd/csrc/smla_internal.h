@@ -137,13 +137,16 @@ __host__ __device__ inline float e2m1_to_f32(uint32_t code) {
   return (code & 8u) ? -m : m;
 }
 // exponent k of the fp4 block scale s = 2^k = 2^ceil(log2(max(amax, 6*2^-126) / 6)); the division
-// is the float32 one of the definition (rounded), the ceiling is exact on its bits
+// is the float32 one of the definition (rounded), the ceiling is exact on its bits.  128, the scale byte 255 (NaN), where amax
+// (fp4_amax: fmaxf would drop a NaN) is not finite: the largest finite one has 126
+__device__ inline float fp4_amax(float a, float x) { return __builtin_elementwise_maximum(a, __builtin_fabsf(x)); }
 __host__ __device__ inline int fp4_scale_exp(float amax) {
-  const float a = fmaxf(amax, 6.0f * 0x1p-126f);
+  const float a = amax < 6.0f * 0x1p-126f ? 6.0f * 0x1p-126f : amax;
   const float v = a / 6.0f;  // >= 2^-126: a normal number
   uint32_t u;
   __builtin_memcpy(&u, &v, 4);
-  return (int)((u >> 23) & 0xffu) - 127 + ((u & 0x7fffffu) ? 1 : 0);
+  const int k = (int)((u >> 23) & 0xffu) - 127 + ((u & 0x7fffffu) ? 1 : 0);
+  return k < 128 ? k : 128;
 }
 // 2^k as float32 for -126 <= k <= 127
 __host__ __device__ inline float exp2i_f32(int k) {
@@ -152,6 +155,8 @@ __host__ __device__ inline float exp2i_f32(int k) {
   __builtin_memcpy(&f, &u, 4);
   return f;
 }
+// the scale of that exponent
+__device__ inline float fp4_scale(int k) { return k < 128 ? exp2i_f32(k) : __builtin_nanf(""); }
 // ue8m0 scale byte b -> 2^(b-127) as float32: 0 gives the subnormal 2^-127, 255 the E8M0 NaN
 __host__ __device__ inline float ue8m0_to_f32(uint32_t b) {
   // selects, not branches: inside unrolled loops a branch splits the schedule

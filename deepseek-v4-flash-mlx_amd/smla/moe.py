@@ -49,7 +49,8 @@ def experts(x, ids, weights, gate, up, down, limit=None):
 
 def pack_fp4(w):
     """(codes [..., K/2], scales [..., K/32]) of weights [..., K] (fp32 or bf16, K a multiple of 32): the nearest e2m1
-    values under a power of two per 32 (``v4mlx/qat.py:23-31`` without the rotation)."""
+    values under a power of two per 32 (``v4mlx/qat.py:23-31`` without the rotation).  32 weights with one that is not finite are
+    NaN, all of them."""
     if w.shape[-1] % 32:
         raise ValueError(f"rows of a multiple of 32 weights are packed, got {w.shape[-1]}")
     codes, scales = qat.fp4_pack(w.reshape(-1, 32), rotate=False)

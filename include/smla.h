@@ -317,7 +317,8 @@ int smla_block_mean_pool(const void* x, int x_dtype, int64_t B, int64_t N, int64
  *                        (NaN in all of a block with a value that is not finite)
  *                        (v4mlx/compressor.py:60-62, apply_sim=True);
  *   SMLA_SIM_ROTATE_FP4  all d channels Hadamard-rotated, then fp4 round-tripped with pow2
- *                        block-32 scales (v4mlx/compressor.py:57-59, rotate=True: the indexer
+ *                        block-32 scales, NaN in all of a block that is not finite
+ *                        (v4mlx/compressor.py:57-59, rotate=True: the indexer
  *                        compressor). */
 enum { SMLA_SIM_NONE = 0, SMLA_SIM_FP8 = 1, SMLA_SIM_ROTATE_FP4 = 2 };
 
@@ -446,6 +447,7 @@ int smla_quant_fp8_pow2(const void* x, int x_dtype, int64_t rows, int64_t D, uin
  *           h = 1, 2, ..., n/2 in float32 (pairs (y[i], y[i+h]) -> (sum, difference));
  *           SMLA_QAT_FP4: per block of 32, s = 2^ceil(log2(max(amax, 6*2^-126) / 6)),
  *           q = e2m1(clip(y / s, +-6)) (round to nearest even, grid 0..6);
+ *           a block with a value that is not finite is NaN in all of it (scale byte 255; its codes are any);
  *           both: rotation first (the indexer key path)
  *   out     [rows, n] fp32 or NULL: the result (with FP4, the round trip q * s)
  *   codes   [rows, n/2] uint8 or NULL: packed e2m1 codes, element 2i in the low nibble of byte

@@ -173,3 +173,23 @@ def test_layer_of_inputs_that_begin_anywhere(dev, T, kind):
         assert torch.equal(layer(y), want)
     flat = torch.empty(T * K + 1, dtype=torch.bfloat16, device=dev)[1:].view(T, K).copy_(x)
     assert torch.equal(layer(flat), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_packed_weights_that_are_not_finite(dev, dtype):
+    """A block of 32 weights that holds a NaN or an infinity is NaN when packed, and the products with it; no other block changes."""
+    from smla import mla, moe
+    announce(f"packed weights not finite {dtype}")
+    N, K = 24, 160
+    g = torch.Generator().manual_seed(3)
+    w = torch.randn(2, N, K, generator=g).to(dtype)
+    clean_codes, clean_scales = moe.pack_fp4(w.to(dev))
+    bad = w.clone()
+    bad[0, 3, 40], bad[0, 5, 159], bad[1, 7, 0], bad[1, 7, 1] = math.nan, math.inf, -math.inf, math.nan
+    codes, scales = moe.pack_fp4(bad.to(dev))
+    hit = ~bad.isfinite().view(2, N, K // 32, 32).all(-1)
+    assert hit.sum() == 3 and (scales.cpu()[hit] == 255).all()
+    assert torch.equal(scales.cpu()[~hit], clean_scales.cpu()[~hit])
+    assert torch.equal(codes.cpu().view(2, N, K // 32, 16)[~hit], clean_codes.cpu().view(2, N, K // 32, 16)[~hit])
+    y = mla.linear_fp4(torch.randn(5, K, generator=g).to(torch.bfloat16).to(dev), codes[0], scales[0])
+    assert y[:, [3, 5]].isnan().all() and y[:, 6:].isfinite().all()
